@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <mutex>
+#include <optional>
 #include <stdexcept>
 #include <string>
 #include <unordered_map>
@@ -137,7 +138,7 @@ struct WithoutGil {
 // its own (or whose words another's would land on).  The lock is held from the look-up to the last launch of a call: another
 // thread on the same stream neither replaces the scratch under it nor puts a launch between its steps.  It is never waited
 // for with the GIL held.
-enum Slot { kSlotShared = 0, kSlotLinear = 1, kSlotRouter = 2, kSlotGemm = 3, kSlots = 4 };        // Python names them in _torch_util.py
+enum Slot { kSlotShared = 0, kSlotLinear = 1, kSlotRouter = 2, kSlotGemm = 3, kSlotW4a16 = 4, kSlots = 5 };        // Python names them in _torch_util.py
 struct StreamScratch {
   std::mutex mu;
   at::Tensor slots[kSlots];
@@ -481,6 +482,110 @@ B200_FN(py_moe_prefill) {
   });
 }
 
+// ------------------------------------------------------------------------------------------ weight-only operators
+
+bool is_float(const at::Tensor& t) { return is_16bit(t) || t.scalar_type() == at::kFloat; }
+bool rows_aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(0) < 2 || t.stride(0) % 8 == 0); }
+
+// w4a16_linear(x, packed, g_scale, N, K, bias or None, out or None, out_dtype or None) -> out
+B200_FN(py_w4a16_linear) {
+  return guarded([&] {
+    want_args(n_args, 8);
+    const at::Tensor &x = tensor(args[0]), &w = tensor(args[1]), &g = tensor(args[2]);
+    const int64_t N = integer(args[3]), K = integer(args[4]);
+    const at::Tensor *bias = maybe_tensor(args[5]), *given = maybe_tensor(args[6]);
+    const int dev = require_cuda({&x, &w, &g, bias, given});
+    require(x.dim() == 2 && is_16bit(x) && x.size(1) == K && x.stride(1) == 1, "x must be [M,K] bf16/f16, unit inner stride");
+    const int64_t M = x.size(0);
+    require(M == 0 || rows_aligned(x), "the rows of x must be 16-byte aligned");
+    require(M < 2 || x.stride(0) >= K, "the rows of x must not overlap");
+    require(w.scalar_type() == at::kByte && w.is_contiguous() && w.nbytes() >= b200fp4_w4a16_packed_bytes(1, N, K, 0), "weight must come from pack_nvfp4_weight");
+    require(is_f32_scalar(g), "g_scale must be one f32");
+    require(bias == nullptr || (bias->dim() == 1 && bias->size(0) == N && is_float(*bias) && bias->is_contiguous()), "bias must be a contiguous [N] tensor in bf16, f16 or f32");
+    at::ScalarType dt = x.scalar_type();
+    if (args[7] != Py_None) {
+      require(THPDtype_Check(args[7]), "out_dtype must be bfloat16, float16 or float32");
+      dt = reinterpret_cast<THPDtype*>(args[7])->scalar_type;
+    } else if (given) {
+      dt = given->scalar_type();
+    }
+    require(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, "out_dtype must be bfloat16, float16 or float32");
+    require(given == nullptr || (given->scalar_type() == dt && is_2d(*given, M, N) && given->is_contiguous()), "out must be a contiguous [M,N] tensor of out_dtype");
+    at::Tensor out;
+    {
+      WithoutGil nogil;
+      c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+      out = given ? *given : empty({M, N}, dt, dev);
+      if (M > 0) {
+        cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+        const Workspace ws(dev, st, b200fp4_w4a16_linear_workspace_bytes(M, N, K), kSlotW4a16);
+        check(b200fp4_w4a16_linear(ptr(x), dtype_code(x.scalar_type()), M > 1 ? x.stride(0) : K, ptr<uint8_t>(w), ptr<float>(g),
+                                   bias ? ptr(*bias) : nullptr, bias ? dtype_code(bias->scalar_type()) : 0, ptr(out), dtype_code(dt), M, N, K,
+                                   ws.data(), ws.bytes(), st),
+              "w4a16_linear");
+      }
+    }
+    if (given) {
+      Py_INCREF(args[6]);
+      return args[6];
+    }
+    return wrap(std::move(out));
+  });
+}
+
+// w4a16_moe(w13, w13_g, w2, w2_g, expert_map or None, H, I, E, hidden, topk_weights, topk_ids, weight_on_input, out or None) -> out
+B200_FN(py_w4a16_moe) {
+  return guarded([&] {
+    want_args(n_args, 13);
+    const at::Tensor &w13 = tensor(args[0]), &g13 = tensor(args[1]), &w2 = tensor(args[2]), &g2 = tensor(args[3]);
+    const at::Tensor* emap = maybe_tensor(args[4]);
+    const int64_t H = integer(args[5]), I = integer(args[6]), E = integer(args[7]);
+    const at::Tensor &x = tensor(args[8]), &tw_in = tensor(args[9]), &ids_in = tensor(args[10]);
+    const int flags = truth(args[11]) ? B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT : 0;
+    const at::Tensor* given = maybe_tensor(args[12]);
+    const int dev = require_cuda({&w13, &g13, &w2, &g2, emap, &x, &tw_in, &ids_in, given});
+    require(x.dim() == 2 && x.size(1) == H && x.is_contiguous() && is_16bit(x), "hidden_states must be a contiguous [M,H] 16-bit tensor");
+    const int64_t M = x.size(0);
+    require(M == 0 || rows_aligned(x), "hidden_states must be 16-byte aligned");
+    require(ids_in.dim() == 2 && ids_in.size(0) == M && ids_in.size(1) > 0 && is_2d(tw_in, M, ids_in.size(1)), "topk_weights and topk_ids must be [M, topk]");
+    require(ids_in.scalar_type() == at::kInt || ids_in.scalar_type() == at::kLong, "topk_ids must be int32 or int64");
+    const int64_t topk = ids_in.size(1);
+    require(w13.nbytes() >= b200fp4_w4a16_packed_bytes(E, 2 * I, H, 1) && w2.nbytes() >= b200fp4_w4a16_packed_bytes(E, H, I, 0) && g13.numel() == 2 * E &&
+                g2.numel() == E,
+            "the weights must come from pack_nvfp4_weight");
+    require(given == nullptr || (is_float(*given) && is_2d(*given, M, H) && given->is_contiguous()), "out must be a contiguous [M,H] tensor in bf16, f16 or f32");
+    at::Tensor out;
+    {
+      WithoutGil nogil;
+      c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+      out = given ? *given : empty({M, H}, x.scalar_type(), dev);
+      if (M > 0) {
+        const at::Tensor ids = (ids_in.scalar_type() == at::kInt ? ids_in : ids_in.to(at::kInt)).contiguous();
+        const at::Tensor tw = (tw_in.scalar_type() == at::kFloat ? tw_in : tw_in.to(at::kFloat)).contiguous();
+        cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+        const size_t bytes = b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I);
+        // A captured call has scratch of its own, from its graph's pool: graphs that are replayed at once share none.
+        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+        const bool captured = cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
+        std::optional<Workspace> ws;
+        at::Tensor own;
+        if (captured) own = empty({(int64_t)bytes}, at::kByte, dev);
+        else ws.emplace(dev, st, bytes);
+        check(b200fp4_w4a16_moe(ptr(x), dtype_code(x.scalar_type()), ptr<float>(tw), ptr<int32_t>(ids), emap ? ptr<int32_t>(*emap) : nullptr,
+                                emap ? emap->numel() : 0, ptr<uint8_t>(w13), ptr<float>(g13), ptr<uint8_t>(w2), ptr<float>(g2), ptr(out),
+                                dtype_code(out.scalar_type()), M, topk, H, I, E, flags, captured ? own.data_ptr() : ws->data(),
+                                captured ? own.nbytes() : ws->bytes(), st),
+              "w4a16_moe");
+      }
+    }
+    if (given) {
+      Py_INCREF(args[12]);
+      return args[12];
+    }
+    return wrap(std::move(out));
+  });
+}
+
 PyMethodDef kMethods[] = {
     {"workspace", (PyCFunction)(void (*)())py_workspace, METH_FASTCALL, nullptr},
     {"scaled_fp4_quant", (PyCFunction)(void (*)())py_quant, METH_FASTCALL, nullptr},
@@ -489,6 +594,8 @@ PyMethodDef kMethods[] = {
     {"moe_router", (PyCFunction)(void (*)())py_router, METH_FASTCALL, nullptr},
     {"moe_bind", (PyCFunction)(void (*)())py_moe_bind, METH_FASTCALL, nullptr},
     {"moe_call", (PyCFunction)(void (*)())py_moe_call, METH_FASTCALL, nullptr},
+    {"w4a16_linear", (PyCFunction)(void (*)())py_w4a16_linear, METH_FASTCALL, nullptr},
+    {"w4a16_moe", (PyCFunction)(void (*)())py_w4a16_moe, METH_FASTCALL, nullptr},
     {"moe_prefill", (PyCFunction)(void (*)())py_moe_prefill, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
