@@ -20,7 +20,6 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <mutex>
-#include <optional>
 #include <stdexcept>
 #include <string>
 #include <unordered_map>
@@ -487,6 +486,27 @@ B200_FN(py_moe_prefill) {
 bool is_float(const at::Tensor& t) { return is_16bit(t) || t.scalar_type() == at::kFloat; }
 bool rows_aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(0) < 2 || t.stride(0) % 8 == 0); }
 
+// Status word and scratch of a call.  The scratch of a captured call is its own, from its graph's pool: graphs that are replayed at once
+// share no more than the status word.
+class Scratch {
+ public:
+  Scratch(int dev, cudaStream_t st, size_t bytes) : captured_(capturing(st)), shared_(dev, st, 256 + (captured_ ? 0 : bytes), kSlotW4a16) {
+    if (captured_ && bytes > 0) own_ = empty({(int64_t)bytes}, at::kByte, dev);
+  }
+  int32_t* status() const { return static_cast<int32_t*>(shared_.data()); }
+  void* data() const { return captured_ ? (own_.defined() ? own_.data_ptr() : nullptr) : static_cast<uint8_t*>(shared_.data()) + 256; }
+  size_t bytes() const { return captured_ ? (own_.defined() ? own_.nbytes() : 0) : shared_.bytes() - 256; }
+
+ private:
+  static bool capturing(cudaStream_t st) {
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    return cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
+  }
+  bool captured_;
+  Workspace shared_;
+  at::Tensor own_;
+};
+
 // w4a16_linear(x, packed, g_scale, N, K, bias or None, out or None, out_dtype or None) -> out
 B200_FN(py_w4a16_linear) {
   return guarded([&] {
@@ -518,10 +538,10 @@ B200_FN(py_w4a16_linear) {
       out = given ? *given : empty({M, N}, dt, dev);
       if (M > 0) {
         cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-        const Workspace ws(dev, st, b200fp4_w4a16_linear_workspace_bytes(M, N, K), kSlotW4a16);
+        const Scratch ws(dev, st, 0);
         check(b200fp4_w4a16_linear(ptr(x), dtype_code(x.scalar_type()), M > 1 ? x.stride(0) : K, ptr<uint8_t>(w), ptr<float>(g),
                                    bias ? ptr(*bias) : nullptr, bias ? dtype_code(bias->scalar_type()) : 0, ptr(out), dtype_code(dt), M, N, K,
-                                   ws.data(), ws.bytes(), st),
+                                   ws.status(), st),
               "w4a16_linear");
       }
     }
@@ -563,18 +583,10 @@ B200_FN(py_w4a16_moe) {
         const at::Tensor ids = (ids_in.scalar_type() == at::kInt ? ids_in : ids_in.to(at::kInt)).contiguous();
         const at::Tensor tw = (tw_in.scalar_type() == at::kFloat ? tw_in : tw_in.to(at::kFloat)).contiguous();
         cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-        const size_t bytes = b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I);
-        // A captured call has scratch of its own, from its graph's pool: graphs that are replayed at once share none.
-        cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-        const bool captured = cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
-        std::optional<Workspace> ws;
-        at::Tensor own;
-        if (captured) own = empty({(int64_t)bytes}, at::kByte, dev);
-        else ws.emplace(dev, st, bytes);
+        const Scratch ws(dev, st, b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I));
         check(b200fp4_w4a16_moe(ptr(x), dtype_code(x.scalar_type()), ptr<float>(tw), ptr<int32_t>(ids), emap ? ptr<int32_t>(*emap) : nullptr,
                                 emap ? emap->numel() : 0, ptr<uint8_t>(w13), ptr<float>(g13), ptr<uint8_t>(w2), ptr<float>(g2), ptr(out),
-                                dtype_code(out.scalar_type()), M, topk, H, I, E, flags, captured ? own.data_ptr() : ws->data(),
-                                captured ? own.nbytes() : ws->bytes(), st),
+                                dtype_code(out.scalar_type()), M, topk, H, I, E, flags, ws.status(), ws.data(), ws.bytes(), st),
               "w4a16_moe");
       }
     }

@@ -5,14 +5,16 @@
 //   linear   columns are tokens
 //   gate/up  columns are the (token, expert) pairs of one expert; a tile's rows are eight gate rows and the same eight up rows, so that a
 //            lane holds both halves of its values and applies SiLU(gate) * up to them
-//   down     two columns a pair, the activation's upper and lower 16 bits: bf16 holds eight significant bits, the sum of two holds
-//            sixteen, at any magnitude that f32 has, so that the value between the projections is not what limits the result
+//   down     two columns a pair, the activation's upper and lower part in f16: their sum has 22 bits, so that the value between the projections is
+//            not what limits the result
 // Work items are (tile, slot); a slot is a run of one expert's pairs that fits the columns.  A block has a contiguous range of them, groups of
 // warps take items in turn and split k among themselves.
 // The layer is two launches without anything that has to outlast them: both find the slots from the routing by themselves, the first sets the
 // counters of the second, in which the block that finishes a tile's last item adds up its pairs in their order.
 #include <algorithm>
+#include <type_traits>
 
+#include "sm100_ptx.cuh"
 #include "w4a16.cuh"
 
 namespace b200fp4 {
@@ -26,6 +28,7 @@ struct PackParams {
   const uint8_t* codes;       // [E, N, K/2]
   const uint8_t* scales;      // [E, N, K/16]
   uint8_t* packed;
+  uint32_t* peaks;            // [E], gated [E][gate, up]: behind the units, zeroed before
   int64_t tiles, units;
   int N, K, gated;
 };
@@ -38,9 +41,10 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
   const int64_t u = unit % p.units, tile = unit / p.units % p.tiles, e = unit / p.units / p.tiles;
   uint8_t* const dst = p.packed + unit * kUnitBytes;
   uint32_t sc = 0;
+  float peak[2] = {0.f, 0.f};
   for (int half = 0; half < 2; ++half) {
     const int64_t k = u * kUnitK + half * 64 + (lane & 3) * 16;
-    uint32_t word[4];
+    uint2 word[2];
     for (int r = 0; r < 2; ++r) {
       // rows of a tile: 16 neighbours, or eight of the gate and the same eight of the up half
       const int64_t row = p.gated ? (tile * 8 + (lane >> 2) < p.N / 2 ? r * (int64_t)(p.N / 2) + tile * 8 + (lane >> 2) : p.N)
@@ -56,21 +60,23 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
           c.y ^= 0x88888888u;
         }
       }
-      sc |= (scale & 0x7F) << (8 * (half * 2 + r));
-      for (int q = 0; q < 2; ++q) {
-        const uint32_t w = q ? c.y : c.x;
-        uint32_t out = 0;
-        for (int i = 0; i < 8; ++i) {
-          constexpr int kSign[4] = {15, 12, 13, 14}, kMag[4] = {6, 3, 0, 9};
-          const uint32_t code = (w >> (4 * i)) & 15;
-          out |= (((code >> 3) << kSign[i >> 1]) | ((code & 7) << kMag[i >> 1])) << (16 * (i & 1));
-        }
-        word[r * 2 + q] = out;
-      }
+      scale &= 0x7F;
+      if (scale == 0x7F) scale = 0x7E;             // NaN, which the caller has refused
+      sc |= scale << (8 * (half * 2 + r));
+      word[r] = c;
+      uint32_t code = 0;
+      for (int i = 0; i < 16; ++i) code = max(code, ((i < 8 ? c.x : c.y) >> (4 * (i & 7))) & 7);
+      const float value = (code < 2 ? 0.5f * code : (1.f + 0.5f * (code & 1)) * (float)(1 << (code >> 1)) * 0.5f) * e4m3_to_f32((uint8_t)scale);
+      peak[p.gated ? r : 0] = fmaxf(peak[p.gated ? r : 0], value);
     }
-    *reinterpret_cast<uint4*>(dst + half * 512 + lane * 16) = make_uint4(word[0], word[1], word[2], word[3]);
+    *reinterpret_cast<uint4*>(dst + half * 512 + lane * 16) = make_uint4(word[0].x, word[0].y, word[1].x, word[1].y);
   }
   *reinterpret_cast<uint32_t*>(dst + kUnitScales + lane * 4) = sc;
+  // magnitudes are not negative: their bits order as they do
+  for (int r = 0; r <= p.gated; ++r) {
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(peak[r]));
+    if (lane == 0) atomicMax(p.peaks + e * (p.gated + 1) + r, top);
+  }
 }
 
 // ------------------------------------------------------------------------------------------ products
@@ -78,11 +84,11 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
 enum Mode { kLinear, kGateUp, kDown };
 
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
-constexpr int kMaxPairs = 4096;                // pairs whose slots a block finds in its shared memory; more are done in turns
+constexpr int kMaxPairs = 2048;                // pairs whose slots a block finds in its shared memory; more are done in turns
 constexpr int kMaxExperts = 4096;
 
 struct RowsParams {
-  const void* x;              // [M, K], rows ldx apart; down: [pair][upper, lower][K] bf16
+  const void* x;              // [M, K], rows ldx apart; down: [pair][upper, lower][K] f16
   int64_t ldx;
   const uint8_t* packed;
   const float* g;             // [E]; gate/up [E][gate, up]
@@ -91,34 +97,50 @@ struct RowsParams {
   int out_dtype, bias_dtype;
   int M, N, K;
   int tiles, units;
+  int cap, rows;              // columns of a slot; rows that there is room for
+  int* status;
+  int clear_status;
   // layer
   const int32_t* ids;         // [M, topk]
   const float* weights;       // [M, topk]
   const int32_t* map;         // [global_E] or null
   int64_t global_E;
   int topk, E, weight_on_input;
-  __nv_bfloat16* act;         // gate/up out
+  const float* peaks;         // gate/up [E][gate, up]
+  __half* act;                // gate/up out
+  float* act_inv;             // [pair]: the reciprocal of the factor that brought its row of act into f16's range
   float* y;                   // down: [pair][N]
   int* counters;              // [tile groups of down]
   int n_counters;
 };
 
-struct SlotLayout {
-  uint32_t count, expert, rank, list, slots, scan, red, bytes;
+// Shared memory of a block.  Rings of weight units, a warp's its own | their barriers | partial sums, two of them in turn | and for the layer: pairs
+// an expert has, then where they begin | expert of a pair | its place among that expert's | pairs by expert | slots | scan | and where rows are
+// staged: their statistics | parts of those | the rows in f16
+struct Layout {
+  uint32_t bars, red, count, expert, rank, list, slots, scan, stats, parts, rows, bytes;
 };
-// Shared memory: pairs an expert has, then where they begin | expert of a pair | its place among that expert's | pairs by expert | slots | scan |
-// partial sums
-__host__ __device__ __forceinline__ SlotLayout slot_layout(int pairs, int E, int cap, uint32_t red_bytes) {
-  SlotLayout l;
-  l.count = 0;
+struct RowStat {
+  float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
+};
+constexpr uint32_t kSmemMost = 227 * 1024;
+
+__host__ __device__ __forceinline__ uint32_t pad16(uint32_t v) { return (v + 15) / 16 * 16; }
+// pairs, E: 0 for a linear layer; rows: staged rows of row_bytes each
+__host__ __device__ __forceinline__ Layout layout_of(uint32_t ring, uint32_t bars, uint32_t red, int pairs, int E, int cap, int rows, uint32_t row_bytes) {
+  Layout l;
+  l.bars = ring;
+  l.red = pad16(l.bars + bars);
+  l.count = l.red + red;
   l.expert = l.count + (uint32_t)E * 4;
-  l.rank = l.expert + ((uint32_t)pairs * 2 + 3) / 4 * 4;
-  l.list = l.rank + ((uint32_t)pairs * 2 + 3) / 4 * 4;
-  l.slots = (l.list + (uint32_t)pairs * 2 + 15) / 16 * 16;
-  const int most = (pairs < E ? pairs : E) + pairs / cap;
-  l.scan = l.slots + (uint32_t)most * 8;
-  l.red = (l.scan + (pairs > 0 ? 2 * kWarps * 4 + 16 : 0) + 15) / 16 * 16;
-  l.bytes = l.red + red_bytes;
+  l.rank = pad16(l.expert + (uint32_t)pairs * 2);
+  l.list = pad16(l.rank + (uint32_t)pairs * 2);
+  l.slots = pad16(l.list + (uint32_t)pairs * 2);
+  l.scan = l.slots + (pairs > 0 ? (uint32_t)((pairs < E ? pairs : E) + pairs / cap) * 8 : 0);
+  l.stats = pad16(l.scan + (pairs > 0 ? 2 * kWarps * 4 + 16 : 0));
+  l.parts = l.stats + (uint32_t)rows * sizeof(RowStat);
+  l.rows = pad16(l.parts + (rows > 0 ? kWarps * kWarps * 8 : 0));
+  l.bytes = l.rows + (uint32_t)rows * row_bytes;
   return l;
 }
 
@@ -130,7 +152,7 @@ __device__ __forceinline__ int local_expert(const RowsParams& p, int pair) {
 
 // Slots of at most `cap` pairs of one expert, experts in order and pairs in theirs, so that every block finds the same; returns their number.
 // One warp counts, 32 pairs at a time: a few steps for a decode batch, and no order of atomics to depend on.
-__device__ int find_slots(const RowsParams& p, unsigned char* smem, const SlotLayout& l, int cap) {
+__device__ int find_slots(const RowsParams& p, unsigned char* smem, const Layout& l, int cap) {
   int* const count = reinterpret_cast<int*>(smem + l.count);
   uint16_t* const expert = reinterpret_cast<uint16_t*>(smem + l.expert);
   uint16_t* const rank = reinterpret_cast<uint16_t*>(smem + l.rank);
@@ -221,36 +243,92 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, size_t at)
   return static_cast<const float*>(p)[at];
 }
 
-// T: type of the operand; kCols: columns of eight; kTiles: row tiles a warp does at once
-template <typename T, int kMode, int kCols, int kTiles>
+// ---- powers of two that bring values into f16's range
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
+
+// The exponent that brings a row whose largest magnitude has these bf16 bits below 2^15.  Rows with infinities or NaN, which only give such
+// again, take the least that no finite value overflows with.
+__device__ __forceinline__ int row_exponent(uint32_t bits) { return min(141 - min((int)(bits >> 7), 254), 126); }
+
+// Largest magnitude (bf16 bits; bf16 only) and sum of squares (layer only) of elements [k0, k1) of a row, all lanes; k0 and k1 multiples of 8
+template <typename T, bool kSquares>
+__device__ __forceinline__ float2 row_part(const T* row, int k0, int k1) {
+  uint32_t top = 0;
+  float sum = 0.f;
+  for (int k = k0 + (threadIdx.x & 31) * 8; k < k1; k += 256) {
+    const uint4 v = ld_u4(row + k);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
+      if constexpr (kSquares) {
+        float2 f;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+        else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        sum += f.x * f.x + f.y * f.y;
+      }
+    }
+  }
+  top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+  if constexpr (kSquares)
+#pragma unroll
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  return make_float2(__uint_as_float(top), sum);
+}
+
+template <int kCols, int kTiles>
+struct Shape {
+  static constexpr int kStages = kCols * kTiles >= 4 ? 2 : (kTiles == 1 ? 5 : 3);      // of a warp's ring
+  static constexpr uint32_t kStageBytes = kTiles * kUnitBytes;
+  static constexpr uint32_t kRing = kWarps * kStages * kStageBytes;
+  static constexpr uint32_t kBars = kWarps * kStages * 8;
+  static constexpr int kSums = kTiles * kCols * 4 * 32;       // of a warp
+  static constexpr uint32_t kRed = 2 * kWarps * kSums * 4;
+};
+
+// XT: type of the activations; kCols: columns of eight; kTiles: row tiles a warp does at once
+template <typename XT, int kMode, int kCols, int kTiles>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParams p) {
-  extern __shared__ __align__(16) unsigned char smem[];
-  constexpr int kCap = (kMode == kDown ? 4 : 8) * kCols;
-  constexpr int kAhead = kTiles == 1 ? 4 : 2;
-  constexpr int kRedFloats = kTiles * kCols * 4 * 32;
+  extern __shared__ __align__(128) unsigned char smem[];
+  using S = Shape<kCols, kTiles>;
+  constexpr bool kConvert = std::is_same<XT, __nv_bfloat16>::value;
+  constexpr bool kStaged = kMode != kDown;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
-  const SlotLayout l = slot_layout(kMode == kLinear ? 0 : p.M * p.topk, kMode == kLinear ? 0 : p.E, kCap, kWarps * kRedFloats * 4);
+  const int cap = p.cap;
+  const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;      // rows are shifted by 16 bytes against each other: no two lanes of a load meet
+  const Layout l = layout_of(S::kRing, S::kBars, S::kRed, kMode == kLinear ? 0 : p.M * p.topk, kMode == kLinear ? 0 : p.E, cap, p.rows, row_bytes);
+  const uint32_t base = smem_u32(smem);
   const int2* const slots = reinterpret_cast<const int2*>(smem + l.slots);
   const uint16_t* const list = reinterpret_cast<const uint16_t*>(smem + l.list);
+  const uint32_t ring = base + warp * (S::kStages * S::kStageBytes), bars = base + l.bars + warp * (S::kStages * 8);
+  if (lane < S::kStages) mbar_init(bars + lane * 8, 1);
+  fence_proxy_async_smem();
+  __syncwarp();
   pdl_wait();
   pdl_launch_dependents();
   int n_slots;
   if constexpr (kMode == kLinear) {
-    n_slots = (p.M + kCap - 1) / kCap;
+    n_slots = (p.M + cap - 1) / cap;
+    if (p.clear_status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
   } else {
-    n_slots = find_slots(p, smem, l, kCap);
-    if (kMode == kGateUp && blockIdx.x == 0)
+    n_slots = find_slots(p, smem, l, cap);
+    if (kMode == kGateUp && blockIdx.x == 0) {
+      if (p.clear_status && threadIdx.x == 0) *p.status = 0;
       for (int i = threadIdx.x; i < p.n_counters; i += kThreads) p.counters[i] = 0;
+    }
     if (kMode == kDown && n_slots == 0) {
       for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < (size_t)p.M * p.N; i += (size_t)gridDim.x * kThreads)
         store_value(p.out, p.out_dtype, i, 0.f);
       return;
     }
   }
+  // Items of a slot are neighbours, or (down) those of a group of tiles
   const int groups_of_tiles = (p.tiles + kTiles - 1) / kTiles;
+  const int fast = kMode == kDown ? n_slots : groups_of_tiles;
   const int64_t n_items = (int64_t)n_slots * groups_of_tiles;
-  const int64_t first = n_items * blockIdx.x / gridDim.x, last = n_items * (blockIdx.x + 1) / gridDim.x;
-  const int n_block = (int)(last - first);
+  const int first = (int)(n_items * blockIdx.x / gridDim.x), last = (int)(n_items * (blockIdx.x + 1) / gridDim.x);
+  const int n_block = last - first;
 
   // Warps that share an item: as few rounds as possible, an item's ending counted as one more unit
   int share = 1, best = 1 << 30;
@@ -262,192 +340,304 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
     }
   }
   const int group = warp / share, in_group = warp - group * share, n_groups = kWarps / share;
-  const int k_first = p.units * in_group / share, k_last = p.units * (in_group + 1) / share, n_units = k_last - k_first;
-  const int n_mine = n_block > group ? (n_block - group + n_groups - 1) / n_groups : 0;
-  const int total = n_mine * n_units;
+  const int k_first = p.units * in_group / share, k_last = p.units * (in_group + 1) / share;
 
-  auto slot_of = [&](int64_t item) { return kMode == kGateUp ? (int)(item / groups_of_tiles) : (int)(item % n_slots); };
-  auto tile_of = [&](int64_t item) { return (kMode == kGateUp ? (int)(item % groups_of_tiles) : (int)(item / n_slots)) * kTiles; };
-
-  struct Unit {
-    uint4 codes[kTiles][2];
-    uint32_t scales[kTiles];
-  } ring[kAhead];
-  // what is loaded next
-  int64_t load_item = first + group;
-  int load_k = k_first;
-  const uint8_t* src[kTiles];
-  auto load = [&](Unit& u) {
-    if (load_k == k_first) {
-      const int tile = tile_of(load_item);
-      const size_t e = kMode == kLinear ? 0 : slots[slot_of(load_item)].x & 0xFFFF;
-#pragma unroll
-      for (int r = 0; r < kTiles; ++r)
-        src[r] = p.packed + ((e * p.tiles + min(tile + r, p.tiles - 1)) * p.units + k_first) * kUnitBytes;
-    }
-#pragma unroll
-    for (int r = 0; r < kTiles; ++r) {
-      u.codes[r][0] = ldg_stream_u4(src[r] + lane * 16);
-      u.codes[r][1] = ldg_stream_u4(src[r] + 512 + lane * 16);
-      u.scales[r] = ldg_stream_u32(src[r] + kUnitScales + lane * 4);
-      src[r] += kUnitBytes;
-    }
-    if (++load_k == k_last) {
-      load_k = k_first;
-      load_item += n_groups;
+  struct Cursor {
+    int item, hi, lo;         // hi * fast + lo
+  };
+  auto start = [&](Cursor& c) {
+    c.item = first + group;
+    c.hi = c.item / fast;
+    c.lo = c.item - c.hi * fast;
+  };
+  auto next = [&](Cursor& c) {
+    c.item += n_groups;
+    c.lo += n_groups;
+    while (c.lo >= fast) {
+      c.lo -= fast;
+      ++c.hi;
     }
   };
-#pragma unroll
-  for (int a = 0; a < kAhead; ++a)
-    if (a < total) load(ring[a]);
+  auto slot_of = [&](const Cursor& c) { return kMode == kDown ? c.lo : c.hi; };
+  auto tile_of = [&](const Cursor& c) { return (kMode == kDown ? c.hi : c.lo) * kTiles; };
 
-  int64_t item = first + group;
-  int k = k_first;
-  float acc[kTiles][kCols][4];
-  const T* col[kCols];
-  for (int i = 0; i < total; i += kAhead) {
+  // ---- the ring: one lane asks for the units, all wait for them
+  Cursor ahead;
+  start(ahead);
+  int ahead_k = k_first, fill = 0;
+  const uint8_t* src = nullptr;
+  size_t tile_step = 0;
+  auto fetch = [&]() {
+    if (ahead.item >= last) return;
+    if (ahead_k == k_first) {
+      const int tile = tile_of(ahead);
+      const size_t e = kMode == kLinear ? 0 : slots[slot_of(ahead)].x & 0xFFFF;
+      src = p.packed + ((e * p.tiles + tile) * p.units + k_first) * kUnitBytes;
+      tile_step = tile + kTiles <= p.tiles ? (size_t)p.units * kUnitBytes : 0;       // a last tile alone is done twice
+    }
+    if (lane == 0) {
+      const uint32_t bar = bars + fill * 8, to = ring + fill * S::kStageBytes;
+      mbar_expect_tx(bar, S::kStageBytes);
 #pragma unroll
-    for (int a = 0; a < kAhead; ++a) {
-      if (i + a >= total) break;
-      if (k == k_first) {
-        const int slot = slot_of(item);
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const int at = c * 8 + row8;
-          int64_t row = -1;
-          if constexpr (kMode == kLinear) {
-            if (slot * kCap + at < p.M) row = slot * kCap + at;
-          } else {
-            const int2 s = slots[slot];
-            const int n = s.x >> 16;
-            if constexpr (kMode == kGateUp) {
-              if (at < n) row = list[s.y + at] / p.topk;
-            } else {
-              if (at / 2 < n) row = (int64_t)list[s.y + at / 2] * 2 + (at & 1);
+      for (int r = 0; r < kTiles; ++r) bulk_load_1d(to + r * kUnitBytes, src + r * tile_step, kUnitBytes, bar);
+    }
+    src += kUnitBytes;
+    if (++fill == S::kStages) fill = 0;
+    if (++ahead_k == k_last) {
+      ahead_k = k_first;
+      next(ahead);
+    }
+  };
+  for (int i = 0; i < S::kStages; ++i) fetch();
+
+  Cursor at;
+  start(at);
+  int stage = 0, turn = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  // Rows are staged for as many slots at a time as there is room for
+  int slot = kStaged && n_block > 0 ? first / fast : 0;
+  for (int end = first; end < last;) {
+    int row0 = 0;
+    if constexpr (!kStaged) {
+      end = last;
+    } else {
+      // slots [slot, stop), rows [row0, row0 + n_rows) of the tokens or of the pairs by expert
+      const int slots_end = (last - 1) / fast + 1;
+      int stop = slot + 1, n_rows;
+      if constexpr (kMode == kLinear) {
+        row0 = slot * cap;
+        n_rows = min(cap, p.M - row0);
+      } else {
+        row0 = slots[slot].y;
+        n_rows = slots[slot].x >> 16;
+        while (stop < slots_end && n_rows + (slots[stop].x >> 16) <= p.rows) n_rows += slots[stop++].x >> 16;
+      }
+      end = min(last, stop * fast);
+      slot = stop;
+      auto row_at = [&](int r) {
+        const int64_t row = kMode == kLinear ? row0 + r : list[row0 + r] / p.topk;
+        return static_cast<const XT*>(p.x) + row * p.ldx;
+      };
+      RowStat* const stats = reinterpret_cast<RowStat*>(smem + l.stats);
+      float2* const parts = reinterpret_cast<float2*>(smem + l.parts);
+      // few rows: several warps a row
+      int n_parts = kWarps;
+      while (n_parts > 1 && n_parts * n_rows > kWarps) n_parts /= 2;
+      const int octets = p.K / 8;
+      __syncthreads();                             // nobody reads the rows before these any more
+      for (int i0 = 0; i0 < n_rows * n_parts; i0 += kWarps) {
+        const int i = i0 + warp, r = i / n_parts, part = i - r * n_parts;
+        const int k0 = octets * part / n_parts * 8, k1 = octets * (part + 1) / n_parts * 8;
+        const bool work = r < n_rows;
+        uint32_t factor = 0;
+        if constexpr (kConvert || kMode == kGateUp) {
+          float2 v = make_float2(0.f, 0.f);
+          if (work) v = row_part<XT, kMode == kGateUp>(row_at(r), k0, k1);
+          if (n_parts > 1) {
+            if (work && lane == 0) parts[r * n_parts + part] = v;
+            __syncthreads();
+            if (work) {
+              v = make_float2(0.f, 0.f);
+              for (int j = 0; j < n_parts; ++j) {
+                const float2 u = parts[r * n_parts + j];
+                v.x = __uint_as_float(max(__float_as_uint(v.x), __float_as_uint(u.x)));
+                v.y += u.y;
+              }
             }
           }
-          col[c] = row >= 0 ? static_cast<const T*>(p.x) + row * p.ldx + quad * 16 : nullptr;
-#pragma unroll
-          for (int r = 0; r < kTiles; ++r)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[r][c][j] = 0.f;
-        }
-      }
-      // ---- one unit
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int at = k * kUnitK + half * 64;
-        const bool inside = at + quad * 16 < p.K;
-        uint32_t b[kCols][8];
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-          if (inside && col[c] != nullptr) {
-            lo = ld_u4(col[c] + at);
-            hi = ld_u4(col[c] + at + 8);
-          }
-          b[c][0] = lo.x, b[c][1] = lo.y, b[c][2] = lo.z, b[c][3] = lo.w;
-          b[c][4] = hi.x, b[c][5] = hi.y, b[c][6] = hi.z, b[c][7] = hi.w;
-        }
-#pragma unroll
-        for (int r = 0; r < kTiles; ++r) {
-          uint32_t s_lo, s_hi;
-          scales_of<T>(ring[a].scales[r], half, s_lo, s_hi);
-          const uint4 w = ring[a].codes[r][half];
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t lo[4], hi[4];
-            codes_to_pairs<T>(q ? w.y : w.x, lo);
-            codes_to_pairs<T>(q ? w.w : w.z, hi);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              lo[j] = mul2<T>(lo[j], s_lo);
-              hi[j] = mul2<T>(hi[j], s_hi);
-            }
-#pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              mma_16x8x16<T>(acc[r][c], lo[0], hi[0], lo[1], hi[1], b[c][q * 4], b[c][q * 4 + 1]);
-              mma_16x8x16<T>(acc[r][c], lo[2], hi[2], lo[3], hi[3], b[c][q * 4 + 2], b[c][q * 4 + 3]);
+          if (work) {
+            const int e = kConvert ? row_exponent(__float_as_uint(v.x)) : 0;
+            factor = (uint32_t)(e + 127) * 0x00800080u;
+            if (part == 0 && lane == 0) {
+              RowStat st = {pow2(-e), 0.f};
+              if constexpr (kMode == kGateUp) {
+                // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the
+                // bound is far above the values costs nothing while act's two parts reach 40 binades down.
+                const int pair = list[row0 + r], x = reinterpret_cast<const uint16_t*>(smem + l.expert)[pair];
+                const float w = p.weight_on_input ? p.weights[pair] : 1.f;
+                const float norm = sqrtf(v.y * (float)p.K) * w;
+                const float bound = fabsf(norm * p.g[2 * x] * p.peaks[2 * x]) * fabsf(norm * p.g[2 * x + 1] * p.peaks[2 * x + 1]);
+                const int up = min(max(14 - ((int)(__float_as_uint(bound) >> 23) - 126), -100), 100);
+                st.act = pow2(up);
+                p.act_inv[pair] = pow2(-up);
+              }
+              stats[r] = st;
             }
           }
         }
-      }
-      if (i + a + kAhead < total) load(ring[a]);
-      if (++k < k_last) continue;
-      // ---- an item's end
-      k = k_first;
-      float* const red = reinterpret_cast<float*>(smem + l.red) + group * share * kRedFloats + lane;
-      if (share > 1) {
-        if (in_group > 0) {
-#pragma unroll
-          for (int r = 0; r < kTiles; ++r)
-#pragma unroll
-            for (int c = 0; c < kCols; ++c)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) red[in_group * kRedFloats + ((r * kCols + c) * 4 + j) * 32] = acc[r][c][j];
+        if (work) {
+          const XT* const row = row_at(r);
+          unsigned char* const to = smem + l.rows + r * row_bytes;
+          for (int k = k0 + lane * 8; k < k1; k += 256) {
+            uint4 v = ld_u4(row + k);
+            if constexpr (kConvert)
+              v = make_uint4(bf16_to_f16_pair(v.x, factor), bf16_to_f16_pair(v.y, factor), bf16_to_f16_pair(v.z, factor), bf16_to_f16_pair(v.w, factor));
+            *reinterpret_cast<uint4*>(to + k * 2) = v;
+          }
+          if (part == n_parts - 1)                 // a unit's k past the row's end
+            for (int k = p.K + lane * 8; k < p.units * kUnitK; k += 256) *reinterpret_cast<uint4*>(to + k * 2) = make_uint4(0, 0, 0, 0);
         }
-        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
-        if (in_group == 0) {
-          for (int s = 1; s < share; ++s)
-#pragma unroll
-            for (int r = 0; r < kTiles; ++r)
-#pragma unroll
-              for (int c = 0; c < kCols; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[r][c][j] += red[s * kRedFloats + ((r * kCols + c) * 4 + j) * 32];
-        }
-        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
       }
-      if (in_group == 0) {
-        const int slot = slot_of(item), tile = tile_of(item);
-        const int2 s = kMode == kLinear ? make_int2(0, 0) : slots[slot];
-        const int e = kMode == kLinear ? 0 : s.x & 0xFFFF;
-        const float scale = p.g[kMode == kGateUp ? 2 * e : e] * kOutScale, up_scale = kMode == kGateUp ? p.g[2 * e + 1] * kOutScale : 0.f;
+      __syncthreads();
+    }
+
+    for (; at.item < end; next(at)) {
+      const int slot_at = slot_of(at);
+      const int2 s = kMode == kLinear ? make_int2(min(cap, p.M - slot_at * cap) << 16, slot_at * cap) : slots[slot_at];
+      const int n = s.x >> 16;                     // columns in use; the others read the first one's row, and nobody reads their sums
+      float acc[kTiles][kCols][4];
+      uint32_t col[kCols];
+      const __half* act[kCols];
 #pragma unroll
-        for (int r = 0; r < kTiles; ++r) {
-          if (tile + r >= p.tiles) break;
+      for (int c = 0; c < kCols; ++c) {
+        const int i = c * 8 + row8;
+        if constexpr (kStaged) col[c] = base + l.rows + (uint32_t)(s.y - row0 + (i < n ? i : 0)) * row_bytes + k_first * (kUnitK * 2) + quad * 32;
+        else act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i / 2 < n ? i / 2 : 0)] * 2 + (i & 1)) * p.ldx + k_first * kUnitK + quad * 16;
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[r][c][j] = 0.f;
+      }
+      for (int k = k_first; k < k_last; ++k) {
+        uint32_t b[2][kCols][8];
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
-            const int at = c * 8 + quad * 2;       // this lane's two columns
-            if constexpr (kMode == kLinear) {
+            uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+            if constexpr (kStaged) {
+              lo = lds128(col[c] + half * 128);
+              hi = lds128(col[c] + half * 128 + 16);
+            } else if (k * kUnitK + half * 64 + quad * 16 < p.K) {
+              lo = ld_u4(act[c] + half * 64);
+              hi = ld_u4(act[c] + half * 64 + 8);
+            }
+            b[half][c][0] = lo.x, b[half][c][1] = lo.y, b[half][c][2] = lo.z, b[half][c][3] = lo.w;
+            b[half][c][4] = hi.x, b[half][c][5] = hi.y, b[half][c][6] = hi.z, b[half][c][7] = hi.w;
+          }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          if constexpr (kStaged) col[c] += kUnitK * 2;
+          else act[c] += kUnitK;
+        }
+        if (ok) ok = mbar_wait_warp(bars + stage * 8, phase, p.status, 61);
+        const uint32_t unit = ring + stage * S::kStageBytes + lane * 16;
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r) {
+          const uint32_t sc = lds32(unit + r * kUnitBytes + kUnitScales - lane * 12);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint4 w = lds128(unit + r * kUnitBytes + half * 512);
+            uint32_t s_lo, s_hi;
+            scales_of(sc, half, s_lo, s_hi);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              uint32_t lo[4], hi[4];
+              codes_to_pairs(q ? w.y : w.x, lo);
+              codes_to_pairs(q ? w.w : w.z, hi);
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
-                const int m = slot * kCap + at + (j & 1), n = (tile + r) * 16 + row8 + (j >> 1) * 8;
-                if (m < p.M && n < p.N) {
-                  float v = acc[r][c][j] * scale;
-                  if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, n);
-                  store_value(p.out, p.out_dtype, (size_t)m * p.N + n, v);
-                }
+                lo[j] = mul2(lo[j], s_lo);
+                hi[j] = mul2(hi[j], s_hi);
               }
-            } else if constexpr (kMode == kGateUp) {
-              const int i_at = (tile + r) * 8 + row8, I = p.N / 2;
 #pragma unroll
-              for (int j = 0; j < 2; ++j) {
-                if (at + j < (s.x >> 16) && i_at < I) {
-                  const int pair = list[s.y + at + j];
-                  const float f = p.weight_on_input ? p.weights[pair] : 1.f;
-                  const float v = silu_f32(acc[r][c][j] * scale * f) * (acc[r][c][2 + j] * up_scale * f);
-                  const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-                  const float rest = v - __bfloat162float(hi);
-                  __nv_bfloat16* const to = p.act + (size_t)pair * 2 * I + i_at;
-                  to[0] = hi;
-                  to[I] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.f);      // an infinite or NaN value is the upper part's alone
-                }
+              for (int c = 0; c < kCols; ++c) {
+                mma_16x8x16(acc[r][c], lo[0], hi[0], lo[1], hi[1], b[half][c][q * 4], b[half][c][q * 4 + 1]);
+                mma_16x8x16(acc[r][c], lo[2], hi[2], lo[3], hi[3], b[half][c][q * 4 + 2], b[half][c][q * 4 + 3]);
               }
-            } else {
-              if (at / 2 < (s.x >> 16)) {
-                float* const to = p.y + (size_t)list[s.y + at / 2] * p.N + (tile + r) * 16 + row8;
-                to[0] = (acc[r][c][0] + acc[r][c][1]) * scale;
-                to[8] = (acc[r][c][2] + acc[r][c][3]) * scale;
+            }
+          }
+        }
+        if (++stage == S::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+        __syncwarp();                              // every lane has read the stage
+        if (ok) fetch();
+      }
+
+      // ---- the item's end.  Sums of a warp: [tile][column of eight][j][lane]; a lane's j are row l / 4 (0, 1) or row l / 4 + 8 (2, 3) and
+      // columns 2 (l % 4) and the next one.
+      const int e = kMode == kLinear ? 0 : s.x & 0xFFFF, tile = tile_of(at);
+      float* const red = reinterpret_cast<float*>(smem + l.red) + ((turn & 1) * kWarps + group * share) * S::kSums;
+      turn ^= 1;
+      if (share > 1) {
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) red[in_group * S::kSums + ((r * kCols + c) * 4 + j) * 32 + lane] = acc[r][c][j];
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
+      }
+      // a pair of sums (j, j + 2: gate and up, or rows eight apart; down: 0, 1 and 2, 3, the two parts) goes to one lane of one warp
+      constexpr int kPairs = kTiles * kCols * 2;   // a lane's
+      for (int i = in_group; i < kPairs; i += share) {
+        const int j = i & 1, c = (i >> 1) % kCols, r = (i >> 1) / kCols;
+        const int ja = kMode == kDown ? 2 * j : j, jb = kMode == kDown ? 2 * j + 1 : j + 2;
+        float va = 0.f, vb = 0.f;
+        if (share > 1) {
+          const float* from = red + ((r * kCols + c) * 4) * 32 + lane;
+          for (int w = 0; w < share; ++w, from += S::kSums) {
+            va += from[ja * 32];
+            vb += from[jb * 32];
+          }
+        } else {
+#pragma unroll
+          for (int rr = 0; rr < kTiles; ++rr)
+#pragma unroll
+            for (int cc = 0; cc < kCols; ++cc)
+#pragma unroll
+              for (int jj = 0; jj < 2; ++jj)
+                if (rr == r && cc == c && jj == j) {
+                  va = acc[rr][cc][kMode == kDown ? 2 * jj : jj];
+                  vb = acc[rr][cc][kMode == kDown ? 2 * jj + 1 : jj + 2];
+                }
+        }
+        if (tile + r >= p.tiles) continue;
+        const int column = c * 8 + quad * 2;
+        if constexpr (kMode == kDown) {
+          if (column / 2 < n) {
+            const int pair = list[s.y + column / 2];
+            p.y[(size_t)pair * p.N + (tile + r) * 16 + j * 8 + row8] = (va + vb) * (p.act_inv[pair] * p.g[e]);
+          }
+        } else if (column + j < n) {
+          const RowStat st = reinterpret_cast<const RowStat*>(smem + l.stats)[s.y - row0 + column + j];
+          if constexpr (kMode == kGateUp) {
+            const int pair = list[s.y + column + j], I = p.N / 2, i_at = (tile + r) * 8 + row8;
+            if (i_at < I) {
+              const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
+              const float v = silu_f32(va * f * p.g[2 * e]) * (vb * f * p.g[2 * e + 1]) * st.act;
+              const __half hi = __float2half_rn(v);
+              const float rest = v - __half2float(hi);
+              __half* const to = p.act + (size_t)pair * 2 * I + i_at;
+              to[0] = hi;
+              to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
+            }
+          } else {
+            const int m = s.y + column + j, row = (tile + r) * 16 + row8;
+            const float f = kConvert ? st.inv : 1.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int at_n = row + h * 8;
+              if (at_n < p.N) {
+                float v = (h ? vb : va) * f * p.g[0];
+                if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, at_n);
+                store_value(p.out, p.out_dtype, (size_t)m * p.N + at_n, v);
               }
             }
           }
         }
       }
-      item += n_groups;
     }
   }
 
+  if (!ok) {                                       // copies that were asked for land before the block's memory goes
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitCycles / 64) {
+    }
+  }
   if constexpr (kMode == kDown) {
     // The block that completes a group of tiles adds up every token's pairs, in the order of the routing.
     const uint16_t* const expert = reinterpret_cast<const uint16_t*>(smem + l.expert);
@@ -455,10 +645,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
     __threadfence();
     __syncthreads();
     if (n_block == 0) return;
-    for (int tg = (int)(first / n_slots); tg <= (int)((last - 1) / n_slots); ++tg) {
+    for (int tg = first / n_slots; tg <= (last - 1) / n_slots; ++tg) {
       if (threadIdx.x == 0) {
-        const int64_t from = max(first, (int64_t)tg * n_slots), to = min(last, (int64_t)(tg + 1) * n_slots);
-        const int done = (int)(to - from);
+        const int done = min(last, (tg + 1) * n_slots) - max(first, tg * n_slots);
         *flag = atomicAdd(&p.counters[tg], done) + done == n_slots;
         __threadfence();
       }
@@ -480,32 +669,45 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
           sum.z += w * v.z;
           sum.w += w * v.w;
         }
-        const size_t at = (size_t)m * p.N + row;
-        store_value(p.out, p.out_dtype, at, sum.x);
-        store_value(p.out, p.out_dtype, at + 1, sum.y);
-        store_value(p.out, p.out_dtype, at + 2, sum.z);
-        store_value(p.out, p.out_dtype, at + 3, sum.w);
+        const size_t to = (size_t)m * p.N + row;
+        store_value(p.out, p.out_dtype, to, sum.x);
+        store_value(p.out, p.out_dtype, to + 1, sum.y);
+        store_value(p.out, p.out_dtype, to + 2, sum.z);
+        store_value(p.out, p.out_dtype, to + 3, sum.w);
       }
     }
   }
 }
 
-template <typename T, int kMode, int kCols, int kTiles>
-int launch_rows(const RowsParams& p, cudaStream_t st) {
-  constexpr uint32_t kRed = kWarps * kTiles * kCols * 4 * 32 * 4;
-  constexpr int kCap = (kMode == kDown ? 4 : 8) * kCols;
+template <typename XT, int kMode, int kCols, int kTiles>
+int launch_rows(RowsParams p, cudaStream_t st) {
+  using S = Shape<kCols, kTiles>;
   static std::once_flag once[64];
   static bool ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200FP4_STATUS_NOT_SUPPORTED;
   std::call_once(once[dev], [&] {
-    ready[dev] = cudaFuncSetAttribute(w4a16_rows_kernel<T, kMode, kCols, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)slot_layout(kMode == kLinear ? 0 : kMaxPairs, kMode == kLinear ? 0 : kMaxExperts, kCap, kRed).bytes) == cudaSuccess;
+    ready[dev] = cudaFuncSetAttribute(w4a16_rows_kernel<XT, kMode, kCols, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost) == cudaSuccess;
     cudaGetLastError();
   });
   if (!ready[dev]) return B200FP4_STATUS_EXECUTION_FAILED;
-  const uint32_t smem = slot_layout(kMode == kLinear ? 0 : p.M * p.topk, kMode == kLinear ? 0 : p.E, kCap, kRed).bytes;
-  if (launch_pdl(w4a16_rows_kernel<T, kMode, kCols, kTiles>, dim3(sm_count()), dim3(kThreads), smem, st, p) != cudaSuccess) {
+  const int pairs = kMode == kLinear ? 0 : p.M * p.topk, E = kMode == kLinear ? 0 : p.E;
+  const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;
+  p.cap = (kMode == kDown ? 4 : 8) * kCols;
+  p.rows = 0;
+  while (kMode != kDown) {
+    // rows that there is room for; a slot has no more columns than that
+    const uint32_t rest = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, p.cap, 1, 0).bytes;
+    const int64_t most = kMode == kLinear ? std::min(p.M, p.cap) : pairs;
+    p.rows = (int)std::min<int64_t>(most, (kSmemMost - std::min(rest, kSmemMost)) / (row_bytes + (uint32_t)sizeof(RowStat)));
+    if (p.rows < 1) return B200FP4_STATUS_NOT_SUPPORTED;
+    if (p.rows >= p.cap || p.rows == most) break;
+    p.cap = p.rows;
+  }
+  if ((int64_t)((kMode == kLinear ? p.M : pairs) / p.cap + (E > 0 ? E : 1)) * p.tiles > 0x7FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
+  const uint32_t smem = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, p.cap, p.rows, row_bytes).bytes;
+  if (smem > kSmemMost) return B200FP4_STATUS_NOT_SUPPORTED;
+  if (launch_pdl(w4a16_rows_kernel<XT, kMode, kCols, kTiles>, dim3(sm_count()), dim3(kThreads), smem, st, p) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
@@ -515,17 +717,16 @@ int launch_rows(const RowsParams& p, cudaStream_t st) {
 template <typename T>
 int launch_linear(const RowsParams& p, cudaStream_t st) {
   if (p.M <= 8) return launch_rows<T, kLinear, 1, 1>(p, st);
-  if (p.M <= 16) return launch_rows<T, kLinear, 2, 2>(p, st);
-  return launch_rows<T, kLinear, 4, 2>(p, st);
+  return launch_rows<T, kLinear, 2, 2>(p, st);
 }
 template <typename T>
 int launch_gate_up(const RowsParams& p, cudaStream_t st) {
-  if ((int64_t)p.M * p.topk <= 4 * (int64_t)p.E) return launch_rows<T, kGateUp, 1, 1>(p, st);
+  if ((int64_t)p.M * p.topk <= 4 * (int64_t)p.E) return launch_rows<T, kGateUp, 1, 2>(p, st);
   return launch_rows<T, kGateUp, 2, 2>(p, st);
 }
 int launch_down(const RowsParams& p, cudaStream_t st) {
-  if ((int64_t)p.M * p.topk <= 2 * (int64_t)p.E) return launch_rows<__nv_bfloat16, kDown, 1, 1>(p, st);
-  return launch_rows<__nv_bfloat16, kDown, 2, 2>(p, st);
+  if ((int64_t)p.M * p.topk <= 2 * (int64_t)p.E) return launch_rows<__half, kDown, 1, 2>(p, st);
+  return launch_rows<__half, kDown, 2, 2>(p, st);
 }
 
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
@@ -533,19 +734,23 @@ bool is_16bit(int dtype) { return dtype == B200FP4_DTYPE_F16 || dtype == B200FP4
 bool is_dtype(int dtype) { return is_16bit(dtype) || dtype == B200FP4_DTYPE_F32; }
 size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 
-constexpr size_t kStatusBytes = 256;
+
+size_t unit_bytes(int64_t E, int64_t N, int64_t K, int gated) {
+  return (size_t)E * (gated ? (N / 2 + 7) / 8 : tiles_of(N)) * units_of(K) * kUnitBytes;
+}
 
 // tokens of a layer whose pairs fit one turn
 int64_t turn_of(int64_t M, int64_t topk) { return std::min(M, std::max<int64_t>(1, kMaxPairs / topk)); }
 
 struct MoeScratch {
-  size_t act, y, counters, bytes;
+  size_t act, act_inv, y, counters, bytes;
 };
 MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I) {
   MoeScratch s;
   const size_t pairs = (size_t)turn_of(M, topk) * topk;
-  s.act = kStatusBytes;
-  s.y = s.act + pad256(pairs * 2 * I * 2);
+  s.act = 0;
+  s.act_inv = s.act + pad256(pairs * 2 * I * 2);
+  s.y = s.act_inv + pad256(pairs * 4);
   s.counters = s.y + pad256(pairs * H * 4);
   s.bytes = s.counters + pad256((size_t)tiles_of(H) * 4);
   return s;
@@ -558,7 +763,7 @@ using namespace b200fp4;
 
 extern "C" size_t b200fp4_w4a16_packed_bytes(int64_t E, int64_t N, int64_t K, int gated) {
   if (E < 1 || N < 1 || K < 16 || K % 16 != 0 || (gated && N % 2 != 0)) return 0;
-  return (size_t)E * (gated ? (N / 2 + 7) / 8 : w4::tiles_of(N)) * w4::units_of(K) * w4::kUnitBytes;
+  return unit_bytes(E, N, K, gated) + (size_t)E * (gated ? 2 : 1) * 4;
 }
 
 extern "C" int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t N, int64_t K, int gated, uint8_t* packed,
@@ -576,26 +781,24 @@ extern "C" int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, i
   p.gated = gated != 0;
   const int64_t n = E * p.tiles * p.units;
   if ((n + 7) / 8 > 0x7FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
+  p.peaks = reinterpret_cast<uint32_t*>(packed + unit_bytes(E, N, K, gated));
+  if (cudaMemsetAsync(p.peaks, 0, (size_t)E * (gated ? 2 : 1) * 4, static_cast<cudaStream_t>(stream)) != cudaSuccess) {
+    cudaGetLastError();
+    return B200FP4_STATUS_EXECUTION_FAILED;
+  }
   w4a16_pack_kernel<<<(unsigned)((n + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(p, n);
   return finish_launch(1);
 }
 
-extern "C" size_t b200fp4_w4a16_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  (void)M, (void)N, (void)K;
-  return kStatusBytes;
-}
-
 extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const float* g_scale, const void* bias,
-                                    int bias_dtype, void* out, int out_dtype, int64_t M, int64_t N, int64_t K, void* workspace,
-                                    size_t workspace_bytes, void* stream) {
+                                    int bias_dtype, void* out, int out_dtype, int64_t M, int64_t N, int64_t K, int32_t* status,
+                                    void* stream) {
   if (M < 0 || N < 1 || K < 16 || K % 16 != 0) return B200FP4_STATUS_INVALID_VALUE;
   if (!is_16bit(x_dtype) || !is_dtype(out_dtype) || (bias != nullptr && !is_dtype(bias_dtype))) return B200FP4_STATUS_INVALID_VALUE;
   if (M == 0) return B200FP4_STATUS_SUCCESS;
-  if (x == nullptr || packed == nullptr || g_scale == nullptr || out == nullptr) return B200FP4_STATUS_INVALID_VALUE;
+  if (x == nullptr || packed == nullptr || g_scale == nullptr || out == nullptr || status == nullptr) return B200FP4_STATUS_INVALID_VALUE;
   if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(out, 16) || ldx % 8 != 0 || (M > 1 && ldx < K)) return B200FP4_STATUS_INVALID_VALUE;
-  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < b200fp4_w4a16_linear_workspace_bytes(M, N, K))
-    return B200FP4_STATUS_ALLOC_FAILED;
-  if (!fits_int(M) || !fits_int(N + 16) || !fits_int(K + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
+  if (!fits_int(M) || !fits_int(N + 64) || !fits_int(K + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
   RowsParams p = {};
   p.x = x;
   p.ldx = ldx;
@@ -610,24 +813,26 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   p.K = (int)K;
   p.tiles = (int)w4::tiles_of(N);
   p.units = (int)w4::units_of(K);
+  p.status = status;
+  p.clear_status = 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(p, st) : launch_linear<__half>(p, st);
 }
 
 extern "C" size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I) {
-  if (M < 1 || topk < 1 || H < 1 || I < 1) return kStatusBytes;
+  if (M < 1 || topk < 1 || H < 1 || I < 1) return 0;
   return moe_scratch(M, topk, H, I).bytes;
 }
 
 extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* topk_weights, const int32_t* topk_ids, const int32_t* expert_map,
                                  int64_t global_E, const uint8_t* w13_packed, const float* w13_g, const uint8_t* w2_packed, const float* w2_g,
-                                 void* out, int out_dtype, int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E, int flags, void* workspace,
-                                 size_t workspace_bytes, void* stream) {
+                                 void* out, int out_dtype, int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E, int flags, int32_t* status,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
   if (M < 0 || topk < 1 || E < 1 || H < 16 || H % 16 != 0 || I < 16 || I % 16 != 0) return B200FP4_STATUS_INVALID_VALUE;
   if (!is_16bit(h_dtype) || !is_dtype(out_dtype) || (flags & ~B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT) != 0) return B200FP4_STATUS_INVALID_VALUE;
   if (M == 0) return B200FP4_STATUS_SUCCESS;
   if (hidden == nullptr || topk_weights == nullptr || topk_ids == nullptr || w13_packed == nullptr || w13_g == nullptr || w2_packed == nullptr ||
-      w2_g == nullptr || out == nullptr || (expert_map != nullptr && global_E < 1))
+      w2_g == nullptr || out == nullptr || status == nullptr || (expert_map != nullptr && global_E < 1))
     return B200FP4_STATUS_INVALID_VALUE;
   if (!aligned(hidden, 16) || !aligned(w13_packed, 16) || !aligned(w2_packed, 16) || !aligned(out, 16)) return B200FP4_STATUS_INVALID_VALUE;
   if (E > kMaxExperts || topk > kMaxPairs || !fits_int(M * topk) || !fits_int(H + 128) || !fits_int(2 * I + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
@@ -640,6 +845,8 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
   for (int64_t m = 0; m < M; m += turn) {
     RowsParams p = {};
     p.M = (int)std::min(turn, M - m);
+    p.status = status;
+    p.clear_status = m == 0;
     p.ids = topk_ids + m * topk;
     p.weights = topk_weights + m * topk;
     p.map = expert_map;
@@ -647,7 +854,9 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.topk = (int)topk;
     p.E = (int)E;
     p.weight_on_input = flags & B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT ? 1 : 0;
-    p.act = reinterpret_cast<__nv_bfloat16*>(ws + s.act);
+    p.act = reinterpret_cast<__half*>(ws + s.act);
+    p.act_inv = reinterpret_cast<float*>(ws + s.act_inv);
+    p.peaks = reinterpret_cast<const float*>(w13_packed + unit_bytes(E, 2 * I, H, 1));
     p.y = reinterpret_cast<float*>(ws + s.y);
     p.counters = reinterpret_cast<int*>(ws + s.counters);
     p.n_counters = (int)w4::tiles_of(H);

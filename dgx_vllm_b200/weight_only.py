@@ -74,8 +74,8 @@ def w4a16_linear(x: torch.Tensor, weight: PackedNvfp4Weight, bias: torch.Tensor 
 
 
 def last_w4a16_status(device=None) -> int:
-    """Status word of the most recent w4a16_linear on the current stream of `device`: 0, or the code of a bounded wait that ran out
-    (that call's result is then not valid).  Synchronises."""
+    """Status word of the most recent w4a16_linear or W4A16MoE on the current stream of `device`: 0, or the code of a bounded wait that ran
+    out (that call's result is then not valid).  Synchronises."""
     return status_word(device, WS_W4A16)
 
 
@@ -84,7 +84,7 @@ class W4A16MoE:
     projection, router-weighted sum, in two launches.  The counterpart of FusedSparseMoE for weights that are not pruned.
 
     w13 [E, 2I, H] packed gated, w2 [E, H, I] packed; expert_map [global_E] int32 maps the router's ids to local experts (-1: not here)
-    or None.  H and I are multiples of 16.  Meant for decode batches: up to 4096 (token, expert) pairs a pass over the
+    or None.  H and I are multiples of 16.  Meant for decode batches: up to 2048 (token, expert) pairs a pass over the
     weights, more in turns."""
 
     def __init__(self, w13: PackedNvfp4Weight, w2: PackedNvfp4Weight, expert_map: torch.Tensor | None = None):

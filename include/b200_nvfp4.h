@@ -485,7 +485,7 @@ B200FP4_API int b200fp4_ep_combine_p2p(const float* parts, int64_t B, int64_t H,
  *   codes  [E, N, K/2] packed E2M1, scales [E, N, K/16] E4M3 (linear), K a multiple of 16, any N
  *   packed b200fp4_w4a16_packed_bytes(E, N, K, gated) bytes (0 for sizes that it refuses), 16-byte aligned
  *   gated  the rows are N/2 gate rows and then N/2 up rows, which the layer wants next to each other
- * Scale bytes 0x7F / 0xFF (NaN) count as 480; a negative scale gives its sign to its codes.
+ * Scale bytes 0x7F / 0xFF (NaN) count as 448; a negative scale gives its sign to its codes.
  * ------------------------------------------------------------------------------------------- */
 B200FP4_API size_t b200fp4_w4a16_packed_bytes(int64_t E, int64_t N, int64_t K, int gated);
 B200FP4_API int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t N, int64_t K, int gated,
@@ -493,23 +493,24 @@ B200FP4_API int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, 
 
 /* out[M,N] = x . W^T * g_scale (+ bias): x [M,K] bf16 or f16, rows ldx elements apart (a multiple of 8, 16-byte aligned), one packed
  * matrix (not gated), g_scale one f32 on the device (weight_scale_2 of a checkpoint), bias [N] of any dtype or NULL, out contiguous
- * in bf16, f16 or f32.  Products of 16-bit values, sums in f32.  The first int of the workspace is a status word: 0, or the code
- * of a bounded wait that ran out. */
-B200FP4_API size_t b200fp4_w4a16_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ * in bf16, f16 or f32.  Products of exact 16-bit values, sums in f32: bf16 rows are brought into f16's range by a power of two each, with
+ * which only what is below 2^-39 of a row's largest magnitude can be rounded.  status (on the device) is 0 after the call, or the code of a
+ * bounded wait that ran out: the result is then not valid. */
 B200FP4_API int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const float* g_scale,
                                      const void* bias, int bias_dtype, void* out, int out_dtype, int64_t M, int64_t N, int64_t K,
-                                     void* workspace, size_t workspace_bytes, void* stream);
+                                     int32_t* status, void* stream);
 
 /* One mixture-of-experts layer: gate/up projection -> SiLU(gate)*up -> down projection -> router-weighted sum, in two launches for up
- * to 4096 (token, expert) pairs; more are done in turns.  Arguments as b200fp4_fused_sparse_moe, with w13 [E, 2I, H] packed gated and
- * w2 [E, H, I] packed, w13_g [E][gate rows, up rows], w2_g [E]; H and I multiples of 16, E and topk up to 4096.  Pairs whose expert (after expert_map) is outside
+ * to 2048 (token, expert) pairs; more are done in turns.  Arguments as b200fp4_fused_sparse_moe, with w13 [E, 2I, H] packed gated and
+ * w2 [E, H, I] packed, w13_g [E][gate rows, up rows], w2_g [E]; H and I multiples of 16, E up to 4096, topk up to 2048.  Pairs whose expert (after expert_map) is outside
  * [0, E) add nothing; a token without any gives zeros.  flags: B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT or 0.  Between the projections a value is kept as
- * the sum of two bf16.  Results do not depend on the order in which blocks run. */
+ * the sum of two f16.  Results do not depend on the order in which blocks run. */
 B200FP4_API size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I);
 B200FP4_API int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* topk_weights, const int32_t* topk_ids,
                                   const int32_t* expert_map, int64_t global_E, const uint8_t* w13_packed, const float* w13_g,
                                   const uint8_t* w2_packed, const float* w2_g, void* out, int out_dtype, int64_t M, int64_t topk,
-                                  int64_t H, int64_t I, int64_t E, int flags, void* workspace, size_t workspace_bytes, void* stream);
+                                  int64_t H, int64_t I, int64_t E, int flags, int32_t* status, void* workspace, size_t workspace_bytes,
+                                  void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * The reference's declared C API, exported under its own names so that a program written against

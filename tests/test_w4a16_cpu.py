@@ -13,10 +13,10 @@ P = 0x100000                                                      # an address n
     (dict(x=0), INVALID), (dict(x=P + 8), INVALID), (dict(x_dtype=2), INVALID), (dict(ldx=60), INVALID), (dict(ldx=48), INVALID), (dict(packed=0), INVALID),
     (dict(packed=P + 8), INVALID), (dict(g=0), INVALID), (dict(bias=P, bias_dtype=7), INVALID), (dict(out=0), INVALID), (dict(out_dtype=3), INVALID),
     (dict(M=-1), INVALID), (dict(N=0), INVALID), (dict(K=72), INVALID), (dict(K=0), INVALID), (dict(M=1 << 33), NOT_SUPPORTED), (dict(N=1 << 33), NOT_SUPPORTED),
-    (dict(workspace=0), ALLOC), (dict(bytes=8), ALLOC), (dict(workspace=P + 16), ALLOC),
+    (dict(status=0), INVALID),
 ])
 def test_refused_linear_queues_nothing(bad, status):
-    a = dict(x=P, x_dtype=1, ldx=64, packed=P, g=P, bias=0, bias_dtype=0, out=P, out_dtype=1, M=2, N=128, K=64, workspace=P, bytes=1 << 40, stream=0)
+    a = dict(x=P, x_dtype=1, ldx=64, packed=P, g=P, bias=0, bias_dtype=0, out=P, out_dtype=1, M=2, N=128, K=64, status=P, stream=0)
     a.update(bad)
     assert _refused_unqueued(lambda L: L.b200fp4_w4a16_linear(*a.values())) == status
 
@@ -24,20 +24,20 @@ def test_refused_linear_queues_nothing(bad, status):
 @pytest.mark.parametrize("bad,status", [
     (dict(hidden=0), INVALID), (dict(hidden=P + 8), INVALID), (dict(h_dtype=2), INVALID), (dict(weights=0), INVALID), (dict(ids=0), INVALID),
     (dict(emap=P), INVALID), (dict(w13=P + 4), INVALID), (dict(w13_g=0), INVALID), (dict(w2=0), INVALID), (dict(w2_g=0), INVALID), (dict(out=P + 4), INVALID),
-    (dict(out_dtype=5), INVALID), (dict(M=-2), INVALID), (dict(topk=0), INVALID), (dict(topk=4097), NOT_SUPPORTED), (dict(H=72), INVALID), (dict(I=24), INVALID),
-    (dict(E=0), INVALID), (dict(E=4097), NOT_SUPPORTED), (dict(flags=2), INVALID), (dict(workspace=0), ALLOC), (dict(bytes=300), ALLOC),
+    (dict(out_dtype=5), INVALID), (dict(M=-2), INVALID), (dict(topk=0), INVALID), (dict(topk=2049), NOT_SUPPORTED), (dict(H=72), INVALID), (dict(I=24), INVALID),
+    (dict(E=0), INVALID), (dict(E=4097), NOT_SUPPORTED), (dict(flags=2), INVALID), (dict(status=0), INVALID), (dict(workspace=0), ALLOC), (dict(bytes=300), ALLOC),
     (dict(M=1 << 31, topk=2), NOT_SUPPORTED),
 ])
 def test_refused_layer_queues_nothing(bad, status):
     a = dict(hidden=P, h_dtype=1, weights=P, ids=P, emap=0, global_E=0, w13=P, w13_g=P, w2=P, w2_g=P, out=P, out_dtype=1, M=2, topk=2, H=64, I=32, E=4,
-             flags=0, workspace=P, bytes=1 << 60, stream=0)
+             flags=0, status=P, workspace=P, bytes=1 << 60, stream=0)
     a.update(bad)
     assert _refused_unqueued(lambda L: L.b200fp4_w4a16_moe(*a.values())) == status
 
 
 @pytest.mark.parametrize("E,N,K,gated,size", [
-    (1, 1, 16, 0, 1152), (1, 16, 128, 0, 1152), (1, 17, 144, 0, 4 * 1152), (3, 32, 256, 1, 12 * 1152), (2, 34, 128, 1, 6 * 1152), (1, 16, 24, 0, 0),
-    (1, 15, 16, 1, 0), (0, 16, 16, 0, 0), (512, 1024, 2048, 1, 512 * 64 * 16 * 1152),
+    (1, 1, 16, 0, 1152 + 4), (1, 16, 128, 0, 1152 + 4), (1, 17, 144, 0, 4 * 1152 + 4), (3, 32, 256, 1, 12 * 1152 + 24), (2, 34, 128, 1, 6 * 1152 + 16), (1, 16, 24, 0, 0),
+    (1, 15, 16, 1, 0), (0, 16, 16, 0, 0), (512, 1024, 2048, 1, 512 * 64 * 16 * 1152 + 4096),
 ])
 def test_packed_bytes(E, N, K, gated, size):
     from dgx_vllm_b200 import _lib
@@ -59,7 +59,7 @@ def test_workspace_covers_a_turn_of_the_layer():
     L = _lib.lib()
     size = L.b200fp4_w4a16_moe_workspace_bytes
     assert size(32, 10, 2048, 512) >= 320 * (2 * 512 * 2 + 2048 * 4)
-    assert size(1 << 20, 10, 2048, 512) == size(409, 10, 2048, 512)               # more pairs are done in turns
+    assert size(1 << 20, 10, 2048, 512) == size(204, 10, 2048, 512)               # more pairs are done in turns
 
 
 def test_no_cpu_path():
