@@ -1,16 +1,16 @@
 // Weight-only NVFP4 (w4a16.cuh): the packing of a checkpoint's weights, the linear layer of few tokens, and the mixture-of-experts layer.
 //
-// One kernel, three uses.  A warp multiplies a tile of 16 packed rows with up to 8 * kCols columns of activations: codes become the
+// One kernel, three uses.  A warp multiplies units of 32 packed rows with up to 8 * kCols columns of activations: codes become the
 // 16-bit A operand in registers, the activations of a lane are the B operand as they lie in memory, sums are f32.
 //   linear   columns are tokens
 //   gate/up  columns are the (token, expert) pairs of one expert; a tile's rows are eight gate rows and the same eight up rows, so that a
 //            lane holds both halves of its values and applies SiLU(gate) * up to them
 //   down     two columns a pair, the activation's upper and lower part in f16: their sum has 22 bits, so that the value between the projections is
 //            not what limits the result
-// Work items are (tile, slot); a slot is a run of one expert's pairs that fits the columns.  A block has a contiguous range of them, groups of
+// Work items are (strip of 32 rows, slot); a slot is a run of one expert's pairs that fits the columns.  A block has a contiguous range of them, groups of
 // warps take items in turn and split k among themselves.
 // The layer is two launches without anything that has to outlast them: both find the slots from the routing by themselves, the first sets the
-// counters of the second, in which the block that finishes a tile's last item adds up its pairs in their order.
+// counters of the second, in which the block that finishes a strip's last item adds up its pairs in their order.
 #include <algorithm>
 #include <type_traits>
 
@@ -29,32 +29,30 @@ struct PackParams {
   const uint8_t* scales;      // [E, N, K/16]
   uint8_t* packed;
   uint32_t* peaks;            // [E], gated [E][gate, up]: behind the units, zeroed before
-  int64_t tiles, units;
+  int64_t strips, units;
   int N, K, gated;
 };
 
-// one warp per unit
-__global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int64_t n_units) {
-  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (unit >= n_units) return;
-  const int lane = threadIdx.x & 31;
-  const int64_t u = unit % p.units, tile = unit / p.units % p.tiles, e = unit / p.units / p.tiles;
+// one warp per tile of a unit
+__global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int64_t n_tiles) {
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (at >= n_tiles) return;
+  const int lane = threadIdx.x & 31, tile = (int)(at & 1);
+  const int64_t unit = at >> 1, u = unit % p.units, strip = unit / p.units % p.strips, e = unit / p.units / p.strips;
   uint8_t* const dst = p.packed + unit * kUnitBytes;
+  const int64_t row0 = (strip * 2 + tile) * (p.gated ? 8 : 16) + (lane >> 2), step = p.gated ? p.N / 2 : 8, rows = p.gated ? p.N / 2 : p.N;
   uint32_t sc = 0;
   float peak[2] = {0.f, 0.f};
   for (int half = 0; half < 2; ++half) {
     const int64_t k = u * kUnitK + half * 64 + (lane & 3) * 16;
     uint2 word[2];
     for (int r = 0; r < 2; ++r) {
-      // rows of a tile: 16 neighbours, or eight of the gate and the same eight of the up half
-      const int64_t row = p.gated ? (tile * 8 + (lane >> 2) < p.N / 2 ? r * (int64_t)(p.N / 2) + tile * 8 + (lane >> 2) : p.N)
-                                  : tile * 16 + r * 8 + (lane >> 2);
       uint32_t scale = 0;
       uint2 c = make_uint2(0, 0);
-      if (row < p.N && k < p.K) {
-        const int64_t at = e * p.N + row;
-        c = *reinterpret_cast<const uint2*>(p.codes + at * (p.K / 2) + k / 2);
-        scale = p.scales[at * (p.K / 16) + k / 16];
+      if ((p.gated ? row0 : row0 + r * 8) < rows && k < p.K) {
+        const int64_t row = e * p.N + row0 + r * step;
+        c = *reinterpret_cast<const uint2*>(p.codes + row * (p.K / 2) + k / 2);
+        scale = p.scales[row * (p.K / 16) + k / 16];
         if (scale & 0x80) {
           c.x ^= 0x88888888u;
           c.y ^= 0x88888888u;
@@ -69,9 +67,9 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
       const float value = (code < 2 ? 0.5f * code : (1.f + 0.5f * (code & 1)) * (float)(1 << (code >> 1)) * 0.5f) * e4m3_to_f32((uint8_t)scale);
       peak[p.gated ? r : 0] = fmaxf(peak[p.gated ? r : 0], value);
     }
-    *reinterpret_cast<uint4*>(dst + half * 512 + lane * 16) = make_uint4(word[0].x, word[0].y, word[1].x, word[1].y);
+    *reinterpret_cast<uint4*>(dst + (tile * 2 + half) * 512 + lane * 16) = make_uint4(word[0].x, word[0].y, word[1].x, word[1].y);
   }
-  *reinterpret_cast<uint32_t*>(dst + kUnitScales + lane * 4) = sc;
+  *reinterpret_cast<uint32_t*>(dst + kUnitScales + lane * 8 + tile * 4) = sc;
   // magnitudes are not negative: their bits order as they do
   for (int r = 0; r <= p.gated; ++r) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(peak[r]));
@@ -96,7 +94,8 @@ struct RowsParams {
   const void* bias;           // [N] or null
   int out_dtype, bias_dtype;
   int M, N, K;
-  int tiles, units;
+  int strips, units;
+  int split;                  // linear: blocks of a cluster, which share the units of an item
   int cap, rows;              // columns of a slot; rows that there is room for
   int* status;
   int clear_status;
@@ -110,15 +109,15 @@ struct RowsParams {
   __half* act;                // gate/up out
   float* act_inv;             // [pair]: the reciprocal of the factor that brought its row of act into f16's range
   float* y;                   // down: [pair][N]
-  int* counters;              // [tile groups of down]
+  int* counters;              // [strips of down]
   int n_counters;
 };
 
 // Shared memory of a block.  Rings of weight units, a warp's its own | their barriers | partial sums, two of them in turn | and for the layer: pairs
 // an expert has, then where they begin | expert of a pair | its place among that expert's | pairs by expert | slots | scan | and where rows are
-// staged: their statistics | parts of those | the rows in f16
+// staged: their statistics | parts of those | the rows in f16 | (linear, split) sums of the block's items
 struct Layout {
-  uint32_t bars, red, count, expert, rank, list, slots, scan, stats, parts, rows, bytes;
+  uint32_t bars, red, count, expert, rank, list, slots, scan, stats, parts, rows, sums, bytes;
 };
 struct RowStat {
   float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
@@ -127,7 +126,8 @@ constexpr uint32_t kSmemMost = 227 * 1024;
 
 __host__ __device__ __forceinline__ uint32_t pad16(uint32_t v) { return (v + 15) / 16 * 16; }
 // pairs, E: 0 for a linear layer; rows: staged rows of row_bytes each
-__host__ __device__ __forceinline__ Layout layout_of(uint32_t ring, uint32_t bars, uint32_t red, int pairs, int E, int cap, int rows, uint32_t row_bytes) {
+__host__ __device__ __forceinline__ Layout layout_of(uint32_t ring, uint32_t bars, uint32_t red, int pairs, int E, int cap, int rows, uint32_t row_bytes,
+                                                      uint32_t sums) {
   Layout l;
   l.bars = ring;
   l.red = pad16(l.bars + bars);
@@ -140,7 +140,8 @@ __host__ __device__ __forceinline__ Layout layout_of(uint32_t ring, uint32_t bar
   l.stats = pad16(l.scan + (pairs > 0 ? 2 * kWarps * 4 + 16 : 0));
   l.parts = l.stats + (uint32_t)rows * sizeof(RowStat);
   l.rows = pad16(l.parts + (rows > 0 ? kWarps * kWarps * 8 : 0));
-  l.bytes = l.rows + (uint32_t)rows * row_bytes;
+  l.sums = l.rows + (uint32_t)rows * row_bytes;
+  l.bytes = l.sums + sums;
   return l;
 }
 
@@ -277,31 +278,68 @@ __device__ __forceinline__ float2 row_part(const T* row, int k0, int k1) {
   return make_float2(__uint_as_float(top), sum);
 }
 
-template <int kCols, int kTiles>
+template <int kCols>
 struct Shape {
-  static constexpr int kStages = kCols * kTiles >= 4 ? 2 : (kTiles == 1 ? 5 : 3);      // of a warp's ring
-  static constexpr uint32_t kStageBytes = kTiles * kUnitBytes;
-  static constexpr uint32_t kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kStages = 3;                            // of a warp's ring
+  static constexpr uint32_t kRing = kWarps * kStages * kUnitBytes;
   static constexpr uint32_t kBars = kWarps * kStages * 8;
-  static constexpr int kSums = kTiles * kCols * 4 * 32;       // of a warp
-  static constexpr uint32_t kRed = 2 * kWarps * kSums * 4;
+  static constexpr int kSums = 2 * kCols * 4 * 32;             // of a warp
+  static constexpr uint32_t kRed = kWarps * kSums * 4;
 };
 
-// XT: type of the activations; kCols: columns of eight; kTiles: row tiles a warp does at once
-template <typename XT, int kMode, int kCols, int kTiles>
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// a unit's 32 rows times kCols columns of eight; b: the columns' operands, [half][column][8]
+template <int kCols>
+__device__ __forceinline__ void multiply_unit(uint32_t unit, int lane, const uint32_t (&b)[2][kCols][8], float (&acc)[2][kCols][4]) {
+  const uint2 sc = lds64(unit + kUnitScales + lane * 8);
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint4 w = lds128(unit + (t * 2 + half) * 512 + lane * 16);
+      const __half2 s = scales_of(t ? sc.y : sc.x, half), s_lo = __low2half2(s), s_hi = __high2half2(s);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t lo[4], hi[4];
+        codes_to_pairs(q ? w.y : w.x, lo);
+        codes_to_pairs(q ? w.w : w.z, hi);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = as_u32(__hmul2(as_half2(lo[j]), s_lo));
+          hi[j] = as_u32(__hmul2(as_half2(hi[j]), s_hi));
+        }
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          mma_16x8x16(acc[t][c], lo[0], hi[0], lo[1], hi[1], b[half][c][q * 4], b[half][c][q * 4 + 1]);
+          mma_16x8x16(acc[t][c], lo[2], hi[2], lo[3], hi[3], b[half][c][q * 4 + 2], b[half][c][q * 4 + 3]);
+        }
+      }
+    }
+}
+
+// XT: type of the activations; kCols: columns of eight
+template <typename XT, int kMode, int kCols>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  using S = Shape<kCols, kTiles>;
+  using S = Shape<kCols>;
   constexpr bool kConvert = std::is_same<XT, __nv_bfloat16>::value;
   constexpr bool kStaged = kMode != kDown;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
-  const int cap = p.cap;
-  const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;      // rows are shifted by 16 bytes against each other: no two lanes of a load meet
-  const Layout l = layout_of(S::kRing, S::kBars, S::kRed, kMode == kLinear ? 0 : p.M * p.topk, kMode == kLinear ? 0 : p.E, cap, p.rows, row_bytes);
+  const int cap = p.cap, split = kMode == kLinear ? p.split : 1;
+  const int rank = kMode == kLinear ? (int)(blockIdx.x % (unsigned)split) : 0;
+  const int unit_first = p.units * rank / split, unit_last = p.units * (rank + 1) / split, own_units = unit_last - unit_first;
+  // rows are shifted by 16 bytes against each other: no two lanes of a load meet
+  const uint32_t row_bytes = (uint32_t)((p.units + split - 1) / split) * (kUnitK * 2) + 16;
+  const Layout l = layout_of(S::kRing, S::kBars, S::kRed, kMode == kLinear ? 0 : p.M * p.topk, kMode == kLinear ? 0 : p.E, cap, p.rows, row_bytes, 0);
   const uint32_t base = smem_u32(smem);
   const int2* const slots = reinterpret_cast<const int2*>(smem + l.slots);
   const uint16_t* const list = reinterpret_cast<const uint16_t*>(smem + l.list);
-  const uint32_t ring = base + warp * (S::kStages * S::kStageBytes), bars = base + l.bars + warp * (S::kStages * 8);
+  const uint32_t ring = base + warp * (S::kStages * kUnitBytes), bars = base + l.bars + warp * (S::kStages * 8);
   if (lane < S::kStages) mbar_init(bars + lane * 8, 1);
   fence_proxy_async_smem();
   __syncwarp();
@@ -323,24 +361,26 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
       return;
     }
   }
-  // Items of a slot are neighbours, or (down) those of a group of tiles
-  const int groups_of_tiles = (p.tiles + kTiles - 1) / kTiles;
-  const int fast = kMode == kDown ? n_slots : groups_of_tiles;
-  const int64_t n_items = (int64_t)n_slots * groups_of_tiles;
-  const int first = (int)(n_items * blockIdx.x / gridDim.x), last = (int)(n_items * (blockIdx.x + 1) / gridDim.x);
+  // Items of a slot are neighbours, or (down) those of a strip
+  const int fast = kMode == kDown ? n_slots : p.strips;
+  const int64_t n_items = (int64_t)n_slots * p.strips;
+  const unsigned cluster = blockIdx.x / (unsigned)split, clusters = gridDim.x / (unsigned)split;
+  const int first = (int)(n_items * cluster / clusters), last = (int)(n_items * (cluster + 1) / clusters);
   const int n_block = last - first;
 
-  // Warps that share an item: as few rounds as possible, an item's ending counted as one more unit
-  int share = 1, best = 1 << 30;
-  for (int s = 1; s <= kWarps && s <= p.units; s *= 2) {
-    const int cost = (n_block * s + kWarps - 1) / kWarps * ((p.units + s - 1) / s + 1);
+  // Warps that share an item.  Busy warps take a unit in about 110 cycles of the SM, a warp alone in 350; an item's ending costs a warp that shares it
+  // about half a unit.
+  int share = 1, best = 0x7FFFFFFF;
+  for (int s = 1; s <= kWarps && s <= own_units; s *= 2) {
+    const int busy = n_block * (2 * own_units + s), alone = (n_block * s + kWarps - 1) / kWarps * ((own_units + s - 1) / s + 1) * 7;
+    const int cost = busy > alone ? busy : alone;
     if (cost < best) {
       best = cost;
       share = s;
     }
   }
   const int group = warp / share, in_group = warp - group * share, n_groups = kWarps / share;
-  const int k_first = p.units * in_group / share, k_last = p.units * (in_group + 1) / share;
+  const int k_first = unit_first + own_units * in_group / share, k_last = unit_first + own_units * (in_group + 1) / share;
 
   struct Cursor {
     int item, hi, lo;         // hi * fast + lo
@@ -359,41 +399,35 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
     }
   };
   auto slot_of = [&](const Cursor& c) { return kMode == kDown ? c.lo : c.hi; };
-  auto tile_of = [&](const Cursor& c) { return (kMode == kDown ? c.hi : c.lo) * kTiles; };
+  auto strip_of = [&](const Cursor& c) { return kMode == kDown ? c.hi : c.lo; };
 
   // ---- the ring: one lane asks for the units, all wait for them
   Cursor ahead;
   start(ahead);
-  int ahead_k = k_first, fill = 0;
+  int ahead_left = 0;
+  uint32_t fill = 0;
   const uint8_t* src = nullptr;
-  size_t tile_step = 0;
   auto fetch = [&]() {
-    if (ahead.item >= last) return;
-    if (ahead_k == k_first) {
-      const int tile = tile_of(ahead);
+    if (ahead_left == 0) {
+      if (ahead.item >= last) return;
       const size_t e = kMode == kLinear ? 0 : slots[slot_of(ahead)].x & 0xFFFF;
-      src = p.packed + ((e * p.tiles + tile) * p.units + k_first) * kUnitBytes;
-      tile_step = tile + kTiles <= p.tiles ? (size_t)p.units * kUnitBytes : 0;       // a last tile alone is done twice
-    }
-    if (lane == 0) {
-      const uint32_t bar = bars + fill * 8, to = ring + fill * S::kStageBytes;
-      mbar_expect_tx(bar, S::kStageBytes);
-#pragma unroll
-      for (int r = 0; r < kTiles; ++r) bulk_load_1d(to + r * kUnitBytes, src + r * tile_step, kUnitBytes, bar);
-    }
-    src += kUnitBytes;
-    if (++fill == S::kStages) fill = 0;
-    if (++ahead_k == k_last) {
-      ahead_k = k_first;
+      src = p.packed + ((e * p.strips + strip_of(ahead)) * p.units + k_first) * kUnitBytes;
+      ahead_left = k_last - k_first;
       next(ahead);
     }
+    if (lane == 0) {
+      mbar_expect_tx(bars + fill * 8, kUnitBytes);
+      bulk_load_1d(ring + fill * kUnitBytes, src, kUnitBytes, bars + fill * 8);
+    }
+    src += kUnitBytes;
+    --ahead_left;
+    if (++fill == S::kStages) fill = 0;
   };
   for (int i = 0; i < S::kStages; ++i) fetch();
 
   Cursor at;
   start(at);
-  int stage = 0, turn = 0;
-  uint32_t phase = 0;
+  uint32_t stage = 0, phase = 0;
   bool ok = true;
   // Rows are staged for as many slots at a time as there is room for
   int slot = kStaged && n_block > 0 ? first / fast : 0;
@@ -424,11 +458,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
       // few rows: several warps a row
       int n_parts = kWarps;
       while (n_parts > 1 && n_parts * n_rows > kWarps) n_parts /= 2;
-      const int octets = p.K / 8;
+      const int k_begin = unit_first * kUnitK, k_end = min(p.K, unit_last * kUnitK), octets = (k_end - k_begin) / 8;
       __syncthreads();                             // nobody reads the rows before these any more
       for (int i0 = 0; i0 < n_rows * n_parts; i0 += kWarps) {
         const int i = i0 + warp, r = i / n_parts, part = i - r * n_parts;
-        const int k0 = octets * part / n_parts * 8, k1 = octets * (part + 1) / n_parts * 8;
+        const int k0 = k_begin + octets * part / n_parts * 8, k1 = k_begin + octets * (part + 1) / n_parts * 8;
         const bool work = r < n_rows;
         uint32_t factor = 0;
         if constexpr (kConvert || kMode == kGateUp) {
@@ -473,34 +507,34 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
             uint4 v = ld_u4(row + k);
             if constexpr (kConvert)
               v = make_uint4(bf16_to_f16_pair(v.x, factor), bf16_to_f16_pair(v.y, factor), bf16_to_f16_pair(v.z, factor), bf16_to_f16_pair(v.w, factor));
-            *reinterpret_cast<uint4*>(to + k * 2) = v;
+            *reinterpret_cast<uint4*>(to + (k - k_begin) * 2) = v;
           }
           if (part == n_parts - 1)                 // a unit's k past the row's end
-            for (int k = p.K + lane * 8; k < p.units * kUnitK; k += 256) *reinterpret_cast<uint4*>(to + k * 2) = make_uint4(0, 0, 0, 0);
+            for (int k = k_end + lane * 8; k < unit_last * kUnitK; k += 256) *reinterpret_cast<uint4*>(to + (k - k_begin) * 2) = make_uint4(0, 0, 0, 0);
         }
       }
       __syncthreads();
     }
 
     for (; at.item < end; next(at)) {
-      const int slot_at = slot_of(at);
+      const int slot_at = slot_of(at), strip = strip_of(at);
       const int2 s = kMode == kLinear ? make_int2(min(cap, p.M - slot_at * cap) << 16, slot_at * cap) : slots[slot_at];
       const int n = s.x >> 16;                     // columns in use; the others read the first one's row, and nobody reads their sums
-      float acc[kTiles][kCols][4];
+      float acc[2][kCols][4];
+      uint32_t b[2][kCols][8];
       uint32_t col[kCols];
       const __half* act[kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
         const int i = c * 8 + row8;
-        if constexpr (kStaged) col[c] = base + l.rows + (uint32_t)(s.y - row0 + (i < n ? i : 0)) * row_bytes + k_first * (kUnitK * 2) + quad * 32;
+        if constexpr (kStaged) col[c] = base + l.rows + (uint32_t)(s.y - row0 + (i < n ? i : 0)) * row_bytes + (k_first - unit_first) * (kUnitK * 2) + quad * 32;
         else act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i / 2 < n ? i / 2 : 0)] * 2 + (i & 1)) * p.ldx + k_first * kUnitK + quad * 16;
 #pragma unroll
-        for (int r = 0; r < kTiles; ++r)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int j = 0; j < 4; ++j) acc[r][c][j] = 0.f;
+          for (int j = 0; j < 4; ++j) acc[t][c][j] = 0.f;
       }
-      for (int k = k_first; k < k_last; ++k) {
-        uint32_t b[2][kCols][8];
+      auto load_columns = [&](int k) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -521,34 +555,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
           if constexpr (kStaged) col[c] += kUnitK * 2;
           else act[c] += kUnitK;
         }
-        if (ok) ok = mbar_wait_warp(bars + stage * 8, phase, p.status, 61);
-        const uint32_t unit = ring + stage * S::kStageBytes + lane * 16;
-#pragma unroll
-        for (int r = 0; r < kTiles; ++r) {
-          const uint32_t sc = lds32(unit + r * kUnitBytes + kUnitScales - lane * 12);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint4 w = lds128(unit + r * kUnitBytes + half * 512);
-            uint32_t s_lo, s_hi;
-            scales_of(sc, half, s_lo, s_hi);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t lo[4], hi[4];
-              codes_to_pairs(q ? w.y : w.x, lo);
-              codes_to_pairs(q ? w.w : w.z, hi);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                lo[j] = mul2(lo[j], s_lo);
-                hi[j] = mul2(hi[j], s_hi);
-              }
-#pragma unroll
-              for (int c = 0; c < kCols; ++c) {
-                mma_16x8x16(acc[r][c], lo[0], hi[0], lo[1], hi[1], b[half][c][q * 4], b[half][c][q * 4 + 1]);
-                mma_16x8x16(acc[r][c], lo[2], hi[2], lo[3], hi[3], b[half][c][q * 4 + 2], b[half][c][q * 4 + 3]);
-              }
-            }
-          }
-        }
+      };
+      for (int k = k_first; k < k_last; ++k) {
+        load_columns(k);
+        if (ok) ok = mbar_wait(bars + stage * 8, phase, p.status, 61);
+        multiply_unit<kCols>(ring + stage * kUnitBytes, lane, b, acc);
         if (++stage == S::kStages) {
           stage = 0;
           phase ^= 1;
@@ -557,55 +568,21 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
         if (ok) fetch();
       }
 
-      // ---- the item's end.  Sums of a warp: [tile][column of eight][j][lane]; a lane's j are row l / 4 (0, 1) or row l / 4 + 8 (2, 3) and
-      // columns 2 (l % 4) and the next one.
-      const int e = kMode == kLinear ? 0 : s.x & 0xFFFF, tile = tile_of(at);
-      float* const red = reinterpret_cast<float*>(smem + l.red) + ((turn & 1) * kWarps + group * share) * S::kSums;
-      turn ^= 1;
-      if (share > 1) {
-#pragma unroll
-        for (int r = 0; r < kTiles; ++r)
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) red[in_group * S::kSums + ((r * kCols + c) * 4 + j) * 32 + lane] = acc[r][c][j];
-        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
-      }
-      // a pair of sums (j, j + 2: gate and up, or rows eight apart; down: 0, 1 and 2, 3, the two parts) goes to one lane of one warp
-      constexpr int kPairs = kTiles * kCols * 2;   // a lane's
-      for (int i = in_group; i < kPairs; i += share) {
-        const int j = i & 1, c = (i >> 1) % kCols, r = (i >> 1) / kCols;
-        const int ja = kMode == kDown ? 2 * j : j, jb = kMode == kDown ? 2 * j + 1 : j + 2;
-        float va = 0.f, vb = 0.f;
-        if (share > 1) {
-          const float* from = red + ((r * kCols + c) * 4) * 32 + lane;
-          for (int w = 0; w < share; ++w, from += S::kSums) {
-            va += from[ja * 32];
-            vb += from[jb * 32];
-          }
-        } else {
-#pragma unroll
-          for (int rr = 0; rr < kTiles; ++rr)
-#pragma unroll
-            for (int cc = 0; cc < kCols; ++cc)
-#pragma unroll
-              for (int jj = 0; jj < 2; ++jj)
-                if (rr == r && cc == c && jj == j) {
-                  va = acc[rr][cc][kMode == kDown ? 2 * jj : jj];
-                  vb = acc[rr][cc][kMode == kDown ? 2 * jj + 1 : jj + 2];
-                }
-        }
-        if (tile + r >= p.tiles) continue;
+      // ---- the item's end.  A lane's sums j are row l / 4 (0, 1) or l / 4 + 8 (2, 3) of a tile and columns 2 (l % 4) and the next one.
+      const int e = kMode == kLinear ? 0 : s.x & 0xFFFF;
+      auto finish = [&](int t, int c, int j, float va, float vb) {
+        // va, vb: sums j and j + 2 (gate and up, or rows eight apart); down: the two parts' sums of row j * 8
         const int column = c * 8 + quad * 2;
         if constexpr (kMode == kDown) {
-          if (column / 2 < n) {
+          const int row = strip * 32 + t * 16 + j * 8 + row8;
+          if (column / 2 < n && row < p.N) {
             const int pair = list[s.y + column / 2];
-            p.y[(size_t)pair * p.N + (tile + r) * 16 + j * 8 + row8] = (va + vb) * (p.act_inv[pair] * p.g[e]);
+            p.y[(size_t)pair * p.N + row] = (va + vb) * (p.act_inv[pair] * p.g[e]);
           }
         } else if (column + j < n) {
           const RowStat st = reinterpret_cast<const RowStat*>(smem + l.stats)[s.y - row0 + column + j];
           if constexpr (kMode == kGateUp) {
-            const int pair = list[s.y + column + j], I = p.N / 2, i_at = (tile + r) * 8 + row8;
+            const int pair = list[s.y + column + j], I = p.N / 2, i_at = strip * 16 + t * 8 + row8;
             if (i_at < I) {
               const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
               const float v = silu_f32(va * f * p.g[2 * e]) * (vb * f * p.g[2 * e + 1]) * st.act;
@@ -616,19 +593,53 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
               to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
             }
           } else {
-            const int m = s.y + column + j, row = (tile + r) * 16 + row8;
+            const int row = strip * 32 + t * 16 + row8;
             const float f = kConvert ? st.inv : 1.f;
+            if (split > 1) {
+              float* const to = reinterpret_cast<float*>(smem + l.sums) + ((at.item - first) * cap + column + j) * 32 + t * 16 + row8;
+              to[0] = va * f;
+              to[8] = vb * f;
+            } else {
+              const int m = s.y + column + j;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int at_n = row + h * 8;
-              if (at_n < p.N) {
-                float v = (h ? vb : va) * f * p.g[0];
-                if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, at_n);
-                store_value(p.out, p.out_dtype, (size_t)m * p.N + at_n, v);
-              }
+              for (int h = 0; h < 2; ++h)
+                if (row + h * 8 < p.N) {
+                  float v = (h ? vb : va) * f * p.g[0];
+                  if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row + h * 8);
+                  store_value(p.out, p.out_dtype, (size_t)m * p.N + row + h * 8, v);
+                }
             }
           }
         }
+      };
+      if (share == 1) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) finish(t, c, j, acc[t][c][kMode == kDown ? 2 * j : j], acc[t][c][kMode == kDown ? 2 * j + 1 : j + 2]);
+      } else {
+        // [warp][tile][column of eight][j][lane]; each warp adds up and finishes its part
+        float* const red = reinterpret_cast<float*>(smem + l.red) + group * share * S::kSums + lane;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int c = 0; c < kCols; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) red[in_group * S::kSums + ((t * kCols + c) * 4 + j) * 32] = acc[t][c][j];
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
+        for (int i = in_group; i < 4 * kCols; i += share) {
+          const int j = i & 1, tc = i >> 1;
+          const float *a_from = red + (tc * 4 + (kMode == kDown ? 2 * j : j)) * 32, *b_from = a_from + (kMode == kDown ? 32 : 64);
+          float va = 0.f, vb = 0.f;
+          for (int w = 0; w < share; ++w) {
+            va += a_from[w * S::kSums];
+            vb += b_from[w * S::kSums];
+          }
+          finish(tc / kCols, tc % kCols, j, va, vb);
+        }
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
       }
     }
   }
@@ -638,24 +649,46 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
     while (clock64() - t0 < kWaitCycles / 64) {
     }
   }
+  if constexpr (kMode == kLinear) {
+    if (split > 1) {
+      // the parts of k are added in their order, each block of the cluster some of the items' values
+      cluster_sync_any();
+      const int count = n_block * cap * 32;
+      for (int i = rank * kThreads + threadIdx.x; i < count; i += split * kThreads) {
+        const int item = first + i / (cap * 32), column = i / 32 % cap, slot_at = item / fast;
+        const int row = (item - slot_at * fast) * 32 + (i & 31), m = slot_at * cap + column;
+        if (m >= p.M || row >= p.N) continue;
+        float v = 0.f;
+        for (int r = 0; r < split; ++r) {
+          float u;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(map_to_cta(base + l.sums + i * 4, r)) : "memory");
+          v += u;
+        }
+        v *= p.g[0];
+        if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
+        store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
+      }
+      cluster_sync_any();                          // nobody leaves while its sums are read
+    }
+  }
   if constexpr (kMode == kDown) {
-    // The block that completes a group of tiles adds up every token's pairs, in the order of the routing.
+    // The block that completes a strip adds up every token's pairs, in the order of the routing.
     const uint16_t* const expert = reinterpret_cast<const uint16_t*>(smem + l.expert);
     int* const flag = reinterpret_cast<int*>(smem + l.scan);
     __threadfence();
     __syncthreads();
     if (n_block == 0) return;
-    for (int tg = first / n_slots; tg <= (last - 1) / n_slots; ++tg) {
+    for (int strip = first / n_slots; strip <= (last - 1) / n_slots; ++strip) {
       if (threadIdx.x == 0) {
-        const int done = min(last, (tg + 1) * n_slots) - max(first, tg * n_slots);
-        *flag = atomicAdd(&p.counters[tg], done) + done == n_slots;
+        const int done = min(last, (strip + 1) * n_slots) - max(first, strip * n_slots);
+        *flag = atomicAdd(&p.counters[strip], done) + done == n_slots;
         __threadfence();
       }
       __syncthreads();
       const bool mine = *flag != 0;
       __syncthreads();
       if (!mine) continue;
-      const int row0 = tg * kTiles * 16, quads = (min(kTiles * 16, p.N - row0)) / 4;
+      const int row0 = strip * 32, quads = (min(32, p.N - row0)) / 4;
       for (int i = threadIdx.x; i < p.M * quads; i += kThreads) {
         const int m = i / quads, row = row0 + (i - m * quads) * 4;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -679,35 +712,63 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
   }
 }
 
-template <typename XT, int kMode, int kCols, int kTiles>
+constexpr int kMaxSplit = 8;
+
+template <typename XT, int kMode, int kCols>
 int launch_rows(RowsParams p, cudaStream_t st) {
-  using S = Shape<kCols, kTiles>;
+  using S = Shape<kCols>;
   static std::once_flag once[64];
   static bool ready[64];
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200FP4_STATUS_NOT_SUPPORTED;
   std::call_once(once[dev], [&] {
-    ready[dev] = cudaFuncSetAttribute(w4a16_rows_kernel<XT, kMode, kCols, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost) == cudaSuccess;
+    ready[dev] = cudaFuncSetAttribute(w4a16_rows_kernel<XT, kMode, kCols>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost) == cudaSuccess;
     cudaGetLastError();
   });
   if (!ready[dev]) return B200FP4_STATUS_EXECUTION_FAILED;
   const int pairs = kMode == kLinear ? 0 : p.M * p.topk, E = kMode == kLinear ? 0 : p.E;
-  const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;
-  p.cap = (kMode == kDown ? 4 : 8) * kCols;
-  p.rows = 0;
-  while (kMode != kDown) {
-    // rows that there is room for; a slot has no more columns than that
-    const uint32_t rest = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, p.cap, 1, 0).bytes;
-    const int64_t most = kMode == kLinear ? std::min(p.M, p.cap) : pairs;
-    p.rows = (int)std::min<int64_t>(most, (kSmemMost - std::min(rest, kSmemMost)) / (row_bytes + (uint32_t)sizeof(RowStat)));
-    if (p.rows < 1) return B200FP4_STATUS_NOT_SUPPORTED;
-    if (p.rows >= p.cap || p.rows == most) break;
-    p.cap = p.rows;
+  unsigned grid = 0;
+  uint32_t smem = 0;
+  int64_t best = INT64_MAX;
+  RowsParams chosen = p;
+  // Blocks that share the k of an item in a cluster (linear): a shorter k leaves room for more rows and spreads few strips over all SMs
+  for (int split = 1; split <= (kMode == kLinear ? kMaxSplit : 1) && split <= p.units; split *= 2) {
+    static ResidentClusters counts[kMaxSplit + 1][64];
+    const int clusters = split == 1 ? sm_count() : resident_clusters_of(counts[split], w4a16_rows_kernel<XT, kMode, kCols>, split, kThreads, kSmemMost);
+    if (clusters < 1) break;
+    RowsParams q = p;
+    const uint32_t own = (uint32_t)((p.units + split - 1) / split), row_bytes = own * (kUnitK * 2) + 16;
+    const int64_t most = kMode == kLinear ? p.M : pairs;
+    q.split = split;
+    q.cap = (kMode == kDown ? 4 : 8) * kCols;
+    q.rows = 0;
+    uint32_t sums = 0;
+    while (kMode != kDown) {
+      // rows that there is room for; a slot has no more columns than that
+      if (kMode == kLinear) q.cap = (int)std::min<int64_t>(q.cap, most);
+      const int64_t items = kMode == kLinear ? (most + q.cap - 1) / q.cap * p.strips : 0;
+      sums = split > 1 ? (uint32_t)std::min<int64_t>((items + clusters - 1) / clusters, 1 << 16) * q.cap * 128 : 0;
+      const uint32_t rest = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, q.cap, 1, 0, sums).bytes;
+      q.rows = (int)std::min<int64_t>(kMode == kLinear ? q.cap : most, rest < kSmemMost ? (kSmemMost - rest) / (row_bytes + (uint32_t)sizeof(RowStat)) : 0);
+      if (q.rows < 1 || q.rows >= q.cap || q.rows == most) break;
+      q.cap = q.rows;
+    }
+    if (kMode != kDown && q.rows < 1) continue;
+    const uint32_t bytes = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, q.cap, q.rows, row_bytes, sums).bytes;
+    if (bytes > kSmemMost) continue;
+    const int64_t slots = kMode == kLinear ? (most + q.cap - 1) / q.cap : std::min(pairs, E) + pairs / q.cap;
+    if (slots * p.strips > 0x3FFFFFFF) continue;
+    // units of the block with the most of them; a cluster costs its synchronisation
+    const int64_t cost = kMode == kLinear ? ((slots * p.strips + clusters - 1) / clusters * own + (split > 1 ? 4 : 0)) : 0;
+    if (cost < best) {
+      best = cost;
+      chosen = q;
+      grid = (unsigned)(kMode == kLinear ? std::min<int64_t>(clusters, slots * p.strips) * split : clusters);
+      smem = bytes;
+    }
   }
-  if ((int64_t)((kMode == kLinear ? p.M : pairs) / p.cap + (E > 0 ? E : 1)) * p.tiles > 0x7FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
-  const uint32_t smem = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, p.cap, p.rows, row_bytes).bytes;
-  if (smem > kSmemMost) return B200FP4_STATUS_NOT_SUPPORTED;
-  if (launch_pdl(w4a16_rows_kernel<XT, kMode, kCols, kTiles>, dim3(sm_count()), dim3(kThreads), smem, st, p) != cudaSuccess) {
+  if (grid == 0) return B200FP4_STATUS_NOT_SUPPORTED;
+  if (launch_pdl_cluster(chosen.split, w4a16_rows_kernel<XT, kMode, kCols>, dim3(grid), dim3(kThreads), smem, st, chosen) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
@@ -716,17 +777,14 @@ int launch_rows(RowsParams p, cudaStream_t st) {
 
 template <typename T>
 int launch_linear(const RowsParams& p, cudaStream_t st) {
-  if (p.M <= 8) return launch_rows<T, kLinear, 1, 1>(p, st);
-  return launch_rows<T, kLinear, 2, 2>(p, st);
+  return p.M <= 8 ? launch_rows<T, kLinear, 1>(p, st) : launch_rows<T, kLinear, 2>(p, st);
 }
 template <typename T>
 int launch_gate_up(const RowsParams& p, cudaStream_t st) {
-  if ((int64_t)p.M * p.topk <= 4 * (int64_t)p.E) return launch_rows<T, kGateUp, 1, 2>(p, st);
-  return launch_rows<T, kGateUp, 2, 2>(p, st);
+  return (int64_t)p.M * p.topk <= 4 * (int64_t)p.E ? launch_rows<T, kGateUp, 1>(p, st) : launch_rows<T, kGateUp, 2>(p, st);
 }
 int launch_down(const RowsParams& p, cudaStream_t st) {
-  if ((int64_t)p.M * p.topk <= 2 * (int64_t)p.E) return launch_rows<__half, kDown, 1, 2>(p, st);
-  return launch_rows<__half, kDown, 2, 2>(p, st);
+  return (int64_t)p.M * p.topk <= 2 * (int64_t)p.E ? launch_rows<__half, kDown, 1>(p, st) : launch_rows<__half, kDown, 2>(p, st);
 }
 
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
@@ -735,8 +793,9 @@ bool is_dtype(int dtype) { return is_16bit(dtype) || dtype == B200FP4_DTYPE_F32;
 size_t pad256(size_t v) { return (v + 255) / 256 * 256; }
 
 
+int64_t packed_strips(int64_t N, int gated) { return gated ? (N / 2 + 15) / 16 : strips_of(N); }
 size_t unit_bytes(int64_t E, int64_t N, int64_t K, int gated) {
-  return (size_t)E * (gated ? (N / 2 + 7) / 8 : tiles_of(N)) * units_of(K) * kUnitBytes;
+  return (size_t)E * packed_strips(N, gated) * units_of(K) * kUnitBytes;
 }
 
 // tokens of a layer whose pairs fit one turn
@@ -752,7 +811,7 @@ MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I) {
   s.act_inv = s.act + pad256(pairs * 2 * I * 2);
   s.y = s.act_inv + pad256(pairs * 4);
   s.counters = s.y + pad256(pairs * H * 4);
-  s.bytes = s.counters + pad256((size_t)tiles_of(H) * 4);
+  s.bytes = s.counters + pad256((size_t)strips_of(H) * 4);
   return s;
 }
 
@@ -774,12 +833,12 @@ extern "C" int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, i
   p.codes = codes;
   p.scales = scales;
   p.packed = packed;
-  p.tiles = gated ? (N / 2 + 7) / 8 : w4::tiles_of(N);
+  p.strips = packed_strips(N, gated);
   p.units = w4::units_of(K);
   p.N = (int)N;
   p.K = (int)K;
   p.gated = gated != 0;
-  const int64_t n = E * p.tiles * p.units;
+  const int64_t n = E * p.strips * p.units * 2;
   if ((n + 7) / 8 > 0x7FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
   p.peaks = reinterpret_cast<uint32_t*>(packed + unit_bytes(E, N, K, gated));
   if (cudaMemsetAsync(p.peaks, 0, (size_t)E * (gated ? 2 : 1) * 4, static_cast<cudaStream_t>(stream)) != cudaSuccess) {
@@ -811,7 +870,7 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   p.M = (int)M;
   p.N = (int)N;
   p.K = (int)K;
-  p.tiles = (int)w4::tiles_of(N);
+  p.strips = (int)w4::strips_of(N);
   p.units = (int)w4::units_of(K);
   p.status = status;
   p.clear_status = 1;
@@ -859,7 +918,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.peaks = reinterpret_cast<const float*>(w13_packed + unit_bytes(E, 2 * I, H, 1));
     p.y = reinterpret_cast<float*>(ws + s.y);
     p.counters = reinterpret_cast<int*>(ws + s.counters);
-    p.n_counters = (int)w4::tiles_of(H);
+    p.n_counters = (int)w4::strips_of(H);
     RowsParams d = p;
     p.x = static_cast<const unsigned char*>(hidden) + (size_t)m * H * 2;
     p.ldx = H;
@@ -867,7 +926,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.g = w13_g;
     p.N = (int)(2 * I);
     p.K = (int)H;
-    p.tiles = (int)((I + 7) / 8);
+    p.strips = (int)((I + 15) / 16);
     p.units = (int)w4::units_of(H);
     d.x = p.act;
     d.ldx = I;
@@ -877,7 +936,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     d.out_dtype = out_dtype;
     d.N = (int)H;
     d.K = (int)I;
-    d.tiles = (int)w4::tiles_of(H);
+    d.strips = (int)w4::strips_of(H);
     d.units = (int)w4::units_of(I);
     int rc = h_dtype == B200FP4_DTYPE_BF16 ? launch_gate_up<__nv_bfloat16>(p, st) : launch_gate_up<__half>(p, st);
     if (rc == B200FP4_STATUS_SUCCESS) rc = launch_down(d, st);

@@ -8,13 +8,14 @@
 // become f16 exactly, after a power of two for each row has brought its largest value below 2^15: what is then below f16's
 // smallest, 2^-39 of that largest value, is the only part that can be rounded.
 //
-// Packed weight: units of 16 rows x 128 of k, 1152 bytes, [matrix][row tile][k / 128][unit].  A unit is laid out for the 16x8x16 matrix
+// Packed weight: units of 32 rows x 128 of k, 2304 bytes, [matrix][32 rows][k / 128][unit].  A unit is two tiles of the 16x8x16 matrix
 // instruction, whose lane l holds rows l / 4 and l / 4 + 8 and four k of each: with the k of an instruction taken from four blocks of 16,
 // lane l needs block l % 4 only, so it converts one scale a row for four instructions, and its operands of a whole block are 16
 // neighbouring values:
-//   codes   [half: 64 of k][lane][16 bytes: row l / 4, k 0..15 | row l / 4 + 8, k 0..15]
-//   scales  [lane][4 bytes: half 0 row l / 4, row l / 4 + 8 | half 1 likewise]
-// Both are read with one coalesced load a lane.  Negative scales give their sign to their codes when the weight is packed.
+//   codes   [tile][half: 64 of k][lane][16 bytes: row l / 4, k 0..15 | row l / 4 + 8, k 0..15]
+//   scales  [lane][tile][4 bytes: half 0 row l / 4, row l / 4 + 8 | half 1 likewise]
+// A lane reads them with wide loads that no other lane's meet.  Negative scales give their sign to their codes when the weight is packed.
+// Gated: the 16 rows of a tile are eight gate rows and the same eight up rows, so that a lane holds both of a value's products.
 // Behind the units: for each matrix the largest magnitude of code times scale, f32 (two of them, gate rows and up rows, where gated).
 #pragma once
 
@@ -23,15 +24,13 @@
 namespace b200fp4 {
 namespace w4 {
 
-constexpr int kUnitBytes = 1152, kUnitScales = 1024, kUnitK = 128, kTileRows = 16;
+constexpr int kUnitBytes = 2304, kUnitScales = 2048, kUnitK = 128, kUnitRows = 32;
 
-__host__ __device__ __forceinline__ int64_t tiles_of(int64_t rows) { return (rows + kTileRows - 1) / kTileRows; }
+__host__ __device__ __forceinline__ int64_t strips_of(int64_t rows) { return (rows + kUnitRows - 1) / kUnitRows; }      // of 32 rows
 __host__ __device__ __forceinline__ int64_t units_of(int64_t K) { return (K + kUnitK - 1) / kUnitK; }
 
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
-  return *reinterpret_cast<const uint32_t*>(&r);
-}
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 
 // Eight codes -> four pairs of f16
 __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&p)[4]) {
@@ -47,21 +46,16 @@ __device__ __forceinline__ void codes_to_pairs(uint32_t w, uint32_t (&p)[4]) {
       : "r"(w));
 }
 
-// The scales of rows l / 4 (lo) and l / 4 + 8 (hi) for one half of a unit, each twice in a register: a byte's fields, moved to those of f16, are
-// the scale times 2^-8
-__device__ __forceinline__ void scales_of(uint32_t bytes, int half, uint32_t& lo, uint32_t& hi) {
-  const uint32_t raw = prmt(bytes, 0u, half ? 0x3424u : 0x1404u) >> 1;
-  const uint32_t s = mul2(raw, 0x5C005C00u);                  // * 2^8
-  lo = prmt(s, s, 0x1010u);
-  hi = prmt(s, s, 0x3232u);
+// The scales of rows l / 4 (x) and l / 4 + 8 (y) for one half of a unit: a byte's fields, moved to those of f16, are the scale times 2^-8
+__device__ __forceinline__ __half2 scales_of(uint32_t bytes, int half) {
+  return __hmul2(as_half2(prmt(bytes, 0u, half ? 0x3424u : 0x1404u) >> 1), as_half2(0x5C005C00u));
 }
 
 // two bf16 times a power of two (twice in `factor`) -> two f16
 __device__ __forceinline__ uint32_t bf16_to_f16_pair(uint32_t x, uint32_t factor) {
   const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&factor));
   const uint32_t b = *reinterpret_cast<const uint32_t*>(&v);
-  const __half2 h = __floats2half2_rn(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u));
-  return *reinterpret_cast<const uint32_t*>(&h);
+  return as_u32(__floats2half2_rn(__uint_as_float(b << 16), __uint_as_float(b & 0xFFFF0000u)));
 }
 
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {

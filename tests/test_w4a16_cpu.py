@@ -36,8 +36,8 @@ def test_refused_layer_queues_nothing(bad, status):
 
 
 @pytest.mark.parametrize("E,N,K,gated,size", [
-    (1, 1, 16, 0, 1152 + 4), (1, 16, 128, 0, 1152 + 4), (1, 17, 144, 0, 4 * 1152 + 4), (3, 32, 256, 1, 12 * 1152 + 24), (2, 34, 128, 1, 6 * 1152 + 16), (1, 16, 24, 0, 0),
-    (1, 15, 16, 1, 0), (0, 16, 16, 0, 0), (512, 1024, 2048, 1, 512 * 64 * 16 * 1152 + 4096),
+    (1, 1, 16, 0, 2304 + 4), (1, 32, 128, 0, 2304 + 4), (1, 33, 144, 0, 4 * 2304 + 4), (3, 32, 256, 1, 6 * 2304 + 24), (2, 34, 128, 1, 4 * 2304 + 16), (1, 16, 24, 0, 0),
+    (1, 15, 16, 1, 0), (0, 16, 16, 0, 0), (512, 1024, 2048, 1, 512 * 32 * 16 * 2304 + 4096),
 ])
 def test_packed_bytes(E, N, K, gated, size):
     from dgx_vllm_b200 import _lib
