@@ -12,6 +12,7 @@
 // The layer is two launches without anything that has to outlast them: both find the slots from the routing by themselves, the first sets the
 // counters of the second, in which the block that finishes a strip's last item adds up its pairs in their order.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "sm100_ptx.cuh"
@@ -79,159 +80,20 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
 
 // ------------------------------------------------------------------------------------------ products
 
-enum Mode { kLinear, kGateUp, kDown };
-
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
-constexpr int kMaxPairs = 2048;                // pairs whose slots a block finds in its shared memory; more are done in turns
-constexpr int kMaxExperts = 4096;
-
-struct RowsParams {
-  const void* x;              // [M, K], rows ldx apart; down: [pair][upper, lower][K] f16
-  int64_t ldx;
-  const uint8_t* packed;
-  const float* g;             // [E]; gate/up [E][gate, up]
-  void* out;                  // linear [M, N]; down [M, N]
-  const void* bias;           // [N] or null
-  int out_dtype, bias_dtype;
-  int M, N, K;
-  int strips, units;
-  int split;                  // linear: blocks of a cluster, which share the units of an item
-  int cap, rows;              // columns of a slot; rows that there is room for
-  int* status;
-  int clear_status;
-  // layer
-  const int32_t* ids;         // [M, topk]
-  const float* weights;       // [M, topk]
-  const int32_t* map;         // [global_E] or null
-  int64_t global_E;
-  int topk, E, weight_on_input;
-  const float* peaks;         // gate/up [E][gate, up]
-  __half* act;                // gate/up out
-  float* act_inv;             // [pair]: the reciprocal of the factor that brought its row of act into f16's range
-  float* y;                   // down: [pair][N]
-  int* counters;              // [strips of down]
-  int n_counters;
-};
-
-// Shared memory of a block.  Rings of weight units, a warp's its own | their barriers | partial sums, two of them in turn | and for the layer: pairs
-// an expert has, then where they begin | expert of a pair | its place among that expert's | pairs by expert | slots | scan | and where rows are
-// staged: their statistics | parts of those | the rows in f16 | (linear, split) sums of the block's items
-struct Layout {
-  uint32_t bars, red, count, expert, rank, list, slots, scan, stats, parts, rows, sums, bytes;
-};
-struct RowStat {
-  float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
-};
 constexpr uint32_t kSmemMost = 227 * 1024;
+constexpr int kStages = 3;                     // units of a warp's ring
+constexpr uint32_t kRingBytes = kWarps * kStages * kUnitBytes, kBarBytes = kWarps * kStages * 8;
 
 __host__ __device__ __forceinline__ uint32_t pad16(uint32_t v) { return (v + 15) / 16 * 16; }
-// pairs, E: 0 for a linear layer; rows: staged rows of row_bytes each
-__host__ __device__ __forceinline__ Layout layout_of(uint32_t ring, uint32_t bars, uint32_t red, int pairs, int E, int cap, int rows, uint32_t row_bytes,
-                                                      uint32_t sums) {
-  Layout l;
-  l.bars = ring;
-  l.red = pad16(l.bars + bars);
-  l.count = l.red + red;
-  l.expert = l.count + (uint32_t)E * 4;
-  l.rank = pad16(l.expert + (uint32_t)pairs * 2);
-  l.list = pad16(l.rank + (uint32_t)pairs * 2);
-  l.slots = pad16(l.list + (uint32_t)pairs * 2);
-  l.scan = l.slots + (pairs > 0 ? (uint32_t)((pairs < E ? pairs : E) + pairs / cap) * 8 : 0);
-  l.stats = pad16(l.scan + (pairs > 0 ? 2 * kWarps * 4 + 16 : 0));
-  l.parts = l.stats + (uint32_t)rows * sizeof(RowStat);
-  l.rows = pad16(l.parts + (rows > 0 ? kWarps * kWarps * 8 : 0));
-  l.sums = l.rows + (uint32_t)rows * row_bytes;
-  l.bytes = l.sums + sums;
-  return l;
-}
+__host__ __device__ __forceinline__ constexpr uint32_t red_bytes(int cols) { return kWarps * 2 * cols * 4 * 32 * 4; }
 
-__device__ __forceinline__ int local_expert(const RowsParams& p, int pair) {
-  int64_t e = p.ids[pair];
-  if (p.map != nullptr) e = e >= 0 && e < p.global_E ? p.map[e] : -1;
-  return e >= 0 && e < p.E ? (int)e : -1;
-}
-
-// Slots of at most `cap` pairs of one expert, experts in order and pairs in theirs, so that every block finds the same; returns their number.
-// One warp counts, 32 pairs at a time: a few steps for a decode batch, and no order of atomics to depend on.
-__device__ int find_slots(const RowsParams& p, unsigned char* smem, const Layout& l, int cap) {
-  int* const count = reinterpret_cast<int*>(smem + l.count);
-  uint16_t* const expert = reinterpret_cast<uint16_t*>(smem + l.expert);
-  uint16_t* const rank = reinterpret_cast<uint16_t*>(smem + l.rank);
-  uint16_t* const list = reinterpret_cast<uint16_t*>(smem + l.list);
-  int2* const slots = reinterpret_cast<int2*>(smem + l.slots);
-  int* const scan = reinterpret_cast<int*>(smem + l.scan);
-  const int P = p.M * p.topk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int e = threadIdx.x; e < p.E; e += kThreads) count[e] = 0;
-  for (int i = threadIdx.x; i < P; i += kThreads) {
-    const int e = local_expert(p, i);
-    expert[i] = (uint16_t)(e < 0 ? 0xFFFF : e);
-  }
-  __syncthreads();
-  if (warp == 0) {
-    for (int i = lane; i - lane < P; i += 32) {
-      const int e = i < P ? expert[i] : 0xFFFF;
-      const uint32_t same = __match_any_sync(0xffffffffu, e), before = same & ((1u << lane) - 1);
-      const int seen = e != 0xFFFF ? count[e] : 0;
-      __syncwarp();
-      if (e != 0xFFFF) {
-        rank[i] = (uint16_t)(seen + __popc(before));
-        if (before == 0) count[e] = seen + __popc(same);
-      }
-      __syncwarp();
-    }
-  }
-  __syncthreads();
-  // a run of experts a thread: sums, an exclusive scan over the threads, then slots and first places
-  const int per = (p.E + kThreads - 1) / kThreads, e0 = min(p.E, (int)threadIdx.x * per), e1 = min(p.E, e0 + per);
-  int pairs = 0, n = 0;
-  for (int e = e0; e < e1; ++e) {
-    pairs += count[e];
-    n += (count[e] + cap - 1) / cap;
-  }
-  int ip = pairs, in = n;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const int a = __shfl_up_sync(0xffffffffu, ip, d), b = __shfl_up_sync(0xffffffffu, in, d);
-    if (lane >= d) {
-      ip += a;
-      in += b;
-    }
-  }
-  if (lane == 31) {
-    scan[warp] = ip;
-    scan[kWarps + warp] = in;
-  }
-  __syncthreads();
-  int total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) {
-      ip += scan[w];
-      in += scan[kWarps + w];
-    }
-    total += scan[kWarps + w];
-  }
-  int at = ip - pairs, slot = in - n;
-  for (int e = e0; e < e1; ++e) {
-    const int c = count[e];
-    for (int i = 0; i < c; i += cap) slots[slot++] = make_int2(e | (min(cap, c - i) << 16), at + i);
-    count[e] = at;
-    at += c;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < P; i += kThreads)
-    if (expert[i] != 0xFFFF) list[count[expert[i]] + rank[i]] = (uint16_t)i;
-  __syncthreads();
-  return total;
-}
-
-__device__ __forceinline__ uint32_t ldg_stream_u32(const void* p) {
-  uint32_t v;
-  asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(v) : "l"(p));
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint4 ld_u4(const void* p) {      // through L1: the warps of a block share activations
-  return *static_cast<const uint4*>(p);
-}
+__device__ __forceinline__ uint4 ld_u4(const void* p) { return *static_cast<const uint4*>(p); }
 
 __device__ __forceinline__ void store_value(void* out, int dtype, size_t at, float v) {
   if (dtype == B200FP4_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
@@ -244,54 +106,45 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, size_t at)
   return static_cast<const float*>(p)[at];
 }
 
-// ---- powers of two that bring values into f16's range
-
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
-
-// The exponent that brings a row whose largest magnitude has these bf16 bits below 2^15.  Rows with infinities or NaN, which only give such
-// again, take the least that no finite value overflows with.
-__device__ __forceinline__ int row_exponent(uint32_t bits) { return min(141 - min((int)(bits >> 7), 254), 126); }
-
-// Largest magnitude (bf16 bits; bf16 only) and sum of squares (layer only) of elements [k0, k1) of a row, all lanes; k0 and k1 multiples of 8
-template <typename T, bool kSquares>
-__device__ __forceinline__ float2 row_part(const T* row, int k0, int k1) {
-  uint32_t top = 0;
-  float sum = 0.f;
-  for (int k = k0 + (threadIdx.x & 31) * 8; k < k1; k += 256) {
-    const uint4 v = ld_u4(row + k);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (std::is_same<T, __nv_bfloat16>::value) top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
-      if constexpr (kSquares) {
-        float2 f;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
-        else f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-        sum += f.x * f.x + f.y * f.y;
-      }
+// A warp's ring of units: one lane asks for them, all wait for them.  Every unit that was asked for is waited for.
+struct Ring {
+  uint32_t units, bars, stage, phase, fill;
+  bool ok;
+  __device__ __forceinline__ void init(uint32_t base, uint32_t bars_at, int warp, int lane) {
+    units = base + warp * (kStages * kUnitBytes);
+    bars = bars_at + warp * (kStages * 8);
+    stage = phase = fill = 0;
+    ok = true;
+    if (lane < kStages) mbar_init(bars + lane * 8, 1);
+    fence_proxy_async_smem();
+    __syncwarp();
+  }
+  __device__ __forceinline__ void ask(const uint8_t* src, int lane) {
+    if (lane == 0) {
+      mbar_expect_tx(bars + fill * 8, kUnitBytes);
+      bulk_load_1d(units + fill * kUnitBytes, src, kUnitBytes, bars + fill * 8);
+    }
+    if (++fill == kStages) fill = 0;
+  }
+  __device__ __forceinline__ uint32_t wait(int* status) {
+    if (ok) ok = mbar_wait(bars + stage * 8, phase, status, 61);
+    return units + stage * kUnitBytes;
+  }
+  __device__ __forceinline__ void advance() {      // every lane has read the unit
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+    __syncwarp();
+  }
+  // after a wait that ran out: copies that were asked for land before the block's memory goes
+  __device__ __forceinline__ void drain() {
+    if (ok) return;
+    const long long t0 = clock64();
+    while (clock64() - t0 < kWaitCycles / 64) {
     }
   }
-  top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-  if constexpr (kSquares)
-#pragma unroll
-    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-  return make_float2(__uint_as_float(top), sum);
-}
-
-template <int kCols>
-struct Shape {
-  static constexpr int kStages = 3;                            // of a warp's ring
-  static constexpr uint32_t kRing = kWarps * kStages * kUnitBytes;
-  static constexpr uint32_t kBars = kWarps * kStages * 8;
-  static constexpr int kSums = 2 * kCols * 4 * 32;             // of a warp
-  static constexpr uint32_t kRed = kWarps * kSums * 4;
 };
-
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-  return v;
-}
 
 // a unit's 32 rows times kCols columns of eight; b: the columns' operands, [half][column][8]
 template <int kCols>
@@ -322,74 +175,568 @@ __device__ __forceinline__ void multiply_unit(uint32_t unit, int lane, const uin
     }
 }
 
+// columns that are rows in shared memory (f16): lane l's are blocks l % 4 of the unit's two halves
+template <int kCols>
+__device__ __forceinline__ void staged_columns(const uint32_t (&col)[kCols], uint32_t at, uint32_t (&b)[2][kCols][8]) {
+#pragma unroll
+  for (int half = 0; half < 2; ++half)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const uint4 lo = lds128(col[c] + at + half * 128), hi = lds128(col[c] + at + half * 128 + 16);
+      b[half][c][0] = lo.x, b[half][c][1] = lo.y, b[half][c][2] = lo.z, b[half][c][3] = lo.w;
+      b[half][c][4] = hi.x, b[half][c][5] = hi.y, b[half][c][6] = hi.z, b[half][c][7] = hi.w;
+    }
+}
+
+// Warps that share the units of an item, as a power of two, given the block's items and the units of one.  The kernels are bound by the instructions that
+// their warps issue, so the busiest of the SM's four schedulers counts (warp w is with scheduler w % 4): a unit is about 440 cycles of a busy scheduler
+// and 600 of a warp alone, an item's ending a third of one where a warp has the item for itself and half of one for each warp that shares it.
+inline float share_cost(int items, int units, int log_share) {
+  const int share = 1 << log_share, rounds = ((items << log_share) + kWarps - 1) / kWarps, schedulers = share < 4 ? 4 / share : 1;
+  const float item = (float)((units + share - 1) / share) + (log_share == 0 ? 0.33f : 0.5f);
+  const float busy = (float)((items + schedulers - 1) / schedulers) * (share > 4 ? share / 4 : 1) * item, alone = rounds * item * 1.4f;
+  return busy > alone ? busy : alone;
+}
+inline int share_of(int items, int units) {
+  int log_share = 0;
+  for (int s = 1; s < 5 && (1 << s) <= units; ++s)
+    if (share_cost(items, units, s) < share_cost(items, units, log_share)) log_share = s;
+  return log_share;
+}
+
+// Sums of the warps that share an item, [warp][tile][column of eight][j][lane]: each warp adds up some of them, in the order of k, and finishes them.
+// A lane's sums j are row l / 4 (0, 1) or l / 4 + 8 (2, 3) of a tile and columns 2 (l % 4) and the next one; finish gets those of j = kFirst[i] and
+// kSecond[i].  Both barriers are the group's.
+template <int kCols, bool kAcross, typename F>
+__device__ __forceinline__ void finish_item(float* red, int share, int in_group, int group, int lane, const float (&acc)[2][kCols][4], F&& finish) {
+  // kAcross: the pair is the two columns of one row (j, j + 1), otherwise the two rows of one column (j, j + 2)
+  constexpr int kSums = 2 * kCols * 4 * 32;
+  if (share == 1) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int c = 0; c < kCols; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) finish(t, c, i, acc[t][c][kAcross ? 2 * i : i], acc[t][c][kAcross ? 2 * i + 1 : i + 2]);
+    return;
+  }
+  float* const own = red + group * share * kSums + lane;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) own[in_group * kSums + ((t * kCols + c) * 4 + j) * 32] = acc[t][c][j];
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
+  for (int u = in_group; u < 4 * kCols; u += share) {
+    const int i = u & 1, tc = u >> 1;
+    const float *a = own + (tc * 4 + (kAcross ? 2 * i : i)) * 32, *b = a + (kAcross ? 32 : 64);
+    float va = 0.f, vb = 0.f;
+#pragma unroll 4
+    for (int w = 0; w < share; ++w) {
+      va += a[w * kSums];
+      vb += b[w * kSums];
+    }
+    finish(kCols == 1 ? tc : tc / kCols, kCols == 1 ? 0 : tc % kCols, i, va, vb);
+  }
+  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
+}
+
+// ---- powers of two that bring values into f16's range
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
+
+// The exponent that brings a row whose largest magnitude has these bf16 bits below 2^15.  Rows with infinities or NaN, which only give such
+// again, take the least that no finite value overflows with.
+__device__ __forceinline__ int row_exponent(uint32_t bits) { return min(141 - min((int)(bits >> 7), 254), 126); }
+
+// Largest magnitude (as bf16 bits, two of them; bf16 only) and sum of squares (kSquares) of eight elements, added to what there is
+template <typename T, bool kSquares>
+__device__ __forceinline__ void look_at(const uint4& v, uint32_t& top, float& sum) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) top = __vmaxu2(top, w[j] & 0x7FFF7FFFu);
+    if constexpr (kSquares) {
+      float2 f;
+      if constexpr (std::is_same<T, __nv_bfloat16>::value) f = make_float2(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xFFFF0000u));
+      else f = __half22float2(as_half2(w[j]));
+      sum += f.x * f.x + f.y * f.y;
+    }
+  }
+}
+
+// Rows [0, n_rows) -> f16 in shared memory, row_bytes apart, elements [k_begin, k_end) and zeros up to k_stop; all threads.  row_at(r): the row's
+// elements; seen(r, factor's reciprocal, sum of squares): called once a row.  Few rows are shared by several warps.
+template <typename T, bool kSquares, typename RowAt, typename Seen>
+__device__ __forceinline__ void stage_rows(int n_rows, int k_begin, int k_end, int k_stop, unsigned char* rows, uint32_t row_bytes, float2* parts, RowAt&& row_at,
+                                           Seen&& seen) {
+  constexpr bool kConvert = std::is_same<T, __nv_bfloat16>::value;
+  constexpr int kHeld = 4;                         // pieces that a lane keeps between looking at them and writing them; others are read again
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int log_parts = 4;
+  while (log_parts > 0 && (n_rows << log_parts) > kWarps) --log_parts;
+  const int n_parts = 1 << log_parts, octets = (k_end - k_begin) >> 3;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n_rows << log_parts; i0 += kWarps) {
+    const int r = (i0 + warp) >> log_parts, part = (i0 + warp) & (n_parts - 1);
+    const bool work = r < n_rows;
+    const int k0 = k_begin + ((octets * part) >> log_parts) * 8 + lane * 8, k1 = work ? k_begin + ((octets * (part + 1)) >> log_parts) * 8 : 0;
+    const T* const row = work ? row_at(r) : nullptr;
+    uint4 held[kHeld];
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+      if (k0 + h * 256 < k1) held[h] = ld_u4(row + k0 + h * 256);
+    uint32_t factor = 0;
+    float inv = 1.f, squares = 0.f;
+    if constexpr (kConvert || kSquares) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h)
+        if (k0 + h * 256 < k1) look_at<T, kSquares>(held[h], top, squares);
+#pragma unroll 2
+      for (int k = k0 + kHeld * 256; k < k1; k += 256) look_at<T, kSquares>(ld_u4(row + k), top, squares);
+      top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+      if constexpr (kSquares)
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+      if (n_parts > 1) {                           // one round then
+        if (lane == 0) parts[warp] = make_float2(__uint_as_float(top), squares);
+        __syncthreads();
+        squares = 0.f;
+        for (int j = 0; j < n_parts; ++j) {        // in the same order for every warp of the row
+          const float2 u = parts[warp - part + j];
+          top = max(top, __float_as_uint(u.x));
+          squares += u.y;
+        }
+      }
+      const int e = kConvert ? row_exponent(top) : 0;
+      factor = (uint32_t)(e + 127) * 0x00800080u;
+      inv = pow2(-e);
+    }
+    if (work) {
+      unsigned char* const to = rows + r * row_bytes - k_begin * 2;
+      auto put = [&](int k, uint4 v) {
+        if constexpr (kConvert)
+          v = make_uint4(bf16_to_f16_pair(v.x, factor), bf16_to_f16_pair(v.y, factor), bf16_to_f16_pair(v.z, factor), bf16_to_f16_pair(v.w, factor));
+        *reinterpret_cast<uint4*>(to + k * 2) = v;
+      };
+#pragma unroll
+      for (int h = 0; h < kHeld; ++h)
+        if (k0 + h * 256 < k1) put(k0 + h * 256, held[h]);
+#pragma unroll 2
+      for (int k = k0 + kHeld * 256; k < k1; k += 256) put(k, ld_u4(row + k));
+      if (part == n_parts - 1)
+        for (int k = k_end + lane * 8; k < k_stop; k += 256) *reinterpret_cast<uint4*>(to + k * 2) = make_uint4(0, 0, 0, 0);
+      if constexpr (kConvert || kSquares)
+        if (part == 0 && lane == 0) seen(r, inv, squares);
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------ linear layer of few tokens
+
+constexpr int kMaxSplit = 8;
+
+struct LinearParams {
+  const void* x;              // [M, K], rows ldx apart
+  int64_t ldx;
+  const uint8_t* packed;
+  const float* g;
+  void* out;                  // [M, N]
+  const void* bias;           // [N] or null
+  int out_dtype, bias_dtype;
+  int M, N, K;
+  int strips, units;
+  int split;                  // blocks of a cluster, which share the units of an item
+  int cap;                    // columns of an item
+  int per, more;              // items of a cluster: `per`, and one more for the first `more` clusters
+  int log_share;
+  int* status;
+};
+
+// Shared memory behind the rings and barriers: partial sums of warps | factors' reciprocals | parts of the rows' statistics | rows in f16 | sums of a
+// cluster's items, [source block][value], of this block's share of the values
+struct LinearLayout {
+  uint32_t red, inv, parts, rows, sums, bytes;
+};
+__host__ __device__ __forceinline__ LinearLayout linear_layout(int cols, int cap, uint32_t row_bytes, int split, int items) {
+  LinearLayout l;
+  l.red = pad16(kRingBytes + kBarBytes);
+  l.inv = l.red + red_bytes(cols);
+  l.parts = pad16(l.inv + (uint32_t)cap * 4);
+  l.rows = l.parts + kWarps * 8;
+  l.sums = l.rows + (uint32_t)cap * row_bytes;
+  // strips of an item are 32 rows: each block of the cluster finishes 32 / split of them
+  l.bytes = l.sums + (split > 1 ? (uint32_t)items * cap * 32 * 4 : 0);
+  return l;
+}
+
 // XT: type of the activations; kCols: columns of eight
-template <typename XT, int kMode, int kCols>
-__global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParams p) {
+template <typename XT, int kCols>
+__global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
-  using S = Shape<kCols>;
   constexpr bool kConvert = std::is_same<XT, __nv_bfloat16>::value;
-  constexpr bool kStaged = kMode != kDown;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
-  const int cap = p.cap, split = kMode == kLinear ? p.split : 1;
-  const int rank = kMode == kLinear ? (int)(blockIdx.x % (unsigned)split) : 0;
-  const int unit_first = p.units * rank / split, unit_last = p.units * (rank + 1) / split, own_units = unit_last - unit_first;
+  const uint32_t base = smem_u32(smem);
+  Ring ring;
+  ring.init(base, base + kRingBytes, warp, lane);
+  const int split = p.split, rank = (int)blockIdx.x & (split - 1), cluster = (int)blockIdx.x / split;      // split: a power of two
+  const int unit_first = p.units * rank / split, own_units = p.units * (rank + 1) / split - unit_first;
+  const int share = 1 << p.log_share, group = warp >> p.log_share, in_group = warp & (share - 1), n_groups = kWarps >> p.log_share;
+  const int k_first = (own_units * in_group) >> p.log_share, n_units = ((own_units * (in_group + 1)) >> p.log_share) - k_first;
+  const int first = cluster * p.per + min(cluster, p.more), last = first + p.per + (cluster < p.more ? 1 : 0);
+  // Strips of a slot of tokens are neighbours
+  int ahead = first + group, ahead_left = 0;
+  const uint8_t* src = nullptr;
+  auto fetch = [&]() {
+    if (ahead_left == 0) {
+      if (ahead >= last) return;
+      src = p.packed + ((size_t)(ahead % p.strips) * p.units + unit_first + k_first) * kUnitBytes;
+      ahead_left = n_units;
+      ahead += n_groups;
+    }
+    ring.ask(src, lane);
+    src += kUnitBytes;
+    --ahead_left;
+  };
+  pdl_wait();
+#pragma unroll 1
+  for (int i = 0; i < kStages; ++i) fetch();
+  pdl_launch_dependents();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
+  if (split > 1) cluster_arrive();                 // the other blocks run before anything is sent to them
   // rows are shifted by 16 bytes against each other: no two lanes of a load meet
   const uint32_t row_bytes = (uint32_t)((p.units + split - 1) / split) * (kUnitK * 2) + 16;
-  const Layout l = layout_of(S::kRing, S::kBars, S::kRed, kMode == kLinear ? 0 : p.M * p.topk, kMode == kLinear ? 0 : p.E, cap, p.rows, row_bytes, 0);
+  const LinearLayout l = linear_layout(kCols, p.cap, row_bytes, split, p.per + (p.more > 0));
+  float* const inv = reinterpret_cast<float*>(smem + l.inv);
+  const float g = *p.g;
+  bool arrived = split == 1;
+  int item = first + group;
+  for (int done = first; done < last;) {
+    // one slot of tokens at a time
+    const int slot = done / p.strips, m0 = slot * p.cap, n = min(p.cap, p.M - m0), end = min(last, (slot + 1) * p.strips);
+    if (done > first) __syncthreads();             // nobody reads the rows before these any more
+    stage_rows<XT, false>(n, unit_first * kUnitK, min(p.K, (unit_first + own_units) * kUnitK), (unit_first + own_units) * kUnitK, smem + l.rows, row_bytes,
+                          reinterpret_cast<float2*>(smem + l.parts), [&](int r) { return static_cast<const XT*>(p.x) + (m0 + r) * p.ldx; },
+                          [&](int r, float v, float) { inv[r] = v; });
+    __syncthreads();
+    uint32_t col[kCols];
+#pragma unroll
+    for (int c = 0; c < kCols; ++c) {
+      const int i = c * 8 + row8;                  // columns past the tokens read the first one's row: nobody reads their sums
+      col[c] = base + l.rows + (i < n ? i : 0) * row_bytes + quad * 32;
+    }
+    for (; item < end; item += n_groups) {
+      float acc[2][kCols][4] = {};
+#pragma unroll 1
+      for (int k = k_first; k < k_first + n_units; ++k) {
+        uint32_t b[2][kCols][8];
+        staged_columns<kCols>(col, k * (kUnitK * 2), b);
+        multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+        ring.advance();
+        if (ring.ok) fetch();
+      }
+      if (!arrived) {
+        cluster_wait();
+        arrived = true;
+      }
+      const int strip = item - slot * p.strips;
+      finish_item<kCols, false>(reinterpret_cast<float*>(smem + l.red), share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb) {
+        const int column = c * 8 + quad * 2 + i, row = t * 16 + row8;
+        if (column >= n) return;
+        const float f = kConvert ? inv[column] : 1.f;
+        if (split > 1) {
+          // value [row of the strip] is finished by block row / (32 / split): [source][item][column][its rows]
+          const int rows = 32 / split;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int at = row + h * 8, owner = at / rows;
+            const uint32_t to = base + l.sums + (((uint32_t)(rank * (p.per + (p.more > 0)) + item - first) * p.cap + column) * rows + at - owner * rows) * 4;
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(to, owner)), "f"((h ? vb : va) * f) : "memory");
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int at = strip * 32 + row + h * 8;
+            if (at < p.N) {
+              float v = (h ? vb : va) * f * g;
+              if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, at);
+              store_value(p.out, p.out_dtype, (size_t)(m0 + column) * p.N + at, v);
+            }
+          }
+        }
+      });
+    }
+    done = end;
+  }
+  ring.drain();
+  if (split > 1) {
+    if (!arrived) cluster_wait();
+    cluster_sync_any();                            // the parts of k have arrived; they are added in their order
+    const int rows = 32 / split, items = p.per + (p.more > 0), count = (last - first) * p.cap * rows;
+    const float* const sums = reinterpret_cast<const float*>(smem + l.sums);
+    for (int i = threadIdx.x; i < count; i += kThreads) {
+      const int r = i & (rows - 1), ic = i / rows, it = first + ic / p.cap, column = ic % p.cap;
+      const int slot = it / p.strips, row = (it - slot * p.strips) * 32 + rank * rows + r, m = slot * p.cap + column;
+      if (m >= p.M || row >= p.N) continue;
+      float v = 0.f;
+      for (int s = 0; s < split; ++s) v += sums[s * items * p.cap * rows + i];
+      v *= g;
+      if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
+      store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
+    }
+  }
+}
+
+template <typename Kernel>
+bool allow_smem(Kernel kernel, std::once_flag (&once)[64], bool (&ready)[64]) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  std::call_once(once[dev], [&] {
+    ready[dev] = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost) == cudaSuccess;
+    cudaGetLastError();
+  });
+  return ready[dev];
+}
+
+template <typename XT, int kCols>
+int launch_linear_of(LinearParams p, cudaStream_t st) {
+  static std::once_flag once[64];
+  static bool ready[64];
+  static ResidentClusters counts[kMaxSplit + 1][64];
+  if (!allow_smem(w4a16_linear_kernel<XT, kCols>, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
+  // Blocks that share the k of an item in a cluster: a shorter k leaves room for more rows, and few strips reach all SMs
+  float best = 1e30f;
+  unsigned grid = 0;
+  uint32_t smem = 0;
+  LinearParams chosen = p;
+  for (int split = 1; split <= kMaxSplit && split <= p.units; split *= 2) {
+    const int clusters = split == 1 ? sm_count() : resident_clusters_of(counts[split], w4a16_linear_kernel<XT, kCols>, split, kThreads, kSmemMost);
+    if (clusters < 1) break;
+    const int own = (p.units + split - 1) / split;
+    const uint32_t row_bytes = (uint32_t)own * (kUnitK * 2) + 16;
+    for (int cap = std::min(8 * kCols, p.M); cap > 0; cap /= 2) {
+      const int64_t items = (int64_t)((p.M + cap - 1) / cap) * p.strips;
+      if (items > 0x3FFFFFFF) break;
+      const int used = (int)std::min<int64_t>(clusters, items), most = (int)((items + used - 1) / used);
+      const uint64_t bytes = (uint64_t)linear_layout(kCols, cap, row_bytes, 1, 0).bytes + (split > 1 ? (uint64_t)most * cap * 128 : 0);
+      if ((uint64_t)own * 256 > kSmemMost || bytes > kSmemMost) continue;
+      // the busiest block's units; a cluster's exchange costs about as much as two
+      const int log_share = share_of(most, p.units / split);
+      const float cost = share_cost(most, own, log_share) + (split > 1 ? 2.f : 0.f);
+      if (cost < best) {
+        best = cost;
+        chosen.split = split;
+        chosen.cap = cap;
+        chosen.per = (int)(items / used);
+        chosen.more = (int)(items % used);
+        chosen.log_share = log_share;
+        grid = (unsigned)(used * split);
+        smem = (uint32_t)bytes;
+      }
+      break;
+    }
+  }
+  if (grid == 0) return B200FP4_STATUS_NOT_SUPPORTED;
+  if (launch_pdl_cluster(chosen.split, w4a16_linear_kernel<XT, kCols>, dim3(grid), dim3(kThreads), smem, st, chosen) != cudaSuccess) {
+    cudaGetLastError();
+    return B200FP4_STATUS_EXECUTION_FAILED;
+  }
+  return finish_launch(1);
+}
+
+template <typename T>
+int launch_linear(const LinearParams& p, cudaStream_t st) {
+  return p.M <= 8 ? launch_linear_of<T, 1>(p, st) : launch_linear_of<T, 2>(p, st);
+}
+
+// ------------------------------------------------------------------------------------------ mixture of experts
+
+constexpr int kMaxPairs = 2048;                // pairs whose slots a block finds in its shared memory; more are done in turns
+constexpr int kMaxExperts = 4096;
+
+struct MoeParams {
+  const void* x;              // gate/up [M, K], rows ldx apart; down: [pair][upper, lower][K] f16
+  int64_t ldx;
+  const uint8_t* packed;
+  const float* g;             // [E]; gate/up [E][gate, up]
+  const float* peaks;         // gate/up: [E][gate, up]
+  int M, N, K;
+  int strips, units;
+  int cap, rows;              // columns of a slot; rows that there is room for
+  int log_share;
+  const int32_t* ids;         // [M, topk]
+  const float* weights;       // [M, topk]
+  const int32_t* map;         // [global_E] or null
+  int64_t global_E;
+  int topk, E, weight_on_input;
+  __half* act;                // gate/up out
+  float* act_inv;             // [pair]: the reciprocal of the factor that brought its row of act into f16's range
+  float* y;                   // down: [pair][N]
+  int* counters;              // [strips of down]
+  int n_counters;
+  void* out;                  // down [M, N]
+  int out_dtype;
+  int* status;
+  int clear_status;
+};
+
+struct RowStat {
+  float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
+};
+// Shared memory behind the rings and barriers: partial sums of warps | expert of a pair | pairs by expert | first place of an expert | slots | scan | routing
+// weights (down) | statistics of the staged rows | parts of those | the rows in f16, and before them the counts
+struct MoeLayout {
+  uint32_t red, expert, list, start, slots, scan, weights, stats, parts, rows, bytes;
+};
+// Bytes of an expert in the table of counts: one for each 32 pairs
+__host__ __device__ __forceinline__ int count_bytes(int pairs) { return (pairs + 511) / 512 * 16; }
+__host__ __device__ __forceinline__ MoeLayout moe_layout(int cols, int pairs, int E, int cap, int rows, uint32_t row_bytes) {
+  MoeLayout l;
+  l.red = pad16(kRingBytes + kBarBytes);
+  l.expert = l.red + red_bytes(cols);
+  l.list = pad16(l.expert + (uint32_t)pairs * 2);
+  l.start = pad16(l.list + (uint32_t)pairs * 2);
+  l.slots = pad16(l.start + (uint32_t)E * 2);
+  l.scan = pad16(l.slots + (uint32_t)((pairs < E ? pairs : E) + pairs / cap) * 8);
+  l.weights = l.scan + kWarps * 4;
+  l.stats = pad16(l.weights + (rows > 0 ? 0 : (uint32_t)pairs * 4));
+  l.parts = pad16(l.stats + (uint32_t)rows * sizeof(RowStat));
+  l.rows = l.parts + kWarps * 8;
+  const uint32_t counts = (uint32_t)E * count_bytes(pairs), staged = (uint32_t)rows * row_bytes;
+  l.bytes = l.rows + (counts > staged ? counts : staged);
+  return l;
+}
+
+__device__ __forceinline__ int local_expert(const MoeParams& p, int pair) {
+  int64_t e = p.ids[pair];
+  if (p.map != nullptr) e = e >= 0 && e < p.global_E ? p.map[e] : -1;
+  return e >= 0 && e < p.E ? (int)e : -1;
+}
+
+// Counts to zero; needs nothing of the call's inputs
+__device__ __forceinline__ void clear_counts(const MoeParams& p, unsigned char* smem, const MoeLayout& l) {
+  for (int i = threadIdx.x; i < p.E * count_bytes(p.M * p.topk) / 16; i += kThreads) *reinterpret_cast<uint4*>(smem + l.rows + i * 16) = make_uint4(0, 0, 0, 0);
+}
+
+// Slots (expert | pairs << 16, first place in the list): runs of at most `cap` pairs of one expert, pairs in their order.  Every block finds the same ones,
+// whatever the order in which its threads run; returns their number.  A warp takes 32 pairs at a time and counts those of the same expert among them
+// into a table [expert][32 pairs]; a pair's place is the sum of its expert's counts before its own 32 and its place among those.
+__device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* smem, const MoeLayout& l) {
+  constexpr int kMost = kMaxPairs / kThreads;
+  const int cap = p.cap, P = p.M * p.topk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bytes = count_bytes(P);
+  uint16_t* const expert = reinterpret_cast<uint16_t*>(smem + l.expert);
+  uint16_t* const list = reinterpret_cast<uint16_t*>(smem + l.list);
+  uint16_t* const start = reinterpret_cast<uint16_t*>(smem + l.start);
+  int2* const slots = reinterpret_cast<int2*>(smem + l.slots);
+  uint32_t* const scan = reinterpret_cast<uint32_t*>(smem + l.scan);
+  int e[kMost], place[kMost];
+  uint32_t leads[kMost];                           // the first pair of an expert: its pairs | its slots << 16
+#pragma unroll
+  for (int q = 0; q < kMost; ++q) {
+    const int i = q * kThreads + threadIdx.x;
+    e[q] = i < P ? local_expert(p, i) : -1;
+    if (i < P) expert[i] = (uint16_t)e[q];
+  }
+  __syncthreads();                                 // the counts are clear
+#pragma unroll
+  for (int q = 0; q < kMost; ++q) {
+    if (q * kThreads >= P) break;
+    const uint32_t same = __match_any_sync(0xffffffffu, e[q]), before = same & ((1u << lane) - 1);
+    place[q] = __popc(before);
+    if (e[q] >= 0 && before == 0) smem[l.rows + e[q] * bytes + q * kWarps + warp] = (unsigned char)__popc(same);
+  }
+  __syncthreads();
+  uint32_t mine = 0;
+#pragma unroll
+  for (int q = 0; q < kMost; ++q) {
+    leads[q] = 0;
+    if (q * kThreads >= P || e[q] < 0) continue;
+    uint32_t before = 0, all = 0;
+    const int at = q * kWarps + warp;              // this pair's 32
+    for (int w = 0; w < bytes / 4; ++w) {
+      const uint32_t c = *reinterpret_cast<const uint32_t*>(smem + l.rows + e[q] * bytes + w * 4);
+      all = __dp4a(c, 0x01010101u, all);
+      const int ahead = at - w * 4;                // bytes of this word that count pairs before
+      if (ahead > 0) before = __dp4a(ahead >= 4 ? c : c & ((1u << (ahead * 8)) - 1), 0x01010101u, before);
+    }
+    place[q] += before;
+    if (place[q] == 0) leads[q] = all | ((all + cap - 1) / cap << 16);
+    mine += leads[q];
+  }
+  // pairs and slots before this thread's: an exclusive scan
+  uint32_t sum = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const uint32_t a = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += a;
+  }
+  if (lane == 31) scan[warp] = sum;
+  __syncthreads();
+  uint32_t warps = lane < kWarps ? scan[lane] : 0;
+#pragma unroll
+  for (int d = 1; d < kWarps; d *= 2) {
+    const uint32_t a = __shfl_up_sync(0xffffffffu, warps, d);
+    if (lane >= d) warps += a;
+  }
+  const uint32_t others = __shfl_sync(0xffffffffu, warps, warp > 0 ? warp - 1 : 0);
+  const int total = (int)(__shfl_sync(0xffffffffu, warps, kWarps - 1) >> 16);
+  uint32_t at = sum - mine + (warp > 0 ? others : 0);
+#pragma unroll
+  for (int q = 0; q < kMost; ++q) {
+    if (leads[q] == 0) continue;
+    const int pairs = leads[q] & 0xFFFF, first = at & 0xFFFF;
+    int slot = at >> 16;
+    start[e[q]] = (uint16_t)first;
+    for (int c = 0; c < pairs; c += cap) slots[slot++] = make_int2(e[q] | (min(cap, pairs - c) << 16), first + c);
+    at += leads[q];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kMost; ++q)
+    if (q * kThreads < P && e[q] >= 0) list[start[e[q]] + place[q]] = (uint16_t)(q * kThreads + threadIdx.x);
+  __syncthreads();
+  return total;
+}
+
+// XT: type of the activations (gate/up); kDown: the second projection; kCols: columns of eight
+template <typename XT, bool kDown, int kCols>
+__global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
   const uint32_t base = smem_u32(smem);
+  const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;      // rows are shifted by 16 bytes against each other: no two lanes of a load meet
+  const MoeLayout l = moe_layout(kCols, p.M * p.topk, p.E, p.cap, p.rows, row_bytes);
+  const uint16_t* const expert = reinterpret_cast<const uint16_t*>(smem + l.expert);
   const int2* const slots = reinterpret_cast<const int2*>(smem + l.slots);
   const uint16_t* const list = reinterpret_cast<const uint16_t*>(smem + l.list);
-  const uint32_t ring = base + warp * (S::kStages * kUnitBytes), bars = base + l.bars + warp * (S::kStages * 8);
-  if (lane < S::kStages) mbar_init(bars + lane * 8, 1);
-  fence_proxy_async_smem();
-  __syncwarp();
-  pdl_wait();
-  pdl_launch_dependents();
-  int n_slots;
-  if constexpr (kMode == kLinear) {
-    n_slots = (p.M + cap - 1) / cap;
-    if (p.clear_status && blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
+  Ring ring;
+  ring.init(base, base + kRingBytes, warp, lane);
+  // The routing is not the first projection's work, and its kernel lets this one start only once what came before it is complete: the second
+  // projection finds its slots and asks for its first weights while the first one ends.
+  clear_counts(p, smem, l);
+  if (!kDown) {
+    pdl_wait();
+    pdl_launch_dependents();
   } else {
-    n_slots = find_slots(p, smem, l, cap);
-    if (kMode == kGateUp && blockIdx.x == 0) {
-      if (p.clear_status && threadIdx.x == 0) *p.status = 0;
-      for (int i = threadIdx.x; i < p.n_counters; i += kThreads) p.counters[i] = 0;
-    }
-    if (kMode == kDown && n_slots == 0) {
-      for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < (size_t)p.M * p.N; i += (size_t)gridDim.x * kThreads)
-        store_value(p.out, p.out_dtype, i, 0.f);
-      return;
-    }
+    for (int i = threadIdx.x; i < p.M * p.topk; i += kThreads)
+      reinterpret_cast<float*>(smem + l.weights)[i] = p.weight_on_input ? 1.f : p.weights[i];
   }
-  // Items of a slot are neighbours, or (down) those of a strip
-  const int fast = kMode == kDown ? n_slots : p.strips;
-  const int64_t n_items = (int64_t)n_slots * p.strips;
-  const unsigned cluster = blockIdx.x / (unsigned)split, clusters = gridDim.x / (unsigned)split;
-  const int first = (int)(n_items * cluster / clusters), last = (int)(n_items * (cluster + 1) / clusters);
-  const int n_block = last - first;
-
-  // Warps that share an item.  Busy warps take a unit in about 110 cycles of the SM, a warp alone in 350; an item's ending costs a warp that shares it
-  // about half a unit.
-  int share = 1, best = 0x7FFFFFFF;
-  for (int s = 1; s <= kWarps && s <= own_units; s *= 2) {
-    const int busy = n_block * (2 * own_units + s), alone = (n_block * s + kWarps - 1) / kWarps * ((own_units + s - 1) / s + 1) * 7;
-    const int cost = busy > alone ? busy : alone;
-    if (cost < best) {
-      best = cost;
-      share = s;
-    }
-  }
-  const int group = warp / share, in_group = warp - group * share, n_groups = kWarps / share;
-  const int k_first = unit_first + own_units * in_group / share, k_last = unit_first + own_units * (in_group + 1) / share;
+  const int n_slots = find_slots(p, smem, l);
+  // Items (strip, slot) of a slot are neighbours, or (down) those of a strip
+  const int fast = kDown ? n_slots : p.strips, n_items = n_slots * p.strips, per = n_items / (int)gridDim.x, more = n_items - per * (int)gridDim.x;
+  const int first = (int)blockIdx.x * per + min((int)blockIdx.x, more), last = first + per + ((int)blockIdx.x < more ? 1 : 0);
+  const int share = 1 << p.log_share, group = warp >> p.log_share, in_group = warp & (share - 1), n_groups = kWarps >> p.log_share;
+  const int k_first = (p.units * in_group) >> p.log_share, n_units = ((p.units * (in_group + 1)) >> p.log_share) - k_first;
 
   struct Cursor {
     int item, hi, lo;         // hi * fast + lo
   };
-  auto start = [&](Cursor& c) {
-    c.item = first + group;
-    c.hi = c.item / fast;
-    c.lo = c.item - c.hi * fast;
-  };
+  Cursor at = {first + group, 0, 0};
+  if (fast > 0) at.hi = at.item / fast;
+  at.lo = at.item - at.hi * fast;
+  Cursor ahead = at;
   auto next = [&](Cursor& c) {
     c.item += n_groups;
     c.lo += n_groups;
@@ -398,309 +745,198 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
       ++c.hi;
     }
   };
-  auto slot_of = [&](const Cursor& c) { return kMode == kDown ? c.lo : c.hi; };
-  auto strip_of = [&](const Cursor& c) { return kMode == kDown ? c.hi : c.lo; };
-
-  // ---- the ring: one lane asks for the units, all wait for them
-  Cursor ahead;
-  start(ahead);
   int ahead_left = 0;
-  uint32_t fill = 0;
   const uint8_t* src = nullptr;
   auto fetch = [&]() {
     if (ahead_left == 0) {
       if (ahead.item >= last) return;
-      const size_t e = kMode == kLinear ? 0 : slots[slot_of(ahead)].x & 0xFFFF;
-      src = p.packed + ((e * p.strips + strip_of(ahead)) * p.units + k_first) * kUnitBytes;
-      ahead_left = k_last - k_first;
+      const size_t e = slots[kDown ? ahead.lo : ahead.hi].x & 0xFFFF;
+      src = p.packed + ((e * p.strips + (kDown ? ahead.hi : ahead.lo)) * p.units + k_first) * kUnitBytes;
+      ahead_left = n_units;
       next(ahead);
     }
-    if (lane == 0) {
-      mbar_expect_tx(bars + fill * 8, kUnitBytes);
-      bulk_load_1d(ring + fill * kUnitBytes, src, kUnitBytes, bars + fill * 8);
-    }
+    ring.ask(src, lane);
     src += kUnitBytes;
     --ahead_left;
-    if (++fill == S::kStages) fill = 0;
   };
-  for (int i = 0; i < S::kStages; ++i) fetch();
+#pragma unroll 1
+  for (int i = 0; i < kStages; ++i) fetch();
+  float* const red = reinterpret_cast<float*>(smem + l.red);
 
-  Cursor at;
-  start(at);
-  uint32_t stage = 0, phase = 0;
-  bool ok = true;
-  // Rows are staged for as many slots at a time as there is room for
-  int slot = kStaged && n_block > 0 ? first / fast : 0;
-  for (int end = first; end < last;) {
-    int row0 = 0;
-    if constexpr (!kStaged) {
-      end = last;
-    } else {
-      // slots [slot, stop), rows [row0, row0 + n_rows) of the tokens or of the pairs by expert
-      const int slots_end = (last - 1) / fast + 1;
-      int stop = slot + 1, n_rows;
-      if constexpr (kMode == kLinear) {
-        row0 = slot * cap;
-        n_rows = min(cap, p.M - row0);
-      } else {
-        row0 = slots[slot].y;
-        n_rows = slots[slot].x >> 16;
-        while (stop < slots_end && n_rows + (slots[stop].x >> 16) <= p.rows) n_rows += slots[stop++].x >> 16;
-      }
+  if constexpr (!kDown) {
+    if (blockIdx.x == 0) {
+      if (p.clear_status && threadIdx.x == 0) *p.status = 0;
+      for (int i = threadIdx.x; i < p.n_counters; i += kThreads) p.counters[i] = 0;
+    }
+    RowStat* const stats = reinterpret_cast<RowStat*>(smem + l.stats);
+    // Rows are staged for as many slots at a time as there is room for: slots [slot, stop), the pairs in places [row0, row0 + n_rows) of the list
+    int slot = last > first ? first / fast : 0;
+    for (int end = first; end < last;) {
+      const int slots_end = (last - 1) / fast + 1, row0 = slots[slot].y;
+      int stop = slot + 1, n_rows = slots[slot].x >> 16;
+      while (stop < slots_end && n_rows + (slots[stop].x >> 16) <= p.rows) n_rows += slots[stop++].x >> 16;
+      if (end > first) __syncthreads();            // nobody reads the rows before these any more
       end = min(last, stop * fast);
       slot = stop;
-      auto row_at = [&](int r) {
-        const int64_t row = kMode == kLinear ? row0 + r : list[row0 + r] / p.topk;
-        return static_cast<const XT*>(p.x) + row * p.ldx;
-      };
-      RowStat* const stats = reinterpret_cast<RowStat*>(smem + l.stats);
-      float2* const parts = reinterpret_cast<float2*>(smem + l.parts);
-      // few rows: several warps a row
-      int n_parts = kWarps;
-      while (n_parts > 1 && n_parts * n_rows > kWarps) n_parts /= 2;
-      const int k_begin = unit_first * kUnitK, k_end = min(p.K, unit_last * kUnitK), octets = (k_end - k_begin) / 8;
-      __syncthreads();                             // nobody reads the rows before these any more
-      for (int i0 = 0; i0 < n_rows * n_parts; i0 += kWarps) {
-        const int i = i0 + warp, r = i / n_parts, part = i - r * n_parts;
-        const int k0 = k_begin + octets * part / n_parts * 8, k1 = k_begin + octets * (part + 1) / n_parts * 8;
-        const bool work = r < n_rows;
-        uint32_t factor = 0;
-        if constexpr (kConvert || kMode == kGateUp) {
-          float2 v = make_float2(0.f, 0.f);
-          if (work) v = row_part<XT, kMode == kGateUp>(row_at(r), k0, k1);
-          if (n_parts > 1) {
-            if (work && lane == 0) parts[r * n_parts + part] = v;
-            __syncthreads();
-            if (work) {
-              v = make_float2(0.f, 0.f);
-              for (int j = 0; j < n_parts; ++j) {
-                const float2 u = parts[r * n_parts + j];
-                v.x = __uint_as_float(max(__float_as_uint(v.x), __float_as_uint(u.x)));
-                v.y += u.y;
-              }
-            }
-          }
-          if (work) {
-            const int e = kConvert ? row_exponent(__float_as_uint(v.x)) : 0;
-            factor = (uint32_t)(e + 127) * 0x00800080u;
-            if (part == 0 && lane == 0) {
-              RowStat st = {pow2(-e), 0.f};
-              if constexpr (kMode == kGateUp) {
-                // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the
-                // bound is far above the values costs nothing while act's two parts reach 40 binades down.
-                const int pair = list[row0 + r], x = reinterpret_cast<const uint16_t*>(smem + l.expert)[pair];
-                const float w = p.weight_on_input ? p.weights[pair] : 1.f;
-                const float norm = sqrtf(v.y * (float)p.K) * w;
-                const float bound = fabsf(norm * p.g[2 * x] * p.peaks[2 * x]) * fabsf(norm * p.g[2 * x + 1] * p.peaks[2 * x + 1]);
-                const int up = min(max(14 - ((int)(__float_as_uint(bound) >> 23) - 126), -100), 100);
-                st.act = pow2(up);
-                p.act_inv[pair] = pow2(-up);
-              }
-              stats[r] = st;
-            }
-          }
-        }
-        if (work) {
-          const XT* const row = row_at(r);
-          unsigned char* const to = smem + l.rows + r * row_bytes;
-          for (int k = k0 + lane * 8; k < k1; k += 256) {
-            uint4 v = ld_u4(row + k);
-            if constexpr (kConvert)
-              v = make_uint4(bf16_to_f16_pair(v.x, factor), bf16_to_f16_pair(v.y, factor), bf16_to_f16_pair(v.z, factor), bf16_to_f16_pair(v.w, factor));
-            *reinterpret_cast<uint4*>(to + (k - k_begin) * 2) = v;
-          }
-          if (part == n_parts - 1)                 // a unit's k past the row's end
-            for (int k = k_end + lane * 8; k < unit_last * kUnitK; k += 256) *reinterpret_cast<uint4*>(to + (k - k_begin) * 2) = make_uint4(0, 0, 0, 0);
-        }
-      }
+      stage_rows<XT, true>(
+          n_rows, 0, p.K, p.units * kUnitK, smem + l.rows, row_bytes, reinterpret_cast<float2*>(smem + l.parts),
+          [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)(list[row0 + r] / p.topk) * p.ldx; },
+          [&](int r, float inv, float squares) {
+            // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the
+            // bound is far above the values costs nothing while act's two parts reach 40 binades down.
+            const int pair = list[row0 + r], x = expert[pair];
+            const float norm = sqrtf(squares * (float)p.K) * (p.weight_on_input ? p.weights[pair] : 1.f);
+            const float bound = fabsf(norm * p.g[2 * x] * p.peaks[2 * x]) * fabsf(norm * p.g[2 * x + 1] * p.peaks[2 * x + 1]);
+            const int up = min(max(14 - ((int)(__float_as_uint(bound) >> 23) - 126), -100), 100);
+            stats[r] = {inv, pow2(up)};
+            p.act_inv[pair] = pow2(-up);
+          });
       __syncthreads();
+      for (; at.item < end; next(at)) {
+        const int2 s = slots[at.hi];
+        const int n = s.x >> 16, e = s.x & 0xFFFF, strip = at.lo;
+        uint32_t col[kCols];
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) {
+          const int i = c * 8 + row8;              // columns past the slot's pairs read the first one's row: nobody reads their sums
+          col[c] = base + l.rows + (s.y - row0 + (i < n ? i : 0)) * row_bytes + quad * 32;
+        }
+        float acc[2][kCols][4] = {};
+#pragma unroll 1
+        for (int k = k_first; k < k_first + n_units; ++k) {
+          uint32_t b[2][kCols][8];
+          staged_columns<kCols>(col, k * (kUnitK * 2), b);
+          multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+          ring.advance();
+          if (ring.ok) fetch();
+        }
+        finish_item<kCols, false>(red, share, in_group, group, lane, acc, [&](int t, int c, int i, float gate, float up) {
+          const int column = c * 8 + quad * 2 + i, I = p.N / 2, i_at = strip * 16 + t * 8 + row8;
+          if (column >= n || i_at >= I) return;
+          const int pair = list[s.y + column];
+          const RowStat st = stats[s.y - row0 + column];
+          const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
+          const float v = silu_f32(gate * f * p.g[2 * e]) * (up * f * p.g[2 * e + 1]) * st.act;
+          const __half hi = __float2half_rn(v);
+          const float rest = v - __half2float(hi);
+          __half* const to = p.act + (size_t)pair * 2 * I + i_at;
+          to[0] = hi;
+          to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
+        });
+      }
     }
-
-    for (; at.item < end; next(at)) {
-      const int slot_at = slot_of(at), strip = strip_of(at);
-      const int2 s = kMode == kLinear ? make_int2(min(cap, p.M - slot_at * cap) << 16, slot_at * cap) : slots[slot_at];
-      const int n = s.x >> 16;                     // columns in use; the others read the first one's row, and nobody reads their sums
-      float acc[2][kCols][4];
-      uint32_t b[2][kCols][8];
-      uint32_t col[kCols];
+    ring.drain();
+  } else {
+    pdl_wait();
+    pdl_launch_dependents();
+    if (n_slots == 0) {
+      for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < (size_t)p.M * p.N; i += (size_t)gridDim.x * kThreads)
+        store_value(p.out, p.out_dtype, i, 0.f);
+      return;
+    }
+    for (; at.item < last; next(at)) {
+      const int2 s = slots[at.lo];
+      const int n = s.x >> 16, e = s.x & 0xFFFF, strip = at.hi;
       const __half* act[kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
-        const int i = c * 8 + row8;
-        if constexpr (kStaged) col[c] = base + l.rows + (uint32_t)(s.y - row0 + (i < n ? i : 0)) * row_bytes + (k_first - unit_first) * (kUnitK * 2) + quad * 32;
-        else act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i / 2 < n ? i / 2 : 0)] * 2 + (i & 1)) * p.ldx + k_first * kUnitK + quad * 16;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[t][c][j] = 0.f;
+        const int i = c * 4 + row8 / 2;            // a pair's columns are its upper and its lower part
+        act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i < n ? i : 0)] * 2 + (row8 & 1)) * p.ldx + quad * 16;
       }
-      auto load_columns = [&](int k) {
+      float acc[2][kCols][4] = {};
+      uint32_t b[2][kCols][8];
+      auto load_columns = [&](int k, uint32_t(&to)[2][kCols][8]) {
 #pragma unroll
         for (int half = 0; half < 2; ++half)
 #pragma unroll
           for (int c = 0; c < kCols; ++c) {
+            const int x = k * kUnitK + half * 64;
             uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-            if constexpr (kStaged) {
-              lo = lds128(col[c] + half * 128);
-              hi = lds128(col[c] + half * 128 + 16);
-            } else if (k * kUnitK + half * 64 + quad * 16 < p.K) {
-              lo = ld_u4(act[c] + half * 64);
-              hi = ld_u4(act[c] + half * 64 + 8);
+            if (x + quad * 16 < p.K) {
+              lo = ld_u4(act[c] + x);
+              hi = ld_u4(act[c] + x + 8);
             }
-            b[half][c][0] = lo.x, b[half][c][1] = lo.y, b[half][c][2] = lo.z, b[half][c][3] = lo.w;
-            b[half][c][4] = hi.x, b[half][c][5] = hi.y, b[half][c][6] = hi.z, b[half][c][7] = hi.w;
+            to[half][c][0] = lo.x, to[half][c][1] = lo.y, to[half][c][2] = lo.z, to[half][c][3] = lo.w;
+            to[half][c][4] = hi.x, to[half][c][5] = hi.y, to[half][c][6] = hi.z, to[half][c][7] = hi.w;
           }
-#pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          if constexpr (kStaged) col[c] += kUnitK * 2;
-          else act[c] += kUnitK;
-        }
       };
-      for (int k = k_first; k < k_last; ++k) {
-        load_columns(k);
-        if (ok) ok = mbar_wait(bars + stage * 8, phase, p.status, 61);
-        multiply_unit<kCols>(ring + stage * kUnitBytes, lane, b, acc);
-        if (++stage == S::kStages) {
-          stage = 0;
-          phase ^= 1;
+      if constexpr (kCols == 1) {                  // a unit ahead, as far as there are registers
+        load_columns(k_first, b);
+#pragma unroll 1
+        for (int k = k_first; k < k_first + n_units; ++k) {
+          uint32_t after[2][kCols][8];
+          load_columns(k + 1, after);
+          multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+          ring.advance();
+          if (ring.ok) fetch();
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) b[half][0][j] = after[half][0][j];
         }
-        __syncwarp();                              // every lane has read the stage
-        if (ok) fetch();
-      }
-
-      // ---- the item's end.  A lane's sums j are row l / 4 (0, 1) or l / 4 + 8 (2, 3) of a tile and columns 2 (l % 4) and the next one.
-      const int e = kMode == kLinear ? 0 : s.x & 0xFFFF;
-      auto finish = [&](int t, int c, int j, float va, float vb) {
-        // va, vb: sums j and j + 2 (gate and up, or rows eight apart); down: the two parts' sums of row j * 8
-        const int column = c * 8 + quad * 2;
-        if constexpr (kMode == kDown) {
-          const int row = strip * 32 + t * 16 + j * 8 + row8;
-          if (column / 2 < n && row < p.N) {
-            const int pair = list[s.y + column / 2];
-            p.y[(size_t)pair * p.N + row] = (va + vb) * (p.act_inv[pair] * p.g[e]);
-          }
-        } else if (column + j < n) {
-          const RowStat st = reinterpret_cast<const RowStat*>(smem + l.stats)[s.y - row0 + column + j];
-          if constexpr (kMode == kGateUp) {
-            const int pair = list[s.y + column + j], I = p.N / 2, i_at = strip * 16 + t * 8 + row8;
-            if (i_at < I) {
-              const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
-              const float v = silu_f32(va * f * p.g[2 * e]) * (vb * f * p.g[2 * e + 1]) * st.act;
-              const __half hi = __float2half_rn(v);
-              const float rest = v - __half2float(hi);
-              __half* const to = p.act + (size_t)pair * 2 * I + i_at;
-              to[0] = hi;
-              to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
-            }
-          } else {
-            const int row = strip * 32 + t * 16 + row8;
-            const float f = kConvert ? st.inv : 1.f;
-            if (split > 1) {
-              float* const to = reinterpret_cast<float*>(smem + l.sums) + ((at.item - first) * cap + column + j) * 32 + t * 16 + row8;
-              to[0] = va * f;
-              to[8] = vb * f;
-            } else {
-              const int m = s.y + column + j;
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                if (row + h * 8 < p.N) {
-                  float v = (h ? vb : va) * f * p.g[0];
-                  if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row + h * 8);
-                  store_value(p.out, p.out_dtype, (size_t)m * p.N + row + h * 8, v);
-                }
-            }
-          }
-        }
-      };
-      if (share == 1) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) finish(t, c, j, acc[t][c][kMode == kDown ? 2 * j : j], acc[t][c][kMode == kDown ? 2 * j + 1 : j + 2]);
       } else {
-        // [warp][tile][column of eight][j][lane]; each warp adds up and finishes its part
-        float* const red = reinterpret_cast<float*>(smem + l.red) + group * share * S::kSums + lane;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int c = 0; c < kCols; ++c)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) red[in_group * S::kSums + ((t * kCols + c) * 4 + j) * 32] = acc[t][c][j];
-        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
-        for (int i = in_group; i < 4 * kCols; i += share) {
-          const int j = i & 1, tc = i >> 1;
-          const float *a_from = red + (tc * 4 + (kMode == kDown ? 2 * j : j)) * 32, *b_from = a_from + (kMode == kDown ? 32 : 64);
-          float va = 0.f, vb = 0.f;
-          for (int w = 0; w < share; ++w) {
-            va += a_from[w * S::kSums];
-            vb += b_from[w * S::kSums];
-          }
-          finish(tc / kCols, tc % kCols, j, va, vb);
+#pragma unroll 1
+        for (int k = k_first; k < k_first + n_units; ++k) {
+          load_columns(k, b);
+          multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+          ring.advance();
+          if (ring.ok) fetch();
         }
-        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
       }
+      finish_item<kCols, true>(red, share, in_group, group, lane, acc, [&](int t, int c, int i, float upper, float lower) {
+        const int column = c * 4 + quad, row = strip * 32 + t * 16 + i * 8 + row8;
+        if (column >= n || row >= p.N) return;
+        const int pair = list[s.y + column];
+        p.y[(size_t)pair * p.N + row] = (upper + lower) * (p.act_inv[pair] * p.g[e]);
+      });
     }
-  }
-
-  if (!ok) {                                       // copies that were asked for land before the block's memory goes
-    const long long t0 = clock64();
-    while (clock64() - t0 < kWaitCycles / 64) {
-    }
-  }
-  if constexpr (kMode == kLinear) {
-    if (split > 1) {
-      // the parts of k are added in their order, each block of the cluster some of the items' values
-      cluster_sync_any();
-      const int count = n_block * cap * 32;
-      for (int i = rank * kThreads + threadIdx.x; i < count; i += split * kThreads) {
-        const int item = first + i / (cap * 32), column = i / 32 % cap, slot_at = item / fast;
-        const int row = (item - slot_at * fast) * 32 + (i & 31), m = slot_at * cap + column;
-        if (m >= p.M || row >= p.N) continue;
-        float v = 0.f;
-        for (int r = 0; r < split; ++r) {
-          float u;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(map_to_cta(base + l.sums + i * 4, r)) : "memory");
-          v += u;
-        }
-        v *= p.g[0];
-        if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
-        store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
-      }
-      cluster_sync_any();                          // nobody leaves while its sums are read
-    }
-  }
-  if constexpr (kMode == kDown) {
+    ring.drain();
     // The block that completes a strip adds up every token's pairs, in the order of the routing.
-    const uint16_t* const expert = reinterpret_cast<const uint16_t*>(smem + l.expert);
-    int* const flag = reinterpret_cast<int*>(smem + l.scan);
+    const float* const weights = reinterpret_cast<const float*>(smem + l.weights);
+    uint32_t* const flag = reinterpret_cast<uint32_t*>(smem + l.scan);
     __threadfence();
     __syncthreads();
-    if (n_block == 0) return;
-    for (int strip = first / n_slots; strip <= (last - 1) / n_slots; ++strip) {
-      if (threadIdx.x == 0) {
-        const int done = min(last, (strip + 1) * n_slots) - max(first, strip * n_slots);
-        *flag = atomicAdd(&p.counters[strip], done) + done == n_slots;
+    if (last == first) return;
+    const int strip_first = first / n_slots, strip_end = (last - 1) / n_slots + 1;
+    for (int strip0 = strip_first; strip0 < strip_end; strip0 += 32) {
+      if (warp == 0) {
+        const int strip = strip0 + lane;
+        bool mine = false;
+        if (strip < strip_end) {
+          const int done = min(last, (strip + 1) * n_slots) - max(first, strip * n_slots);
+          mine = atomicAdd(&p.counters[strip], done) + done == n_slots;
+        }
+        const uint32_t mask = __ballot_sync(0xffffffffu, mine);
         __threadfence();
+        if (lane == 0) *flag = mask;
       }
       __syncthreads();
-      const bool mine = *flag != 0;
+      const uint32_t mask = *flag;
       __syncthreads();
-      if (!mine) continue;
-      const int row0 = strip * 32, quads = (min(32, p.N - row0)) / 4;
-      for (int i = threadIdx.x; i < p.M * quads; i += kThreads) {
-        const int m = i / quads, row = row0 + (i - m * quads) * 4;
+      const int per_strip = p.M * 8, count = __popc(mask) * per_strip;
+      for (int i = threadIdx.x; i < count; i += kThreads) {
+        const int nth = i / per_strip, m = (i - nth * per_strip) >> 3, row = (strip0 + __fns(mask, 0, nth + 1)) * 32 + (i & 7) * 4;
+        if (row >= p.N) continue;
         float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < p.topk; ++s) {
-          const int pair = m * p.topk + s;
-          if (expert[pair] == 0xFFFF) continue;
-          const float w = p.weight_on_input ? 1.f : p.weights[pair];
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(p.y + (size_t)pair * p.N + row));
-          sum.x += w * v.x;
-          sum.y += w * v.y;
-          sum.z += w * v.z;
-          sum.w += w * v.w;
+        for (int s0 = 0; s0 < p.topk; s0 += 8) {
+          float4 v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int pair = m * p.topk + s0 + u;
+            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (s0 + u < p.topk && expert[pair] != 0xFFFF) v[u] = __ldcg(reinterpret_cast<const float4*>(p.y + (size_t)pair * p.N + row));
+          }
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int pair = m * p.topk + s0 + u;
+            if (s0 + u < p.topk && expert[pair] != 0xFFFF) {
+              const float w = weights[pair];
+              sum.x += w * v[u].x;
+              sum.y += w * v[u].y;
+              sum.z += w * v[u].z;
+              sum.w += w * v[u].w;
+            }
+          }
         }
         const size_t to = (size_t)m * p.N + row;
         store_value(p.out, p.out_dtype, to, sum.x);
@@ -712,63 +948,31 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_rows_kernel(const RowsParam
   }
 }
 
-constexpr int kMaxSplit = 8;
-
-template <typename XT, int kMode, int kCols>
-int launch_rows(RowsParams p, cudaStream_t st) {
-  using S = Shape<kCols>;
+template <typename XT, bool kDown, int kCols>
+int launch_moe_of(MoeParams p, cudaStream_t st) {
   static std::once_flag once[64];
   static bool ready[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200FP4_STATUS_NOT_SUPPORTED;
-  std::call_once(once[dev], [&] {
-    ready[dev] = cudaFuncSetAttribute(w4a16_rows_kernel<XT, kMode, kCols>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMost) == cudaSuccess;
-    cudaGetLastError();
-  });
-  if (!ready[dev]) return B200FP4_STATUS_EXECUTION_FAILED;
-  const int pairs = kMode == kLinear ? 0 : p.M * p.topk, E = kMode == kLinear ? 0 : p.E;
-  unsigned grid = 0;
-  uint32_t smem = 0;
-  int64_t best = INT64_MAX;
-  RowsParams chosen = p;
-  // Blocks that share the k of an item in a cluster (linear): a shorter k leaves room for more rows and spreads few strips over all SMs
-  for (int split = 1; split <= (kMode == kLinear ? kMaxSplit : 1) && split <= p.units; split *= 2) {
-    static ResidentClusters counts[kMaxSplit + 1][64];
-    const int clusters = split == 1 ? sm_count() : resident_clusters_of(counts[split], w4a16_rows_kernel<XT, kMode, kCols>, split, kThreads, kSmemMost);
-    if (clusters < 1) break;
-    RowsParams q = p;
-    const uint32_t own = (uint32_t)((p.units + split - 1) / split), row_bytes = own * (kUnitK * 2) + 16;
-    const int64_t most = kMode == kLinear ? p.M : pairs;
-    q.split = split;
-    q.cap = (kMode == kDown ? 4 : 8) * kCols;
-    q.rows = 0;
-    uint32_t sums = 0;
-    while (kMode != kDown) {
-      // rows that there is room for; a slot has no more columns than that
-      if (kMode == kLinear) q.cap = (int)std::min<int64_t>(q.cap, most);
-      const int64_t items = kMode == kLinear ? (most + q.cap - 1) / q.cap * p.strips : 0;
-      sums = split > 1 ? (uint32_t)std::min<int64_t>((items + clusters - 1) / clusters, 1 << 16) * q.cap * 128 : 0;
-      const uint32_t rest = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, q.cap, 1, 0, sums).bytes;
-      q.rows = (int)std::min<int64_t>(kMode == kLinear ? q.cap : most, rest < kSmemMost ? (kSmemMost - rest) / (row_bytes + (uint32_t)sizeof(RowStat)) : 0);
-      if (q.rows < 1 || q.rows >= q.cap || q.rows == most) break;
-      q.cap = q.rows;
-    }
-    if (kMode != kDown && q.rows < 1) continue;
-    const uint32_t bytes = layout_of(S::kRing, S::kBars, S::kRed, pairs, E, q.cap, q.rows, row_bytes, sums).bytes;
-    if (bytes > kSmemMost) continue;
-    const int64_t slots = kMode == kLinear ? (most + q.cap - 1) / q.cap : std::min(pairs, E) + pairs / q.cap;
-    if (slots * p.strips > 0x3FFFFFFF) continue;
-    // units of the block with the most of them; a cluster costs its synchronisation
-    const int64_t cost = kMode == kLinear ? ((slots * p.strips + clusters - 1) / clusters * own + (split > 1 ? 4 : 0)) : 0;
-    if (cost < best) {
-      best = cost;
-      chosen = q;
-      grid = (unsigned)(kMode == kLinear ? std::min<int64_t>(clusters, slots * p.strips) * split : clusters);
-      smem = bytes;
-    }
+  if (!allow_smem(w4a16_moe_kernel<XT, kDown, kCols>, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
+  const int pairs = p.M * p.topk;
+  const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;
+  p.cap = (kDown ? 4 : 8) * kCols;
+  p.rows = 0;
+  while (!kDown) {
+    // rows that there is room for; a slot has no more columns than that
+    const uint32_t rest = moe_layout(kCols, pairs, p.E, p.cap, 0, 0).rows + 16;      // the counts lie where the rows come
+    p.rows = rest < kSmemMost ? (int)std::min<uint32_t>((uint32_t)pairs, (kSmemMost - rest) / (row_bytes + (uint32_t)sizeof(RowStat))) : 0;
+    if (p.rows < 1) return B200FP4_STATUS_NOT_SUPPORTED;
+    if (p.rows >= p.cap || p.rows == pairs) break;
+    p.cap = p.rows;
   }
-  if (grid == 0) return B200FP4_STATUS_NOT_SUPPORTED;
-  if (launch_pdl_cluster(chosen.split, w4a16_rows_kernel<XT, kMode, kCols>, dim3(grid), dim3(kThreads), smem, st, chosen) != cudaSuccess) {
+  const uint32_t smem = moe_layout(kCols, pairs, p.E, p.cap, p.rows, row_bytes).bytes;
+  if (smem > kSmemMost || (int64_t)(std::min(pairs, p.E) + pairs / p.cap) * p.strips > 0x3FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
+  // Items as far as they can be foretold: what a router without favourites would give
+  const double local = (double)pairs * p.E / (double)(p.map != nullptr ? std::max<int64_t>(p.global_E, p.E) : p.E);
+  const double each = std::min(1.0, local / ((double)p.M * p.E)), reached = p.E * (1.0 - std::pow(1.0 - each, p.M));
+  const double slots = std::max(1.0, std::max(reached, local / p.cap));
+  p.log_share = share_of((int)(slots * p.strips / sm_count()) + 1, p.units);
+  if (launch_pdl(w4a16_moe_kernel<XT, kDown, kCols>, dim3(sm_count()), dim3(kThreads), smem, st, p) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
@@ -776,15 +980,11 @@ int launch_rows(RowsParams p, cudaStream_t st) {
 }
 
 template <typename T>
-int launch_linear(const RowsParams& p, cudaStream_t st) {
-  return p.M <= 8 ? launch_rows<T, kLinear, 1>(p, st) : launch_rows<T, kLinear, 2>(p, st);
+int launch_gate_up(const MoeParams& p, cudaStream_t st) {
+  return (int64_t)p.M * p.topk <= 4 * (int64_t)p.E ? launch_moe_of<T, false, 1>(p, st) : launch_moe_of<T, false, 2>(p, st);
 }
-template <typename T>
-int launch_gate_up(const RowsParams& p, cudaStream_t st) {
-  return (int64_t)p.M * p.topk <= 4 * (int64_t)p.E ? launch_rows<T, kGateUp, 1>(p, st) : launch_rows<T, kGateUp, 2>(p, st);
-}
-int launch_down(const RowsParams& p, cudaStream_t st) {
-  return (int64_t)p.M * p.topk <= 2 * (int64_t)p.E ? launch_rows<__half, kDown, 1>(p, st) : launch_rows<__half, kDown, 2>(p, st);
+int launch_down(const MoeParams& p, cudaStream_t st) {
+  return (int64_t)p.M * p.topk <= 2 * (int64_t)p.E ? launch_moe_of<__half, true, 1>(p, st) : launch_moe_of<__half, true, 2>(p, st);
 }
 
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
@@ -798,15 +998,17 @@ size_t unit_bytes(int64_t E, int64_t N, int64_t K, int gated) {
   return (size_t)E * packed_strips(N, gated) * units_of(K) * kUnitBytes;
 }
 
+// pairs of a turn: the table of counts takes 32 KB (64 KB from 2049 experts)
+int64_t pairs_of_turn(int64_t E) { return E <= 512 ? kMaxPairs : (E <= 1024 ? kMaxPairs / 2 : kMaxPairs / 4); }
 // tokens of a layer whose pairs fit one turn
-int64_t turn_of(int64_t M, int64_t topk) { return std::min(M, std::max<int64_t>(1, kMaxPairs / topk)); }
+int64_t turn_of(int64_t M, int64_t topk, int64_t E) { return std::min(M, std::max<int64_t>(1, pairs_of_turn(E) / topk)); }
 
 struct MoeScratch {
   size_t act, act_inv, y, counters, bytes;
 };
-MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I) {
+MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E) {
   MoeScratch s;
-  const size_t pairs = (size_t)turn_of(M, topk) * topk;
+  const size_t pairs = (size_t)turn_of(M, topk, E) * topk;
   s.act = 0;
   s.act_inv = s.act + pad256(pairs * 2 * I * 2);
   s.y = s.act_inv + pad256(pairs * 4);
@@ -858,7 +1060,7 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   if (x == nullptr || packed == nullptr || g_scale == nullptr || out == nullptr || status == nullptr) return B200FP4_STATUS_INVALID_VALUE;
   if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(out, 16) || ldx % 8 != 0 || (M > 1 && ldx < K)) return B200FP4_STATUS_INVALID_VALUE;
   if (!fits_int(M) || !fits_int(N + 64) || !fits_int(K + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
-  RowsParams p = {};
+  LinearParams p = {};
   p.x = x;
   p.ldx = ldx;
   p.packed = packed;
@@ -873,14 +1075,13 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   p.strips = (int)w4::strips_of(N);
   p.units = (int)w4::units_of(K);
   p.status = status;
-  p.clear_status = 1;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(p, st) : launch_linear<__half>(p, st);
 }
 
-extern "C" size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I) {
-  if (M < 1 || topk < 1 || H < 1 || I < 1) return 0;
-  return moe_scratch(M, topk, H, I).bytes;
+extern "C" size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E) {
+  if (M < 1 || topk < 1 || H < 1 || I < 1 || E < 1) return 0;
+  return moe_scratch(M, topk, H, I, E).bytes;
 }
 
 extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* topk_weights, const int32_t* topk_ids, const int32_t* expert_map,
@@ -894,15 +1095,15 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
       w2_g == nullptr || out == nullptr || status == nullptr || (expert_map != nullptr && global_E < 1))
     return B200FP4_STATUS_INVALID_VALUE;
   if (!aligned(hidden, 16) || !aligned(w13_packed, 16) || !aligned(w2_packed, 16) || !aligned(out, 16)) return B200FP4_STATUS_INVALID_VALUE;
-  if (E > kMaxExperts || topk > kMaxPairs || !fits_int(M * topk) || !fits_int(H + 128) || !fits_int(2 * I + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
-  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I))
+  if (E > kMaxExperts || topk > pairs_of_turn(E) || !fits_int(M * topk) || !fits_int(H + 128) || !fits_int(2 * I + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
+  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I, E))
     return B200FP4_STATUS_ALLOC_FAILED;
-  const MoeScratch s = moe_scratch(M, topk, H, I);
+  const MoeScratch s = moe_scratch(M, topk, H, I, E);
   unsigned char* const ws = static_cast<unsigned char*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t turn = turn_of(M, topk);
+  const int64_t turn = turn_of(M, topk, E);
   for (int64_t m = 0; m < M; m += turn) {
-    RowsParams p = {};
+    MoeParams p = {};
     p.M = (int)std::min(turn, M - m);
     p.status = status;
     p.clear_status = m == 0;
@@ -919,7 +1120,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.y = reinterpret_cast<float*>(ws + s.y);
     p.counters = reinterpret_cast<int*>(ws + s.counters);
     p.n_counters = (int)w4::strips_of(H);
-    RowsParams d = p;
+    MoeParams d = p;
     p.x = static_cast<const unsigned char*>(hidden) + (size_t)m * H * 2;
     p.ldx = H;
     p.packed = w13_packed;
