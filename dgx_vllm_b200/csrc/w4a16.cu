@@ -17,6 +17,7 @@
 
 #include "sm100_ptx.cuh"
 #include "w4a16.cuh"
+#include "w4a16_linear.cuh"
 
 namespace b200fp4 {
 namespace {
@@ -68,7 +69,7 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
       const float value = (code < 2 ? 0.5f * code : (1.f + 0.5f * (code & 1)) * (float)(1 << (code >> 1)) * 0.5f) * e4m3_to_f32((uint8_t)scale);
       peak[p.gated ? r : 0] = fmaxf(peak[p.gated ? r : 0], value);
     }
-    *reinterpret_cast<uint4*>(dst + (tile * 2 + half) * 512 + lane * 16) = make_uint4(word[0].x, word[0].y, word[1].x, word[1].y);
+    *reinterpret_cast<uint4*>(dst + (tile * 2 + half) * 512 + chunk_at(lane >> 2, lane & 3)) = make_uint4(word[0].x, word[0].y, word[1].x, word[1].y);
   }
   *reinterpret_cast<uint32_t*>(dst + kUnitScales + lane * 8 + tile * 4) = sc;
   // magnitudes are not negative: their bits order as they do
@@ -148,13 +149,13 @@ struct Ring {
 
 // a unit's 32 rows times kCols columns of eight; b: the columns' operands, [half][column][8]
 template <int kCols>
-__device__ __forceinline__ void multiply_unit(uint32_t unit, int lane, const uint32_t (&b)[2][kCols][8], float (&acc)[2][kCols][4]) {
+__device__ __forceinline__ void multiply_unit(uint32_t unit, int lane, uint32_t chunk, const uint32_t (&b)[2][kCols][8], float (&acc)[2][kCols][4]) {
   const uint2 sc = lds64(unit + kUnitScales + lane * 8);
 #pragma unroll
   for (int half = 0; half < 2; ++half)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint4 w = lds128(unit + (t * 2 + half) * 512 + lane * 16);
+      const uint4 w = lds128(unit + (t * 2 + half) * 512 + chunk);
       const __half2 s = scales_of(t ? sc.y : sc.x, half), s_lo = __low2half2(s), s_hi = __high2half2(s);
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
@@ -378,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr bool kConvert = std::is_same<XT, __nv_bfloat16>::value;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
-  const uint32_t base = smem_u32(smem);
+  const uint32_t base = smem_u32(smem), chunk = chunk_at(row8, quad);
   Ring ring;
   ring.init(base, base + kRingBytes, warp, lane);
   const int split = p.split, rank = (int)blockIdx.x & (split - 1), cluster = (int)blockIdx.x / split;      // split: a power of two
@@ -433,7 +434,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
       for (int k = k_first; k < k_first + n_units; ++k) {
         uint32_t b[2][kCols][8];
         staged_columns<kCols>(col, k * (kUnitK * 2), b);
-        multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+        multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
         ring.advance();
         if (ring.ok) fetch();
       }
@@ -546,8 +547,25 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
   return finish_launch(1);
 }
 
+constexpr int kFewTokens = 16;
+
 template <typename T>
-int launch_linear(const LinearParams& p, cudaStream_t st) {
+int launch_linear(const LinearCall& c, cudaStream_t st) {
+  LinearParams p = {};
+  p.x = c.x;
+  p.ldx = c.ldx;
+  p.packed = c.packed;
+  p.g = c.g;
+  p.out = c.out;
+  p.out_dtype = c.out_dtype;
+  p.bias = c.bias;
+  p.bias_dtype = c.bias_dtype;
+  p.M = (int)c.M;
+  p.N = (int)c.N;
+  p.K = (int)c.K;
+  p.strips = (int)strips_of(c.N);
+  p.units = (int)units_of(c.K);
+  p.status = c.status;
   return p.M <= 8 ? launch_linear_of<T, 1>(p, st) : launch_linear_of<T, 2>(p, st);
 }
 
@@ -705,7 +723,7 @@ template <typename XT, bool kDown, int kCols>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
-  const uint32_t base = smem_u32(smem);
+  const uint32_t base = smem_u32(smem), chunk = chunk_at(row8, quad);
   const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;      // rows are shifted by 16 bytes against each other: no two lanes of a load meet
   const MoeLayout l = moe_layout(kCols, p.M * p.topk, p.E, p.cap, p.rows, row_bytes);
   const uint16_t* const expert = reinterpret_cast<const uint16_t*>(smem + l.expert);
@@ -806,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         for (int k = k_first; k < k_first + n_units; ++k) {
           uint32_t b[2][kCols][8];
           staged_columns<kCols>(col, k * (kUnitK * 2), b);
-          multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
           ring.advance();
           if (ring.ok) fetch();
         }
@@ -866,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         for (int k = k_first; k < k_first + n_units; ++k) {
           uint32_t after[2][kCols][8];
           load_columns(k + 1, after);
-          multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
           ring.advance();
           if (ring.ok) fetch();
 #pragma unroll
@@ -878,7 +896,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
 #pragma unroll 1
         for (int k = k_first; k < k_first + n_units; ++k) {
           load_columns(k, b);
-          multiply_unit<kCols>(ring.wait(p.status), lane, b, acc);
+          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
           ring.advance();
           if (ring.ok) fetch();
         }
@@ -1060,23 +1078,10 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   if (x == nullptr || packed == nullptr || g_scale == nullptr || out == nullptr || status == nullptr) return B200FP4_STATUS_INVALID_VALUE;
   if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(out, 16) || ldx % 8 != 0 || (M > 1 && ldx < K)) return B200FP4_STATUS_INVALID_VALUE;
   if (!fits_int(M) || !fits_int(N + 64) || !fits_int(K + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
-  LinearParams p = {};
-  p.x = x;
-  p.ldx = ldx;
-  p.packed = packed;
-  p.g = g_scale;
-  p.out = out;
-  p.out_dtype = out_dtype;
-  p.bias = bias;
-  p.bias_dtype = bias_dtype;
-  p.M = (int)M;
-  p.N = (int)N;
-  p.K = (int)K;
-  p.strips = (int)w4::strips_of(N);
-  p.units = (int)w4::units_of(K);
-  p.status = status;
+  const LinearCall c = {x, x_dtype, ldx, packed, g_scale, bias, bias_dtype, out, out_dtype, M, N, K, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(p, st) : launch_linear<__half>(p, st);
+  if (M > kFewTokens) return launch_w4a16_gemm(c, st);
+  return x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(c, st) : launch_linear<__half>(c, st);
 }
 
 extern "C" size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E) {

@@ -12,9 +12,10 @@
 // instruction, whose lane l holds rows l / 4 and l / 4 + 8 and four k of each: with the k of an instruction taken from four blocks of 16,
 // lane l needs block l % 4 only, so it converts one scale a row for four instructions, and its operands of a whole block are 16
 // neighbouring values:
-//   codes   [tile][half: 64 of k][lane][16 bytes: row l / 4, k 0..15 | row l / 4 + 8, k 0..15]
+//   codes   [tile][half: 64 of k][chunk_at(l / 4, l % 4)][16 bytes: row l / 4, k 0..15 | row l / 4 + 8, k 0..15]
 //   scales  [lane][tile][4 bytes: half 0 row l / 4, row l / 4 + 8 | half 1 likewise]
-// A lane reads them with wide loads that no other lane's meet.  Negative scales give their sign to their codes when the weight is packed.
+// The chunks are ordered so that no two lanes meet in a bank when each reads its 16 bytes, nor when a lane is one of 32 rows and reads the 8 bytes of a
+// block (the decoding of w4a16_gemm.cu).  Negative scales give their sign to their codes when the weight is packed.
 // Gated: the 16 rows of a tile are eight gate rows and the same eight up rows, so that a lane holds both of a value's products.
 // Behind the units: for each matrix the largest magnitude of code times scale, f32 (two of them, gate rows and up rows, where gated).
 #pragma once
@@ -28,6 +29,9 @@ constexpr int kUnitBytes = 2304, kUnitScales = 2048, kUnitK = 128, kUnitRows = 3
 
 __host__ __device__ __forceinline__ int64_t strips_of(int64_t rows) { return (rows + kUnitRows - 1) / kUnitRows; }      // of 32 rows
 __host__ __device__ __forceinline__ int64_t units_of(int64_t K) { return (K + kUnitK - 1) / kUnitK; }
+
+// where the chunk of row r8 (and r8 + 8) and block t of a half begins
+__device__ __forceinline__ uint32_t chunk_at(int r8, int t) { return (uint32_t)(t * 8 + ((r8 + 2 * t) & 7)) * 16; }
 
 __device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 __device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }

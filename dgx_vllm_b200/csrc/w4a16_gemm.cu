@@ -1,0 +1,428 @@
+// Weight-only NVFP4 linear of many tokens: out[M,N] = x . W^T * g (+ bias) on the tcgen05 tensor cores.
+//
+// The 128 rows of an MMA are rows of the weight, the tokens are its columns.  Decoding warps turn packed units (w4a16.cuh) into 16-bit values and write
+// them straight into tensor memory, from where the MMA takes its A operand: a decoded weight never is in shared memory, and it is decoded once for
+// up to 192 tokens.  The activations are the B operand as they lie in memory, brought in by TMA, in the type they have: products are exact in bf16
+// and in f16 alike.
+// Roles (18 warps): 0 copies, 1 MMAs and tensor memory, 2-5 epilogue, 6-17 decoding (three sets of four, each 32 rows of the tile and every third 64 of k).
+// Tensor memory: two accumulators of up to 192 columns, four A stages of 32 (128 rows x 64 of k).  Persistent blocks, one to an SM; where there are too few
+// tiles for them, a cluster shares the k of one and adds up its parts through distributed shared memory, each block some of the tokens.
+// Every wait is bounded (status word), tensor memory is always freed.
+#include <algorithm>
+#include <type_traits>
+
+#include "sm100_ptx.cuh"
+#include "w4a16_linear.cuh"
+#include "w4a16.cuh"
+
+namespace b200fp4 {
+namespace {
+
+using namespace w4;
+
+constexpr int kMmaRows = 128, kMostTokens = 192;
+constexpr int kDecodeSets = 3, kFirstDecode = 6;
+constexpr int kThreads = 32 * (kFirstDecode + 4 * kDecodeSets);
+constexpr int kAStages = 4, kWStages = 4;       // A operands in tensor memory, packed units of 128 rows x 128 of k in shared memory
+constexpr int kBMost = 8;                       // token stages, as many as 120 KB hold
+constexpr uint32_t kWStageBytes = 4 * kUnitBytes, kBBytes = 120 * 1024;
+constexpr uint32_t kAccCols = kMostTokens, kACol = 2 * kAccCols;      // tensor-memory columns: accumulators, then A
+static_assert(kACol + kAStages * 32 <= 512, "tensor memory budget");
+constexpr uint32_t kSmemBytes = 1024 + kBBytes + kWStages * kWStageBytes + 512;
+constexpr int kMaxSplit = 8;
+
+struct GemmParams {
+  const uint8_t* packed;
+  const float* g;
+  const void* bias;
+  void* out;
+  int bias_dtype, out_dtype;
+  int M, N, K;
+  int strips, units;
+  int tokens;                 // columns of a tile, a multiple of 16
+  int row_tiles, tiles;       // tiles: row tiles x token tiles, row tiles first
+  int split;                  // blocks of a cluster, which share the units of a tile (then each block has one)
+  int b_stages;
+  int* status;
+};
+
+// two f16 that hold E2M1 values -> two bf16 times 2^-112: sign, and exponent and mantissa three places down
+__device__ __forceinline__ uint32_t f16_to_bf16_bits(uint32_t h) { return (h & 0x80008000u) | ((h >> 3) & 0x0FFF0FFFu); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t scaled(uint32_t pair, uint32_t scale);
+template <>
+__device__ __forceinline__ uint32_t scaled<__half>(uint32_t pair, uint32_t scale) {
+  return as_u32(__hmul2(as_half2(pair), as_half2(scale)));
+}
+template <>
+__device__ __forceinline__ uint32_t scaled<__nv_bfloat16>(uint32_t pair, uint32_t scale) {
+  const uint32_t b = f16_to_bf16_bits(pair);
+  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&scale));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+// E4M3 byte -> the scale twice in a register: f16, or bf16 times 2^112 (which takes back what f16_to_bf16_bits leaves)
+template <typename T>
+__device__ __forceinline__ uint32_t scale_pair(uint32_t byte);
+template <>
+__device__ __forceinline__ uint32_t scale_pair<__half>(uint32_t byte) {
+  return as_u32(__hmul2(as_half2(byte * 0x00800080u), as_half2(0x5C005C00u)));      // fields in place: times 2^-8
+}
+template <>
+__device__ __forceinline__ uint32_t scale_pair<__nv_bfloat16>(uint32_t byte) {
+  const uint32_t raw = byte * 0x00100010u, f1 = 0x7F007F00u, f2 = 0x74007400u;      // times 2^-120; 2^127, 2^105
+  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&raw), *reinterpret_cast<const __nv_bfloat162*>(&f1));
+  r = __hmul2(r, *reinterpret_cast<const __nv_bfloat162*>(&f2));
+  return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+__device__ __forceinline__ void tcgen05_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+      "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// D += A . B^T, A in tensor memory
+__device__ __forceinline__ void tcgen05_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+__device__ __forceinline__ void store_value(void* out, int dtype, size_t at, float v) {
+  if (dtype == B200FP4_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else if (dtype == B200FP4_DTYPE_F16) static_cast<__half*>(out)[at] = __float2half_rn(v);
+  else static_cast<float*>(out)[at] = v;
+}
+__device__ __forceinline__ float load_value(const void* p, int dtype, size_t at) {
+  if (dtype == B200FP4_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
+  if (dtype == B200FP4_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[at]);
+  return static_cast<const float*>(p)[at];
+}
+
+// a position in a ring of `size` stages
+struct Slot {
+  uint32_t at = 0, phase = 0;
+  __device__ __forceinline__ void next(uint32_t size) {
+    if (++at == size) {
+      at = 0;
+      phase ^= 1;
+    }
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const GemmParams p) {
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t base = smem_u32(smem), w_ring = base + kBBytes, bars = w_ring + kWStages * kWStageBytes;
+  const uint32_t b_full = bars, b_empty = b_full + 8 * kBMost, w_full = b_empty + 8 * kBMost, w_empty = w_full + 8 * kWStages;
+  const uint32_t a_full = w_empty + 8 * kWStages, a_empty = a_full + 8 * kAStages, acc_full = a_empty + 8 * kAStages, acc_empty = acc_full + 16;
+  const uint32_t tmem_ptr = acc_empty + 16;
+  const int tokens = p.tokens, split = p.split, b_stages = p.b_stages;
+  const uint32_t b_bytes = (uint32_t)tokens * 128;
+  const int rank = split > 1 ? (int)blockIdx.x & (split - 1) : 0;
+  const int first_tile = (int)blockIdx.x / split, step = (int)gridDim.x / split;
+  const int unit_first = p.units * rank / split, n_units = p.units * (rank + 1) / split - unit_first;
+  int* const status = p.status;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBMost; ++i) {
+      mbar_init(b_full + 8 * i, 1);
+      mbar_init(b_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < kWStages; ++i) {
+      mbar_init(w_full + 8 * i, 1);
+      mbar_init(w_empty + 8 * i, 8);              // four warps for each of its 64 of k
+    }
+    for (int i = 0; i < kAStages; ++i) {
+      mbar_init(a_full + 8 * i, 4);
+      mbar_init(a_empty + 8 * i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(acc_full + 8 * i, 1);
+      mbar_init(acc_empty + 8 * i, 4);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    fence_proxy_async_smem();
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_ptr), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem = lds32(tmem_ptr);
+  pdl_wait();
+  pdl_launch_dependents();
+  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ copies
+    const bool leader = elect_one();
+    Slot b, w;
+    bool ok = true;
+    b.phase = w.phase = 1;
+    for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
+      const int row_tile = tile % p.row_tiles, token0 = tile / p.row_tiles * tokens;
+      const int strip0 = row_tile * 4, strips = min(4, p.strips - strip0);
+      const uint8_t* src = p.packed + ((size_t)strip0 * p.units + unit_first) * kUnitBytes;
+      for (int u = 0; u < n_units && ok; ++u, src += kUnitBytes) {
+        ok = mbar_wait_warp(w_empty + 8 * w.at, w.phase, status, 71);
+        if (!ok) break;
+        if (leader) {
+          const uint32_t bar = w_full + 8 * w.at, to = w_ring + w.at * kWStageBytes;
+          mbar_expect_tx(bar, (uint32_t)strips * kUnitBytes);
+          for (int s = 0; s < strips; ++s) bulk_load_1d(to + s * kUnitBytes, src + (size_t)s * p.units * kUnitBytes, kUnitBytes, bar);
+        }
+        w.next(kWStages);
+        for (int half = 0; half < 2; ++half) {
+          ok = mbar_wait_warp(b_empty + 8 * b.at, b.phase, status, 72);
+          if (!ok) break;
+          if (leader) {
+            mbar_expect_tx(b_full + 8 * b.at, b_bytes);
+            tma_load_2d(base + b.at * b_bytes, &map_x, ((unit_first + u) * 2 + half) * 128, token0, b_full + 8 * b.at);
+          }
+          b.next(b_stages);
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMAs
+    const bool leader = elect_one();
+    // f32 accumulators, A and B both f16 or both bf16, K-major, M = 128, N = tokens
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(tokens >> 3) << 17) | ((uint32_t)(kMmaRows >> 4) << 24);
+    const uint64_t b0 = desc_kmajor<128>(base);
+    Slot b, a, acc;
+    bool ok = true;
+    acc.phase = 1;
+    for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
+      ok = mbar_wait_warp(acc_empty + 8 * acc.at, acc.phase, status, 73);
+      if (!ok) break;
+      tcgen05_fence_after();
+      const uint32_t d = tmem + acc.at * kAccCols;
+      for (int k = 0; k < 2 * n_units; ++k) {
+        ok = mbar_wait_warp(b_full + 8 * b.at, b.phase, status, 74) && mbar_wait_warp(a_full + 8 * a.at, a.phase, status, 75);
+        if (!ok) break;
+        tcgen05_fence_after();
+        if (leader) {
+          const uint64_t desc = b0 + (uint64_t)((b.at * b_bytes) >> 4);
+          const uint32_t from = tmem + kACol + a.at * 32;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) tcgen05_mma_ts(d, from + i * 8, desc + i * 2, idesc, (k > 0 || i > 0) ? 1u : 0u);
+          tcgen05_commit(b_empty + 8 * b.at);
+          tcgen05_commit(a_empty + 8 * a.at);
+          if (k == 2 * n_units - 1) tcgen05_commit(acc_full + 8 * acc.at);
+        }
+        __syncwarp();
+        b.next(b_stages);
+        a.next(kAStages);
+      }
+      acc.next(2);
+    }
+  } else if (warp >= kFirstDecode) {
+    // ------------------------------------------------------------------ decoding: a lane is a row
+    const int set = (warp - kFirstDecode) >> 2, quarter = warp & 3, r8 = lane & 7, upper = (lane >> 3) & 1, tile16 = lane >> 4;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    uint32_t code_at[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) code_at[t] = quarter * kUnitBytes + tile16 * 1024 + chunk_at(r8, t) + upper * 8;
+    const uint32_t scale_at = quarter * kUnitBytes + kUnitScales + r8 * 32 + tile16 * 4, scale_shift = upper * 8;
+    bool ok = true;
+    uint32_t turn = 0;                             // of all steps of 64 of k; this set takes every third
+    for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
+      for (int k = 0; k < 2 * n_units; ++k, ++turn) {
+        if (turn % kDecodeSets != (uint32_t)set) continue;
+        const uint32_t ws = (turn >> 1) % kWStages, as = turn % kAStages;
+        ok = mbar_wait_warp(w_full + 8 * ws, ((turn >> 1) / kWStages) & 1, status, 76);
+        if (!ok) break;
+        const uint32_t unit = w_ring + ws * kWStageBytes, half = turn & 1;
+        uint2 code[4];
+        uint32_t sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          code[t] = lds64(unit + code_at[t] + half * 512);
+          sc[t] = (lds32(unit + scale_at + t * 8) >> (scale_shift + half * 16)) & 0x7Fu;
+        }
+        uint32_t v[32];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          uint32_t pair[8];
+          codes_to_pairs(code[t].x, *reinterpret_cast<uint32_t(*)[4]>(&pair[0]));
+          codes_to_pairs(code[t].y, *reinterpret_cast<uint32_t(*)[4]>(&pair[4]));
+          const uint32_t s = scale_pair<T>(sc[t]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[t * 8 + i] = scaled<T>(pair[i], s);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(w_empty + 8 * ws);
+        if (turn >= kAStages) {
+          ok = mbar_wait_warp(a_empty + 8 * as, (turn / kAStages - 1) & 1, status, 77);
+          if (!ok) break;
+        }
+        tcgen05_fence_after();
+        tcgen05_st_32x32(tmem + kACol + lanes + as * 32, v);
+        tcgen05_wait_st();
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(a_full + 8 * as);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------------ epilogue: a lane is a row of the weight, a column a token
+    const int quarter = warp & 3;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const float g = *p.g;
+    Slot acc;
+    for (int tile = first_tile; tile < p.tiles; tile += step) {
+      const int row = tile % p.row_tiles * kMmaRows + quarter * 32 + lane, token0 = tile / p.row_tiles * tokens, n = min(tokens, p.M - token0);
+      const float bias = p.bias != nullptr && row < p.N && split == 1 ? load_value(p.bias, p.bias_dtype, row) : 0.f;
+      if (!mbar_wait_warp(acc_full + 8 * acc.at, acc.phase, status, 78)) break;
+      tcgen05_fence_after();
+      if (split > 1) break;                        // the only tile: its sums go to the cluster below
+      for (int c = 0; c < n; c += 32) {
+        uint32_t r[32];
+        tcgen05_ld_32x32(tmem + lanes + acc.at * kAccCols + c, r);
+        tcgen05_wait_ld();
+        if (row < p.N) {
+          const size_t at = (size_t)(token0 + c) * p.N + row;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (c + i < n) store_value(p.out, p.out_dtype, at + (size_t)i * p.N, __uint_as_float(r[i]) * g + bias);
+        }
+      }
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_empty + 8 * acc.at);
+      acc.next(2);
+    }
+  }
+  __syncwarp();
+  if (split > 1) {
+    // Token t of the tile is finished by block t / (tokens / split): [source][its tokens][128 rows] of f32, where the token stages were
+    cluster_sync_any();                            // all MMAs of the cluster have read theirs
+    const int own = tokens / split, tile = first_tile;
+    if (warp >= 2 && warp < 6) {
+      const int quarter = warp & 3;
+      for (int c = 0; c < tokens; c += 16) {
+        uint32_t r[16];
+        tcgen05_ld_32x16(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
+        tcgen05_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int t = c + i, owner = t / own;
+          const uint32_t to = base + ((uint32_t)(rank * own + t - owner * own) * kMmaRows + quarter * 32 + lane) * 4;
+          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(map_to_cta(to, owner)), "r"(r[i]) : "memory");
+        }
+      }
+    }
+    cluster_sync_any();
+    const float g = *p.g;
+    const int row0 = tile % p.row_tiles * kMmaRows, token0 = tile / p.row_tiles * tokens + rank * own;
+    const float* const sums = reinterpret_cast<const float*>(smem);
+    for (int i = threadIdx.x; i < own * kMmaRows; i += kThreads) {
+      const int m = token0 + i / kMmaRows, row = row0 + i % kMmaRows;
+      if (m >= p.M || row >= p.N) continue;
+      float v = 0.f;
+      for (int s = 0; s < split; ++s) v += sums[s * own * kMmaRows + i];
+      v *= g;
+      if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
+      store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
+    }
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tcgen05_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+template <typename T>
+int launch_gemm(const LinearCall& c, cudaStream_t st) {
+  static std::once_flag once[64];
+  static bool ready[64];
+  static ResidentClusters counts[kMaxSplit + 1][64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200FP4_STATUS_NOT_SUPPORTED;
+  std::call_once(once[dev], [&] {
+    ready[dev] = cudaFuncSetAttribute(w4a16_gemm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) == cudaSuccess;
+    cudaGetLastError();
+  });
+  if (!ready[dev]) return B200FP4_STATUS_EXECUTION_FAILED;
+  GemmParams p = {};
+  p.packed = c.packed;
+  p.g = c.g;
+  p.bias = c.bias;
+  p.bias_dtype = c.bias_dtype;
+  p.out = c.out;
+  p.out_dtype = c.out_dtype;
+  p.M = (int)c.M;
+  p.N = (int)c.N;
+  p.K = (int)c.K;
+  p.strips = (int)strips_of(c.N);
+  p.units = (int)units_of(c.K);
+  p.row_tiles = (int)((c.N + kMmaRows - 1) / kMmaRows);
+  p.status = c.status;
+  const int sms = sm_count();
+  // Tokens of a tile and blocks that share one: the least time of the busiest block, in cycles.  64 of k take the MMAs two cycles a token, the copies one for each
+  // 57 bytes, and decoding 200.
+  double best = 1e30;
+  unsigned grid = 0;
+  const int64_t least = (c.M + kMostTokens - 1) / kMostTokens;
+  for (int64_t tt = least; tt <= least + 3; ++tt) {
+    const int tokens = (int)(((c.M + tt - 1) / tt + 15) / 16 * 16);
+    const int64_t token_tiles = (c.M + tokens - 1) / tokens, tiles = token_tiles * p.row_tiles;
+    if (tiles > 0x3FFFFFFF) continue;
+    for (int split = 1; split <= kMaxSplit && split <= p.units; split *= 2) {
+      const int clusters = split == 1 ? sms : resident_clusters_of(counts[split], w4a16_gemm_kernel<T>, split, kThreads, kSmemBytes);
+      if (clusters < 1) break;
+      if (split > 1 && tiles > clusters) break;    // a cluster does one tile
+      const double unit = std::max(std::max(4.0 * tokens, 400.0), (2.0 * tokens * 128 + 4.0 * kUnitBytes) / 57.0);
+      const double waves = (double)((tiles + clusters - 1) / clusters);
+      const double cost = waves * ((p.units + split - 1) / split * unit) + 2000.0 + tokens * 20.0 + (split > 1 ? 2000.0 + tokens * 20.0 : 0.0);
+      if (cost < best) {
+        best = cost;
+        p.tokens = tokens;
+        p.tiles = (int)tiles;
+        p.split = split;
+        p.b_stages = (int)std::min<uint32_t>(kBMost, kBBytes / ((uint32_t)tokens * 128));
+        grid = (unsigned)(std::min<int64_t>(clusters, tiles) * split);
+      }
+    }
+  }
+  if (grid == 0) return B200FP4_STATUS_NOT_SUPPORTED;
+  CUtensorMap map;
+  if (!make_rows_map(&map, c.x, (uint64_t)c.M, (uint64_t)c.K * 2, (uint64_t)(c.M > 1 ? c.ldx : c.K) * 2, (uint32_t)p.tokens, 128)) return B200FP4_STATUS_INTERNAL_ERROR;
+  if (launch_pdl_cluster(p.split, w4a16_gemm_kernel<T>, dim3(grid), dim3(kThreads), kSmemBytes, st, map, p) != cudaSuccess) {
+    cudaGetLastError();
+    return B200FP4_STATUS_EXECUTION_FAILED;
+  }
+  return finish_launch(1);
+}
+
+}  // namespace
+
+int launch_w4a16_gemm(const LinearCall& c, cudaStream_t st) {
+  return c.x_dtype == B200FP4_DTYPE_BF16 ? launch_gemm<__nv_bfloat16>(c, st) : launch_gemm<__half>(c, st);
+}
+
+}  // namespace b200fp4
