@@ -41,8 +41,9 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
   if (at >= n_tiles) return;
   const int lane = threadIdx.x & 31, tile = (int)(at & 1);
   const int64_t unit = at >> 1, u = unit % p.units, strip = unit / p.units % p.strips, e = unit / p.units / p.strips;
-  uint8_t* const dst = p.packed + unit * kUnitBytes;
-  const int64_t row0 = (strip * 2 + tile) * (p.gated ? 8 : 16) + (lane >> 2), step = p.gated ? p.N / 2 : 8, rows = p.gated ? p.N / 2 : p.N;
+  int step;
+  uint8_t* const dst = p.packed + (e * p.strips * p.units + strip_at(strip, p.strips, p.units, u, step)) * kUnitBytes;
+  const int64_t row0 = (strip * 2 + tile) * (p.gated ? 8 : 16) + (lane >> 2), apart = p.gated ? p.N / 2 : 8, rows = p.gated ? p.N / 2 : p.N;
   uint32_t sc = 0;
   float peak[2] = {0.f, 0.f};
   for (int half = 0; half < 2; ++half) {
@@ -52,7 +53,7 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
       uint32_t scale = 0;
       uint2 c = make_uint2(0, 0);
       if ((p.gated ? row0 : row0 + r * 8) < rows && k < p.K) {
-        const int64_t row = e * p.N + row0 + r * step;
+        const int64_t row = e * p.N + row0 + r * apart;
         c = *reinterpret_cast<const uint2*>(p.codes + row * (p.K / 2) + k / 2);
         scale = p.scales[row * (p.K / 16) + k / 16];
         if (scale & 0x80) {
@@ -388,17 +389,17 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   const int k_first = (own_units * in_group) >> p.log_share, n_units = ((own_units * (in_group + 1)) >> p.log_share) - k_first;
   const int first = cluster * p.per + min(cluster, p.more), last = first + p.per + (cluster < p.more ? 1 : 0);
   // Strips of a slot of tokens are neighbours
-  int ahead = first + group, ahead_left = 0;
+  int ahead = first + group, ahead_left = 0, src_step = 0;
   const uint8_t* src = nullptr;
   auto fetch = [&]() {
     if (ahead_left == 0) {
       if (ahead >= last) return;
-      src = p.packed + ((size_t)(ahead % p.strips) * p.units + unit_first + k_first) * kUnitBytes;
+      src = p.packed + strip_at(ahead % p.strips, p.strips, p.units, unit_first + k_first, src_step) * kUnitBytes;
       ahead_left = n_units;
       ahead += n_groups;
     }
     ring.ask(src, lane);
-    src += kUnitBytes;
+    src += src_step * kUnitBytes;
     --ahead_left;
   };
   pdl_wait();
@@ -763,18 +764,18 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       ++c.hi;
     }
   };
-  int ahead_left = 0;
+  int ahead_left = 0, src_step = 0;
   const uint8_t* src = nullptr;
   auto fetch = [&]() {
     if (ahead_left == 0) {
       if (ahead.item >= last) return;
       const size_t e = slots[kDown ? ahead.lo : ahead.hi].x & 0xFFFF;
-      src = p.packed + ((e * p.strips + (kDown ? ahead.hi : ahead.lo)) * p.units + k_first) * kUnitBytes;
+      src = p.packed + (e * p.strips * p.units + strip_at(kDown ? ahead.hi : ahead.lo, p.strips, p.units, k_first, src_step)) * kUnitBytes;
       ahead_left = n_units;
       next(ahead);
     }
     ring.ask(src, lane);
-    src += kUnitBytes;
+    src += src_step * kUnitBytes;
     --ahead_left;
   };
 #pragma unroll 1

@@ -8,7 +8,8 @@
 // become f16 exactly, after a power of two for each row has brought its largest value below 2^15: what is then below f16's
 // smallest, 2^-39 of that largest value, is the only part that can be rounded.
 //
-// Packed weight: units of 32 rows x 128 of k, 2304 bytes, [matrix][32 rows][k / 128][unit].  A unit is two tiles of the 16x8x16 matrix
+// Packed weight: units of 32 rows x 128 of k, 2304 bytes, [matrix][128 rows][k / 128][32 rows][unit] (fewer rows in a last block): one copy brings 128 rows x 128 of
+// k, and one a unit.  A unit is two tiles of the 16x8x16 matrix
 // instruction, whose lane l holds rows l / 4 and l / 4 + 8 and four k of each: with the k of an instruction taken from four blocks of 16,
 // lane l needs block l % 4 only, so it converts one scale a row for four instructions, and its operands of a whole block are 16
 // neighbouring values:
@@ -29,6 +30,13 @@ constexpr int kUnitBytes = 2304, kUnitScales = 2048, kUnitK = 128, kUnitRows = 3
 
 __host__ __device__ __forceinline__ int64_t strips_of(int64_t rows) { return (rows + kUnitRows - 1) / kUnitRows; }      // of 32 rows
 __host__ __device__ __forceinline__ int64_t units_of(int64_t K) { return (K + kUnitK - 1) / kUnitK; }
+
+// Units of a matrix before those of a strip of 32 rows, and from one 128 of k to the next
+__host__ __device__ __forceinline__ int64_t strip_at(int64_t strip, int64_t strips, int64_t units, int64_t unit, int& step) {
+  const int64_t block = strip & ~(int64_t)3;
+  step = (int)(strips - block < 4 ? strips - block : 4);
+  return block * units + unit * step + (strip - block);
+}
 
 // where the chunk of row r8 (and r8 + 8) and block t of a half begins
 __device__ __forceinline__ uint32_t chunk_at(int r8, int t) { return (uint32_t)(t * 8 + ((r8 + 2 * t) & 7)) * 16; }

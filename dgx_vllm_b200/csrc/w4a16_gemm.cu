@@ -4,8 +4,10 @@
 // them straight into tensor memory, from where the MMA takes its A operand: a decoded weight never is in shared memory, and it is decoded once for
 // up to 192 tokens.  The activations are the B operand as they lie in memory, brought in by TMA, in the type they have: products are exact in bf16
 // and in f16 alike.
-// Roles (18 warps): 0 copies, 1 MMAs and tensor memory, 2-5 epilogue, 6-17 decoding (three sets of four, each 32 rows of the tile and every third 64 of k).
-// Tensor memory: two accumulators of up to 192 columns, four A stages of 32 (128 rows x 64 of k).  Persistent blocks, one to an SM; where there are too few
+// Roles (23 warps): 0 copies of the weight, 22 of the tokens, 1 MMAs and tensor memory, 2-5 epilogue, 6-21 decoding (four sets of four, a warp 32 rows of the tile
+// and every fourth 128 of k).  One warp that brought in weight and tokens, four copies for 128 rows, took 1040 cycles for 128 of k and was what all waited for.
+// Tensor memory: accumulators, and the rest for A stages of 64 columns (128 rows x 128 of k): the MMA warp's waits, MMAs and commits take 300 cycles a
+// stage however few the tokens are.  Persistent blocks, one to an SM; where there are too few
 // tiles for them, a cluster shares the k of one and adds up its parts through distributed shared memory, each block some of the tokens.
 // Every wait is bounded (status word), tensor memory is always freed.
 #include <algorithm>
@@ -21,14 +23,13 @@ namespace {
 using namespace w4;
 
 constexpr int kMmaRows = 128, kMostTokens = 192;
-constexpr int kDecodeSets = 3, kFirstDecode = 6;
-constexpr int kThreads = 32 * (kFirstDecode + 4 * kDecodeSets);
-constexpr int kAStages = 4, kWStages = 4;       // A operands in tensor memory, packed units of 128 rows x 128 of k in shared memory
-constexpr int kBMost = 8;                       // token stages, as many as 120 KB hold
-constexpr uint32_t kWStageBytes = 4 * kUnitBytes, kBBytes = 120 * 1024;
-constexpr uint32_t kAccCols = kMostTokens, kACol = 2 * kAccCols;      // tensor-memory columns: accumulators, then A
-static_assert(kACol + kAStages * 32 <= 512, "tensor memory budget");
-constexpr uint32_t kSmemBytes = 1024 + kBBytes + kWStages * kWStageBytes + 512;
+constexpr int kDecodeSets = 4, kFirstDecode = 6, kTokenWarp = kFirstDecode + 4 * kDecodeSets;
+constexpr int kThreads = 32 * (kTokenWarp + 1);
+// Stages at most; how many there are goes by the tokens of a tile.  A: 128 rows x 128 of k in tensor memory, beside the accumulators; W: packed units of 128
+// rows x 128 of k; B: tokens x 128 of k, two boxes of 64.
+constexpr int kAMost = 6, kWMost = 12, kBMost = 6;
+constexpr uint32_t kWStageBytes = 4 * kUnitBytes, kRingBytes = 212 * 1024;
+constexpr uint32_t kSmemBytes = 1024 + kRingBytes + 1024;
 constexpr int kMaxSplit = 8;
 
 struct GemmParams {
@@ -42,13 +43,15 @@ struct GemmParams {
   int tokens;                 // columns of a tile, a multiple of 16
   int row_tiles, tiles;       // tiles: row tiles x token tiles, row tiles first
   int split;                  // blocks of a cluster, which share the units of a tile (then each block has one)
-  int b_stages;
+  int a_stages, b_stages, w_stages;
+  int sets;                   // decoding sets at work: no more than A or W stages, since a set that is further ahead would take a stage's round for the one before
+  uint32_t acc_cols;          // columns of an accumulator
+  int accs;                   // accumulators: two where a block does several tiles
   int* status;
 };
 
-// two f16 that hold E2M1 values -> two bf16 times 2^-112: sign, and exponent and mantissa three places down
-__device__ __forceinline__ uint32_t f16_to_bf16_bits(uint32_t h) { return (h & 0x80008000u) | ((h >> 3) & 0x0FFF0FFFu); }
-
+// A pair of codes' f16 values times a block's scale, in the operand's type; both products are exact.  To bf16 by way of two f32, which a mixed-precision
+// multiplication gives at once: 54 cycles of an SM for 32 rows x 64 of k, against 75 where the bits are moved and multiplied in bf16, and 34 in f16.
 template <typename T>
 __device__ __forceinline__ uint32_t scaled(uint32_t pair, uint32_t scale);
 template <>
@@ -57,23 +60,23 @@ __device__ __forceinline__ uint32_t scaled<__half>(uint32_t pair, uint32_t scale
 }
 template <>
 __device__ __forceinline__ uint32_t scaled<__nv_bfloat16>(uint32_t pair, uint32_t scale) {
-  const uint32_t b = f16_to_bf16_bits(pair);
-  const __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&scale));
-  return *reinterpret_cast<const uint32_t*>(&r);
+  uint32_t r;
+  asm("{\n"
+      ".reg .b16 lo, hi, s, unused;\n"
+      ".reg .f32 a, b;\n"
+      "mov.b32 {lo, hi}, %1;\n"
+      "mov.b32 {s, unused}, %2;\n"
+      "fma.rn.f32.f16 a, lo, s, 0f80000000;\n"
+      "fma.rn.f32.f16 b, hi, s, 0f80000000;\n"
+      "cvt.rn.bf16x2.f32 %0, b, a;\n"
+      "}\n"
+      : "=r"(r)
+      : "r"(pair), "r"(scale));
+  return r;
 }
-// E4M3 byte -> the scale twice in a register: f16, or bf16 times 2^112 (which takes back what f16_to_bf16_bits leaves)
-template <typename T>
-__device__ __forceinline__ uint32_t scale_pair(uint32_t byte);
-template <>
-__device__ __forceinline__ uint32_t scale_pair<__half>(uint32_t byte) {
+// E4M3 byte -> the scale twice in a register, f16
+__device__ __forceinline__ uint32_t scale_pair(uint32_t byte) {
   return as_u32(__hmul2(as_half2(byte * 0x00800080u), as_half2(0x5C005C00u)));      // fields in place: times 2^-8
-}
-template <>
-__device__ __forceinline__ uint32_t scale_pair<__nv_bfloat16>(uint32_t byte) {
-  const uint32_t raw = byte * 0x00100010u, f1 = 0x7F007F00u, f2 = 0x74007400u;      // times 2^-120; 2^127, 2^105
-  __nv_bfloat162 r = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&raw), *reinterpret_cast<const __nv_bfloat162*>(&f1));
-  r = __hmul2(r, *reinterpret_cast<const __nv_bfloat162*>(&f2));
-  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 __device__ __forceinline__ void tcgen05_st_32x32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -130,12 +133,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t base = smem_u32(smem), w_ring = base + kBBytes, bars = w_ring + kWStages * kWStageBytes;
-  const uint32_t b_full = bars, b_empty = b_full + 8 * kBMost, w_full = b_empty + 8 * kBMost, w_empty = w_full + 8 * kWStages;
-  const uint32_t a_full = w_empty + 8 * kWStages, a_empty = a_full + 8 * kAStages, acc_full = a_empty + 8 * kAStages, acc_empty = acc_full + 16;
+  const uint32_t base = smem_u32(smem), bars = base + kRingBytes;
+  const uint32_t b_full = bars, b_empty = b_full + 8 * kBMost, w_full = b_empty + 8 * kBMost, w_empty = w_full + 8 * kWMost;
+  const uint32_t a_full = w_empty + 8 * kWMost, a_empty = a_full + 8 * kAMost, acc_full = a_empty + 8 * kAMost, acc_empty = acc_full + 16;
   const uint32_t tmem_ptr = acc_empty + 16;
   const int tokens = p.tokens, split = p.split, b_stages = p.b_stages;
-  const uint32_t b_bytes = (uint32_t)tokens * 128;
+  const uint32_t a_stages = p.a_stages, w_stages = p.w_stages, acc_cols = p.acc_cols, a_col = acc_cols * p.accs;
+  const uint32_t b_half = (uint32_t)tokens * 128, b_bytes = 2 * b_half, w_ring = base + b_stages * b_bytes;
   const int rank = split > 1 ? (int)blockIdx.x & (split - 1) : 0;
   const int first_tile = (int)blockIdx.x / split, step = (int)gridDim.x / split;
   const int unit_first = p.units * rank / split, n_units = p.units * (rank + 1) / split - unit_first;
@@ -145,11 +149,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       mbar_init(b_full + 8 * i, 1);
       mbar_init(b_empty + 8 * i, 1);
     }
-    for (int i = 0; i < kWStages; ++i) {
+    for (int i = 0; i < kWMost; ++i) {
       mbar_init(w_full + 8 * i, 1);
-      mbar_init(w_empty + 8 * i, 8);              // four warps for each of its 64 of k
+      mbar_init(w_empty + 8 * i, 4);
     }
-    for (int i = 0; i < kAStages; ++i) {
+    for (int i = 0; i < kAMost; ++i) {
       mbar_init(a_full + 8 * i, 4);
       mbar_init(a_empty + 8 * i, 1);
     }
@@ -174,34 +178,46 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
 
   if (warp == 0) {
-    // ------------------------------------------------------------------ copies
+    // ------------------------------------------------------------------ copies of the weight
     const bool leader = elect_one();
-    Slot b, w;
+    Slot w;
     bool ok = true;
-    b.phase = w.phase = 1;
+    w.phase = 1;
     for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
-      const int row_tile = tile % p.row_tiles, token0 = tile / p.row_tiles * tokens;
-      const int strip0 = row_tile * 4, strips = min(4, p.strips - strip0);
-      const uint8_t* src = p.packed + ((size_t)strip0 * p.units + unit_first) * kUnitBytes;
-      for (int u = 0; u < n_units && ok; ++u, src += kUnitBytes) {
+      const int strip0 = tile % p.row_tiles * 4;
+      int strips;
+      const uint8_t* src = p.packed + strip_at(strip0, p.strips, p.units, unit_first, strips) * kUnitBytes;
+      const uint32_t bytes = (uint32_t)strips * kUnitBytes;
+      for (int u = 0; u < n_units; ++u, src += bytes) {
         ok = mbar_wait_warp(w_empty + 8 * w.at, w.phase, status, 71);
         if (!ok) break;
         if (leader) {
-          const uint32_t bar = w_full + 8 * w.at, to = w_ring + w.at * kWStageBytes;
-          mbar_expect_tx(bar, (uint32_t)strips * kUnitBytes);
-          for (int s = 0; s < strips; ++s) bulk_load_1d(to + s * kUnitBytes, src + (size_t)s * p.units * kUnitBytes, kUnitBytes, bar);
-        }
-        w.next(kWStages);
-        for (int half = 0; half < 2; ++half) {
-          ok = mbar_wait_warp(b_empty + 8 * b.at, b.phase, status, 72);
-          if (!ok) break;
-          if (leader) {
-            mbar_expect_tx(b_full + 8 * b.at, b_bytes);
-            tma_load_2d(base + b.at * b_bytes, &map_x, ((unit_first + u) * 2 + half) * 128, token0, b_full + 8 * b.at);
-          }
-          b.next(b_stages);
+          mbar_expect_tx(w_full + 8 * w.at, bytes);
+          bulk_load_1d(w_ring + w.at * kWStageBytes, src, bytes, w_full + 8 * w.at);
         }
         __syncwarp();
+        w.next(w_stages);
+      }
+    }
+  } else if (warp == kTokenWarp) {
+    // ------------------------------------------------------------------ copies of the tokens
+    const bool leader = elect_one();
+    Slot b;
+    bool ok = true;
+    b.phase = 1;
+    for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
+      const int token0 = tile / p.row_tiles * tokens;
+      for (int u = 0; u < n_units; ++u) {
+        ok = mbar_wait_warp(b_empty + 8 * b.at, b.phase, status, 72);
+        if (!ok) break;
+        if (leader) {
+          const uint32_t bar = b_full + 8 * b.at, to = base + b.at * b_bytes;
+          mbar_expect_tx(bar, b_bytes);
+          tma_load_2d(to, &map_x, (unit_first + u) * 256, token0, bar);
+          tma_load_2d(to + b_half, &map_x, (unit_first + u) * 256 + 128, token0, bar);
+        }
+        __syncwarp();
+        b.next(b_stages);
       }
     }
   } else if (warp == 1) {
@@ -218,25 +234,26 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       ok = mbar_wait_warp(acc_empty + 8 * acc.at, acc.phase, status, 73);
       if (!ok) break;
       tcgen05_fence_after();
-      const uint32_t d = tmem + acc.at * kAccCols;
-      for (int k = 0; k < 2 * n_units; ++k) {
+      const uint32_t d = tmem + acc.at * acc_cols;
+      for (int u = 0; u < n_units; ++u) {
         ok = mbar_wait_warp(b_full + 8 * b.at, b.phase, status, 74) && mbar_wait_warp(a_full + 8 * a.at, a.phase, status, 75);
         if (!ok) break;
         tcgen05_fence_after();
         if (leader) {
           const uint64_t desc = b0 + (uint64_t)((b.at * b_bytes) >> 4);
-          const uint32_t from = tmem + kACol + a.at * 32;
+          const uint32_t from = tmem + a_col + a.at * 64;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) tcgen05_mma_ts(d, from + i * 8, desc + i * 2, idesc, (k > 0 || i > 0) ? 1u : 0u);
-          tcgen05_commit(b_empty + 8 * b.at);
+          for (int i = 0; i < 8; ++i)
+            tcgen05_mma_ts(d, from + i * 8, desc + (i & 3) * 2 + (i >> 2) * (b_half >> 4), idesc, (u > 0 || i > 0) ? 1u : 0u);
           tcgen05_commit(a_empty + 8 * a.at);
-          if (k == 2 * n_units - 1) tcgen05_commit(acc_full + 8 * acc.at);
+          tcgen05_commit(b_empty + 8 * b.at);
+          if (u == n_units - 1) tcgen05_commit(acc_full + 8 * acc.at);
         }
         __syncwarp();
+        a.next(a_stages);
         b.next(b_stages);
-        a.next(kAStages);
       }
-      acc.next(2);
+      acc.next(p.accs);
     }
   } else if (warp >= kFirstDecode) {
     // ------------------------------------------------------------------ decoding: a lane is a row
@@ -247,43 +264,51 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     for (int t = 0; t < 4; ++t) code_at[t] = quarter * kUnitBytes + tile16 * 1024 + chunk_at(r8, t) + upper * 8;
     const uint32_t scale_at = quarter * kUnitBytes + kUnitScales + r8 * 32 + tile16 * 4, scale_shift = upper * 8;
     bool ok = true;
-    uint32_t turn = 0;                             // of all steps of 64 of k; this set takes every third
-    for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
-      for (int k = 0; k < 2 * n_units; ++k, ++turn) {
-        if (turn % kDecodeSets != (uint32_t)set) continue;
-        const uint32_t ws = (turn >> 1) % kWStages, as = turn % kAStages;
-        ok = mbar_wait_warp(w_full + 8 * ws, ((turn >> 1) / kWStages) & 1, status, 76);
-        if (!ok) break;
-        const uint32_t unit = w_ring + ws * kWStageBytes, half = turn & 1;
-        uint2 code[4];
-        uint32_t sc[4];
+    // each set every `sets`th unit of all that the block does
+    int tiles = 0;
+    for (int tile = first_tile; tile < p.tiles; tile += step) ++tiles;
+    const int turns = set < p.sets ? tiles * n_units : 0;
+    Slot w, a;
+    a.phase = 1;                                   // the first round finds its stages free
+    for (int i = 0; i < set; ++i) {
+      w.next(w_stages);
+      a.next(a_stages);
+    }
+    for (int turn = set; turn < turns; turn += p.sets) {
+      ok = mbar_wait_warp(w_full + 8 * w.at, w.phase, status, 76);
+      if (!ok) break;
+      const uint32_t unit = w_ring + w.at * kWStageBytes;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          code[t] = lds64(unit + code_at[t] + half * 512);
-          sc[t] = (lds32(unit + scale_at + t * 8) >> (scale_shift + half * 16)) & 0x7Fu;
-        }
+      for (int half = 0; half < 2; ++half) {
         uint32_t v[32];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
+          const uint2 code = lds64(unit + code_at[t] + half * 512);
           uint32_t pair[8];
-          codes_to_pairs(code[t].x, *reinterpret_cast<uint32_t(*)[4]>(&pair[0]));
-          codes_to_pairs(code[t].y, *reinterpret_cast<uint32_t(*)[4]>(&pair[4]));
-          const uint32_t s = scale_pair<T>(sc[t]);
+          codes_to_pairs(code.x, *reinterpret_cast<uint32_t(*)[4]>(&pair[0]));
+          codes_to_pairs(code.y, *reinterpret_cast<uint32_t(*)[4]>(&pair[4]));
+          const uint32_t s = scale_pair((lds32(unit + scale_at + t * 8) >> (scale_shift + half * 16)) & 0x7Fu);
 #pragma unroll
           for (int i = 0; i < 8; ++i) v[t * 8 + i] = scaled<T>(pair[i], s);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(w_empty + 8 * ws);
-        if (turn >= kAStages) {
-          ok = mbar_wait_warp(a_empty + 8 * as, (turn / kAStages - 1) & 1, status, 77);
+        if (half == 0) {
+          ok = mbar_wait_warp(a_empty + 8 * a.at, a.phase, status, 77);
           if (!ok) break;
+          tcgen05_fence_after();
+        } else {
+          __syncwarp();
+          if (lane == 0) mbar_arrive(w_empty + 8 * w.at);
         }
-        tcgen05_fence_after();
-        tcgen05_st_32x32(tmem + kACol + lanes + as * 32, v);
-        tcgen05_wait_st();
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(a_full + 8 * as);
+        tcgen05_st_32x32(tmem + a_col + lanes + a.at * 64 + half * 32, v);
+      }
+      if (!ok) break;
+      tcgen05_wait_st();
+      tcgen05_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(a_full + 8 * a.at);
+      for (int i = 0; i < p.sets; ++i) {
+        w.next(w_stages);
+        a.next(a_stages);
       }
     }
   } else {
@@ -300,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       if (split > 1) break;                        // the only tile: its sums go to the cluster below
       for (int c = 0; c < n; c += 32) {
         uint32_t r[32];
-        tcgen05_ld_32x32(tmem + lanes + acc.at * kAccCols + c, r);
+        tcgen05_ld_32x32(tmem + lanes + acc.at * acc_cols + c, r);
         tcgen05_wait_ld();
         if (row < p.N) {
           const size_t at = (size_t)(token0 + c) * p.N + row;
@@ -312,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       tcgen05_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(acc_empty + 8 * acc.at);
-      acc.next(2);
+      acc.next(p.accs);
     }
   }
   __syncwarp();
@@ -383,8 +408,8 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
   p.row_tiles = (int)((c.N + kMmaRows - 1) / kMmaRows);
   p.status = c.status;
   const int sms = sm_count();
-  // Tokens of a tile and blocks that share one: the least time of the busiest block, in cycles.  64 of k take the MMAs two cycles a token, the copies one for each
-  // 57 bytes, and decoding 200.
+  // Tokens of a tile and blocks that share one: the least time of the busiest block, in cycles.  128 of k take the MMAs four cycles a token, the copies one for each
+  // 57 bytes, and decoding and issue 450.
   double best = 1e30;
   unsigned grid = 0;
   const int64_t least = (c.M + kMostTokens - 1) / kMostTokens;
@@ -396,7 +421,7 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
       const int clusters = split == 1 ? sms : resident_clusters_of(counts[split], w4a16_gemm_kernel<T>, split, kThreads, kSmemBytes);
       if (clusters < 1) break;
       if (split > 1 && tiles > clusters) break;    // a cluster does one tile
-      const double unit = std::max(std::max(4.0 * tokens, 400.0), (2.0 * tokens * 128 + 4.0 * kUnitBytes) / 57.0);
+      const double unit = std::max(std::max(4.0 * tokens, 450.0), (2.0 * tokens * 128 + 4.0 * kUnitBytes) / 57.0);
       const double waves = (double)((tiles + clusters - 1) / clusters);
       const double cost = waves * ((p.units + split - 1) / split * unit) + 2000.0 + tokens * 20.0 + (split > 1 ? 2000.0 + tokens * 20.0 : 0.0);
       if (cost < best) {
@@ -404,7 +429,14 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
         p.tokens = tokens;
         p.tiles = (int)tiles;
         p.split = split;
-        p.b_stages = (int)std::min<uint32_t>(kBMost, kBBytes / ((uint32_t)tokens * 128));
+        // Tensor memory: accumulators (two where a block has several tiles), the rest for A.  Shared memory: 120 KB of tokens at most, the rest for packed units, whose
+        // copies take longest.
+        p.accs = tiles > clusters ? 2 : 1;
+        p.acc_cols = (uint32_t)(tokens + 31) / 32 * 32;
+        p.a_stages = (int)std::min<uint32_t>(kAMost, (512 - p.accs * p.acc_cols) / 64);
+        p.b_stages = (int)std::min<uint32_t>(kBMost, 120 * 1024 / ((uint32_t)tokens * 256));
+        p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - (uint32_t)p.b_stages * tokens * 256) / kWStageBytes);
+        p.sets = std::min(kDecodeSets, std::min(p.a_stages, p.w_stages));
         grid = (unsigned)(std::min<int64_t>(clusters, tiles) * split);
       }
     }

@@ -45,6 +45,10 @@ def _linear(M, N, K, dtype, out_dtype=None, bias_dtype=None, pad=0, exact=True, 
     (257, 129, 176, F16, F32, None, 0),
     (300, 640, 2048, BF16, None, BF16, 0),
     (1029, 384, 512, F16, None, None, 0),
+    (577, 6465, 256, BF16, F32, None, 0),         # more tiles of the widest kind than blocks: two accumulators, few stages
+    (2000, 1300, 144, F16, None, F32, 0),
+    (18, 20000, 64, BF16, None, None, 8),         # more narrow ones
+    (48, 96, 8208, F16, F32, None, 0),            # one tile for a cluster
 ])
 def test_linear_exact(M, N, K, dtype, out_dtype, bias_dtype, pad):
     y, ref, _ = _linear(M, N, K, dtype, out_dtype, bias_dtype, pad)
