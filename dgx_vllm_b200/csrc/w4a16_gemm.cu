@@ -4,7 +4,7 @@
 // them straight into tensor memory, from where the MMA takes its A operand: a decoded weight never is in shared memory, and it is decoded once for
 // up to 192 tokens.  The activations are the B operand as they lie in memory, brought in by TMA, in the type they have: products are exact in bf16
 // and in f16 alike.
-// Roles (23 warps): 0 copies of the weight, 22 of the tokens, 1 MMAs and tensor memory, 2-5 epilogue, 6-21 decoding (four sets of four, a warp 32 rows of the tile
+// Roles (23 warps): 0 copies of the weight, 22 of the tokens, 1 MMAs and tensor memory, 2-5 (in the end 2-21) epilogue, 6-21 decoding (four sets of four, a warp 32 rows of the tile
 // and every fourth 128 of k).  One warp that brought in weight and tokens, four copies for 128 rows, took 1040 cycles for 128 of k and was what all waited for.
 // Tensor memory: accumulators, and the rest for A stages of 64 columns (128 rows x 128 of k): the MMA warp's waits, MMAs and commits take 300 cycles a
 // stage however few the tokens are.  Persistent blocks, one to an SM; where there are too few
@@ -25,9 +25,9 @@ using namespace w4;
 constexpr int kMmaRows = 128, kMostTokens = 192;
 constexpr int kDecodeSets = 4, kFirstDecode = 6, kTokenWarp = kFirstDecode + 4 * kDecodeSets;
 constexpr int kThreads = 32 * (kTokenWarp + 1);
-// Stages at most; how many there are goes by the tokens of a tile.  A: 128 rows x 128 of k in tensor memory, beside the accumulators; W: packed units of 128
-// rows x 128 of k; B: tokens x 128 of k, two boxes of 64.
-constexpr int kAMost = 6, kWMost = 12, kBMost = 6;
+// Stages at most; how many there are goes by the tokens of a tile.  Of the MMA's operands: 128 rows x 128 of k in tensor memory, beside the accumulators, and
+// tokens x 128 of k in shared memory, two boxes of 64; of packed units of 128 rows x 128 of k.
+constexpr int kMost = 6, kWMost = 12;
 constexpr uint32_t kWStageBytes = 4 * kUnitBytes, kRingBytes = 212 * 1024;
 constexpr uint32_t kSmemBytes = 1024 + kRingBytes + 1024;
 constexpr int kMaxSplit = 8;
@@ -43,8 +43,8 @@ struct GemmParams {
   int tokens;                 // columns of a tile, a multiple of 16
   int row_tiles, tiles;       // tiles: row tiles x token tiles, row tiles first
   int split;                  // blocks of a cluster, which share the units of a tile (then each block has one)
-  int a_stages, b_stages, w_stages;
-  int sets;                   // decoding sets at work: no more than A or W stages, since a set that is further ahead would take a stage's round for the one before
+  int stages, w_stages;
+  int sets;                   // decoding sets at work: no more than stages of either kind, since a set that is further ahead would take a stage's round for the one before
   uint32_t acc_cols;          // columns of an accumulator
   int accs;                   // accumulators: two where a block does several tiles
   int* status;
@@ -134,28 +134,23 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t base = smem_u32(smem), bars = base + kRingBytes;
-  const uint32_t b_full = bars, b_empty = b_full + 8 * kBMost, w_full = b_empty + 8 * kBMost, w_empty = w_full + 8 * kWMost;
-  const uint32_t a_full = w_empty + 8 * kWMost, a_empty = a_full + 8 * kAMost, acc_full = a_empty + 8 * kAMost, acc_empty = acc_full + 16;
-  const uint32_t tmem_ptr = acc_empty + 16;
-  const int tokens = p.tokens, split = p.split, b_stages = p.b_stages;
-  const uint32_t a_stages = p.a_stages, w_stages = p.w_stages, acc_cols = p.acc_cols, a_col = acc_cols * p.accs;
-  const uint32_t b_half = (uint32_t)tokens * 128, b_bytes = 2 * b_half, w_ring = base + b_stages * b_bytes;
+  const uint32_t full = bars, empty = full + 8 * kMost, w_full = empty + 8 * kMost, w_empty = w_full + 8 * kWMost;
+  const uint32_t acc_full = w_empty + 8 * kWMost, acc_empty = acc_full + 16, tmem_ptr = acc_empty + 16;
+  const int tokens = p.tokens, split = p.split;
+  const uint32_t stages = p.stages, w_stages = p.w_stages, acc_cols = p.acc_cols, a_col = acc_cols * p.accs;
+  const uint32_t b_half = (uint32_t)tokens * 128, b_bytes = 2 * b_half, w_ring = base + stages * b_bytes;
   const int rank = split > 1 ? (int)blockIdx.x & (split - 1) : 0;
   const int first_tile = (int)blockIdx.x / split, step = (int)gridDim.x / split;
   const int unit_first = p.units * rank / split, n_units = p.units * (rank + 1) / split - unit_first;
   int* const status = p.status;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBMost; ++i) {
-      mbar_init(b_full + 8 * i, 1);
-      mbar_init(b_empty + 8 * i, 1);
+    for (int i = 0; i < kMost; ++i) {
+      mbar_init(full + 8 * i, 5);                  // the tokens, and each of a set's four warps
+      mbar_init(empty + 8 * i, 1);
     }
     for (int i = 0; i < kWMost; ++i) {
       mbar_init(w_full + 8 * i, 1);
       mbar_init(w_empty + 8 * i, 4);
-    }
-    for (int i = 0; i < kAMost; ++i) {
-      mbar_init(a_full + 8 * i, 4);
-      mbar_init(a_empty + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(acc_full + 8 * i, 1);
@@ -208,16 +203,16 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
       const int token0 = tile / p.row_tiles * tokens;
       for (int u = 0; u < n_units; ++u) {
-        ok = mbar_wait_warp(b_empty + 8 * b.at, b.phase, status, 72);
+        ok = mbar_wait_warp(empty + 8 * b.at, b.phase, status, 72);
         if (!ok) break;
         if (leader) {
-          const uint32_t bar = b_full + 8 * b.at, to = base + b.at * b_bytes;
+          const uint32_t bar = full + 8 * b.at, to = base + b.at * b_bytes;
           mbar_expect_tx(bar, b_bytes);
           tma_load_2d(to, &map_x, (unit_first + u) * 256, token0, bar);
           tma_load_2d(to + b_half, &map_x, (unit_first + u) * 256 + 128, token0, bar);
         }
         __syncwarp();
-        b.next(b_stages);
+        b.next(stages);
       }
     }
   } else if (warp == 1) {
@@ -227,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(tokens >> 3) << 17) | ((uint32_t)(kMmaRows >> 4) << 24);
     const uint64_t b0 = desc_kmajor<128>(base);
-    Slot b, a, acc;
+    Slot op, acc;
     bool ok = true;
     acc.phase = 1;
     for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
@@ -236,22 +231,21 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       tcgen05_fence_after();
       const uint32_t d = tmem + acc.at * acc_cols;
       for (int u = 0; u < n_units; ++u) {
-        ok = mbar_wait_warp(b_full + 8 * b.at, b.phase, status, 74) && mbar_wait_warp(a_full + 8 * a.at, a.phase, status, 75);
+        // One wait and one commit for 128 of k: with barriers of their own for the two operands the loop took 650 cycles for few tokens.
+        ok = mbar_wait_warp(full + 8 * op.at, op.phase, status, 74);
         if (!ok) break;
         tcgen05_fence_after();
         if (leader) {
-          const uint64_t desc = b0 + (uint64_t)((b.at * b_bytes) >> 4);
-          const uint32_t from = tmem + a_col + a.at * 64;
+          const uint64_t desc = b0 + (uint64_t)((op.at * b_bytes) >> 4);
+          const uint32_t from = tmem + a_col + op.at * 64;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             tcgen05_mma_ts(d, from + i * 8, desc + (i & 3) * 2 + (i >> 2) * (b_half >> 4), idesc, (u > 0 || i > 0) ? 1u : 0u);
-          tcgen05_commit(a_empty + 8 * a.at);
-          tcgen05_commit(b_empty + 8 * b.at);
+          tcgen05_commit(empty + 8 * op.at);
           if (u == n_units - 1) tcgen05_commit(acc_full + 8 * acc.at);
         }
         __syncwarp();
-        a.next(a_stages);
-        b.next(b_stages);
+        op.next(stages);
       }
       acc.next(p.accs);
     }
@@ -272,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     a.phase = 1;                                   // the first round finds its stages free
     for (int i = 0; i < set; ++i) {
       w.next(w_stages);
-      a.next(a_stages);
+      a.next(stages);
     }
     for (int turn = set; turn < turns; turn += p.sets) {
       ok = mbar_wait_warp(w_full + 8 * w.at, w.phase, status, 76);
@@ -292,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
           for (int i = 0; i < 8; ++i) v[t * 8 + i] = scaled<T>(pair[i], s);
         }
         if (half == 0) {
-          ok = mbar_wait_warp(a_empty + 8 * a.at, a.phase, status, 77);
+          ok = mbar_wait_warp(empty + 8 * a.at, a.phase, status, 77);
           if (!ok) break;
           tcgen05_fence_after();
         } else {
@@ -305,72 +299,99 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       tcgen05_wait_st();
       tcgen05_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(a_full + 8 * a.at);
+      if (lane == 0) mbar_arrive(full + 8 * a.at);
       for (int i = 0; i < p.sets; ++i) {
         w.next(w_stages);
-        a.next(a_stages);
+        a.next(stages);
       }
-    }
-  } else {
-    // ------------------------------------------------------------------ epilogue: a lane is a row of the weight, a column a token
-    const int quarter = warp & 3;
-    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    const float g = *p.g;
-    Slot acc;
-    for (int tile = first_tile; tile < p.tiles; tile += step) {
-      const int row = tile % p.row_tiles * kMmaRows + quarter * 32 + lane, token0 = tile / p.row_tiles * tokens, n = min(tokens, p.M - token0);
-      const float bias = p.bias != nullptr && row < p.N && split == 1 ? load_value(p.bias, p.bias_dtype, row) : 0.f;
-      if (!mbar_wait_warp(acc_full + 8 * acc.at, acc.phase, status, 78)) break;
-      tcgen05_fence_after();
-      if (split > 1) break;                        // the only tile: its sums go to the cluster below
-      for (int c = 0; c < n; c += 32) {
-        uint32_t r[32];
-        tcgen05_ld_32x32(tmem + lanes + acc.at * acc_cols + c, r);
-        tcgen05_wait_ld();
-        if (row < p.N) {
-          const size_t at = (size_t)(token0 + c) * p.N + row;
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i < n) store_value(p.out, p.out_dtype, at + (size_t)i * p.N, __uint_as_float(r[i]) * g + bias);
-        }
-      }
-      tcgen05_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(acc_empty + 8 * acc.at);
-      acc.next(p.accs);
     }
   }
   __syncwarp();
-  if (split > 1) {
-    // Token t of the tile is finished by block t / (tokens / split): [source][its tokens][128 rows] of f32, where the token stages were
-    cluster_sync_any();                            // all MMAs of the cluster have read theirs
-    const int own = tokens / split, tile = first_tile;
-    if (warp >= 2 && warp < 6) {
-      const int quarter = warp & 3;
-      for (int c = 0; c < tokens; c += 16) {
-        uint32_t r[16];
-        tcgen05_ld_32x16(tmem + ((uint32_t)(quarter * 32) << 16) + c, r);
-        tcgen05_wait_ld();
+  // ---------------------------------------------------------------------- epilogue: a lane is a row of the weight, a column a token
+  const int quarter = warp & 3;
+  const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+  // columns from, from + by, ... of a tile of n tokens, 32 at a time
+  auto write_columns = [&](uint32_t acc, int row, int token0, int n, int from, int by, float g) {
+    const float bias = p.bias != nullptr && row < p.N ? load_value(p.bias, p.bias_dtype, row) : 0.f;
+    for (int c = from; c < n; c += by) {
+      uint32_t r[32];
+      tcgen05_ld_32x32(tmem + lanes + acc + c, r);
+      tcgen05_wait_ld();
+      if (row >= p.N) continue;
+      const size_t at = (size_t)(token0 + c) * p.N + row;
+      const int most = n - c;
+      if (p.out_dtype == B200FP4_DTYPE_BF16) {
+        __nv_bfloat16* const to = static_cast<__nv_bfloat16*>(p.out) + at;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int t = c + i, owner = t / own;
-          const uint32_t to = base + ((uint32_t)(rank * own + t - owner * own) * kMmaRows + quarter * 32 + lane) * 4;
-          asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(map_to_cta(to, owner)), "r"(r[i]) : "memory");
-        }
+        for (int i = 0; i < 32; ++i)
+          if (i < most) to[(size_t)i * p.N] = __float2bfloat16_rn(__uint_as_float(r[i]) * g + bias);
+      } else if (p.out_dtype == B200FP4_DTYPE_F16) {
+        __half* const to = static_cast<__half*>(p.out) + at;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i < most) to[(size_t)i * p.N] = __float2half_rn(__uint_as_float(r[i]) * g + bias);
+      } else {
+        float* const to = static_cast<float*>(p.out) + at;
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+          if (i < most) to[(size_t)i * p.N] = __uint_as_float(r[i]) * g + bias;
       }
     }
-    cluster_sync_any();
+  };
+  if (p.accs > 1) {
+    // several tiles: four warps, while the others go on
+    if (warp >= 2 && warp < kFirstDecode) {
+      const float g = *p.g;
+      Slot acc;
+      for (int tile = first_tile; tile < p.tiles; tile += step) {
+        const int token0 = tile / p.row_tiles * tokens;
+        if (!mbar_wait_warp(acc_full + 8 * acc.at, acc.phase, status, 78)) break;
+        tcgen05_fence_after();
+        write_columns(acc.at * acc_cols, tile % p.row_tiles * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), 0, 32, g);
+        tcgen05_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + 8 * acc.at);
+        acc.next(2);
+      }
+    }
+  } else {
+    // one tile: all warps that are left, five to a quarter of tensor memory
+    const bool work = warp >= 2 && warp < kTokenWarp;
+    const int nth = (warp - 2) >> 2, row_tile = first_tile % p.row_tiles, token0 = first_tile / p.row_tiles * tokens;
+    bool ok = true;
+    if (work) ok = mbar_wait_warp(acc_full, 0, status, 79);
+    tcgen05_fence_after();
     const float g = *p.g;
-    const int row0 = tile % p.row_tiles * kMmaRows, token0 = tile / p.row_tiles * tokens + rank * own;
-    const float* const sums = reinterpret_cast<const float*>(smem);
-    for (int i = threadIdx.x; i < own * kMmaRows; i += kThreads) {
-      const int m = token0 + i / kMmaRows, row = row0 + i % kMmaRows;
-      if (m >= p.M || row >= p.N) continue;
-      float v = 0.f;
-      for (int s = 0; s < split; ++s) v += sums[s * own * kMmaRows + i];
-      v *= g;
-      if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
-      store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
+    if (split == 1) {
+      if (work && ok) write_columns(0, row_tile * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), nth * 32, 5 * 32, g);
+    } else {
+      // Token t of the tile is finished by block t / (tokens / split): [source][its tokens][128 rows] of f32, where the token stages were
+      cluster_sync_any();                          // all MMAs of the cluster have read theirs
+      const int own = tokens / split;
+      if (work)
+        for (int c = nth * 16; c < tokens; c += 5 * 16) {
+          uint32_t r[16];
+          tcgen05_ld_32x16(tmem + lanes + c, r);
+          tcgen05_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int t = c + i, owner = t / own;
+            const uint32_t to = base + ((uint32_t)(rank * own + t - owner * own) * kMmaRows + quarter * 32 + lane) * 4;
+            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(map_to_cta(to, owner)), "r"(r[i]) : "memory");
+          }
+        }
+      cluster_sync_any();
+      const int row0 = row_tile * kMmaRows, first = token0 + rank * own;
+      const float* const sums = reinterpret_cast<const float*>(smem);
+      for (int i = threadIdx.x; i < own * kMmaRows; i += kThreads) {
+        const int m = first + i / kMmaRows, row = row0 + i % kMmaRows;
+        if (m >= p.M || row >= p.N) continue;
+        float v = 0.f;
+        for (int s = 0; s < split; ++s) v += sums[s * own * kMmaRows + i];
+        v *= g;
+        if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
+        store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
+      }
     }
   }
   tcgen05_fence_before();
@@ -429,14 +450,13 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
         p.tokens = tokens;
         p.tiles = (int)tiles;
         p.split = split;
-        // Tensor memory: accumulators (two where a block has several tiles), the rest for A.  Shared memory: 120 KB of tokens at most, the rest for packed units, whose
+        // Tensor memory: accumulators (two where a block has several tiles), the rest for the weight.  Shared memory: 144 KB of tokens at most, the rest for packed units, whose
         // copies take longest.
         p.accs = tiles > clusters ? 2 : 1;
         p.acc_cols = (uint32_t)(tokens + 31) / 32 * 32;
-        p.a_stages = (int)std::min<uint32_t>(kAMost, (512 - p.accs * p.acc_cols) / 64);
-        p.b_stages = (int)std::min<uint32_t>(kBMost, 120 * 1024 / ((uint32_t)tokens * 256));
-        p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - (uint32_t)p.b_stages * tokens * 256) / kWStageBytes);
-        p.sets = std::min(kDecodeSets, std::min(p.a_stages, p.w_stages));
+        p.stages = (int)std::min<uint32_t>(kMost, std::min<uint32_t>((512 - p.accs * p.acc_cols) / 64, 144 * 1024 / ((uint32_t)tokens * 256)));
+        p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - (uint32_t)p.stages * tokens * 256) / kWStageBytes);
+        p.sets = std::min(kDecodeSets, std::min(p.stages, p.w_stages));
         grid = (unsigned)(std::min<int64_t>(clusters, tiles) * split);
       }
     }
