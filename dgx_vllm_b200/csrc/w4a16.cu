@@ -5,8 +5,8 @@
 //   linear   columns are tokens
 //   gate/up  columns are the (token, expert) pairs of one expert; a tile's rows are eight gate rows and the same eight up rows, so that a
 //            lane holds both halves of its values and applies SiLU(gate) * up to them
-//   down     two columns a pair, the activation's upper and lower part in f16: their sum has 22 bits, so that the value between the projections is
-//            not what limits the result
+//   down     the value between the projections in f16, brought into its range by a power of two for each pair: eleven bits, where a bf16 result keeps eight.  For an
+//            f16 or f32 result it is two f16, upper and lower part, in two columns: their sum has 22 bits
 // Work items are (strip of 32 rows, slot); a slot is a run of one expert's pairs that fits the columns.  A block has a contiguous range of them, groups of
 // warps take items in turn and split k among themselves.
 // The layer is two launches without anything that has to outlast them: both find the slots from the routing by themselves, the first sets the
@@ -84,8 +84,10 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
 
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr uint32_t kSmemMost = 227 * 1024;
-constexpr int kStages = 3;                     // units of a warp's ring
-constexpr uint32_t kRingBytes = kWarps * kStages * kUnitBytes, kBarBytes = kWarps * kStages * 8;
+// Units of a warp's ring: three, two where partial sums and rows for more columns need the room.  Two keep as much of HBM busy, but bear less unevenness.
+__host__ __device__ __forceinline__ constexpr int stages_of(int cols) { return cols == 1 ? 3 : 2; }
+__host__ __device__ __forceinline__ constexpr uint32_t ring_bytes(int cols) { return kWarps * stages_of(cols) * kUnitBytes; }
+__host__ __device__ __forceinline__ constexpr uint32_t bar_bytes(int cols) { return kWarps * stages_of(cols) * 8; }
 
 __host__ __device__ __forceinline__ uint32_t pad16(uint32_t v) { return (v + 15) / 16 * 16; }
 __host__ __device__ __forceinline__ constexpr uint32_t red_bytes(int cols) { return kWarps * 2 * cols * 4 * 32 * 4; }
@@ -109,6 +111,7 @@ __device__ __forceinline__ float load_value(const void* p, int dtype, size_t at)
 }
 
 // A warp's ring of units: one lane asks for them, all wait for them.  Every unit that was asked for is waited for.
+template <int kStages>
 struct Ring {
   uint32_t units, bars, stage, phase, fill;
   bool ok;
@@ -364,7 +367,7 @@ struct LinearLayout {
 };
 __host__ __device__ __forceinline__ LinearLayout linear_layout(int cols, int cap, uint32_t row_bytes, int split, int items) {
   LinearLayout l;
-  l.red = pad16(kRingBytes + kBarBytes);
+  l.red = pad16(ring_bytes(cols) + bar_bytes(cols));
   l.inv = l.red + red_bytes(cols);
   l.parts = pad16(l.inv + (uint32_t)cap * 4);
   l.rows = l.parts + kWarps * 8;
@@ -381,8 +384,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   constexpr bool kConvert = std::is_same<XT, __nv_bfloat16>::value;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
   const uint32_t base = smem_u32(smem), chunk = chunk_at(row8, quad);
-  Ring ring;
-  ring.init(base, base + kRingBytes, warp, lane);
+  Ring<stages_of(kCols)> ring;
+  ring.init(base, base + ring_bytes(kCols), warp, lane);
   const int split = p.split, rank = (int)blockIdx.x & (split - 1), cluster = (int)blockIdx.x / split;      // split: a power of two
   const int unit_first = p.units * rank / split, own_units = p.units * (rank + 1) / split - unit_first;
   const int share = 1 << p.log_share, group = warp >> p.log_share, in_group = warp & (share - 1), n_groups = kWarps >> p.log_share;
@@ -404,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   };
   pdl_wait();
 #pragma unroll 1
-  for (int i = 0; i < kStages; ++i) fetch();
+  for (int i = 0; i < stages_of(kCols); ++i) fetch();
   pdl_launch_dependents();
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
   if (split > 1) cluster_arrive();                 // the other blocks run before anything is sent to them
@@ -576,7 +579,7 @@ constexpr int kMaxPairs = 2048;                // pairs whose slots a block find
 constexpr int kMaxExperts = 4096;
 
 struct MoeParams {
-  const void* x;              // gate/up [M, K], rows ldx apart; down: [pair][upper, lower][K] f16
+  const void* x;              // gate/up [M, K], rows ldx apart; down: [pair][part][K] f16
   int64_t ldx;
   const uint8_t* packed;
   const float* g;             // [E]; gate/up [E][gate, up]
@@ -613,7 +616,7 @@ struct MoeLayout {
 __host__ __device__ __forceinline__ int count_bytes(int pairs) { return (pairs + 511) / 512 * 16; }
 __host__ __device__ __forceinline__ MoeLayout moe_layout(int cols, int pairs, int E, int cap, int rows, uint32_t row_bytes) {
   MoeLayout l;
-  l.red = pad16(kRingBytes + kBarBytes);
+  l.red = pad16(ring_bytes(cols) + bar_bytes(cols));
   l.expert = l.red + red_bytes(cols);
   l.list = pad16(l.expert + (uint32_t)pairs * 2);
   l.start = pad16(l.list + (uint32_t)pairs * 2);
@@ -652,6 +655,7 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
   uint32_t* const scan = reinterpret_cast<uint32_t*>(smem + l.scan);
   int e[kMost], place[kMost];
   uint32_t leads[kMost];                           // the first pair of an expert: its pairs | its slots << 16
+  const bool busy = warp * 32 < P;                 // a warp without pairs only comes to the barriers
 #pragma unroll
   for (int q = 0; q < kMost; ++q) {
     const int i = q * kThreads + threadIdx.x;
@@ -662,6 +666,7 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
 #pragma unroll
   for (int q = 0; q < kMost; ++q) {
     if (q * kThreads >= P) break;
+    if (q * kThreads + warp * 32 >= P) break;
     const uint32_t same = __match_any_sync(0xffffffffu, e[q]), before = same & ((1u << lane) - 1);
     place[q] = __popc(before);
     if (e[q] >= 0 && before == 0) smem[l.rows + e[q] * bytes + q * kWarps + warp] = (unsigned char)__popc(same);
@@ -674,11 +679,17 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
     if (q * kThreads >= P || e[q] < 0) continue;
     uint32_t before = 0, all = 0;
     const int at = q * kWarps + warp;              // this pair's 32
-    for (int w = 0; w < bytes / 4; ++w) {
-      const uint32_t c = *reinterpret_cast<const uint32_t*>(smem + l.rows + e[q] * bytes + w * 4);
-      all = __dp4a(c, 0x01010101u, all);
-      const int ahead = at - w * 4;                // bytes of this word that count pairs before
-      if (ahead > 0) before = __dp4a(ahead >= 4 ? c : c & ((1u << (ahead * 8)) - 1), 0x01010101u, before);
+#pragma unroll
+    for (int v = 0; v < kMost; ++v) {
+      if (v * 16 >= bytes) break;
+      const uint4 c4 = *reinterpret_cast<const uint4*>(smem + l.rows + e[q] * bytes + v * 16);
+      const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        all = __dp4a(c[w], 0x01010101u, all);
+        const int ahead = at - v * 16 - w * 4;     // bytes of this word that count pairs before
+        if (ahead > 0) before = __dp4a(ahead >= 4 ? c[w] : c[w] & ((1u << (ahead * 8)) - 1), 0x01010101u, before);
+      }
     }
     place[q] += before;
     if (place[q] == 0) leads[q] = all | ((all + cap - 1) / cap << 16);
@@ -686,11 +697,12 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
   }
   // pairs and slots before this thread's: an exclusive scan
   uint32_t sum = mine;
+  if (busy)
 #pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const uint32_t a = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += a;
-  }
+    for (int d = 1; d < 32; d *= 2) {
+      const uint32_t a = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += a;
+    }
   if (lane == 31) scan[warp] = sum;
   __syncthreads();
   uint32_t warps = lane < kWarps ? scan[lane] : 0;
@@ -719,8 +731,8 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
   return total;
 }
 
-// XT: type of the activations (gate/up); kDown: the second projection; kCols: columns of eight
-template <typename XT, bool kDown, int kCols>
+// XT: type of the activations (gate/up); kDown: the second projection; kCols: columns of eight; kParts: f16 parts of a value between the projections
+template <typename XT, bool kDown, int kCols, int kParts>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
@@ -730,8 +742,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   const uint16_t* const expert = reinterpret_cast<const uint16_t*>(smem + l.expert);
   const int2* const slots = reinterpret_cast<const int2*>(smem + l.slots);
   const uint16_t* const list = reinterpret_cast<const uint16_t*>(smem + l.list);
-  Ring ring;
-  ring.init(base, base + kRingBytes, warp, lane);
+  Ring<stages_of(kCols)> ring;
+  ring.init(base, base + ring_bytes(kCols), warp, lane);
   // The routing is not the first projection's work, and its kernel lets this one start only once what came before it is complete: the second
   // projection finds its slots and asks for its first weights while the first one ends.
   clear_counts(p, smem, l);
@@ -779,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     --ahead_left;
   };
 #pragma unroll 1
-  for (int i = 0; i < kStages; ++i) fetch();
+  for (int i = 0; i < stages_of(kCols); ++i) fetch();
   float* const red = reinterpret_cast<float*>(smem + l.red);
 
   if constexpr (!kDown) {
@@ -797,19 +809,28 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       if (end > first) __syncthreads();            // nobody reads the rows before these any more
       end = min(last, stop * fast);
       slot = stop;
+      // asked for before the rows, needed behind them
+      float gate_peak = 0.f, up_peak = 0.f, w = 1.f;
+      const int own = (int)threadIdx.x < n_rows ? list[row0 + threadIdx.x] : -1;
+      if (own >= 0) {
+        const int x = expert[own];
+        gate_peak = p.g[2 * x] * p.peaks[2 * x];
+        up_peak = p.g[2 * x + 1] * p.peaks[2 * x + 1];
+        if (p.weight_on_input) w = p.weights[own];
+      }
       stage_rows<XT, true>(
           n_rows, 0, p.K, p.units * kUnitK, smem + l.rows, row_bytes, reinterpret_cast<float2*>(smem + l.parts),
           [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)(list[row0 + r] / p.topk) * p.ldx; },
-          [&](int r, float inv, float squares) {
-            // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the
-            // bound is far above the values costs nothing while act's two parts reach 40 binades down.
-            const int pair = list[row0 + r], x = expert[pair];
-            const float norm = sqrtf(squares * (float)p.K) * (p.weight_on_input ? p.weights[pair] : 1.f);
-            const float bound = fabsf(norm * p.g[2 * x] * p.peaks[2 * x]) * fabsf(norm * p.g[2 * x + 1] * p.peaks[2 * x + 1]);
-            const int up = min(max(14 - ((int)(__float_as_uint(bound) >> 23) - 126), -100), 100);
-            stats[r] = {inv, pow2(up)};
-            p.act_inv[pair] = pow2(-up);
-          });
+          [&](int r, float inv, float squares) { stats[r] = {inv, squares}; });
+      __syncthreads();
+      if (own >= 0) {
+        // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the bound is
+        // far above the values costs little: f16 reaches 40 binades down.
+        const float norm = sqrtf(stats[threadIdx.x].act * (float)p.K) * w, bound = fabsf(norm * gate_peak) * fabsf(norm * up_peak);
+        const int up = min(max(14 - ((int)(__float_as_uint(bound) >> 23) - 126), -100), 100);
+        stats[threadIdx.x].act = pow2(up);
+        p.act_inv[own] = pow2(-up);
+      }
       __syncthreads();
       for (; at.item < end; next(at)) {
         const int2 s = slots[at.hi];
@@ -838,9 +859,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
           const float v = silu_f32(gate * f * p.g[2 * e]) * (up * f * p.g[2 * e + 1]) * st.act;
           const __half hi = __float2half_rn(v);
           const float rest = v - __half2float(hi);
-          __half* const to = p.act + (size_t)pair * 2 * I + i_at;
+          __half* const to = p.act + (size_t)pair * kParts * I + i_at;
           to[0] = hi;
-          to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
+          if (kParts == 2) to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
         });
       }
     }
@@ -859,8 +880,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       const __half* act[kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
-        const int i = c * 4 + row8 / 2;            // a pair's columns are its upper and its lower part
-        act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i < n ? i : 0)] * 2 + (row8 & 1)) * p.ldx + quad * 16;
+        const int i = (c * 8 + row8) / kParts;     // a pair's columns are its parts
+        act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i < n ? i : 0)] * kParts + (kParts == 2 ? row8 & 1 : 0)) * p.ldx + quad * 16;
       }
       float acc[2][kCols][4] = {};
       uint32_t b[2][kCols][8];
@@ -902,11 +923,19 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
           if (ring.ok) fetch();
         }
       }
-      finish_item<kCols, true>(red, share, in_group, group, lane, acc, [&](int t, int c, int i, float upper, float lower) {
-        const int column = c * 4 + quad, row = strip * 32 + t * 16 + i * 8 + row8;
-        if (column >= n || row >= p.N) return;
+      finish_item<kCols, kParts == 2>(red, share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb) {
+        // two parts: the columns of one pair in one row; one: two rows of one pair
+        const int column = kParts == 2 ? c * 4 + quad : c * 8 + quad * 2 + i, row = strip * 32 + t * 16 + row8 + (kParts == 2 ? i * 8 : 0);
+        if (column >= n) return;
         const int pair = list[s.y + column];
-        p.y[(size_t)pair * p.N + row] = (upper + lower) * (p.act_inv[pair] * p.g[e]);
+        const float f = p.act_inv[pair] * p.g[e];
+        float* const to = p.y + (size_t)pair * p.N + row;
+        if (kParts == 2) {
+          if (row < p.N) to[0] = (va + vb) * f;
+        } else {
+          if (row < p.N) to[0] = va * f;
+          if (row + 8 < p.N) to[8] = vb * f;
+        }
       });
     }
     ring.drain();
@@ -933,55 +962,73 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       const uint32_t mask = *flag;
       __syncthreads();
       const int per_strip = p.M * 8, count = __popc(mask) * per_strip;
-      for (int i = threadIdx.x; i < count; i += kThreads) {
-        const int nth = i / per_strip, m = (i - nth * per_strip) >> 3, row = (strip0 + __fns(mask, 0, nth + 1)) * 32 + (i & 7) * 4;
-        if (row >= p.N) continue;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s0 = 0; s0 < p.topk; s0 += 8) {
-          float4 v[8];
+      // four outputs of a token each, two of them and eight of their pairs at a time: all that is asked for is on its way before the first is needed
+      for (int i0 = threadIdx.x; i0 < count; i0 += 2 * kThreads) {
+        int m[2], row[2];
+        bool inside[2];
+        float4 sum[2];
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int pair = m * p.topk + s0 + u;
-            v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-            if (s0 + u < p.topk && expert[pair] != 0xFFFF) v[u] = __ldcg(reinterpret_cast<const float4*>(p.y + (size_t)pair * p.N + row));
-          }
-#pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int pair = m * p.topk + s0 + u;
-            if (s0 + u < p.topk && expert[pair] != 0xFFFF) {
-              const float w = weights[pair];
-              sum.x += w * v[u].x;
-              sum.y += w * v[u].y;
-              sum.z += w * v[u].z;
-              sum.w += w * v[u].w;
-            }
-          }
+        for (int h = 0; h < 2; ++h) {
+          const int i = i0 + h * kThreads, nth = i / per_strip;
+          m[h] = (i - nth * per_strip) >> 3;
+          row[h] = i < count ? (strip0 + __fns(mask, 0, nth + 1)) * 32 + (i & 7) * 4 : p.N;
+          inside[h] = row[h] < p.N;
+          sum[h] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
-        const size_t to = (size_t)m * p.N + row;
-        store_value(p.out, p.out_dtype, to, sum.x);
-        store_value(p.out, p.out_dtype, to + 1, sum.y);
-        store_value(p.out, p.out_dtype, to + 2, sum.z);
-        store_value(p.out, p.out_dtype, to + 3, sum.w);
+        for (int s0 = 0; s0 < p.topk; s0 += 8) {
+          float4 v[2][8];
+          float w[2][8];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              const int pair = m[h] * p.topk + s0 + u;
+              v[h][u] = make_float4(0.f, 0.f, 0.f, 0.f);
+              w[h][u] = 0.f;
+              if (inside[h] && s0 + u < p.topk && expert[pair] != 0xFFFF) {
+                v[h][u] = __ldcg(reinterpret_cast<const float4*>(p.y + (size_t)pair * p.N + row[h]));
+                w[h][u] = weights[pair];
+              }
+            }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              sum[h].x += w[h][u] * v[h][u].x;
+              sum[h].y += w[h][u] * v[h][u].y;
+              sum[h].z += w[h][u] * v[h][u].z;
+              sum[h].w += w[h][u] * v[h][u].w;
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!inside[h]) continue;
+          const size_t to = (size_t)m[h] * p.N + row[h];
+          store_value(p.out, p.out_dtype, to, sum[h].x);
+          store_value(p.out, p.out_dtype, to + 1, sum[h].y);
+          store_value(p.out, p.out_dtype, to + 2, sum[h].z);
+          store_value(p.out, p.out_dtype, to + 3, sum[h].w);
+        }
       }
     }
   }
 }
 
-template <typename XT, bool kDown, int kCols>
+template <typename XT, bool kDown, int kCols, int kParts>
 int launch_moe_of(MoeParams p, cudaStream_t st) {
   static std::once_flag once[64];
   static bool ready[64];
-  if (!allow_smem(w4a16_moe_kernel<XT, kDown, kCols>, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
+  if (!allow_smem(w4a16_moe_kernel<XT, kDown, kCols, kParts>, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
   const int pairs = p.M * p.topk;
   const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;
-  p.cap = (kDown ? 4 : 8) * kCols;
+  p.cap = 8 * kCols / (kDown ? kParts : 1);
   p.rows = 0;
   while (!kDown) {
     // rows that there is room for; a slot has no more columns than that
     const uint32_t rest = moe_layout(kCols, pairs, p.E, p.cap, 0, 0).rows + 16;      // the counts lie where the rows come
-    p.rows = rest < kSmemMost ? (int)std::min<uint32_t>((uint32_t)pairs, (kSmemMost - rest) / (row_bytes + (uint32_t)sizeof(RowStat))) : 0;
+    p.rows = rest < kSmemMost ? (int)std::min<uint32_t>((uint32_t)std::min(pairs, kThreads), (kSmemMost - rest) / (row_bytes + (uint32_t)sizeof(RowStat))) : 0;
     if (p.rows < 1) return B200FP4_STATUS_NOT_SUPPORTED;
-    if (p.rows >= p.cap || p.rows == pairs) break;
+    if (p.rows >= std::min(p.cap, pairs)) break;
     p.cap = p.rows;
   }
   const uint32_t smem = moe_layout(kCols, pairs, p.E, p.cap, p.rows, row_bytes).bytes;
@@ -991,19 +1038,29 @@ int launch_moe_of(MoeParams p, cudaStream_t st) {
   const double each = std::min(1.0, local / ((double)p.M * p.E)), reached = p.E * (1.0 - std::pow(1.0 - each, p.M));
   const double slots = std::max(1.0, std::max(reached, local / p.cap));
   p.log_share = share_of((int)(slots * p.strips / sm_count()) + 1, p.units);
-  if (launch_pdl(w4a16_moe_kernel<XT, kDown, kCols>, dim3(sm_count()), dim3(kThreads), smem, st, p) != cudaSuccess) {
+  if (launch_pdl(w4a16_moe_kernel<XT, kDown, kCols, kParts>, dim3(sm_count()), dim3(kThreads), smem, st, p) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
   return finish_launch(1);
 }
 
-template <typename T>
-int launch_gate_up(const MoeParams& p, cudaStream_t st) {
-  return (int64_t)p.M * p.topk <= 4 * (int64_t)p.E ? launch_moe_of<T, false, 1>(p, st) : launch_moe_of<T, false, 2>(p, st);
+// Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  Up to as many pairs an expert as
+// one column of eight holds, few have more.
+template <typename T, int kParts>
+int launch_gate_up(const MoeParams& p, double each, cudaStream_t st) {
+  return each <= 7 ? launch_moe_of<T, false, 1, kParts>(p, st) : launch_moe_of<T, false, 2, kParts>(p, st);
 }
-int launch_down(const MoeParams& p, cudaStream_t st) {
-  return (int64_t)p.M * p.topk <= 2 * (int64_t)p.E ? launch_moe_of<__half, true, 1>(p, st) : launch_moe_of<__half, true, 2>(p, st);
+template <int kParts>
+int launch_down(const MoeParams& p, double each, cudaStream_t st) {
+  return each * kParts <= 7 ? launch_moe_of<__half, true, 1, kParts>(p, st) : launch_moe_of<__half, true, 2, kParts>(p, st);
+}
+template <int kParts>
+int launch_layer(const MoeParams& up, const MoeParams& down, int h_dtype, cudaStream_t st) {
+  // pairs of an expert of this call, as a router without favourites gives them
+  const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
+  const int rc = h_dtype == B200FP4_DTYPE_BF16 ? launch_gate_up<__nv_bfloat16, kParts>(up, each, st) : launch_gate_up<__half, kParts>(up, each, st);
+  return rc == B200FP4_STATUS_SUCCESS ? launch_down<kParts>(down, each, st) : rc;
 }
 
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
@@ -1145,8 +1202,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     d.K = (int)I;
     d.strips = (int)w4::strips_of(H);
     d.units = (int)w4::units_of(I);
-    int rc = h_dtype == B200FP4_DTYPE_BF16 ? launch_gate_up<__nv_bfloat16>(p, st) : launch_gate_up<__half>(p, st);
-    if (rc == B200FP4_STATUS_SUCCESS) rc = launch_down(d, st);
+    const int rc = out_dtype == B200FP4_DTYPE_BF16 ? launch_layer<1>(p, d, h_dtype, st) : launch_layer<2>(p, d, h_dtype, st);
     if (rc != B200FP4_STATUS_SUCCESS) return rc;
   }
   return B200FP4_STATUS_SUCCESS;
