@@ -90,7 +90,7 @@ SIGNATURES = {
     "b200fp4_w4a16_packed_bytes": (_sz, [_i64, _i64, _i64, _i32]),
     "b200fp4_w4a16_pack": (_i32, [_vp, _vp, _i64, _i64, _i64, _i32, _vp, _vp]),
     "b200fp4_w4a16_linear": (_i32, [_vp, _i32, _i64, _vp, _vp, _vp, _i32, _vp, _i32, _i64, _i64, _i64, _vp, _vp]),
-    "b200fp4_w4a16_moe_workspace_bytes": (_sz, [_i64] * 5),
+    "b200fp4_w4a16_moe_workspace_bytes": (_sz, [_i64] * 4),
     "b200fp4_w4a16_moe": (_i32, [_vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i64, _i64, _i64, _i64, _i32,
                                  _vp, _vp, _sz, _vp]),
     "b200fp4_fused_sparse_moe_host_async": (_i32, [_vp, _i32, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp,

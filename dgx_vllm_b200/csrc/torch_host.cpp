@@ -583,7 +583,7 @@ B200_FN(py_w4a16_moe) {
         const at::Tensor ids = (ids_in.scalar_type() == at::kInt ? ids_in : ids_in.to(at::kInt)).contiguous();
         const at::Tensor tw = (tw_in.scalar_type() == at::kFloat ? tw_in : tw_in.to(at::kFloat)).contiguous();
         cudaStream_t st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
-        const Scratch ws(dev, st, b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I, E));
+        const Scratch ws(dev, st, b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I));
         check(b200fp4_w4a16_moe(ptr(x), dtype_code(x.scalar_type()), ptr<float>(tw), ptr<int32_t>(ids), emap ? ptr<int32_t>(*emap) : nullptr,
                                 emap ? emap->numel() : 0, ptr<uint8_t>(w13), ptr<float>(g13), ptr<uint8_t>(w2), ptr<float>(g2), ptr(out),
                                 dtype_code(out.scalar_type()), M, topk, H, I, E, flags, ws.status(), ws.data(), ws.bytes(), st),

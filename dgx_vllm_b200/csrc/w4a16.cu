@@ -273,53 +273,76 @@ __device__ __forceinline__ void look_at(const uint4& v, uint32_t& top, float& su
 
 // Rows [0, n_rows) -> f16 in shared memory, row_bytes apart, elements [k_begin, k_end) and zeros up to k_stop; all threads.  row_at(r): the row's
 // elements; seen(r, factor's reciprocal, sum of squares): called once a row.  Few rows are shared by several warps.
-template <typename T, bool kSquares, typename RowAt, typename Seen>
-__device__ __forceinline__ void stage_rows(int n_rows, int k_begin, int k_end, int k_stop, unsigned char* rows, uint32_t row_bytes, float2* parts, RowAt&& row_at,
-                                           Seen&& seen) {
-  constexpr bool kConvert = std::is_same<T, __nv_bfloat16>::value;
-  constexpr int kHeld = 4;                         // pieces that a lane keeps between looking at them and writing them; others are read again
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  int log_parts = 4;
-  while (log_parts > 0 && (n_rows << log_parts) > kWarps) --log_parts;
-  const int n_parts = 1 << log_parts, octets = (k_end - k_begin) >> 3;
-#pragma unroll 1
-  for (int i0 = 0; i0 < n_rows << log_parts; i0 += kWarps) {
-    const int r = (i0 + warp) >> log_parts, part = (i0 + warp) & (n_parts - 1);
-    const bool work = r < n_rows;
-    const int k0 = k_begin + ((octets * part) >> log_parts) * 8 + lane * 8, k1 = work ? k_begin + ((octets * (part + 1)) >> log_parts) * 8 : 0;
-    const T* const row = work ? row_at(r) : nullptr;
-    uint4 held[kHeld];
+// In two steps: what ask() loads is on its way before a block asks for its weights, behind which it would wait for some 2 us.
+template <typename T, bool kSquares>
+struct StagedRows {
+  static constexpr bool kConvert = std::is_same<T, __nv_bfloat16>::value;
+  static constexpr int kHeld = 4;                  // pieces that a lane holds; others are read when they are needed
+  int n_rows, k_begin, k_end, log_parts;
+  uint4 held[kHeld];
+
+  __device__ __forceinline__ void range(int part, int& k0, int& k1) const {
+    const int octets = (k_end - k_begin) >> 3;
+    k0 = k_begin + ((octets * part) >> log_parts) * 8 + (threadIdx.x & 31) * 8;
+    k1 = k_begin + ((octets * (part + 1)) >> log_parts) * 8;
+  }
+  __device__ __forceinline__ void hold(const T* row, int k0, int k1) {
 #pragma unroll
     for (int h = 0; h < kHeld; ++h)
       if (k0 + h * 256 < k1) held[h] = ld_u4(row + k0 + h * 256);
-    uint32_t factor = 0;
-    float inv = 1.f, squares = 0.f;
-    if constexpr (kConvert || kSquares) {
-      uint32_t top = 0;
+  }
+  template <typename RowAt>
+  __device__ __forceinline__ void ask(int rows, int begin, int end, RowAt&& row_at) {
+    n_rows = rows;
+    k_begin = begin;
+    k_end = end;
+    log_parts = 4;
+    while (log_parts > 0 && (n_rows << log_parts) > kWarps) --log_parts;
+    const int warp = threadIdx.x >> 5, r = warp >> log_parts;
+    int k0, k1;
+    range(warp & ((1 << log_parts) - 1), k0, k1);
+    if (r < n_rows) hold(row_at(r), k0, k1);
+  }
+  template <typename RowAt, typename Seen>
+  __device__ __forceinline__ void finish(int k_stop, unsigned char* rows, uint32_t row_bytes, float2* parts, RowAt&& row_at, Seen&& seen) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n_parts = 1 << log_parts;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n_rows << log_parts; i0 += kWarps) {
+      const int r = (i0 + warp) >> log_parts, part = (i0 + warp) & (n_parts - 1);
+      const bool work = r < n_rows;
+      int k0, k1;
+      range(part, k0, k1);
+      if (!work) k1 = 0;
+      const T* const row = work ? row_at(r) : nullptr;
+      if (i0 > 0) hold(row, k0, k1);
+      uint32_t factor = 0;
+      float inv = 1.f, squares = 0.f;
+      if constexpr (kConvert || kSquares) {
+        uint32_t top = 0;
 #pragma unroll
-      for (int h = 0; h < kHeld; ++h)
-        if (k0 + h * 256 < k1) look_at<T, kSquares>(held[h], top, squares);
+        for (int h = 0; h < kHeld; ++h)
+          if (k0 + h * 256 < k1) look_at<T, kSquares>(held[h], top, squares);
 #pragma unroll 2
-      for (int k = k0 + kHeld * 256; k < k1; k += 256) look_at<T, kSquares>(ld_u4(row + k), top, squares);
-      top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
-      if constexpr (kSquares)
+        for (int k = k0 + kHeld * 256; k < k1; k += 256) look_at<T, kSquares>(ld_u4(row + k), top, squares);
+        top = __reduce_max_sync(0xffffffffu, max(top & 0xFFFFu, top >> 16));
+        if constexpr (kSquares)
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) squares += __shfl_xor_sync(0xffffffffu, squares, d);
-      if (n_parts > 1) {                           // one round then
-        if (lane == 0) parts[warp] = make_float2(__uint_as_float(top), squares);
-        __syncthreads();
-        squares = 0.f;
-        for (int j = 0; j < n_parts; ++j) {        // in the same order for every warp of the row
-          const float2 u = parts[warp - part + j];
-          top = max(top, __float_as_uint(u.x));
-          squares += u.y;
+          for (int d = 16; d > 0; d /= 2) squares += __shfl_xor_sync(0xffffffffu, squares, d);
+        if (n_parts > 1) {                         // one round then
+          if (lane == 0) parts[warp] = make_float2(__uint_as_float(top), squares);
+          __syncthreads();
+          squares = 0.f;
+          for (int j = 0; j < n_parts; ++j) {      // in the same order for every warp of the row
+            const float2 u = parts[warp - part + j];
+            top = max(top, __float_as_uint(u.x));
+            squares += u.y;
+          }
         }
+        const int e = kConvert ? row_exponent(top) : 0;
+        factor = (uint32_t)(e + 127) * 0x00800080u;
+        inv = pow2(-e);
       }
-      const int e = kConvert ? row_exponent(top) : 0;
-      factor = (uint32_t)(e + 127) * 0x00800080u;
-      inv = pow2(-e);
-    }
-    if (work) {
+      if (!work) continue;
       unsigned char* const to = rows + r * row_bytes - k_begin * 2;
       auto put = [&](int k, uint4 v) {
         if constexpr (kConvert)
@@ -337,7 +360,7 @@ __device__ __forceinline__ void stage_rows(int n_rows, int k_begin, int k_end, i
         if (part == 0 && lane == 0) seen(r, inv, squares);
     }
   }
-}
+};
 
 // ------------------------------------------------------------------------------------------ linear layer of few tokens
 
@@ -397,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   auto fetch = [&]() {
     if (ahead_left == 0) {
       if (ahead >= last) return;
-      src = p.packed + strip_at(ahead % p.strips, p.strips, p.units, unit_first + k_first, src_step) * kUnitBytes;
+      src = p.packed + (size_t)strip_at(ahead % p.strips, p.strips, p.units, unit_first + k_first, src_step) * kUnitBytes;
       ahead_left = n_units;
       ahead += n_groups;
     }
@@ -405,7 +428,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
     src += src_step * kUnitBytes;
     --ahead_left;
   };
+  const int k_begin = unit_first * kUnitK, k_stop = (unit_first + own_units) * kUnitK, k_end = min(p.K, k_stop);
+  StagedRows<XT, false> staged;
+  int m0 = first / p.strips * p.cap;
+  auto row_at = [&](int r) { return static_cast<const XT*>(p.x) + (m0 + r) * p.ldx; };
   pdl_wait();
+  staged.ask(min(p.cap, p.M - m0), k_begin, k_end, row_at);
 #pragma unroll 1
   for (int i = 0; i < stages_of(kCols); ++i) fetch();
   pdl_launch_dependents();
@@ -420,11 +448,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   int item = first + group;
   for (int done = first; done < last;) {
     // one slot of tokens at a time
-    const int slot = done / p.strips, m0 = slot * p.cap, n = min(p.cap, p.M - m0), end = min(last, (slot + 1) * p.strips);
-    if (done > first) __syncthreads();             // nobody reads the rows before these any more
-    stage_rows<XT, false>(n, unit_first * kUnitK, min(p.K, (unit_first + own_units) * kUnitK), (unit_first + own_units) * kUnitK, smem + l.rows, row_bytes,
-                          reinterpret_cast<float2*>(smem + l.parts), [&](int r) { return static_cast<const XT*>(p.x) + (m0 + r) * p.ldx; },
-                          [&](int r, float v, float) { inv[r] = v; });
+    const int slot = done / p.strips, end = min(last, (slot + 1) * p.strips);
+    m0 = slot * p.cap;
+    const int n = min(p.cap, p.M - m0);
+    if (done > first) {
+      __syncthreads();                             // nobody reads the rows before these any more
+      staged.ask(n, k_begin, k_end, row_at);
+    }
+    staged.finish(k_stop, smem + l.rows, row_bytes, reinterpret_cast<float2*>(smem + l.parts), row_at, [&](int r, float v, float) { inv[r] = v; });
     __syncthreads();
     uint32_t col[kCols];
 #pragma unroll
@@ -607,26 +638,25 @@ struct MoeParams {
 struct RowStat {
   float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
 };
-// Shared memory behind the rings and barriers: partial sums of warps | expert of a pair | pairs by expert | first place of an expert | slots | scan | routing
-// weights (down) | statistics of the staged rows | parts of those | the rows in f16, and before them the counts
+// Shared memory behind the rings and barriers: partial sums of warps | expert of a pair | pairs by expert, and as they came | first place of an expert | slots | scan |
+// routing weights (down) | statistics of the staged rows | parts of those | the rows in f16, and before them an expert's pairs
 struct MoeLayout {
-  uint32_t red, expert, list, start, slots, scan, weights, stats, parts, rows, bytes;
+  uint32_t red, expert, list, came, start, slots, scan, weights, stats, parts, rows, bytes;
 };
-// Bytes of an expert in the table of counts: one for each 32 pairs
-__host__ __device__ __forceinline__ int count_bytes(int pairs) { return (pairs + 511) / 512 * 16; }
 __host__ __device__ __forceinline__ MoeLayout moe_layout(int cols, int pairs, int E, int cap, int rows, uint32_t row_bytes) {
   MoeLayout l;
   l.red = pad16(ring_bytes(cols) + bar_bytes(cols));
   l.expert = l.red + red_bytes(cols);
   l.list = pad16(l.expert + (uint32_t)pairs * 2);
-  l.start = pad16(l.list + (uint32_t)pairs * 2);
+  l.came = pad16(l.list + (uint32_t)pairs * 2);
+  l.start = pad16(l.came + (uint32_t)pairs * 2);
   l.slots = pad16(l.start + (uint32_t)E * 2);
   l.scan = pad16(l.slots + (uint32_t)((pairs < E ? pairs : E) + pairs / cap) * 8);
-  l.weights = l.scan + kWarps * 4;
+  l.weights = l.scan + 36 * 4;
   l.stats = pad16(l.weights + (rows > 0 ? 0 : (uint32_t)pairs * 4));
   l.parts = pad16(l.stats + (uint32_t)rows * sizeof(RowStat));
   l.rows = l.parts + kWarps * 8;
-  const uint32_t counts = (uint32_t)E * count_bytes(pairs), staged = (uint32_t)rows * row_bytes;
+  const uint32_t counts = pad16((uint32_t)E * 4), staged = (uint32_t)rows * row_bytes;
   l.bytes = l.rows + (counts > staged ? counts : staged);
   return l;
 }
@@ -637,72 +667,48 @@ __device__ __forceinline__ int local_expert(const MoeParams& p, int pair) {
   return e >= 0 && e < p.E ? (int)e : -1;
 }
 
-// Counts to zero; needs nothing of the call's inputs
+// An expert's pairs to zero; needs nothing of the call's inputs
 __device__ __forceinline__ void clear_counts(const MoeParams& p, unsigned char* smem, const MoeLayout& l) {
-  for (int i = threadIdx.x; i < p.E * count_bytes(p.M * p.topk) / 16; i += kThreads) *reinterpret_cast<uint4*>(smem + l.rows + i * 16) = make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < p.E; i += kThreads) reinterpret_cast<int*>(smem + l.rows)[i] = 0;
 }
 
-// Slots (expert | pairs << 16, first place in the list): runs of at most `cap` pairs of one expert, pairs in their order.  Every block finds the same ones,
-// whatever the order in which its threads run; returns their number.  A warp takes 32 pairs at a time and counts those of the same expert among them
-// into a table [expert][32 pairs]; a pair's place is the sum of its expert's counts before its own 32 and its place among those.
+// Slots (expert | pairs << 16, first place in the list): runs of at most `cap` pairs of one expert, experts in order and pairs in theirs.  Every block finds the
+// same ones, whatever the order in which its threads run: pairs are counted and gathered by expert as they come, and then each takes the place that the number
+// of smaller ones in its expert's run gives it.  Returns the number of slots.
 __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* smem, const MoeLayout& l) {
   constexpr int kMost = kMaxPairs / kThreads;
-  const int cap = p.cap, P = p.M * p.topk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, bytes = count_bytes(P);
+  const int cap = p.cap, P = p.M * p.topk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint16_t* const expert = reinterpret_cast<uint16_t*>(smem + l.expert);
   uint16_t* const list = reinterpret_cast<uint16_t*>(smem + l.list);
+  uint16_t* const came = reinterpret_cast<uint16_t*>(smem + l.came);
   uint16_t* const start = reinterpret_cast<uint16_t*>(smem + l.start);
   int2* const slots = reinterpret_cast<int2*>(smem + l.slots);
   uint32_t* const scan = reinterpret_cast<uint32_t*>(smem + l.scan);
-  int e[kMost], place[kMost];
-  uint32_t leads[kMost];                           // the first pair of an expert: its pairs | its slots << 16
-  const bool busy = warp * 32 < P;                 // a warp without pairs only comes to the barriers
+  int* const count = reinterpret_cast<int*>(smem + l.rows);
+  int e[kMost], at[kMost];
 #pragma unroll
   for (int q = 0; q < kMost; ++q) {
     const int i = q * kThreads + threadIdx.x;
     e[q] = i < P ? local_expert(p, i) : -1;
-    if (i < P) expert[i] = (uint16_t)e[q];
   }
   __syncthreads();                                 // the counts are clear
 #pragma unroll
   for (int q = 0; q < kMost; ++q) {
-    if (q * kThreads >= P) break;
-    if (q * kThreads + warp * 32 >= P) break;
-    const uint32_t same = __match_any_sync(0xffffffffu, e[q]), before = same & ((1u << lane) - 1);
-    place[q] = __popc(before);
-    if (e[q] >= 0 && before == 0) smem[l.rows + e[q] * bytes + q * kWarps + warp] = (unsigned char)__popc(same);
+    const int i = q * kThreads + threadIdx.x;
+    if (i < P) expert[i] = (uint16_t)e[q];
+    at[q] = e[q] >= 0 ? atomicAdd(&count[e[q]], 1) : 0;
   }
   __syncthreads();
+  // a run of experts a thread; their pairs | slots << 16, and an exclusive scan of those over the threads
+  const int per = (p.E + kThreads - 1) / kThreads, e0 = min(p.E, (int)threadIdx.x * per), e1 = min(p.E, e0 + per);
   uint32_t mine = 0;
-#pragma unroll
-  for (int q = 0; q < kMost; ++q) {
-    leads[q] = 0;
-    if (q * kThreads >= P || e[q] < 0) continue;
-    uint32_t before = 0, all = 0;
-    const int at = q * kWarps + warp;              // this pair's 32
-#pragma unroll
-    for (int v = 0; v < kMost; ++v) {
-      if (v * 16 >= bytes) break;
-      const uint4 c4 = *reinterpret_cast<const uint4*>(smem + l.rows + e[q] * bytes + v * 16);
-      const uint32_t c[4] = {c4.x, c4.y, c4.z, c4.w};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        all = __dp4a(c[w], 0x01010101u, all);
-        const int ahead = at - v * 16 - w * 4;     // bytes of this word that count pairs before
-        if (ahead > 0) before = __dp4a(ahead >= 4 ? c[w] : c[w] & ((1u << (ahead * 8)) - 1), 0x01010101u, before);
-      }
-    }
-    place[q] += before;
-    if (place[q] == 0) leads[q] = all | ((all + cap - 1) / cap << 16);
-    mine += leads[q];
-  }
-  // pairs and slots before this thread's: an exclusive scan
+  for (int x = e0; x < e1; ++x) mine += (uint32_t)count[x] | ((uint32_t)(count[x] + cap - 1) / cap << 16);
   uint32_t sum = mine;
-  if (busy)
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const uint32_t a = __shfl_up_sync(0xffffffffu, sum, d);
-      if (lane >= d) sum += a;
-    }
+  for (int d = 1; d < 32; d *= 2) {
+    const uint32_t a = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += a;
+  }
   if (lane == 31) scan[warp] = sum;
   __syncthreads();
   uint32_t warps = lane < kWarps ? scan[lane] : 0;
@@ -713,20 +719,27 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
   }
   const uint32_t others = __shfl_sync(0xffffffffu, warps, warp > 0 ? warp - 1 : 0);
   const int total = (int)(__shfl_sync(0xffffffffu, warps, kWarps - 1) >> 16);
-  uint32_t at = sum - mine + (warp > 0 ? others : 0);
-#pragma unroll
-  for (int q = 0; q < kMost; ++q) {
-    if (leads[q] == 0) continue;
-    const int pairs = leads[q] & 0xFFFF, first = at & 0xFFFF;
-    int slot = at >> 16;
-    start[e[q]] = (uint16_t)first;
-    for (int c = 0; c < pairs; c += cap) slots[slot++] = make_int2(e[q] | (min(cap, pairs - c) << 16), first + c);
-    at += leads[q];
+  uint32_t next = sum - mine + (warp > 0 ? others : 0);
+  for (int x = e0; x < e1; ++x) {
+    const int pairs = count[x], first = next & 0xFFFF;
+    int slot = next >> 16;
+    start[x] = (uint16_t)first;
+    for (int c = 0; c < pairs; c += cap) slots[slot++] = make_int2(x | (min(cap, pairs - c) << 16), first + c);
+    next = (next & 0xFFFF0000u) + ((uint32_t)(slot - (int)(next >> 16)) << 16) + first + pairs;
   }
   __syncthreads();
 #pragma unroll
   for (int q = 0; q < kMost; ++q)
-    if (q * kThreads < P && e[q] >= 0) list[start[e[q]] + place[q]] = (uint16_t)(q * kThreads + threadIdx.x);
+    if (e[q] >= 0) came[start[e[q]] + at[q]] = (uint16_t)(q * kThreads + threadIdx.x);
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kMost; ++q) {
+    if (e[q] < 0) continue;
+    const int i = q * kThreads + threadIdx.x, first = start[e[q]], n = count[e[q]];
+    int place = first;
+    for (int j = first; j < first + n; ++j) place += came[j] < i;
+    list[place] = (uint16_t)i;
+  }
   __syncthreads();
   return total;
 }
@@ -781,8 +794,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   auto fetch = [&]() {
     if (ahead_left == 0) {
       if (ahead.item >= last) return;
-      const size_t e = slots[kDown ? ahead.lo : ahead.hi].x & 0xFFFF;
-      src = p.packed + (e * p.strips * p.units + strip_at(kDown ? ahead.hi : ahead.lo, p.strips, p.units, k_first, src_step)) * kUnitBytes;
+      const int e = slots[kDown ? ahead.lo : ahead.hi].x & 0xFFFF;
+      src = p.packed + (size_t)(e * p.strips * p.units + strip_at(kDown ? ahead.hi : ahead.lo, p.strips, p.units, k_first, src_step)) * kUnitBytes;
       ahead_left = n_units;
       next(ahead);
     }
@@ -790,8 +803,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     src += src_step * kUnitBytes;
     --ahead_left;
   };
-#pragma unroll 1
-  for (int i = 0; i < stages_of(kCols); ++i) fetch();
   float* const red = reinterpret_cast<float*>(smem + l.red);
 
   if constexpr (!kDown) {
@@ -801,15 +812,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     }
     RowStat* const stats = reinterpret_cast<RowStat*>(smem + l.stats);
     // Rows are staged for as many slots at a time as there is room for: slots [slot, stop), the pairs in places [row0, row0 + n_rows) of the list
+    StagedRows<XT, true> staged;
     int slot = last > first ? first / fast : 0;
     for (int end = first; end < last;) {
       const int slots_end = (last - 1) / fast + 1, row0 = slots[slot].y;
       int stop = slot + 1, n_rows = slots[slot].x >> 16;
       while (stop < slots_end && n_rows + (slots[stop].x >> 16) <= p.rows) n_rows += slots[stop++].x >> 16;
       if (end > first) __syncthreads();            // nobody reads the rows before these any more
-      end = min(last, stop * fast);
-      slot = stop;
-      // asked for before the rows, needed behind them
+      auto row_at = [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)(list[row0 + r] / p.topk) * p.ldx; };
+      staged.ask(n_rows, 0, p.K, row_at);
       float gate_peak = 0.f, up_peak = 0.f, w = 1.f;
       const int own = (int)threadIdx.x < n_rows ? list[row0 + threadIdx.x] : -1;
       if (own >= 0) {
@@ -818,10 +829,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         up_peak = p.g[2 * x + 1] * p.peaks[2 * x + 1];
         if (p.weight_on_input) w = p.weights[own];
       }
-      stage_rows<XT, true>(
-          n_rows, 0, p.K, p.units * kUnitK, smem + l.rows, row_bytes, reinterpret_cast<float2*>(smem + l.parts),
-          [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)(list[row0 + r] / p.topk) * p.ldx; },
-          [&](int r, float inv, float squares) { stats[r] = {inv, squares}; });
+      if (end == first)
+#pragma unroll 1
+        for (int i = 0; i < stages_of(kCols); ++i) fetch();
+      end = min(last, stop * fast);
+      slot = stop;
+      staged.finish(p.units * kUnitK, smem + l.rows, row_bytes, reinterpret_cast<float2*>(smem + l.parts), row_at,
+                    [&](int r, float inv, float squares) { stats[r] = {inv, squares}; });
       __syncthreads();
       if (own >= 0) {
         // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the bound is
@@ -867,6 +881,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     }
     ring.drain();
   } else {
+#pragma unroll 1
+    for (int i = 0; i < stages_of(kCols); ++i) fetch();
     pdl_wait();
     pdl_launch_dependents();
     if (n_slots == 0) {
@@ -941,12 +957,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     ring.drain();
     // The block that completes a strip adds up every token's pairs, in the order of the routing.
     const float* const weights = reinterpret_cast<const float*>(smem + l.weights);
-    uint32_t* const flag = reinterpret_cast<uint32_t*>(smem + l.scan);
+    int* const done_strips = reinterpret_cast<int*>(smem + l.scan);
+    int& n_done = done_strips[32];
     __threadfence();
     __syncthreads();
     if (last == first) return;
     const int strip_first = first / n_slots, strip_end = (last - 1) / n_slots + 1;
     for (int strip0 = strip_first; strip0 < strip_end; strip0 += 32) {
+      if (strip0 > strip_first) __syncthreads();
       if (warp == 0) {
         const int strip = strip0 + lane;
         bool mine = false;
@@ -956,12 +974,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         }
         const uint32_t mask = __ballot_sync(0xffffffffu, mine);
         __threadfence();
-        if (lane == 0) *flag = mask;
+        if (mine) done_strips[__popc(mask & ((1u << lane) - 1))] = strip;
+        if (lane == 0) n_done = __popc(mask);
       }
       __syncthreads();
-      const uint32_t mask = *flag;
-      __syncthreads();
-      const int per_strip = p.M * 8, count = __popc(mask) * per_strip;
+      const int per_strip = p.M * 8, count = n_done * per_strip;
       // four outputs of a token each, two of them and eight of their pairs at a time: all that is asked for is on its way before the first is needed
       for (int i0 = threadIdx.x; i0 < count; i0 += 2 * kThreads) {
         int m[2], row[2];
@@ -971,7 +988,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         for (int h = 0; h < 2; ++h) {
           const int i = i0 + h * kThreads, nth = i / per_strip;
           m[h] = (i - nth * per_strip) >> 3;
-          row[h] = i < count ? (strip0 + __fns(mask, 0, nth + 1)) * 32 + (i & 7) * 4 : p.N;
+          row[h] = i < count ? done_strips[nth] * 32 + (i & 7) * 4 : p.N;
           inside[h] = row[h] < p.N;
           sum[h] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
@@ -1074,17 +1091,15 @@ size_t unit_bytes(int64_t E, int64_t N, int64_t K, int gated) {
   return (size_t)E * packed_strips(N, gated) * units_of(K) * kUnitBytes;
 }
 
-// pairs of a turn: the table of counts takes 32 KB (64 KB from 2049 experts)
-int64_t pairs_of_turn(int64_t E) { return E <= 512 ? kMaxPairs : (E <= 1024 ? kMaxPairs / 2 : kMaxPairs / 4); }
 // tokens of a layer whose pairs fit one turn
-int64_t turn_of(int64_t M, int64_t topk, int64_t E) { return std::min(M, std::max<int64_t>(1, pairs_of_turn(E) / topk)); }
+int64_t turn_of(int64_t M, int64_t topk) { return std::min(M, std::max<int64_t>(1, kMaxPairs / topk)); }
 
 struct MoeScratch {
   size_t act, act_inv, y, counters, bytes;
 };
-MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E) {
+MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I) {
   MoeScratch s;
-  const size_t pairs = (size_t)turn_of(M, topk, E) * topk;
+  const size_t pairs = (size_t)turn_of(M, topk) * topk;
   s.act = 0;
   s.act_inv = s.act + pad256(pairs * 2 * I * 2);
   s.y = s.act_inv + pad256(pairs * 4);
@@ -1142,9 +1157,9 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   return x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(c, st) : launch_linear<__half>(c, st);
 }
 
-extern "C" size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E) {
-  if (M < 1 || topk < 1 || H < 1 || I < 1 || E < 1) return 0;
-  return moe_scratch(M, topk, H, I, E).bytes;
+extern "C" size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I) {
+  if (M < 1 || topk < 1 || H < 1 || I < 1) return 0;
+  return moe_scratch(M, topk, H, I).bytes;
 }
 
 extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* topk_weights, const int32_t* topk_ids, const int32_t* expert_map,
@@ -1158,13 +1173,15 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
       w2_g == nullptr || out == nullptr || status == nullptr || (expert_map != nullptr && global_E < 1))
     return B200FP4_STATUS_INVALID_VALUE;
   if (!aligned(hidden, 16) || !aligned(w13_packed, 16) || !aligned(w2_packed, 16) || !aligned(out, 16)) return B200FP4_STATUS_INVALID_VALUE;
-  if (E > kMaxExperts || topk > pairs_of_turn(E) || !fits_int(M * topk) || !fits_int(H + 128) || !fits_int(2 * I + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
-  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I, E))
+  if (E > kMaxExperts || topk > kMaxPairs || !fits_int(M * topk) || !fits_int(H + 128) || !fits_int(2 * I + 128) || !fits_int(E * (2 * I / 32 + 1) * (H / 128 + 1)) ||
+      !fits_int(E * (H / 32 + 1) * (I / 128 + 1)))
+    return B200FP4_STATUS_NOT_SUPPORTED;
+  if (workspace == nullptr || !aligned(workspace, 256) || workspace_bytes < b200fp4_w4a16_moe_workspace_bytes(M, topk, H, I))
     return B200FP4_STATUS_ALLOC_FAILED;
-  const MoeScratch s = moe_scratch(M, topk, H, I, E);
+  const MoeScratch s = moe_scratch(M, topk, H, I);
   unsigned char* const ws = static_cast<unsigned char*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int64_t turn = turn_of(M, topk, E);
+  const int64_t turn = turn_of(M, topk);
   for (int64_t m = 0; m < M; m += turn) {
     MoeParams p = {};
     p.M = (int)std::min(turn, M - m);

@@ -32,8 +32,9 @@ __host__ __device__ __forceinline__ int64_t strips_of(int64_t rows) { return (ro
 __host__ __device__ __forceinline__ int64_t units_of(int64_t K) { return (K + kUnitK - 1) / kUnitK; }
 
 // Units of a matrix before those of a strip of 32 rows, and from one 128 of k to the next
-__host__ __device__ __forceinline__ int64_t strip_at(int64_t strip, int64_t strips, int64_t units, int64_t unit, int& step) {
-  const int64_t block = strip & ~(int64_t)3;
+template <typename Int>
+__host__ __device__ __forceinline__ Int strip_at(Int strip, Int strips, Int units, Int unit, int& step) {
+  const Int block = strip & ~(Int)3;
   step = (int)(strips - block < 4 ? strips - block : 4);
   return block * units + unit * step + (strip - block);
 }

@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
       const int strip0 = tile % p.row_tiles * 4;
       int strips;
-      const uint8_t* src = p.packed + strip_at(strip0, p.strips, p.units, unit_first, strips) * kUnitBytes;
+      const uint8_t* src = p.packed + (size_t)strip_at(strip0, p.strips, p.units, unit_first, strips) * kUnitBytes;
       const uint32_t bytes = (uint32_t)strips * kUnitBytes;
       for (int u = 0; u < n_units; ++u, src += bytes) {
         ok = mbar_wait_warp(w_empty + 8 * w.at, w.phase, status, 71);

@@ -501,11 +501,11 @@ B200FP4_API int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, co
                                      int32_t* status, void* stream);
 
 /* One mixture-of-experts layer: gate/up projection -> SiLU(gate)*up -> down projection -> router-weighted sum, in two launches for up
- * to 2048 (token, expert) pairs (1024 from 513 experts, 512 from 1025); more are done in turns.  Arguments as b200fp4_fused_sparse_moe, with w13 [E, 2I, H] packed gated and
- * w2 [E, H, I] packed, w13_g [E][gate rows, up rows], w2_g [E]; H and I multiples of 16, E up to 4096, topk up to the pairs of a turn.  Pairs whose expert (after expert_map) is outside
+ * to 2048 (token, expert) pairs; more are done in turns.  Arguments as b200fp4_fused_sparse_moe, with w13 [E, 2I, H] packed gated and
+ * w2 [E, H, I] packed, w13_g [E][gate rows, up rows], w2_g [E]; H and I multiples of 16, E up to 4096, topk up to 2048.  Pairs whose expert (after expert_map) is outside
  * [0, E) add nothing; a token without any gives zeros.  flags: B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT or 0.  Between the projections a value is kept as
  * the sum of two f16.  Results do not depend on the order in which blocks run. */
-B200FP4_API size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I, int64_t E);
+B200FP4_API size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I);
 B200FP4_API int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* topk_weights, const int32_t* topk_ids,
                                   const int32_t* expert_map, int64_t global_E, const uint8_t* w13_packed, const float* w13_g,
                                   const uint8_t* w2_packed, const float* w2_g, void* out, int out_dtype, int64_t M, int64_t topk,

@@ -58,8 +58,8 @@ def test_workspace_covers_a_turn_of_the_layer():
     from dgx_vllm_b200 import _lib
     L = _lib.lib()
     size = L.b200fp4_w4a16_moe_workspace_bytes
-    assert size(32, 10, 2048, 512, 512) >= 320 * (2 * 512 * 2 + 2048 * 4)
-    assert size(1 << 20, 10, 2048, 512, 512) == size(204, 10, 2048, 512, 512)               # more pairs are done in turns
+    assert size(32, 10, 2048, 512) >= 320 * (2 * 512 * 2 + 2048 * 4)
+    assert size(1 << 20, 10, 2048, 512) == size(204, 10, 2048, 512)               # more pairs are done in turns
 
 
 def test_no_cpu_path():
