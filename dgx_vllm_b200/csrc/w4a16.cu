@@ -669,6 +669,7 @@ __device__ __forceinline__ int local_expert(const MoeParams& p, int pair) {
 
 // An expert's pairs to zero; needs nothing of the call's inputs
 __device__ __forceinline__ void clear_counts(const MoeParams& p, unsigned char* smem, const MoeLayout& l) {
+  if (p.M * p.topk <= 32) return;                  // found without
   for (int i = threadIdx.x; i < p.E; i += kThreads) reinterpret_cast<int*>(smem + l.rows)[i] = 0;
 }
 
@@ -685,6 +686,30 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
   int2* const slots = reinterpret_cast<int2*>(smem + l.slots);
   uint32_t* const scan = reinterpret_cast<uint32_t*>(smem + l.scan);
   int* const count = reinterpret_cast<int*>(smem + l.rows);
+  if (P <= 32) {
+    // Every warp finds all of them and writes the same; slots in the order of their first pairs.
+    const int e = lane < P ? local_expert(p, lane) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, e);
+    const int before = __popc(same & ((1u << lane) - 1)), chunk = before / cap, place = before - chunk * cap;
+    const bool leads = e >= 0 && place == 0;
+    const int size = leads ? min(cap, __popc(same) - before) : 0;
+    const uint32_t leaders = __ballot_sync(0xffffffffu, leads);
+    int first = size;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int a = __shfl_up_sync(0xffffffffu, first, d);
+      if (lane >= d) first += a;
+    }
+    first -= size;
+    uint32_t rest = same;
+    for (int c = 0; c < before - place; ++c) rest &= rest - 1;
+    const int at = __shfl_sync(0xffffffffu, first, e >= 0 ? __ffs((int)rest) - 1 : 0) + place;
+    if (lane < P) expert[lane] = (uint16_t)e;
+    if (leads) slots[__popc(leaders & ((1u << lane) - 1))] = make_int2(e | (size << 16), first);
+    if (e >= 0) list[at] = (uint16_t)lane;
+    __syncwarp();
+    return __popc(leaders);
+  }
   int e[kMost], at[kMost];
 #pragma unroll
   for (int q = 0; q < kMost; ++q) {
@@ -821,12 +846,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       if (end > first) __syncthreads();            // nobody reads the rows before these any more
       auto row_at = [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)(list[row0 + r] / p.topk) * p.ldx; };
       staged.ask(n_rows, 0, p.K, row_at);
-      float gate_peak = 0.f, up_peak = 0.f, w = 1.f;
+      float2 g = {0.f, 0.f}, peak = {0.f, 0.f};
+      float w = 1.f;
       const int own = (int)threadIdx.x < n_rows ? list[row0 + threadIdx.x] : -1;
       if (own >= 0) {
-        const int x = expert[own];
-        gate_peak = p.g[2 * x] * p.peaks[2 * x];
-        up_peak = p.g[2 * x + 1] * p.peaks[2 * x + 1];
+        g = reinterpret_cast<const float2*>(p.g)[expert[own]];
+        peak = reinterpret_cast<const float2*>(p.peaks)[expert[own]];
         if (p.weight_on_input) w = p.weights[own];
       }
       if (end == first)
@@ -840,7 +865,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       if (own >= 0) {
         // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the bound is
         // far above the values costs little: f16 reaches 40 binades down.
-        const float norm = sqrtf(stats[threadIdx.x].act * (float)p.K) * w, bound = fabsf(norm * gate_peak) * fabsf(norm * up_peak);
+        const float norm = sqrtf(stats[threadIdx.x].act * (float)p.K) * w, bound = fabsf(norm * (g.x * peak.x)) * fabsf(norm * (g.y * peak.y));
         const int up = min(max(14 - ((int)(__float_as_uint(bound) >> 23) - 126), -100), 100);
         stats[threadIdx.x].act = pow2(up);
         p.act_inv[own] = pow2(-up);
@@ -1172,7 +1197,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
   if (hidden == nullptr || topk_weights == nullptr || topk_ids == nullptr || w13_packed == nullptr || w13_g == nullptr || w2_packed == nullptr ||
       w2_g == nullptr || out == nullptr || status == nullptr || (expert_map != nullptr && global_E < 1))
     return B200FP4_STATUS_INVALID_VALUE;
-  if (!aligned(hidden, 16) || !aligned(w13_packed, 16) || !aligned(w2_packed, 16) || !aligned(out, 16)) return B200FP4_STATUS_INVALID_VALUE;
+  if (!aligned(hidden, 16) || !aligned(w13_packed, 16) || !aligned(w13_g, 8) || !aligned(w2_packed, 16) || !aligned(out, 16)) return B200FP4_STATUS_INVALID_VALUE;
   if (E > kMaxExperts || topk > kMaxPairs || !fits_int(M * topk) || !fits_int(H + 128) || !fits_int(2 * I + 128) || !fits_int(E * (2 * I / 32 + 1) * (H / 128 + 1)) ||
       !fits_int(E * (H / 32 + 1) * (I / 128 + 1)))
     return B200FP4_STATUS_NOT_SUPPORTED;
