@@ -582,7 +582,7 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
   return finish_launch(1);
 }
 
-constexpr int kFewTokens = 16;
+constexpr int kFewTokens = 8;
 
 template <typename T>
 int launch_linear(const LinearCall& c, cudaStream_t st) {

@@ -47,6 +47,7 @@ struct GemmParams {
   int sets;                   // decoding sets at work: no more than stages of either kind, since a set that is further ahead would take a stage's round for the one before
   uint32_t acc_cols;          // columns of an accumulator
   int accs;                   // accumulators: two where a block does several tiles
+  uint32_t sums_at;           // split: where the cluster's sums go; 0: where the token stages were
   int* status;
 };
 
@@ -89,15 +90,43 @@ __device__ __forceinline__ void tcgen05_st_32x32(uint32_t taddr, const uint32_t 
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-// D += A . B^T, A in tensor memory
-__device__ __forceinline__ void tcgen05_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// D += A . B^T, A in tensor memory; by the lane whose `issue` is set.  Predicates instead of a branch: in a branch of one lane every operand is moved to the uniform
+// registers that the instruction wants.
+__device__ __forceinline__ void tcgen05_mma_ts(uint32_t issue, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_desc_lo, uint32_t b_desc_hi, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p, q;\n"
+      ".reg .b64 b;\n"
+      "mov.b64 b, {%2, %3};\n"
+      "setp.ne.b32 p, %5, 0;\n"
+      "setp.ne.b32 q, %6, 0;\n"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_desc_lo), "r"(b_desc_hi), "r"(idesc), "r"(accumulate), "r"(issue)
+      : "memory");
+}
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
       "{\n"
       ".reg .pred p;\n"
-      "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
-      "}\n" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void tcgen05_commit_if(uint32_t issue, uint32_t bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred q;\n"
+      "setp.ne.b32 q, %1, 0;\n"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(bar),
+      "r"(issue)
       : "memory");
 }
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
@@ -171,6 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
+  if (split > 1) cluster_arrive();                 // the other blocks run before anything is sent to them
 
   if (warp == 0) {
     // ------------------------------------------------------------------ copies of the weight
@@ -222,6 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
     const uint32_t idesc = (1u << 4) | (kType << 7) | (kType << 10) | ((uint32_t)(tokens >> 3) << 17) | ((uint32_t)(kMmaRows >> 4) << 24);
     const uint64_t b0 = desc_kmajor<128>(base);
+    const uint32_t b0_lo = (uint32_t)b0, b0_hi = (uint32_t)(b0 >> 32);      // a stage's address does not reach the upper half
+    bool ready = false;
     Slot op, acc;
     bool ok = true;
     acc.phase = 1;
@@ -231,21 +263,20 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       tcgen05_fence_after();
       const uint32_t d = tmem + acc.at * acc_cols;
       for (int u = 0; u < n_units; ++u) {
-        // One wait and one commit for 128 of k: with barriers of their own for the two operands the loop took 650 cycles for few tokens.
-        ok = mbar_wait_warp(full + 8 * op.at, op.phase, status, 74);
+        // One wait and one commit for 128 of k: with barriers of their own for the two operands the loop took 650 cycles for few tokens.  The next stage is looked at
+        // while this one's MMAs are issued.
+        if (!ready) ok = mbar_wait_warp(full + 8 * op.at, op.phase, status, 74);
         if (!ok) break;
         tcgen05_fence_after();
-        if (leader) {
-          const uint64_t desc = b0 + (uint64_t)((op.at * b_bytes) >> 4);
-          const uint32_t from = tmem + a_col + op.at * 64;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            tcgen05_mma_ts(d, from + i * 8, desc + (i & 3) * 2 + (i >> 2) * (b_half >> 4), idesc, (u > 0 || i > 0) ? 1u : 0u);
-          tcgen05_commit(empty + 8 * op.at);
-          if (u == n_units - 1) tcgen05_commit(acc_full + 8 * acc.at);
-        }
-        __syncwarp();
+        const uint32_t desc = b0_lo + ((op.at * b_bytes) >> 4), from = tmem + a_col + op.at * 64, done = empty + 8 * op.at;
         op.next(stages);
+        const bool next = mbar_test_wait(full + 8 * op.at, op.phase);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          tcgen05_mma_ts(leader, d, from + i * 8, desc + (i & 3) * 2 + (i >> 2) * (b_half >> 4), b0_hi, idesc, (u > 0 || i > 0) ? 1u : 0u);
+        tcgen05_commit_if(leader, done);
+        if (u == n_units - 1) tcgen05_commit_if(leader, acc_full + 8 * acc.at);
+        ready = __all_sync(0xffffffffu, next);
       }
       acc.next(p.accs);
     }
@@ -365,9 +396,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     if (split == 1) {
       if (work && ok) write_columns(0, row_tile * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), nth * 32, 5 * 32, g);
     } else {
-      // Token t of the tile is finished by block t / (tokens / split): [source][its tokens][128 rows] of f32, where the token stages were
-      cluster_sync_any();                          // all MMAs of the cluster have read theirs
+      // Token t of the tile is finished by block t / (tokens / split): [source][its tokens][128 rows] of f32
+      cluster_wait();
+      if (p.sums_at == 0) cluster_sync_any();      // all MMAs of the cluster have read their token stages
       const int own = tokens / split;
+      const uint32_t sums_base = base + p.sums_at;
       if (work)
         for (int c = nth * 16; c < tokens; c += 5 * 16) {
           uint32_t r[16];
@@ -376,13 +409,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int t = c + i, owner = t / own;
-            const uint32_t to = base + ((uint32_t)(rank * own + t - owner * own) * kMmaRows + quarter * 32 + lane) * 4;
+            const uint32_t to = sums_base + ((uint32_t)(rank * own + t - owner * own) * kMmaRows + quarter * 32 + lane) * 4;
             asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(map_to_cta(to, owner)), "r"(r[i]) : "memory");
           }
         }
       cluster_sync_any();
       const int row0 = row_tile * kMmaRows, first = token0 + rank * own;
-      const float* const sums = reinterpret_cast<const float*>(smem);
+      const float* const sums = reinterpret_cast<const float*>(smem + p.sums_at);
       for (int i = threadIdx.x; i < own * kMmaRows; i += kThreads) {
         const int m = first + i / kMmaRows, row = row0 + i % kMmaRows;
         if (m >= p.M || row >= p.N) continue;
@@ -455,7 +488,10 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
         p.accs = tiles > clusters ? 2 : 1;
         p.acc_cols = (uint32_t)(tokens + 31) / 32 * 32;
         p.stages = (int)std::min<uint32_t>(kMost, std::min<uint32_t>((512 - p.accs * p.acc_cols) / 64, 144 * 1024 / ((uint32_t)tokens * 256)));
-        p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - (uint32_t)p.stages * tokens * 256) / kWStageBytes);
+        // A cluster's sums have room of their own where they are small: nobody waits for the others' MMAs then.
+        const uint32_t sums = split > 1 && tokens <= 64 ? (uint32_t)tokens * kMmaRows * 4 : 0;
+        p.sums_at = sums > 0 ? kRingBytes - sums : 0;
+        p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - sums - (uint32_t)p.stages * tokens * 256) / kWStageBytes);
         p.sets = std::min(kDecodeSets, std::min(p.stages, p.w_stages));
         grid = (unsigned)(std::min<int64_t>(clusters, tiles) * split);
       }
