@@ -180,6 +180,48 @@ __device__ __forceinline__ void multiply_unit(uint32_t unit, int lane, uint32_t 
     }
 }
 
+// The same for one or two tokens, without a multiplication by a scale for every pair of values: a column holds one block of 16 of a token's k and zeros elsewhere, so that
+// a matrix instruction's sums stay apart by block (kTokens = 1: the eight blocks of the unit; 2: the four of a half, for each token), and a scale goes with the
+// block's sum.  268 instructions a unit become 200.  Lane l has columns 2 (l % 4) and the next one: part[tile][row l / 4, l / 4 + 8] gets their sum.
+template <int kTokens>
+__device__ __forceinline__ void multiply_unit_by_block(uint32_t unit, int lane, uint32_t chunk, const uint32_t (&b)[2][8], float (&part)[2][2]) {
+  const int row8 = lane >> 2, quad = lane & 3;
+  const uint32_t scales = unit + kUnitScales + row8 * 32;
+  float d[2][4];
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (half == 0 || kTokens == 2)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) d[t][j] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint4 w = lds128(unit + (t * 2 + half) * 512 + chunk);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        uint32_t lo[4], hi[4];
+        codes_to_pairs(q ? w.y : w.x, lo);
+        codes_to_pairs(q ? w.w : w.z, hi);
+        mma_16x8x16(d[t], lo[0], hi[0], lo[1], hi[1], b[half][q * 4], b[half][q * 4 + 1]);
+        mma_16x8x16(d[t], lo[2], hi[2], lo[3], hi[3], b[half][q * 4 + 2], b[half][q * 4 + 3]);
+      }
+    }
+    if (half == 0 && kTokens == 1) continue;
+    // scales of this lane's two blocks: [tile][half: row l / 4, row l / 4 + 8]
+    const int first = (quad & 1) * 2;
+    const uint2 s0 = lds64(scales + first * 8), s1 = lds64(scales + first * 8 + 8);
+    const bool upper = kTokens == 1 ? quad >= 2 : half == 1;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint32_t w0 = t ? s0.y : s0.x, w1 = t ? s1.y : s1.x;
+      const float2 f0 = __half22float2(e4m3_pair(upper ? w0 >> 16 : w0)), f1 = __half22float2(e4m3_pair(upper ? w1 >> 16 : w1));
+      part[t][0] += d[t][0] * f0.x + d[t][1] * f1.x;
+      part[t][1] += d[t][2] * f0.y + d[t][3] * f1.y;
+    }
+  }
+}
+
 // columns that are rows in shared memory (f16): lane l's are blocks l % 4 of the unit's two halves
 template <int kCols>
 __device__ __forceinline__ void staged_columns(const uint32_t (&col)[kCols], uint32_t at, uint32_t (&b)[2][kCols][8]) {
@@ -193,14 +235,12 @@ __device__ __forceinline__ void staged_columns(const uint32_t (&col)[kCols], uin
     }
 }
 
-// Warps that share the units of an item, as a power of two, given the block's items and the units of one.  The kernels are bound by the instructions that
-// their warps issue, so the busiest of the SM's four schedulers counts (warp w is with scheduler w % 4): a unit is about 440 cycles of a busy scheduler
-// and 600 of a warp alone, an item's ending a third of one where a warp has the item for itself and half of one for each warp that shares it.
+// Warps that share the units of an item, as a power of two, given the block's items and the units of one.  A unit takes a warp 750 cycles, and 350 of its scheduler
+// (an SM has four, warp w is with scheduler w % 4); an item's ending a third of a unit where a warp has the item for itself, else nearly one.
 inline float share_cost(int items, int units, int log_share) {
-  const int share = 1 << log_share, rounds = ((items << log_share) + kWarps - 1) / kWarps, schedulers = share < 4 ? 4 / share : 1;
-  const float item = (float)((units + share - 1) / share) + (log_share == 0 ? 0.33f : 0.5f);
-  const float busy = (float)((items + schedulers - 1) / schedulers) * (share > 4 ? share / 4 : 1) * item, alone = rounds * item * 1.4f;
-  return busy > alone ? busy : alone;
+  const int share = 1 << log_share, full = (items << log_share) / kWarps, rest = (items << log_share) % kWarps;
+  const float item = (float)((units + share - 1) / share) + (log_share == 0 ? 0.33f : 0.9f);
+  return item * (float)(full * 1400 + (rest > 0 ? std::max(750, (rest + 3) / 4 * 350) : 0));
 }
 inline int share_of(int items, int units) {
   int log_share = 0;
@@ -400,8 +440,8 @@ __host__ __device__ __forceinline__ LinearLayout linear_layout(int cols, int cap
   return l;
 }
 
-// XT: type of the activations; kCols: columns of eight
-template <typename XT, int kCols>
+// XT: type of the activations; kCols: columns of eight; kTokens: 1 or 2 where there are no more, else 0
+template <typename XT, int kCols, int kTokens>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr bool kConvert = std::is_same<XT, __nv_bfloat16>::value;
@@ -465,13 +505,45 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
     }
     for (; item < end; item += n_groups) {
       float acc[2][kCols][4] = {};
+      if constexpr (kTokens > 0) {
+        // this lane's column: block (l / 4) % 4 of a half, of the first half and then the second or of token l / 16
+        const int token = kTokens == 2 ? row8 >> 2 : 0;
+        const bool mine0 = kTokens == 2 ? (row8 & 3) == quad : row8 == quad, mine1 = kTokens == 2 ? mine0 : row8 == quad + 4;
+        const uint32_t row = base + l.rows + token * row_bytes + quad * 32;
+        float part[2][2] = {};
+        uint32_t b[2][8] = {};
 #pragma unroll 1
-      for (int k = k_first; k < k_first + n_units; ++k) {
-        uint32_t b[2][kCols][8];
-        staged_columns<kCols>(col, k * (kUnitK * 2), b);
-        multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
-        ring.advance();
-        if (ring.ok) fetch();
+        for (int k = k_first; k < k_first + n_units; ++k) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half)
+            if (half ? mine1 : mine0) {
+              const uint4 lo = lds128(row + k * (kUnitK * 2) + half * 128), hi = lds128(row + k * (kUnitK * 2) + half * 128 + 16);
+              b[half][0] = lo.x, b[half][1] = lo.y, b[half][2] = lo.z, b[half][3] = lo.w;
+              b[half][4] = hi.x, b[half][5] = hi.y, b[half][6] = hi.z, b[half][7] = hi.w;
+            }
+          multiply_unit_by_block<kTokens>(ring.wait(p.status), lane, chunk, b, part);
+          ring.advance();
+          if (ring.ok) fetch();
+        }
+        // a token's blocks: four lanes, or two; the second token's sums to where columns 0 and 1 are
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float v = part[t][r] + __shfl_xor_sync(0xffffffffu, part[t][r], 1);
+            const float other = __shfl_xor_sync(0xffffffffu, v, 2);
+            acc[t][0][r * 2] = kTokens == 1 ? v + other : v;
+            if (kTokens == 2) acc[t][0][r * 2 + 1] = other;
+          }
+      } else {
+#pragma unroll 1
+        for (int k = k_first; k < k_first + n_units; ++k) {
+          uint32_t b[2][kCols][8];
+          staged_columns<kCols>(col, k * (kUnitK * 2), b);
+          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
+          ring.advance();
+          if (ring.ok) fetch();
+        }
       }
       if (!arrived) {
         cluster_wait();
@@ -536,19 +608,19 @@ bool allow_smem(Kernel kernel, std::once_flag (&once)[64], bool (&ready)[64]) {
   return ready[dev];
 }
 
-template <typename XT, int kCols>
+template <typename XT, int kCols, int kTokens>
 int launch_linear_of(LinearParams p, cudaStream_t st) {
   static std::once_flag once[64];
   static bool ready[64];
   static ResidentClusters counts[kMaxSplit + 1][64];
-  if (!allow_smem(w4a16_linear_kernel<XT, kCols>, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
+  if (!allow_smem(w4a16_linear_kernel<XT, kCols, kTokens>, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
   // Blocks that share the k of an item in a cluster: a shorter k leaves room for more rows, and few strips reach all SMs
   float best = 1e30f;
   unsigned grid = 0;
   uint32_t smem = 0;
   LinearParams chosen = p;
   for (int split = 1; split <= kMaxSplit && split <= p.units; split *= 2) {
-    const int clusters = split == 1 ? sm_count() : resident_clusters_of(counts[split], w4a16_linear_kernel<XT, kCols>, split, kThreads, kSmemMost);
+    const int clusters = split == 1 ? sm_count() : resident_clusters_of(counts[split], w4a16_linear_kernel<XT, kCols, kTokens>, split, kThreads, kSmemMost);
     if (clusters < 1) break;
     const int own = (p.units + split - 1) / split;
     const uint32_t row_bytes = (uint32_t)own * (kUnitK * 2) + 16;
@@ -558,9 +630,9 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
       const int used = (int)std::min<int64_t>(clusters, items), most = (int)((items + used - 1) / used);
       const uint64_t bytes = (uint64_t)linear_layout(kCols, cap, row_bytes, 1, 0).bytes + (split > 1 ? (uint64_t)most * cap * 128 : 0);
       if ((uint64_t)own * 256 > kSmemMost || bytes > kSmemMost) continue;
-      // the busiest block's units; a cluster's exchange costs about as much as two
+      // the busiest block's units; a cluster's exchange costs some 1500 cycles
       const int log_share = share_of(most, p.units / split);
-      const float cost = share_cost(most, own, log_share) + (split > 1 ? 2.f : 0.f);
+      const float cost = share_cost(most, own, log_share) + (split > 1 ? 1500.f : 0.f);
       if (cost < best) {
         best = cost;
         chosen.split = split;
@@ -575,14 +647,16 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
     }
   }
   if (grid == 0) return B200FP4_STATUS_NOT_SUPPORTED;
-  if (launch_pdl_cluster(chosen.split, w4a16_linear_kernel<XT, kCols>, dim3(grid), dim3(kThreads), smem, st, chosen) != cudaSuccess) {
+  if (launch_pdl_cluster(chosen.split, w4a16_linear_kernel<XT, kCols, kTokens>, dim3(grid), dim3(kThreads), smem, st, chosen) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
   return finish_launch(1);
 }
 
-constexpr int kFewTokens = 8;
+// Up to eight tokens fill the columns of one instruction; with up to sixteen, two of them, the tcgen05 kernel is the faster one but for the smallest weights: M=16, us from
+// Python, this / that: N=K=2048 5.7 / 5.9, N=3001 K=4144 9.7 / 7.9, N=K=4096 10.1 / 8.1, N=14336 K=4096 19.7 / 15.1.
+bool few_tokens(const LinearCall& c) { return c.M <= 8 || (c.M <= 16 && strips_of(c.N) * units_of(c.K) <= 1536); }
 
 template <typename T>
 int launch_linear(const LinearCall& c, cudaStream_t st) {
@@ -601,7 +675,9 @@ int launch_linear(const LinearCall& c, cudaStream_t st) {
   p.strips = (int)strips_of(c.N);
   p.units = (int)units_of(c.K);
   p.status = c.status;
-  return p.M <= 8 ? launch_linear_of<T, 1>(p, st) : launch_linear_of<T, 2>(p, st);
+  if (p.M == 1) return launch_linear_of<T, 1, 1>(p, st);
+  if (p.M == 2) return launch_linear_of<T, 1, 2>(p, st);
+  return p.M <= 8 ? launch_linear_of<T, 1, 0>(p, st) : launch_linear_of<T, 2, 0>(p, st);
 }
 
 // ------------------------------------------------------------------------------------------ mixture of experts
@@ -1178,7 +1254,7 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   if (!fits_int(M) || !fits_int(N + 64) || !fits_int(K + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
   const LinearCall c = {x, x_dtype, ldx, packed, g_scale, bias, bias_dtype, out, out_dtype, M, N, K, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M > kFewTokens) return launch_w4a16_gemm(c, st);
+  if (!few_tokens(c)) return launch_w4a16_gemm(c, st);
   return x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(c, st) : launch_linear<__half>(c, st);
 }
 

@@ -64,6 +64,13 @@ __device__ __forceinline__ __half2 scales_of(uint32_t bytes, int half) {
   return __hmul2(as_half2(prmt(bytes, 0u, half ? 0x3424u : 0x1404u) >> 1), as_half2(0x5C005C00u));
 }
 
+// two E4M3 bytes -> two f16
+__device__ __forceinline__ __half2 e4m3_pair(uint32_t bytes) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)bytes));
+  return as_half2(r);
+}
+
 // two bf16 times a power of two (twice in `factor`) -> two f16
 __device__ __forceinline__ uint32_t bf16_to_f16_pair(uint32_t x, uint32_t factor) {
   const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&factor));

@@ -6,6 +6,7 @@ with shape-only fake implementations).
     cutlass_scaled_fp4_mm(out!, a, b, block_scale_a, block_scale_b, alpha) -> ()        vllm _C::cutlass_scaled_fp4_mm
     cutlass_fp4_group_mm(out!, a, b, a_scales, b_scales, alphas, problem_sizes, expert_offsets, sf_offsets) -> ()
     batched_sparse_v7 / fused_sparse_moe_v7                                             sparse_fp4_v7.cu:744-749
+    w4a16_linear / w4a16_moe                                                            weight-only NVFP4 (weight_only.py)
 
 `install_into_vllm()` points vllm._custom_ops at them (the B200 counterpart of the reference's
 CMake/patch step cmake_patch_gb10_nvfp4_v6_full_kernels.sh:50-64 and of sparse_v7_moe_patch.patch_vllm)."""
@@ -13,6 +14,7 @@ from __future__ import annotations
 
 import torch
 
+from . import _lib as _native
 from . import grouped_moe, ops, sparse_fp4_v7
 
 _lib = torch.library.Library("b200_nvfp4", "DEF")
@@ -26,6 +28,9 @@ _lib.define("batched_sparse_v7(Tensor A, Tensor B_comp_T, Tensor Meta_T_pk, Tens
 _lib.define("fused_sparse_moe_v7(Tensor hidden_states, Tensor topk_weights, Tensor topk_ids, Tensor expert_map, "
             "Tensor w13_comp, Tensor w13_meta, Tensor w13_scale, Tensor w13_g_scales, Tensor w2_comp, Tensor w2_meta, "
             "Tensor w2_scale, Tensor w2_g_scales, int inter_size, bool apply_router_weight_on_input) -> Tensor")
+_lib.define("w4a16_linear(Tensor x, Tensor packed, Tensor g_scale, int N, Tensor? bias, ScalarType? out_dtype) -> Tensor")
+_lib.define("w4a16_moe(Tensor hidden_states, Tensor topk_weights, Tensor topk_ids, Tensor? expert_map, Tensor w13_packed, "
+            "Tensor w13_g_scale, Tensor w2_packed, Tensor w2_g_scale, int inter_size, bool apply_router_weight_on_input) -> Tensor")
 
 
 def _quant_cuda(input, input_scale, is_sf_swizzled_layout):
@@ -59,7 +64,21 @@ def _fused_cuda(hidden_states, topk_weights, topk_ids, expert_map, w13_comp, w13
                                              apply_router_weight_on_input)
 
 
+def _w4a16_linear_cuda(x, packed, g_scale, N, bias, out_dtype):
+    return _native.host().w4a16_linear(x, packed, g_scale, N, x.shape[1], bias, None, out_dtype)
+
+
+def _w4a16_moe_cuda(hidden_states, topk_weights, topk_ids, expert_map, w13_packed, w13_g_scale, w2_packed, w2_g_scale, inter_size,
+                    apply_router_weight_on_input):
+    if expert_map is not None:
+        expert_map = None if expert_map.numel() == 0 else expert_map.to(torch.int32).contiguous()
+    return _native.host().w4a16_moe(w13_packed, w13_g_scale, w2_packed, w2_g_scale, expert_map, hidden_states.shape[1], inter_size, w2_g_scale.numel(),
+                                    hidden_states, topk_weights, topk_ids, apply_router_weight_on_input, None)
+
+
 _lib.impl("scaled_fp4_quant", _quant_cuda, "CUDA")
+_lib.impl("w4a16_linear", _w4a16_linear_cuda, "CUDA")
+_lib.impl("w4a16_moe", _w4a16_moe_cuda, "CUDA")
 _lib.impl("cutlass_scaled_fp4_mm", _mm_cuda, "CUDA")
 _lib.impl("cutlass_fp4_group_mm", _group_mm_cuda, "CUDA")
 _lib.impl("batched_sparse_v7", _sparse_cuda, "CUDA")
@@ -70,6 +89,9 @@ torch.library.register_fake("b200_nvfp4::cutlass_fp4_group_mm", lambda *a: None,
 torch.library.register_fake("b200_nvfp4::batched_sparse_v7",
                             lambda A, B, M, S, g, ids: A.new_empty((A.shape[0], B.shape[2])), lib=_lib)
 torch.library.register_fake("b200_nvfp4::fused_sparse_moe_v7", lambda h, *a: torch.empty_like(h), lib=_lib)
+torch.library.register_fake("b200_nvfp4::w4a16_linear", lambda x, packed, g, N, bias, out_dtype: x.new_empty(
+    (x.shape[0], N), dtype=x.dtype if out_dtype is None else out_dtype), lib=_lib)
+torch.library.register_fake("b200_nvfp4::w4a16_moe", lambda h, *a: torch.empty_like(h), lib=_lib)
 
 
 def install_into_vllm() -> None:

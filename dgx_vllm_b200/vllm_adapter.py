@@ -9,9 +9,13 @@ Sparse MoE experts -- the counterpart of the reference's sparse_kernel patch
                                 original tensors by zero-stride stubs that keep their shapes (:300-326)
   * `patch_vllm`                installs it on ModelOptNvFp4FusedMoE, gated by VLLM_NVFP4_SPARSE_V7=1 like the
                                 reference (:334-362), and routes vLLM's dense NVFP4 entry points here
+Dense NVFP4 experts with 16-bit activations (what MarlinExperts does, weights as they are in the checkpoint):
+  * `make_w4a16_apply_fn`, `process_moe_layer_weight_only`   the same hook over weight_only.W4A16MoE;
+                                `patch_vllm(weight_only=True)` or B200_NVFP4_WEIGHT_ONLY=1 installs it in place of the 2:4 one
 Dense NVFP4 linears:
   * `Nvfp4LinearCore` / `linear_kernel_class()`   an NvFp4LinearKernel (vllm/model_executor/kernels/linear/nvfp4/
-                                base.py) whose quantizer and GEMM are this library's.
+                                base.py) whose quantizer and GEMM are this library's;
+  * `Nvfp4WeightOnlyLinearCore` / `linear_kernel_class(weight_only=True)`   the same with 16-bit activations
 
 Nothing here imports vLLM at module import time; `patch_vllm` and `linear_kernel_class` do when called."""
 from __future__ import annotations
@@ -108,15 +112,70 @@ def process_moe_layer(method, layer, original: Callable, convert_fn: Optional[Ca
     return True
 
 
+def make_w4a16_apply_fn(w13, w2, fused_fn: Optional[Callable] = None):
+    """The function vLLM calls in place of MarlinExperts.apply (same 15 positional arguments, no self) over weights packed by
+    weight_only.pack_nvfp4_weight: writes output[:M] and returns output.  `fused_fn(hidden, topk_weights, topk_ids, expert_map, on_input)`,
+    when given, replaces the CUDA layer (tests on CPU)."""
+    layer = []
+
+    def w4a16_apply(output, hidden_states, w1, w2_, topk_weights, topk_ids, activation, global_num_experts, expert_map,
+                    a1q_scale, a2_scale, workspace13, workspace2, expert_tokens_meta, apply_router_weight_on_input):
+        if str(getattr(activation, "value", activation)).lower() != "silu":
+            raise RuntimeError(f"weight-only experts apply SiLU(gate) * up, not {activation}")
+        if fused_fn is not None:
+            result = fused_fn(hidden_states, topk_weights.float(), topk_ids, expert_map, apply_router_weight_on_input)
+        else:
+            if expert_map is not None and not expert_map.is_cuda:
+                expert_map = expert_map.to(hidden_states.device)
+            if not layer:
+                from .weight_only import W4A16MoE
+                layer.append(W4A16MoE(w13, w2))
+            result = layer[0](hidden_states.contiguous(), topk_weights, topk_ids, apply_router_weight_on_input, expert_map=expert_map)
+        output[:hidden_states.shape[0]] = result.to(output.dtype)
+        return output
+
+    return w4a16_apply
+
+
+def process_moe_layer_weight_only(method, layer, original: Callable, pack_fn: Optional[Callable] = None, device=None,
+                                  make_apply: Callable = make_w4a16_apply_fn) -> bool:
+    """process_moe_layer without the pruning: the checkpoint tensors are packed as they are.  `pack_fn(codes [E,N,K/2], scales
+    [E,N,K/16], g_scales, gated=, device=)` defaults to weight_only.pack_nvfp4_weight; gate and up rows keep a factor each where the
+    checkpoint has two.  Returns True when `apply` was replaced."""
+    src = {name: getattr(layer, name).data.clone() for name in _STUBBED_PARAMS}
+    original(method, layer)
+    experts = getattr(getattr(method, "moe_mk", None), "fused_experts", None)
+    if experts is None:
+        logger.warning("[b200 weight-only] moe_mk.fused_experts not found: layer left on vLLM's own kernels")
+        return False
+    if pack_fn is None:
+        from .weight_only import pack_nvfp4_weight as pack_fn
+    if device is None:
+        device = src["w13_weight"].device if src["w13_weight"].is_cuda else "cuda"
+    g2 = src["w2_weight_scale_2"]
+    w13 = pack_fn(src["w13_weight"], src["w13_weight_scale"], src["w13_weight_scale_2"], gated=True, device=device)
+    w2 = pack_fn(src["w2_weight"], src["w2_weight_scale"], g2[:, 0] if g2.dim() > 1 else g2, gated=False, device=device)
+    experts.apply = make_apply(w13, w2)
+    freed = sum(_zero_stride_stub(getattr(layer, name)) for name in _STUBBED_PARAMS if hasattr(layer, name))
+    if torch.cuda.is_available():
+        torch.cuda.empty_cache()
+    logger.info("[b200 weight-only] %d experts packed, %.1f MB of repacked weights released", src["w13_weight"].shape[0], freed / 1e6)
+    return True
+
+
 _original_process_weights = None
 
 
-def patch_vllm(force: bool = False) -> bool:
+def patch_vllm(force: bool = False, weight_only: Optional[bool] = None) -> bool:
     """Install the hook on vLLM's ModelOptNvFp4FusedMoE and route its dense NVFP4 ops to this library.  Like the
-    reference's module it acts only when VLLM_NVFP4_SPARSE_V7=1 (or force=True).  Idempotent."""
+    reference's module it acts only when VLLM_NVFP4_SPARSE_V7=1, or B200_NVFP4_WEIGHT_ONLY=1 for experts whose weights are not
+    pruned (or force=True; weight_only chooses between the two hooks).  Idempotent."""
     global _original_process_weights
-    if not force and os.environ.get("VLLM_NVFP4_SPARSE_V7", "0") != "1":
+    asked = {name: os.environ.get(name, "0") == "1" for name in ("VLLM_NVFP4_SPARSE_V7", "B200_NVFP4_WEIGHT_ONLY")}
+    if not force and not any(asked.values()):
         return False
+    if weight_only is None:
+        weight_only = asked["B200_NVFP4_WEIGHT_ONLY"] and not asked["VLLM_NVFP4_SPARSE_V7"]
     if _original_process_weights is not None:
         return True
     from vllm.model_executor.layers.quantization.modelopt import ModelOptNvFp4FusedMoE
@@ -124,12 +183,14 @@ def patch_vllm(force: bool = False) -> bool:
     from .torch_ops import install_into_vllm
     _original_process_weights = ModelOptNvFp4FusedMoE.process_weights_after_loading
 
+    process = process_moe_layer_weight_only if weight_only else process_moe_layer
+
     def patched(self, layer):
-        process_moe_layer(self, layer, _original_process_weights)
+        process(self, layer, _original_process_weights)
 
     ModelOptNvFp4FusedMoE.process_weights_after_loading = patched
     install_into_vllm()
-    logger.info("[b200 sparse] vLLM patched: sparse 2:4 MoE experts and dense NVFP4 ops run on libb200nvfp4")
+    logger.info("[b200] vLLM patched: %s MoE experts and dense NVFP4 ops run on libb200nvfp4", "weight-only" if weight_only else "sparse 2:4")
     return True
 
 
@@ -164,6 +225,36 @@ class Nvfp4LinearCore:
         return out.view(*out_shape)
 
 
+class Nvfp4WeightOnlyLinearCore:
+    """process_weights_after_loading / apply_weights of a dense NVFP4 linear with 16-bit activations.  The layer carries the attributes that
+    Nvfp4LinearCore's does; alpha times input_global_scale_inv is the weight's own factor, the activations' global scale is not used."""
+
+    def __init__(self, pack_fn: Optional[Callable] = None, linear_fn: Optional[Callable] = None):
+        self._pack, self._linear = pack_fn, linear_fn
+
+    def process_weights_after_loading(self, layer) -> None:
+        if self._pack is None:
+            from .weight_only import pack_nvfp4_weight
+            pack = pack_nvfp4_weight
+        else:
+            pack = self._pack
+        g = layer.alpha.detach().float() * layer.input_global_scale_inv.detach().float()
+        layer.w4a16_weight = pack(layer.weight.data, layer.weight_scale.data, g.reshape(1))
+        for name in ("weight", "weight_scale"):
+            _zero_stride_stub(getattr(layer, name))
+
+    def apply_weights(self, layer, x: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+        out_shape = [*x.shape[:-1], layer.output_size_per_partition]
+        x2 = x.reshape(-1, x.shape[-1])
+        if self._linear is None:
+            from .weight_only import w4a16_linear as linear
+            if x2.stride(-1) != 1 or x2.data_ptr() % 16 or (x2.shape[0] > 1 and x2.stride(0) % 8):
+                x2 = x2.clone(memory_format=torch.contiguous_format)          # rows of some slice that are not 16-byte aligned
+        else:
+            linear = self._linear
+        return linear(x2, layer.w4a16_weight, bias).view(*out_shape)
+
+
 def swizzle_blockscale(sf_linear: torch.Tensor) -> torch.Tensor:
     """[rows, K/16] e4m3 block scales -> the padded 128x4 tile layout the GEMM reads (swizzle_blockscale,
     vllm/model_executor/layers/quantization/utils/nvfp4_utils.py:38-51), on the GPU."""
@@ -179,12 +270,12 @@ def swizzle_blockscale(sf_linear: torch.Tensor) -> torch.Tensor:
     return out.view(torch.float8_e4m3fn)
 
 
-def linear_kernel_class():
-    """An NvFp4LinearKernel subclass for vLLM's kernel registry (imports vLLM)."""
+def linear_kernel_class(weight_only: bool = False):
+    """An NvFp4LinearKernel subclass for vLLM's kernel registry (imports vLLM); weight_only: with 16-bit activations."""
     from vllm.model_executor.kernels.linear.nvfp4.base import NvFp4LinearKernel
 
     class B200NvFp4LinearKernel(NvFp4LinearKernel):
-        _core = Nvfp4LinearCore()
+        _core = Nvfp4WeightOnlyLinearCore() if weight_only else Nvfp4LinearCore()
 
         @classmethod
         def is_supported(cls, compute_capability=None):
@@ -205,5 +296,5 @@ def linear_kernel_class():
     return B200NvFp4LinearKernel
 
 
-if os.environ.get("VLLM_NVFP4_SPARSE_V7", "0") == "1" and os.environ.get("B200_NVFP4_AUTOPATCH", "0") == "1":
+if os.environ.get("B200_NVFP4_AUTOPATCH", "0") == "1":
     patch_vllm()

@@ -93,15 +93,19 @@ class W4A16MoE:
         require(w13.N == 2 * self.I and w2.N == self.H and w2.E == self.E, "w13 must be [E, 2I, H] and w2 [E, H, I]")
         require(self.H % 16 == 0 and self.I % 16 == 0, "H and I must be multiples of 16")
         self.device = require_cuda(w13.packed, w13.g_scale, w2.packed, w2.g_scale)
-        emap = None
-        if expert_map is not None and expert_map.numel() > 0:
-            require_cuda(w13.packed, expert_map)
-            emap = expert_map.to(torch.int32).contiguous()
-        self._bound = (w13.packed, w13.g_scale, w2.packed, w2.g_scale, emap, self.H, self.I, self.E)
+        self._weights = (w13.packed, w13.g_scale, w2.packed, w2.g_scale)
+        self._sizes = (self.H, self.I, self.E)
+        self._map = self._as_map(expert_map)
         self._call = _lib.host().w4a16_moe
 
+    @staticmethod
+    def _as_map(expert_map):
+        return None if expert_map is None or expert_map.numel() == 0 else expert_map.to(torch.int32).contiguous()
+
     def __call__(self, hidden_states: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
-                 apply_router_weight_on_input: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+                 apply_router_weight_on_input: bool = False, out: torch.Tensor | None = None,
+                 expert_map: torch.Tensor | None = None) -> torch.Tensor:
         """hidden_states [M,H] bf16/f16, topk_weights [M,topk] f32, topk_ids [M,topk] int32 -> [M,H] in the activation dtype (or in `out`'s,
-        which may also be f32).  Pairs whose expert is not here add nothing."""
-        return self._call(*self._bound, hidden_states, topk_weights, topk_ids, apply_router_weight_on_input, out)
+        which may also be f32).  Pairs whose expert is not here add nothing.  expert_map: in place of the layer's own."""
+        emap = self._map if expert_map is None else self._as_map(expert_map)
+        return self._call(*self._weights, emap, *self._sizes, hidden_states, topk_weights, topk_ids, apply_router_weight_on_input, out)

@@ -4,6 +4,7 @@ the dense NVFP4 linear kernel's two methods.  The conversion and the ops are inj
 import types
 
 import numpy as np
+import pytest
 import torch
 
 import oracle
@@ -129,3 +130,68 @@ def test_dense_linear_kernel_methods_with_oracle_stand_ins():
     assert tuple(out.shape) == (2, M // 2, N) and out.dtype == torch.bfloat16
     ref = oracle.nvfp4_linear(bf16_bits(x.reshape(M, K)), gx, wc, wsf, gw) + 1.0
     assert np.max(np.abs(out.float().numpy().reshape(M, N) - ref)) <= 1e-2 * np.max(np.abs(ref))
+
+
+def test_weight_only_moe_hook_packs_swaps_apply_and_stubs_the_originals():
+    from dgx_vllm_b200 import vllm_adapter as va
+    E, I, H = 3, 16, 32
+    layer, w13, w2 = _fake_moe_layer(E, I, H)
+    factors = layer.w13_weight_scale_2.data.clone()
+    factors[:, 1] *= 2                                                       # gate and up rows with a factor each
+    layer.w13_weight_scale_2.data = factors.clone()
+    method = types.SimpleNamespace(moe_mk=None)
+
+    def original(m, l):
+        l.w13_weight.data.zero_()
+        m.moe_mk = types.SimpleNamespace(fused_experts=types.SimpleNamespace(apply=None))
+
+    packed = []
+
+    def pack(codes, scales, g, gated, device):
+        packed.append((codes.clone(), scales.clone(), g.clone(), gated))
+        return len(packed)
+
+    assert va.process_moe_layer_weight_only(method, layer, original, pack_fn=pack, device="cpu", make_apply=lambda a, b: ("apply", a, b))
+    assert method.moe_mk.fused_experts.apply == ("apply", 1, 2)
+    (c13, s13, g13, gated13), (c2, s2, g2, gated2) = packed
+    assert gated13 and not gated2 and torch.equal(c13, w13["codes"]) and torch.equal(c2, w2["codes"]) and torch.equal(s2, w2["sf"])
+    assert torch.equal(g13, factors) and tuple(g2.shape) == (E,)
+    for n in va._STUBBED_PARAMS:
+        assert set(getattr(layer, n).data.stride()) == {0}
+    layer, _, _ = _fake_moe_layer()
+    assert not va.process_moe_layer_weight_only(types.SimpleNamespace(), layer, lambda m, l: None, pack_fn=pack, device="cpu")
+
+
+def test_weight_only_apply_closure_call_shape():
+    from dgx_vllm_b200 import vllm_adapter as va
+    seen = {}
+
+    def fused(hidden, tw, ids, emap, on_input):
+        seen.update(tw=tw.dtype, emap=emap, on_input=on_input)
+        return hidden.float() * 3
+
+    fn = va.make_w4a16_apply_fn(None, None, fused_fn=fused)
+    out = torch.zeros(4, 32, dtype=torch.bfloat16)
+    args = (out, torch.ones(3, 32, dtype=torch.bfloat16), None, None, torch.ones(3, 2, dtype=torch.bfloat16), torch.zeros(3, 2, dtype=torch.int64))
+    assert fn(*args, types.SimpleNamespace(value="silu"), 8, None, None, None, None, None, None, False) is out
+    assert torch.all(out[:3] == 3) and torch.all(out[3:] == 0) and seen == dict(tw=torch.float32, emap=None, on_input=False)
+    with pytest.raises(RuntimeError):
+        fn(*args, "gelu", 8, None, None, None, None, None, None, False)
+
+
+def test_weight_only_linear_kernel_methods():
+    from dgx_vllm_b200 import vllm_adapter as va
+    layer = types.SimpleNamespace(weight=torch.nn.Parameter(torch.zeros(8, 16, dtype=torch.uint8), requires_grad=False),
+                                  weight_scale=torch.nn.Parameter(torch.zeros(8, 2, dtype=torch.uint8), requires_grad=False),
+                                  input_global_scale_inv=torch.tensor([4.0]), alpha=torch.tensor([0.5]), output_size_per_partition=8)
+    seen = {}
+
+    def pack(codes, scales, g):
+        seen["g"] = float(g)
+        return "packed"
+
+    core = va.Nvfp4WeightOnlyLinearCore(pack_fn=pack, linear_fn=lambda x, w, bias: torch.zeros(x.shape[0], 8) + (0 if bias is None else bias))
+    core.process_weights_after_loading(layer)
+    assert layer.w4a16_weight == "packed" and seen["g"] == 2.0 and set(layer.weight.data.stride()) == {0}
+    assert tuple(core.apply_weights(layer, torch.zeros(2, 3, 32)).shape) == (2, 3, 8)
+    assert bool((core.apply_weights(layer, torch.zeros(5, 32), torch.ones(8)) == 1).all())

@@ -32,6 +32,10 @@ def _linear(M, N, K, dtype, out_dtype=None, bias_dtype=None, pad=0, exact=True, 
     (1, 1, 16, BF16, F32, None, 0),               # smallest
     (1, 16, 128, F16, F32, None, 0),              # one whole unit
     (2, 17, 144, BF16, None, None, 8),            # one past a tile and a unit; a slice of a wider tensor
+    (1, 300, 4112, BF16, None, BF16, 0),          # a token with a block of k a column
+    (2, 600, 8208, F16, F32, None, 8),            # two
+    (2, 64, 128, BF16, F32, None, 0),
+    (3, 64, 128, F16, F32, None, 0),              # one more
     (7, 40, 112, F16, None, F16, 0),              # a unit that ends early, a bias
     (8, 129, 2064, BF16, F32, F32, 16),           # all columns of one instruction, k split unevenly
     (9, 33, 256, F16, F32, BF16, 0),              # one more: two of them
@@ -334,3 +338,51 @@ def test_threads_on_one_stream():
     torch.cuda.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_custom_ops():
+    import dgx_vllm_b200.torch_ops  # noqa: F401
+    from dgx_vllm_b200.weight_only import pack_nvfp4_weight, w4a16_linear
+    codes, block = make_weight(1, 96, 128, 4)
+    w = pack_nvfp4_weight(codes[0], block[0], torch.ones(1, device="cuda"))
+    x, bias = make_x(5, 128, 1, BF16), torch.ones(96, device="cuda")
+    torch.library.opcheck(torch.ops.b200_nvfp4.w4a16_linear.default, (x, w.packed, w.g_scale, 96, bias, F32), test_utils=("test_schema", "test_faketensor"))
+    assert torch.equal(torch.ops.b200_nvfp4.w4a16_linear(x, w.packed, w.g_scale, 96, bias, F32), w4a16_linear(x, w, bias, out_dtype=F32))
+    layer, x, weights, ids, emap, _, _ = _layer(6, 4, 128, 64, 2, BF16, parallel=2)
+    got = torch.ops.b200_nvfp4.w4a16_moe(x, weights, ids, emap, *layer._weights, 64, False)
+    assert torch.equal(got, layer(x, weights, ids))
+    torch.library.opcheck(torch.ops.b200_nvfp4.w4a16_moe.default, (x, weights, ids, emap, *layer._weights, 64, False), test_utils=("test_schema", "test_faketensor"))
+
+
+def test_vllm_adapter_on_the_device():
+    """A checkpoint layer through the weight-loading hooks: experts and a linear, against the plain forms."""
+    import types
+    from dgx_vllm_b200 import vllm_adapter as va
+    E, H, I, M, topk = 5, 128, 64, 9, 2
+    c13, b13 = make_weight(E, 2 * I, H, 1)
+    c2, b2 = make_weight(E, H, I, 2)
+    g13 = (torch.rand(E, 2, generator=torch.Generator().manual_seed(1)) + 0.5).cuda() / (12.0 * H ** 0.5)
+    g2 = torch.full((E, 2), 1.0 / (3.0 * I ** 0.5), device="cuda")
+    P = lambda t: torch.nn.Parameter(t, requires_grad=False)
+    layer = types.SimpleNamespace(w13_weight=P(c13), w2_weight=P(c2), w13_weight_scale=P(b13), w2_weight_scale=P(b2), w13_weight_scale_2=P(g13),
+                                  w2_weight_scale_2=P(g2))
+    W13, W2 = values(c13, b13, g13.repeat_interleave(I, 1)), values(c2, b2, g2[:, :1].expand(E, H))
+    experts = types.SimpleNamespace(apply=None)
+    assert va.process_moe_layer_weight_only(types.SimpleNamespace(moe_mk=types.SimpleNamespace(fused_experts=experts)), layer, lambda m, l: None)
+    x = make_x(M, H, 3, BF16)
+    weights = torch.rand(M, topk, generator=torch.Generator().manual_seed(2)).cuda()
+    for n in (E, 2 * E):
+        ids = torch.randint(0, n, (M, topk), generator=torch.Generator().manual_seed(n)).cuda()
+        emap = None if n == E else torch.cat((torch.full((E,), -1), torch.arange(E))).to(torch.int32).cuda()
+        out = torch.full((M + 2, H), 5.0, dtype=BF16, device="cuda")
+        experts.apply(out, x, None, None, weights, ids, "silu", n, emap, None, None, None, None, None, False)
+        _check(out[:M], x, weights, ids, emap, W13, W2)
+        assert bool((out[M:] == 5).all())
+    codes, block = make_weight(1, 48, 64, 6)
+    lin = types.SimpleNamespace(weight=P(codes[0]), weight_scale=P(block[0]), input_global_scale_inv=torch.tensor([8.0], device="cuda"),
+                                alpha=torch.tensor([0.0625], device="cuda"), output_size_per_partition=48)
+    core = va.Nvfp4WeightOnlyLinearCore()
+    core.process_weights_after_loading(lin)
+    x = make_x(6, 64, 1, BF16, pad=4)                                          # rows that are 8 bytes off
+    y = core.apply_weights(lin, x.view(6, 64) if x.is_contiguous() else x, None)
+    assert torch.equal(y, (x.double() @ values(codes, block, torch.full((1, 1), 0.5, device="cuda"))[0].T).to(BF16))
