@@ -695,6 +695,8 @@ struct MoeParams {
   int strips, units;
   int cap, rows;              // columns of a slot; rows that there is room for
   int log_share;
+  int split;                  // whole strips: blocks of a cluster, which share the slots of a strip
+  float rcp_topk, rcp_grid, rcp_strips;
   const int32_t* ids;         // [M, topk]
   const float* weights;       // [M, topk]
   const int32_t* map;         // [global_E] or null
@@ -715,11 +717,11 @@ struct RowStat {
   float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
 };
 // Shared memory behind the rings and barriers: partial sums of warps | expert of a pair | pairs by expert, and as they came | first place of an expert | slots | scan |
-// routing weights (down) | statistics of the staged rows | parts of those | the rows in f16, and before them an expert's pairs
+// routing weights (down) | statistics of the staged rows | parts of those | the rows in f16, and before them an expert's pairs | products of whole strips
 struct MoeLayout {
-  uint32_t red, expert, list, came, start, slots, scan, weights, stats, parts, rows, bytes;
+  uint32_t red, expert, list, came, start, slots, scan, weights, stats, parts, rows, y, bytes;
 };
-__host__ __device__ __forceinline__ MoeLayout moe_layout(int cols, int pairs, int E, int cap, int rows, uint32_t row_bytes) {
+__host__ __device__ __forceinline__ MoeLayout moe_layout(int cols, int pairs, int E, int cap, int rows, uint32_t row_bytes, int whole_strips) {
   MoeLayout l;
   l.red = pad16(ring_bytes(cols) + bar_bytes(cols));
   l.expert = l.red + red_bytes(cols);
@@ -733,9 +735,45 @@ __host__ __device__ __forceinline__ MoeLayout moe_layout(int cols, int pairs, in
   l.parts = pad16(l.stats + (uint32_t)rows * sizeof(RowStat));
   l.rows = l.parts + kWarps * 8;
   const uint32_t counts = pad16((uint32_t)E * 4), staged = (uint32_t)rows * row_bytes;
-  l.bytes = l.rows + (counts > staged ? counts : staged);
+  l.y = l.rows + (counts > staged ? counts : staged);
+  l.bytes = l.y + (uint32_t)whole_strips * pairs * 128;
   return l;
 }
+
+// n / d for 0 <= n, given 1 / d: a float's product is off by less than one for n below 2^22
+__device__ __forceinline__ int quotient(int n, int d, float rcp) {
+  if (n >= 1 << 22) return n / d;
+  int q = __float2int_rz(__int2float_rn(n) * rcp);
+  const int r = n - q * d;
+  q += r >= d ? 1 : 0;
+  q -= r < 0 ? 1 : 0;
+  return q;
+}
+
+// Items of a block of the down projection, of the pairs' slots and the strips of the result: a run of all of them, strip by strip; or a cluster has whole strips
+// and each of its blocks some of the slots.
+struct DownItems {
+  int first, last, fast;      // items; slots of a strip
+  int strip0, strip_step, slot0;
+  __device__ __forceinline__ void of(int block, int grid, float rcp_grid, int n_slots, int strips, int split, bool whole) {
+    strip0 = slot0 = 0;
+    strip_step = 1;
+    fast = n_slots;
+    if (whole) {
+      const int cluster = block / split, clusters = grid / split, rank = block & (split - 1);
+      slot0 = n_slots * rank / split;
+      fast = n_slots * (rank + 1) / split - slot0;
+      strip0 = cluster;
+      strip_step = clusters;
+      first = 0;
+      last = cluster < strips ? (strips - cluster + clusters - 1) / clusters * fast : 0;
+    } else {
+      const int n = n_slots * strips, per = quotient(n, grid, rcp_grid), more = n - per * grid;
+      first = block * per + min(block, more);
+      last = first + per + (block < more ? 1 : 0);
+    }
+  }
+};
 
 __device__ __forceinline__ int local_expert(const MoeParams& p, int pair) {
   int64_t e = p.ids[pair];
@@ -845,19 +883,23 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
   return total;
 }
 
-// XT: type of the activations (gate/up); kDown: the second projection; kCols: columns of eight; kParts: f16 parts of a value between the projections
-template <typename XT, bool kDown, int kCols, int kParts>
+enum Projection { kGateUp, kDownItems, kDownStrips };       // kDownStrips: whole strips
+
+// XT: type of the activations (gate/up); kCols: columns of eight; kParts: f16 parts of a value between the projections
+template <typename XT, int kMode, int kCols, int kParts>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
+  constexpr bool kDown = kMode != kGateUp, kWhole = kMode == kDownStrips;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row8 = lane >> 2, quad = lane & 3;
   const uint32_t base = smem_u32(smem), chunk = chunk_at(row8, quad);
   const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;      // rows are shifted by 16 bytes against each other: no two lanes of a load meet
-  const MoeLayout l = moe_layout(kCols, p.M * p.topk, p.E, p.cap, p.rows, row_bytes);
+  const MoeLayout l = moe_layout(kCols, p.M * p.topk, p.E, p.cap, p.rows, row_bytes, 0);
   const uint16_t* const expert = reinterpret_cast<const uint16_t*>(smem + l.expert);
   const int2* const slots = reinterpret_cast<const int2*>(smem + l.slots);
   const uint16_t* const list = reinterpret_cast<const uint16_t*>(smem + l.list);
   Ring<stages_of(kCols)> ring;
   ring.init(base, base + ring_bytes(kCols), warp, lane);
+  if (kWhole && p.split > 1) cluster_arrive();     // the other blocks run before anything is sent to them
   // The routing is not the first projection's work, and its kernel lets this one start only once what came before it is complete: the second
   // projection finds its slots and asks for its first weights while the first one ends.
   clear_counts(p, smem, l);
@@ -870,8 +912,16 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   }
   const int n_slots = find_slots(p, smem, l);
   // Items (strip, slot) of a slot are neighbours, or (down) those of a strip
-  const int fast = kDown ? n_slots : p.strips, n_items = n_slots * p.strips, per = n_items / (int)gridDim.x, more = n_items - per * (int)gridDim.x;
-  const int first = (int)blockIdx.x * per + min((int)blockIdx.x, more), last = first + per + ((int)blockIdx.x < more ? 1 : 0);
+  DownItems d;
+  if constexpr (kDown) {
+    d.of(blockIdx.x, gridDim.x, p.rcp_grid, n_slots, p.strips, p.split, kWhole);
+  } else {
+    const int n = n_slots * p.strips, per = quotient(n, gridDim.x, p.rcp_grid), more = n - per * (int)gridDim.x;
+    d.first = (int)blockIdx.x * per + min((int)blockIdx.x, more);
+    d.last = d.first + per + ((int)blockIdx.x < more ? 1 : 0);
+    d.fast = p.strips;
+  }
+  const int first = d.first, last = d.last, fast = d.fast;
   const int share = 1 << p.log_share, group = warp >> p.log_share, in_group = warp & (share - 1), n_groups = kWarps >> p.log_share;
   const int k_first = (p.units * in_group) >> p.log_share, n_units = ((p.units * (in_group + 1)) >> p.log_share) - k_first;
 
@@ -879,7 +929,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     int item, hi, lo;         // hi * fast + lo
   };
   Cursor at = {first + group, 0, 0};
-  if (fast > 0) at.hi = at.item / fast;
+  if (fast > 0) at.hi = quotient(at.item, fast, kDown ? __frcp_rn((float)fast) : p.rcp_strips);
   at.lo = at.item - at.hi * fast;
   Cursor ahead = at;
   auto next = [&](Cursor& c) {
@@ -895,8 +945,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   auto fetch = [&]() {
     if (ahead_left == 0) {
       if (ahead.item >= last) return;
-      const int e = slots[kDown ? ahead.lo : ahead.hi].x & 0xFFFF;
-      src = p.packed + (size_t)(e * p.strips * p.units + strip_at(kDown ? ahead.hi : ahead.lo, p.strips, p.units, k_first, src_step)) * kUnitBytes;
+      const int e = slots[kDown ? d.slot0 + ahead.lo : ahead.hi].x & 0xFFFF, strip = kDown ? d.strip0 + ahead.hi * d.strip_step : ahead.lo;
+      src = p.packed + (size_t)(e * p.strips * p.units + strip_at(strip, p.strips, p.units, k_first, src_step)) * kUnitBytes;
       ahead_left = n_units;
       next(ahead);
     }
@@ -914,13 +964,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     RowStat* const stats = reinterpret_cast<RowStat*>(smem + l.stats);
     // Rows are staged for as many slots at a time as there is room for: slots [slot, stop), the pairs in places [row0, row0 + n_rows) of the list
     StagedRows<XT, true> staged;
-    int slot = last > first ? first / fast : 0;
+    int slot = last > first ? quotient(first, fast, p.rcp_strips) : 0;
     for (int end = first; end < last;) {
-      const int slots_end = (last - 1) / fast + 1, row0 = slots[slot].y;
+      const int slots_end = quotient(last - 1, fast, p.rcp_strips) + 1, row0 = slots[slot].y;
       int stop = slot + 1, n_rows = slots[slot].x >> 16;
       while (stop < slots_end && n_rows + (slots[stop].x >> 16) <= p.rows) n_rows += slots[stop++].x >> 16;
       if (end > first) __syncthreads();            // nobody reads the rows before these any more
-      auto row_at = [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)(list[row0 + r] / p.topk) * p.ldx; };
+      auto row_at = [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)quotient(list[row0 + r], p.topk, p.rcp_topk) * p.ldx; };
       staged.ask(n_rows, 0, p.K, row_at);
       float2 g = {0.f, 0.f}, peak = {0.f, 0.f};
       float w = 1.f;
@@ -986,14 +1036,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     for (int i = 0; i < stages_of(kCols); ++i) fetch();
     pdl_wait();
     pdl_launch_dependents();
+    if (kWhole && p.split > 1) cluster_wait();
     if (n_slots == 0) {
       for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < (size_t)p.M * p.N; i += (size_t)gridDim.x * kThreads)
         store_value(p.out, p.out_dtype, i, 0.f);
       return;
     }
     for (; at.item < last; next(at)) {
-      const int2 s = slots[at.lo];
-      const int n = s.x >> 16, e = s.x & 0xFFFF, strip = at.hi;
+      const int2 s = slots[d.slot0 + at.lo];
+      const int n = s.x >> 16, e = s.x & 0xFFFF, strip = d.strip0 + at.hi * d.strip_step;
       const __half* act[kCols];
 #pragma unroll
       for (int c = 0; c < kCols; ++c) {
@@ -1042,22 +1093,48 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       }
       finish_item<kCols, kParts == 2>(red, share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb) {
         // two parts: the columns of one pair in one row; one: two rows of one pair
-        const int column = kParts == 2 ? c * 4 + quad : c * 8 + quad * 2 + i, row = strip * 32 + t * 16 + row8 + (kParts == 2 ? i * 8 : 0);
+        const int column = kParts == 2 ? c * 4 + quad : c * 8 + quad * 2 + i, in_strip = t * 16 + row8 + (kParts == 2 ? i * 8 : 0), row = strip * 32 + in_strip;
         if (column >= n) return;
         const int pair = list[s.y + column];
         const float f = p.act_inv[pair] * p.g[e];
-        float* const to = p.y + (size_t)pair * p.N + row;
-        if (kParts == 2) {
-          if (row < p.N) to[0] = (va + vb) * f;
+        if constexpr (kWhole) {
+          // [strip of the cluster][pair][32 rows], in its first block
+          const uint32_t to = base + l.y + (uint32_t)((at.hi * p.M * p.topk + pair) * 32 + in_strip) * 4;
+          const uint32_t cluster_to = p.split > 1 ? map_to_cta(to, 0) : to;
+          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to), "f"(kParts == 2 ? (va + vb) * f : va * f) : "memory");
+          if (kParts == 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to + 32), "f"(vb * f) : "memory");
         } else {
-          if (row < p.N) to[0] = va * f;
-          if (row + 8 < p.N) to[8] = vb * f;
+          float* const to = p.y + (size_t)pair * p.N + row;
+          if (kParts == 2) {
+            if (row < p.N) to[0] = (va + vb) * f;
+          } else {
+            if (row < p.N) to[0] = va * f;
+            if (row + 8 < p.N) to[8] = vb * f;
+          }
         }
       });
     }
     ring.drain();
-    // The block that completes a strip adds up every token's pairs, in the order of the routing.
     const float* const weights = reinterpret_cast<const float*>(smem + l.weights);
+    if constexpr (kWhole) {
+      // every token's pairs are added up in the order of the routing
+      if (p.split > 1) cluster_sync_any();
+      else __syncthreads();
+      if ((int)blockIdx.x % p.split != 0 || d.strip0 >= p.strips) return;
+      const int P = p.M * p.topk, count = ((p.strips - d.strip0 + d.strip_step - 1) / d.strip_step) * p.M * 32;
+      for (int i = threadIdx.x; i < count; i += kThreads) {
+        const int hi = (i >> 5) / p.M, m = (i >> 5) - hi * p.M, row = (d.strip0 + hi * d.strip_step) * 32 + (i & 31);
+        if (row >= p.N) continue;
+        const float* const y = reinterpret_cast<const float*>(smem + l.y) + (hi * P + m * p.topk) * 32 + (i & 31);
+        float sum = 0.f;
+#pragma unroll 4
+        for (int s = 0; s < p.topk; ++s)
+          if (expert[m * p.topk + s] != 0xFFFF) sum += weights[m * p.topk + s] * y[s * 32];
+        store_value(p.out, p.out_dtype, (size_t)m * p.N + row, sum);
+      }
+      return;
+    }
+    // The block that completes a strip adds up every token's pairs, in the order of the routing.
     int* const done_strips = reinterpret_cast<int*>(smem + l.scan);
     int& n_done = done_strips[32];
     __threadfence();
@@ -1132,53 +1209,116 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   }
 }
 
-template <typename XT, bool kDown, int kCols, int kParts>
-int launch_moe_of(MoeParams p, cudaStream_t st) {
+struct MoePlan {
+  MoeParams p;
+  uint32_t smem;
+  unsigned grid;
+  double items;               // of the busiest block, if the slots are as many as foretold
+};
+
+// Slots of a call as far as they can be foretold: what a router without favourites would give
+double slots_of(const MoeParams& p, int cap) {
+  const double pairs = (double)p.M * p.topk, local = pairs * p.E / (double)(p.map != nullptr ? std::max<int64_t>(p.global_E, p.E) : p.E);
+  const double each = std::min(1.0, local / ((double)p.M * p.E)), reached = p.E * (1.0 - std::pow(1.0 - each, p.M));
+  return std::max(1.0, std::max(reached, local / cap));
+}
+
+// What a launch would be, without launching; a status other than success where there is no room for it
+template <typename XT, int kMode, int kCols, int kParts>
+int plan_moe(const MoeParams& given, MoePlan& plan) {
   static std::once_flag once[64];
   static bool ready[64];
-  if (!allow_smem(w4a16_moe_kernel<XT, kDown, kCols, kParts>, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
-  const int pairs = p.M * p.topk;
+  static ResidentClusters counts[kMaxSplit + 1][64];
+  constexpr auto kernel = w4a16_moe_kernel<XT, kMode, kCols, kParts>;
+  if (!allow_smem(kernel, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
+  MoeParams p = given;
+  const int pairs = p.M * p.topk, sms = sm_count();
   const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;
-  p.cap = 8 * kCols / (kDown ? kParts : 1);
+  p.cap = 8 * kCols / (kMode == kGateUp ? 1 : kParts);
   p.rows = 0;
-  while (!kDown) {
+  p.split = 1;
+  while (kMode == kGateUp) {
     // rows that there is room for; a slot has no more columns than that
-    const uint32_t rest = moe_layout(kCols, pairs, p.E, p.cap, 0, 0).rows + 16;      // the counts lie where the rows come
+    const uint32_t rest = moe_layout(kCols, pairs, p.E, p.cap, 0, 0, 0).rows + 16;      // the counts lie where the rows come
     p.rows = rest < kSmemMost ? (int)std::min<uint32_t>((uint32_t)std::min(pairs, kThreads), (kSmemMost - rest) / (row_bytes + (uint32_t)sizeof(RowStat))) : 0;
     if (p.rows < 1) return B200FP4_STATUS_NOT_SUPPORTED;
     if (p.rows >= std::min(p.cap, pairs)) break;
     p.cap = p.rows;
   }
-  const uint32_t smem = moe_layout(kCols, pairs, p.E, p.cap, p.rows, row_bytes).bytes;
-  if (smem > kSmemMost || (int64_t)(std::min(pairs, p.E) + pairs / p.cap) * p.strips > 0x3FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
-  // Items as far as they can be foretold: what a router without favourites would give
-  const double local = (double)pairs * p.E / (double)(p.map != nullptr ? std::max<int64_t>(p.global_E, p.E) : p.E);
-  const double each = std::min(1.0, local / ((double)p.M * p.E)), reached = p.E * (1.0 - std::pow(1.0 - each, p.M));
-  const double slots = std::max(1.0, std::max(reached, local / p.cap));
-  p.log_share = share_of((int)(slots * p.strips / sm_count()) + 1, p.units);
-  if (launch_pdl(w4a16_moe_kernel<XT, kDown, kCols, kParts>, dim3(sm_count()), dim3(kThreads), smem, st, p) != cudaSuccess) {
+  if ((int64_t)(std::min(pairs, p.E) + pairs / p.cap) * p.strips > 0x3FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
+  const double slots = slots_of(p, p.cap);
+  int strips = 0;
+  double items = slots * p.strips / sms;
+  plan.grid = (unsigned)sms;
+  if (kMode == kDownStrips) {
+    // blocks of a cluster: the fewest items of a block
+    items = 1e30;
+    for (int split = 1; split <= kMaxSplit; split *= 2) {
+      const int clusters = std::min(p.strips, split == 1 ? sms : resident_clusters_of(counts[split], kernel, split, kThreads, kSmemMost));
+      if (clusters < 1) break;
+      const int own = (p.strips + clusters - 1) / clusters;
+      const double most = own * std::ceil(slots / split);
+      if (most < items) {
+        items = most;
+        strips = own;
+        p.split = split;
+        plan.grid = (unsigned)(clusters * split);
+      }
+    }
+    if (strips == 0) return B200FP4_STATUS_NOT_SUPPORTED;
+  }
+  plan.smem = moe_layout(kCols, pairs, p.E, p.cap, p.rows, row_bytes, strips).bytes;
+  if (plan.smem > kSmemMost) return B200FP4_STATUS_NOT_SUPPORTED;
+  plan.items = items;
+  p.log_share = share_of((int)std::min(items, 1e6) + 1, p.units);
+  p.rcp_topk = 1.f / (float)p.topk;
+  p.rcp_grid = 1.f / (float)plan.grid;
+  p.rcp_strips = 1.f / (float)p.strips;
+  plan.p = p;
+  return B200FP4_STATUS_SUCCESS;
+}
+
+template <typename XT, int kMode, int kCols, int kParts>
+int launch_moe(const MoePlan& plan, cudaStream_t st) {
+  if (launch_pdl_cluster(plan.p.split, w4a16_moe_kernel<XT, kMode, kCols, kParts>, dim3(plan.grid), dim3(kThreads), plan.smem, st, plan.p) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
   return finish_launch(1);
 }
 
-// Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  Up to as many pairs an expert as
-// one column of eight holds, few have more.
-template <typename T, int kParts>
-int launch_gate_up(const MoeParams& p, double each, cudaStream_t st) {
-  return each <= 7 ? launch_moe_of<T, false, 1, kParts>(p, st) : launch_moe_of<T, false, 2, kParts>(p, st);
+// Both projections are planned before the first is launched.
+template <typename T, int kUpCols, int kMode, int kDownCols, int kParts>
+int launch_both(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
+  MoePlan u, d;
+  int rc = plan_moe<T, kGateUp, kUpCols, kParts>(up, u);
+  if (rc == B200FP4_STATUS_SUCCESS) rc = plan_moe<__half, kMode, kDownCols, kParts>(down, d);
+  if (rc != B200FP4_STATUS_SUCCESS) return rc;
+  rc = launch_moe<T, kGateUp, kUpCols, kParts>(u, st);
+  return rc == B200FP4_STATUS_SUCCESS ? launch_moe<__half, kMode, kDownCols, kParts>(d, st) : rc;
 }
-template <int kParts>
-int launch_down(const MoeParams& p, double each, cudaStream_t st) {
-  return each * kParts <= 7 ? launch_moe_of<__half, true, 1, kParts>(p, st) : launch_moe_of<__half, true, 2, kParts>(p, st);
+
+template <typename T, int kParts>
+int launch_layer_of(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
+  // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  Up to as many pairs an expert as
+  // one column of eight holds, few have more.
+  const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
+  if (each <= 7) {
+    if (each * kParts > 7) return launch_both<T, 1, kDownItems, 2, kParts>(up, down, st);
+    // Whole strips: nothing goes through memory and no block waits for a counter, 1.4 us less for one token (H = 2048, ten experts of 512: 14.0 us against
+    // 15.4), but the blocks' shares are less even.  A block reads 36 units in some 2 us: from there on the items are spread over all blocks (12 tokens, eight experts
+    // of 4096 and H = 4096, a surplus of 41 units: 53 us against 57).
+    MoePlan strips;
+    if (plan_moe<__half, kDownStrips, 1, kParts>(down, strips) == B200FP4_STATUS_SUCCESS &&
+        (strips.items - slots_of(down, strips.p.cap) * down.strips / sm_count()) * down.units < 36)
+      return launch_both<T, 1, kDownStrips, 1, kParts>(up, down, st);
+    return launch_both<T, 1, kDownItems, 1, kParts>(up, down, st);
+  }
+  return launch_both<T, 2, kDownItems, 2, kParts>(up, down, st);
 }
 template <int kParts>
 int launch_layer(const MoeParams& up, const MoeParams& down, int h_dtype, cudaStream_t st) {
-  // pairs of an expert of this call, as a router without favourites gives them
-  const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
-  const int rc = h_dtype == B200FP4_DTYPE_BF16 ? launch_gate_up<__nv_bfloat16, kParts>(up, each, st) : launch_gate_up<__half, kParts>(up, each, st);
-  return rc == B200FP4_STATUS_SUCCESS ? launch_down<kParts>(down, each, st) : rc;
+  return h_dtype == B200FP4_DTYPE_BF16 ? launch_layer_of<__nv_bfloat16, kParts>(up, down, st) : launch_layer_of<__half, kParts>(up, down, st);
 }
 
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
