@@ -249,11 +249,39 @@ inline int share_of(int items, int units) {
   return log_share;
 }
 
+// A run of items is done in phases: rounds of an item a warp, then the rest by groups of warps, so that no warp is without work for more than a part of an item.
+// share: log2 of the warps of a group.  The plan has that of each number of items under a round, four bits each.
+struct Phase {
+  int count, share;
+};
+__device__ __forceinline__ Phase next_phase(int rest, uint64_t plan) {
+  if (rest >= kWarps) return {rest & -kWarps, 0};
+  const int share = (int)(plan >> (rest * 4)) & 15, most = kWarps >> share;
+  return {rest < most ? rest : most, share};
+}
+inline uint64_t phase_plan(int units) {
+  static_assert(kWarps == 16, "a plan has 16 numbers of four bits");
+  uint64_t plan = 0;
+  float cost[kWarps] = {};
+  for (int rest = 1; rest < kWarps; ++rest) {
+    int best = 0;
+    cost[rest] = 1e30f;
+    for (int s = 0; s < 5 && (s == 0 || (1 << s) <= units); ++s) {
+      const int count = std::min(rest, kWarps >> s);
+      const float all = share_cost(count, units, s) + cost[rest - count] + 400.f;
+      if (all < cost[rest]) cost[rest] = all, best = s;
+    }
+    plan |= (uint64_t)best << (rest * 4);
+  }
+  return plan;
+}
+
 // Sums of the warps that share an item, [warp][tile][column of eight][j][lane]: each warp adds up some of them, in the order of k, and finishes them.
 // A lane's sums j are row l / 4 (0, 1) or l / 4 + 8 (2, 3) of a tile and columns 2 (l % 4) and the next one; finish gets those of j = kFirst[i] and
-// kSecond[i].  Both barriers are the group's.
+// kSecond[i].  Both barriers are the group's, whichever others there are at the time.
 template <int kCols, bool kAcross, typename F>
-__device__ __forceinline__ void finish_item(float* red, int share, int in_group, int group, int lane, const float (&acc)[2][kCols][4], F&& finish) {
+__device__ __forceinline__ void finish_item(float* red, int log_share, int in_group, int group, int lane, const float (&acc)[2][kCols][4], F&& finish) {
+  const int share = 1 << log_share;
   // kAcross: the pair is the two columns of one row (j, j + 1), otherwise the two rows of one column (j, j + 2)
   constexpr int kSums = 2 * kCols * 4 * 32;
   if (share == 1) {
@@ -272,7 +300,7 @@ __device__ __forceinline__ void finish_item(float* red, int share, int in_group,
     for (int c = 0; c < kCols; ++c)
 #pragma unroll
       for (int j = 0; j < 4; ++j) own[in_group * kSums + ((t * kCols + c) * 4 + j) * 32] = acc[t][c][j];
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"((kWarps >> log_share) + group), "r"(share * 32) : "memory");
   for (int u = in_group; u < 4 * kCols; u += share) {
     const int i = u & 1, tc = u >> 1;
     const float *a = own + (tc * 4 + (kAcross ? 2 * i : i)) * 32, *b = a + (kAcross ? 32 : 64);
@@ -284,7 +312,7 @@ __device__ __forceinline__ void finish_item(float* red, int share, int in_group,
     }
     finish(kCols == 1 ? tc : tc / kCols, kCols == 1 ? 0 : tc % kCols, i, va, vb);
   }
-  asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(share * 32) : "memory");
+  asm volatile("bar.sync %0, %1;" ::"r"((kWarps >> log_share) + group), "r"(share * 32) : "memory");
 }
 
 // ---- powers of two that bring values into f16's range
@@ -550,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
         arrived = true;
       }
       const int strip = item - slot * p.strips;
-      finish_item<kCols, false>(reinterpret_cast<float*>(smem + l.red), share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb) {
+      finish_item<kCols, false>(reinterpret_cast<float*>(smem + l.red), p.log_share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb) {
         const int column = c * 8 + quad * 2 + i, row = t * 16 + row8;
         if (column >= n) return;
         const float f = kConvert ? inv[column] : 1.f;
@@ -694,7 +722,7 @@ struct MoeParams {
   int M, N, K;
   int strips, units;
   int cap, rows;              // columns of a slot; rows that there is room for
-  int log_share;
+  uint64_t phases;
   int split;                  // whole strips: blocks of a cluster, which share the slots of a strip
   float rcp_topk, rcp_grid, rcp_strips;
   const int32_t* ids;         // [M, topk]
@@ -922,33 +950,50 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     d.fast = p.strips;
   }
   const int first = d.first, last = d.last, fast = d.fast;
-  const int share = 1 << p.log_share, group = warp >> p.log_share, in_group = warp & (share - 1), n_groups = kWarps >> p.log_share;
-  const int k_first = (p.units * in_group) >> p.log_share, n_units = ((p.units * (in_group + 1)) >> p.log_share) - k_first;
-
-  struct Cursor {
-    int item, hi, lo;         // hi * fast + lo
+  const float rcp_fast = kDown ? __frcp_rn((float)fast) : p.rcp_strips;
+  // Gate/up: rows are staged for as many slots at a time as there is room for: a turn's items end before slot stop
+  auto turn_of = [&](int slot, int& n_rows) {
+    int stop = slot + 1;
+    n_rows = slots[slot].x >> 16;
+#pragma unroll 1
+    while (stop < n_slots && stop * fast < last && n_rows + (slots[stop].x >> 16) <= p.rows) n_rows += slots[stop++].x >> 16;
+    return stop;
   };
-  Cursor at = {first + group, 0, 0};
-  if (fast > 0) at.hi = quotient(at.item, fast, kDown ? __frcp_rn((float)fast) : p.rcp_strips);
-  at.lo = at.item - at.hi * fast;
-  Cursor ahead = at;
-  auto next = [&](Cursor& c) {
-    c.item += n_groups;
-    c.lo += n_groups;
-    while (c.lo >= fast) {
-      c.lo -= fast;
-      ++c.hi;
-    }
+  // This warp's part of an item
+  struct Part {
+    int group, in_group, k_first, n_units;
   };
-  int ahead_left = 0, src_step = 0;
+  auto part_of = [&](int log_share) {
+    Part part;
+    part.group = warp >> log_share;
+    part.in_group = warp & ((1 << log_share) - 1);
+    part.k_first = (p.units * part.in_group) >> log_share;
+    part.n_units = ((p.units * (part.in_group + 1)) >> log_share) - part.k_first;
+    return part;
+  };
+  // Weights are asked for ahead of the items, in the same order
+  int ahead = first, ahead_share = 4, phase_end = first, turn_end = kDown ? last : first, ahead_left = 0, src_step = 0;
   const uint8_t* src = nullptr;
   auto fetch = [&]() {
-    if (ahead_left == 0) {
-      if (ahead.item >= last) return;
-      const int e = slots[kDown ? d.slot0 + ahead.lo : ahead.hi].x & 0xFFFF, strip = kDown ? d.strip0 + ahead.hi * d.strip_step : ahead.lo;
-      src = p.packed + (size_t)(e * p.strips * p.units + strip_at(strip, p.strips, p.units, k_first, src_step)) * kUnitBytes;
-      ahead_left = n_units;
-      next(ahead);
+    if (__builtin_expect(ahead_left == 0, 0)) {
+      ahead += kWarps >> ahead_share;
+#pragma unroll 1
+      while (ahead >= phase_end) {
+        if (phase_end >= last) return;
+        if (!kDown && phase_end == turn_end) {
+          int n_rows;
+          turn_end = min(last, turn_of(quotient(phase_end, fast, rcp_fast), n_rows) * fast);
+        }
+        const Phase phase = next_phase(turn_end - phase_end, p.phases);
+        ahead_share = phase.share;
+        ahead = phase_end + (warp >> ahead_share);
+        phase_end += phase.count;
+      }
+      const Part part = part_of(ahead_share);
+      const int hi = quotient(ahead, fast, rcp_fast), lo = ahead - hi * fast;
+      const int e = slots[kDown ? d.slot0 + lo : hi].x & 0xFFFF, strip = kDown ? d.strip0 + hi * d.strip_step : lo;
+      src = p.packed + (size_t)(e * p.strips * p.units + strip_at(strip, p.strips, p.units, part.k_first, src_step)) * kUnitBytes;
+      ahead_left = part.n_units;
     }
     ring.ask(src, lane);
     src += src_step * kUnitBytes;
@@ -962,13 +1007,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       for (int i = threadIdx.x; i < p.n_counters; i += kThreads) p.counters[i] = 0;
     }
     RowStat* const stats = reinterpret_cast<RowStat*>(smem + l.stats);
-    // Rows are staged for as many slots at a time as there is room for: slots [slot, stop), the pairs in places [row0, row0 + n_rows) of the list
+    // slots [slot, stop) of a turn, the pairs in places [row0, row0 + n_rows) of the list
     StagedRows<XT, true> staged;
-    int slot = last > first ? quotient(first, fast, p.rcp_strips) : 0;
+    int slot = last > first ? quotient(first, fast, rcp_fast) : 0;
     for (int end = first; end < last;) {
-      const int slots_end = quotient(last - 1, fast, p.rcp_strips) + 1, row0 = slots[slot].y;
-      int stop = slot + 1, n_rows = slots[slot].x >> 16;
-      while (stop < slots_end && n_rows + (slots[stop].x >> 16) <= p.rows) n_rows += slots[stop++].x >> 16;
+      int n_rows, done = end;
+      const int row0 = slots[slot].y, stop = turn_of(slot, n_rows);
       if (end > first) __syncthreads();            // nobody reads the rows before these any more
       auto row_at = [&](int r) { return static_cast<const XT*>(p.x) + (int64_t)quotient(list[row0 + r], p.topk, p.rcp_topk) * p.ldx; };
       staged.ask(n_rows, 0, p.K, row_at);
@@ -997,37 +1041,43 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         p.act_inv[own] = pow2(-up);
       }
       __syncthreads();
-      for (; at.item < end; next(at)) {
-        const int2 s = slots[at.hi];
-        const int n = s.x >> 16, e = s.x & 0xFFFF, strip = at.lo;
-        uint32_t col[kCols];
+      while (done < end) {
+        const Phase phase = next_phase(end - done, p.phases);
+        const Part part = part_of(phase.share);
+        for (int item = done + part.group; item < done + phase.count; item += kWarps >> phase.share) {
+          const int hi = quotient(item, fast, rcp_fast), strip = item - hi * fast;
+          const int2 s = slots[hi];
+          const int n = s.x >> 16, e = s.x & 0xFFFF;
+          uint32_t col[kCols];
 #pragma unroll
-        for (int c = 0; c < kCols; ++c) {
-          const int i = c * 8 + row8;              // columns past the slot's pairs read the first one's row: nobody reads their sums
-          col[c] = base + l.rows + (s.y - row0 + (i < n ? i : 0)) * row_bytes + quad * 32;
-        }
-        float acc[2][kCols][4] = {};
+          for (int c = 0; c < kCols; ++c) {
+            const int i = c * 8 + row8;              // columns past the slot's pairs read the first one's row: nobody reads their sums
+            col[c] = base + l.rows + (s.y - row0 + (i < n ? i : 0)) * row_bytes + quad * 32;
+          }
+          float acc[2][kCols][4] = {};
 #pragma unroll 1
-        for (int k = k_first; k < k_first + n_units; ++k) {
-          uint32_t b[2][kCols][8];
-          staged_columns<kCols>(col, k * (kUnitK * 2), b);
-          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
-          ring.advance();
-          if (ring.ok) fetch();
+          for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
+            uint32_t b[2][kCols][8];
+            staged_columns<kCols>(col, k * (kUnitK * 2), b);
+            multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
+            ring.advance();
+            if (ring.ok) fetch();
+          }
+          finish_item<kCols, false>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float gate, float up) {
+            const int column = c * 8 + quad * 2 + i, I = p.N / 2, i_at = strip * 16 + t * 8 + row8;
+            if (column >= n || i_at >= I) return;
+            const int pair = list[s.y + column];
+            const RowStat st = stats[s.y - row0 + column];
+            const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
+            const float v = silu_f32(gate * f * p.g[2 * e]) * (up * f * p.g[2 * e + 1]) * st.act;
+            const __half hi = __float2half_rn(v);
+            const float rest = v - __half2float(hi);
+            __half* const to = p.act + (size_t)pair * kParts * I + i_at;
+            to[0] = hi;
+            if (kParts == 2) to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
+          });
         }
-        finish_item<kCols, false>(red, share, in_group, group, lane, acc, [&](int t, int c, int i, float gate, float up) {
-          const int column = c * 8 + quad * 2 + i, I = p.N / 2, i_at = strip * 16 + t * 8 + row8;
-          if (column >= n || i_at >= I) return;
-          const int pair = list[s.y + column];
-          const RowStat st = stats[s.y - row0 + column];
-          const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
-          const float v = silu_f32(gate * f * p.g[2 * e]) * (up * f * p.g[2 * e + 1]) * st.act;
-          const __half hi = __float2half_rn(v);
-          const float rest = v - __half2float(hi);
-          __half* const to = p.act + (size_t)pair * kParts * I + i_at;
-          to[0] = hi;
-          if (kParts == 2) to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
-        });
+        done += phase.count;
       }
     }
     ring.drain();
@@ -1042,77 +1092,83 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         store_value(p.out, p.out_dtype, i, 0.f);
       return;
     }
-    for (; at.item < last; next(at)) {
-      const int2 s = slots[d.slot0 + at.lo];
-      const int n = s.x >> 16, e = s.x & 0xFFFF, strip = d.strip0 + at.hi * d.strip_step;
-      const __half* act[kCols];
+    for (int done = first; done < last;) {
+      const Phase phase = next_phase(last - done, p.phases);
+      const Part part = part_of(phase.share);
+      for (int item = done + part.group; item < done + phase.count; item += kWarps >> phase.share) {
+        const int strip_nth = quotient(item, fast, rcp_fast);
+        const int2 s = slots[d.slot0 + item - strip_nth * fast];
+        const int n = s.x >> 16, e = s.x & 0xFFFF, strip = d.strip0 + strip_nth * d.strip_step;
+        const __half* act[kCols];
 #pragma unroll
-      for (int c = 0; c < kCols; ++c) {
-        const int i = (c * 8 + row8) / kParts;     // a pair's columns are its parts
-        act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i < n ? i : 0)] * kParts + (kParts == 2 ? row8 & 1 : 0)) * p.ldx + quad * 16;
-      }
-      float acc[2][kCols][4] = {};
-      uint32_t b[2][kCols][8];
-      auto load_columns = [&](int k, uint32_t(&to)[2][kCols][8]) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int c = 0; c < kCols; ++c) {
-            const int x = k * kUnitK + half * 64;
-            uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-            if (x + quad * 16 < p.K) {
-              lo = ld_u4(act[c] + x);
-              hi = ld_u4(act[c] + x + 8);
-            }
-            to[half][c][0] = lo.x, to[half][c][1] = lo.y, to[half][c][2] = lo.z, to[half][c][3] = lo.w;
-            to[half][c][4] = hi.x, to[half][c][5] = hi.y, to[half][c][6] = hi.z, to[half][c][7] = hi.w;
-          }
-      };
-      if constexpr (kCols == 1) {                  // a unit ahead, as far as there are registers
-        load_columns(k_first, b);
-#pragma unroll 1
-        for (int k = k_first; k < k_first + n_units; ++k) {
-          uint32_t after[2][kCols][8];
-          load_columns(k + 1, after);
-          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
-          ring.advance();
-          if (ring.ok) fetch();
+        for (int c = 0; c < kCols; ++c) {
+          const int i = (c * 8 + row8) / kParts;     // a pair's columns are its parts
+          act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i < n ? i : 0)] * kParts + (kParts == 2 ? row8 & 1 : 0)) * p.ldx + quad * 16;
+        }
+        float acc[2][kCols][4] = {};
+        uint32_t b[2][kCols][8];
+        auto load_columns = [&](int k, uint32_t(&to)[2][kCols][8]) {
 #pragma unroll
           for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) b[half][0][j] = after[half][0][j];
-        }
-      } else {
+            for (int c = 0; c < kCols; ++c) {
+              const int x = k * kUnitK + half * 64;
+              uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
+              if (x + quad * 16 < p.K) {
+                lo = ld_u4(act[c] + x);
+                hi = ld_u4(act[c] + x + 8);
+              }
+              to[half][c][0] = lo.x, to[half][c][1] = lo.y, to[half][c][2] = lo.z, to[half][c][3] = lo.w;
+              to[half][c][4] = hi.x, to[half][c][5] = hi.y, to[half][c][6] = hi.z, to[half][c][7] = hi.w;
+            }
+        };
+        if constexpr (kCols == 1) {                  // a unit ahead, as far as there are registers
+          load_columns(part.k_first, b);
 #pragma unroll 1
-        for (int k = k_first; k < k_first + n_units; ++k) {
-          load_columns(k, b);
-          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
-          ring.advance();
-          if (ring.ok) fetch();
-        }
-      }
-      finish_item<kCols, kParts == 2>(red, share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb) {
-        // two parts: the columns of one pair in one row; one: two rows of one pair
-        const int column = kParts == 2 ? c * 4 + quad : c * 8 + quad * 2 + i, in_strip = t * 16 + row8 + (kParts == 2 ? i * 8 : 0), row = strip * 32 + in_strip;
-        if (column >= n) return;
-        const int pair = list[s.y + column];
-        const float f = p.act_inv[pair] * p.g[e];
-        if constexpr (kWhole) {
-          // [strip of the cluster][pair][32 rows], in its first block
-          const uint32_t to = base + l.y + (uint32_t)((at.hi * p.M * p.topk + pair) * 32 + in_strip) * 4;
-          const uint32_t cluster_to = p.split > 1 ? map_to_cta(to, 0) : to;
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to), "f"(kParts == 2 ? (va + vb) * f : va * f) : "memory");
-          if (kParts == 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to + 32), "f"(vb * f) : "memory");
+          for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
+            uint32_t after[2][kCols][8];
+            load_columns(k + 1, after);
+            multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
+            ring.advance();
+            if (ring.ok) fetch();
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+#pragma unroll
+              for (int j = 0; j < 8; ++j) b[half][0][j] = after[half][0][j];
+          }
         } else {
-          float* const to = p.y + (size_t)pair * p.N + row;
-          if (kParts == 2) {
-            if (row < p.N) to[0] = (va + vb) * f;
-          } else {
-            if (row < p.N) to[0] = va * f;
-            if (row + 8 < p.N) to[8] = vb * f;
+#pragma unroll 1
+          for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
+            load_columns(k, b);
+            multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
+            ring.advance();
+            if (ring.ok) fetch();
           }
         }
-      });
+        finish_item<kCols, kParts == 2>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float va, float vb) {
+          // two parts: the columns of one pair in one row; one: two rows of one pair
+          const int column = kParts == 2 ? c * 4 + quad : c * 8 + quad * 2 + i, in_strip = t * 16 + row8 + (kParts == 2 ? i * 8 : 0), row = strip * 32 + in_strip;
+          if (column >= n) return;
+          const int pair = list[s.y + column];
+          const float f = p.act_inv[pair] * p.g[e];
+          if constexpr (kWhole) {
+            // [strip of the cluster][pair][32 rows], in its first block
+            const uint32_t to = base + l.y + (uint32_t)((strip_nth * p.M * p.topk + pair) * 32 + in_strip) * 4;
+            const uint32_t cluster_to = p.split > 1 ? map_to_cta(to, 0) : to;
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to), "f"(kParts == 2 ? (va + vb) * f : va * f) : "memory");
+            if (kParts == 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to + 32), "f"(vb * f) : "memory");
+          } else {
+            float* const to = p.y + (size_t)pair * p.N + row;
+            if (kParts == 2) {
+              if (row < p.N) to[0] = (va + vb) * f;
+            } else {
+              if (row < p.N) to[0] = va * f;
+              if (row + 8 < p.N) to[8] = vb * f;
+            }
+          }
+        });
+      }
+      done += phase.count;
     }
     ring.drain();
     const float* const weights = reinterpret_cast<const float*>(smem + l.weights);
@@ -1270,7 +1326,7 @@ int plan_moe(const MoeParams& given, MoePlan& plan) {
   plan.smem = moe_layout(kCols, pairs, p.E, p.cap, p.rows, row_bytes, strips).bytes;
   if (plan.smem > kSmemMost) return B200FP4_STATUS_NOT_SUPPORTED;
   plan.items = items;
-  p.log_share = share_of((int)std::min(items, 1e6) + 1, p.units);
+  p.phases = phase_plan(p.units);
   p.rcp_topk = 1.f / (float)p.topk;
   p.rcp_grid = 1.f / (float)plan.grid;
   p.rcp_strips = 1.f / (float)p.strips;
