@@ -486,6 +486,12 @@ B200_FN(py_moe_prefill) {
 bool is_float(const at::Tensor& t) { return is_16bit(t) || t.scalar_type() == at::kFloat; }
 bool rows_aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && (t.size(0) < 2 || t.stride(0) % 8 == 0); }
 
+// Whether a [rows, cols] tensor that is read, rows `ld` elements apart, and a contiguous result share memory
+bool meet(const at::Tensor& read, int64_t rows, int64_t cols, int64_t ld, const at::Tensor& written) {
+  const char *r = static_cast<const char*>(read.data_ptr()), *w = static_cast<const char*>(written.data_ptr());
+  return rows > 0 && cols > 0 && r < w + written.nbytes() && w < r + ((rows - 1) * ld + cols) * (int64_t)read.element_size();
+}
+
 // Status word and scratch of a call.  The scratch of a captured call is its own, from its graph's pool: graphs that are replayed at once
 // share no more than the status word.
 class Scratch {
@@ -531,6 +537,7 @@ B200_FN(py_w4a16_linear) {
     }
     require(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, "out_dtype must be bfloat16, float16 or float32");
     require(given == nullptr || (given->scalar_type() == dt && is_2d(*given, M, N) && given->is_contiguous()), "out must be a contiguous [M,N] tensor of out_dtype");
+    require(given == nullptr || !meet(x, M, K, M > 1 ? x.stride(0) : K, *given), "out must not overlap x");
     at::Tensor out;
     {
       WithoutGil nogil;
@@ -574,6 +581,9 @@ B200_FN(py_w4a16_moe) {
                 g2.numel() == E,
             "the weights must come from pack_nvfp4_weight");
     require(given == nullptr || (is_float(*given) && is_2d(*given, M, H) && given->is_contiguous()), "out must be a contiguous [M,H] tensor in bf16, f16 or f32");
+    // In place is right: a row of hidden_states is read for the last time before its result is written.
+    require(given == nullptr || (given->data_ptr() == x.data_ptr() && given->nbytes() == x.nbytes()) || !meet(x, M, H, H, *given),
+            "out must be hidden_states or not overlap it");
     at::Tensor out;
     {
       WithoutGil nogil;

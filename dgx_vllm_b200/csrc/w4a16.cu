@@ -1035,8 +1035,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       if (own >= 0) {
         // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the bound is
         // far above the values costs little: f16 reaches 40 binades down.
-        const float norm = sqrtf(stats[threadIdx.x].act * (float)p.K) * w, bound = fabsf(norm * (g.x * peak.x)) * fabsf(norm * (g.y * peak.y));
-        const int up = min(max(14 - ((int)(__float_as_uint(bound) >> 23) - 126), -100), 100);
+        // Where the squares have left f32's range, |x| <= 2^16 inv sqrt(K) is the bound that is left.
+        const float squares = stats[threadIdx.x].act, root = sqrtf((float)p.K);
+        const float norm = (squares > 1e-30f && squares < 1e30f ? sqrtf(squares) : 65536.f * stats[threadIdx.x].inv * root) * root * w;
+        const float bound = fabsf(norm * (g.x * peak.x)) * fabsf(norm * (g.y * peak.y));
+        const int up = min(14 - ((int)(__float_as_uint(bound) >> 23) - 126), 100);        // from -115, an infinite bound
         stats[threadIdx.x].act = pow2(up);
         p.act_inv[own] = pow2(-up);
       }
@@ -1450,8 +1453,11 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   if (!fits_int(M) || !fits_int(N + 64) || !fits_int(K + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
   const LinearCall c = {x, x_dtype, ldx, packed, g_scale, bias, bias_dtype, out, out_dtype, M, N, K, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (!few_tokens(c)) return launch_w4a16_gemm(c, st);
-  return x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(c, st) : launch_linear<__half>(c, st);
+  if (few_tokens(c)) {
+    const int rc = x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(c, st) : launch_linear<__half>(c, st);
+    if (rc != B200FP4_STATUS_NOT_SUPPORTED) return rc;        // rows too long for shared memory (K above some 400,000) are not for this kernel
+  }
+  return launch_w4a16_gemm(c, st);
 }
 
 extern "C" size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I) {

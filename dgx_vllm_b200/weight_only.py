@@ -68,7 +68,7 @@ def w4a16_linear(x: torch.Tensor, weight: PackedNvfp4Weight, bias: torch.Tensor 
     """y[M,N] = x @ W^T (+ bias) with the weight's exact values and f32 sums, rounded once.
 
     x [M,K] bf16 or f16: unit inner stride, rows 16-byte aligned (they may be strided); bias [N] bf16, f16 or f32; out contiguous
-    [M,N], or out_dtype bf16, f16 or f32 (the dtype of x by default)."""
+    [M,N] and not in x's memory, or out_dtype bf16, f16 or f32 (the dtype of x by default)."""
     require(weight.E == 1 and not weight.gated, "w4a16_linear takes one matrix that is not packed gated")
     return _lib.host().w4a16_linear(x, weight.packed, weight.g_scale, weight.N, weight.K, bias, out, out_dtype)
 
@@ -106,6 +106,7 @@ class W4A16MoE:
                  apply_router_weight_on_input: bool = False, out: torch.Tensor | None = None,
                  expert_map: torch.Tensor | None = None) -> torch.Tensor:
         """hidden_states [M,H] bf16/f16, topk_weights [M,topk] f32, topk_ids [M,topk] int32 -> [M,H] in the activation dtype (or in `out`'s,
-        which may also be f32).  Pairs whose expert is not here add nothing.  expert_map: in place of the layer's own."""
+        which may also be f32; out may be hidden_states itself).  Pairs whose expert is not here add nothing.  expert_map: in place of
+        the layer's own."""
         emap = self._map if expert_map is None else self._as_map(expert_map)
         return self._call(*self._weights, emap, *self._sizes, hidden_states, topk_weights, topk_ids, apply_router_weight_on_input, out)

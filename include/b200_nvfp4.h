@@ -493,7 +493,7 @@ B200FP4_API int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, 
 
 /* out[M,N] = x . W^T * g_scale (+ bias): x [M,K] bf16 or f16, rows ldx elements apart (a multiple of 8, 16-byte aligned), one packed
  * matrix (not gated), g_scale one f32 on the device (weight_scale_2 of a checkpoint), bias [N] of any dtype or NULL, out contiguous
- * in bf16, f16 or f32.  Products of exact 16-bit values, sums in f32: bf16 rows are brought into f16's range by a power of two each, with
+ * in bf16, f16 or f32, not in x's memory.  Products of exact 16-bit values, sums in f32: bf16 rows are brought into f16's range by a power of two each, with
  * which only what is below 2^-39 of a row's largest magnitude can be rounded.  status (on the device) is 0 after the call, or the code of a
  * bounded wait that ran out: the result is then not valid. */
 B200FP4_API int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const float* g_scale,
@@ -502,9 +502,11 @@ B200FP4_API int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, co
 
 /* One mixture-of-experts layer: gate/up projection -> SiLU(gate)*up -> down projection -> router-weighted sum, in two launches for up
  * to 2048 (token, expert) pairs; more are done in turns.  Arguments as b200fp4_fused_sparse_moe, with w13 [E, 2I, H] packed gated and
- * w2 [E, H, I] packed, w13_g [E][gate rows, up rows], w2_g [E]; H and I multiples of 16, E up to 4096, topk up to 2048.  Pairs whose expert (after expert_map) is outside
- * [0, E) add nothing; a token without any gives zeros.  flags: B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT or 0.  Between the projections a value is kept as
- * the sum of two f16.  Results do not depend on the order in which blocks run. */
+ * w2 [E, H, I] packed, w13_g [E][gate rows, up rows] (8-byte aligned), w2_g [E]; H and I multiples of 16, H as long as a row fits in shared
+ * memory (some 50,000), E up to 4096, topk up to 2048.  out may be hidden (of the same type) or other memory.  Pairs whose expert (after
+ * expert_map) is outside [0, E) add nothing; a token without any gives zeros.  flags: B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT or 0.  Between the
+ * projections a value is kept in one f16, with a power of two for each pair, where the result is bf16, else as the sum of two.  Results do not
+ * depend on the order in which blocks run.  The workspace is a call's own until the call is done. */
 B200FP4_API size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I);
 B200FP4_API int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* topk_weights, const int32_t* topk_ids,
                                   const int32_t* expert_map, int64_t global_E, const uint8_t* w13_packed, const float* w13_g,
