@@ -92,23 +92,7 @@ __host__ __device__ __forceinline__ constexpr uint32_t bar_bytes(int cols) { ret
 __host__ __device__ __forceinline__ uint32_t pad16(uint32_t v) { return (v + 15) / 16 * 16; }
 __host__ __device__ __forceinline__ constexpr uint32_t red_bytes(int cols) { return kWarps * 2 * cols * 4 * 32 * 4; }
 
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ uint4 ld_u4(const void* p) { return *static_cast<const uint4*>(p); }
-
-__device__ __forceinline__ void store_value(void* out, int dtype, size_t at, float v) {
-  if (dtype == B200FP4_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-  else if (dtype == B200FP4_DTYPE_F16) static_cast<__half*>(out)[at] = __float2half_rn(v);
-  else static_cast<float*>(out)[at] = v;
-}
-__device__ __forceinline__ float load_value(const void* p, int dtype, size_t at) {
-  if (dtype == B200FP4_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
-  if (dtype == B200FP4_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[at]);
-  return static_cast<const float*>(p)[at];
-}
 
 // A warp's ring of units: one lane asks for them, all wait for them.  Every unit that was asked for is waited for.
 template <int kStages>
@@ -249,7 +233,8 @@ inline int share_of(int items, int units) {
   return log_share;
 }
 
-// A run of items is done in phases: rounds of an item a warp, then the rest by groups of warps, so that no warp is without work for more than a part of an item.
+// A run of items is done in phases: rounds of an item a warp, then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
+// size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 14.3 / 14.0.
 // share: log2 of the warps of a group.  The plan has that of each number of items under a round, four bits each.
 struct Phase {
   int count, share;
@@ -468,6 +453,9 @@ __host__ __device__ __forceinline__ LinearLayout linear_layout(int cols, int cap
   return l;
 }
 
+// The linear layer of few tokens: bound by the copies of the weight, then by decoding it.  An SM's 16 warps decode and multiply a unit in 87 cycles with one column of eight
+// (131 with two), and its share of HBM brings one in 98, so that a layer reaches the copy rate only where it is large: N=14336 K=4096, 33 MB, takes 9.2 us for one token
+// and 11.4 for eight, of which 2 are the launch and the row, 1.5 the first units' way and 5.1 the floor; N=K=2048 4.4, most of it launch.
 // XT: type of the activations; kCols: columns of eight; kTokens: 1 or 2 where there are no more, else 0
 template <typename XT, int kCols, int kTokens>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearParams p) {
@@ -658,7 +646,8 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
       const int used = (int)std::min<int64_t>(clusters, items), most = (int)((items + used - 1) / used);
       const uint64_t bytes = (uint64_t)linear_layout(kCols, cap, row_bytes, 1, 0).bytes + (split > 1 ? (uint64_t)most * cap * 128 : 0);
       if ((uint64_t)own * 256 > kSmemMost || bytes > kSmemMost) continue;
-      // the busiest block's units; a cluster's exchange costs some 1500 cycles
+      // The busiest block's units; a cluster's exchange costs some 1500 cycles.  Shared / not shared, us: M=1 N=512 K=16384 6.8 / 8.9, M=8 N=512 K=4096 5.2 / 6.1;
+      // by this rule not shared: M=1 N=K=4096 5.2, N=14336 K=4096 9.2.
       const int log_share = share_of(most, p.units / split);
       const float cost = share_cost(most, own, log_share) + (split > 1 ? 1500.f : 0.f);
       if (cost < best) {
@@ -703,6 +692,7 @@ int launch_linear(const LinearCall& c, cudaStream_t st) {
   p.strips = (int)strips_of(c.N);
   p.units = (int)units_of(c.K);
   p.status = c.status;
+  // One or two tokens, a block of k a column / a token a column, us: N=14336 K=4096 9.2 / 10.0 for one and 9.8 / 10.0 for two, N=K=2048 the same.
   if (p.M == 1) return launch_linear_of<T, 1, 1>(p, st);
   if (p.M == 2) return launch_linear_of<T, 1, 2>(p, st);
   return p.M <= 8 ? launch_linear_of<T, 1, 0>(p, st) : launch_linear_of<T, 2, 0>(p, st);
@@ -913,6 +903,9 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
 
 enum Projection { kGateUp, kDownItems, kDownStrips };       // kDownStrips: whole strips
 
+// Bound by the copies of the experts that the routing reaches: 32 tokens, ten of 512 experts, H=2048 I=512, take 91-94 us, gate/up 46 of them at 6.1 TB/s and down 26 at
+// 5.3; the rest is finding the slots (2 us), rows and first units (3), the down projection's start (3) and the strips' last sums (4).  128 tokens 180-187.  Two
+// launches: every value of the first projection is needed by the second, which finds its slots and asks for its first weights while the first one ends.
 // XT: type of the activations (gate/up); kCols: columns of eight; kParts: f16 parts of a value between the projections
 template <typename XT, int kMode, int kCols, int kParts>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
@@ -1359,8 +1352,9 @@ int launch_both(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
 
 template <typename T, int kParts>
 int launch_layer_of(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
-  // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  Up to as many pairs an expert as
-  // one column of eight holds, few have more.
+  // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  One / two of them in both
+  // projections, us, eight experts of 4096, H = 4096, bf16: 7.25 pairs an expert 68 / 73, nine 78 / 75, eleven 87 / 78; 64 experts of 768, H = 2048: eight 59.7 / 59.0, twelve
+  // 77 / 69.  Below seven few experts have more pairs than one column of eight holds.
   const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
   if (each <= 7) {
     if (each * kParts > 7) return launch_both<T, 1, kDownItems, 2, kParts>(up, down, st);

@@ -84,5 +84,23 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
+// outputs and biases of any of the three types
+__device__ __forceinline__ void store_value(void* out, int dtype, size_t at, float v) {
+  if (dtype == B200FP4_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
+  else if (dtype == B200FP4_DTYPE_F16) static_cast<__half*>(out)[at] = __float2half_rn(v);
+  else static_cast<float*>(out)[at] = v;
+}
+__device__ __forceinline__ float load_value(const void* p, int dtype, size_t at) {
+  if (dtype == B200FP4_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
+  if (dtype == B200FP4_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[at]);
+  return static_cast<const float*>(p)[at];
+}
+
 }  // namespace w4
 }  // namespace b200fp4

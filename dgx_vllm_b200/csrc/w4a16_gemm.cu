@@ -10,6 +10,9 @@
 // stage however few the tokens are.  Persistent blocks, one to an SM; where there are too few
 // tiles for them, a cluster shares the k of one and adds up its parts through distributed shared memory, each block some of the tokens.
 // Every wait is bounded (status word), tensor memory is always freed.
+// Bound: with many tokens by the tensor cores, M=4096 N=14336 K=4096 400 us, 1.20 PFLOP/s under the power cap (73 % of the measured burst rate, 88 % of the sustained one), the
+// tensor pipe busy 73 % of active cycles; with few by decoding and the MMA warp's turn, some 450 cycles for 128 of k where HBM brings them in 390: M=32 N=4096 K=14336 15.1 us
+// (33 MB, floor 5.3), M=333 N=K=4096 15.6 (0.72 PFLOP/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -129,23 +132,6 @@ __device__ __forceinline__ void tcgen05_commit_if(uint32_t issue, uint32_t bar) 
       "r"(issue)
       : "memory");
 }
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
-  return v;
-}
-
-__device__ __forceinline__ void store_value(void* out, int dtype, size_t at, float v) {
-  if (dtype == B200FP4_DTYPE_BF16) static_cast<__nv_bfloat16*>(out)[at] = __float2bfloat16_rn(v);
-  else if (dtype == B200FP4_DTYPE_F16) static_cast<__half*>(out)[at] = __float2half_rn(v);
-  else static_cast<float*>(out)[at] = v;
-}
-__device__ __forceinline__ float load_value(const void* p, int dtype, size_t at) {
-  if (dtype == B200FP4_DTYPE_BF16) return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[at]);
-  if (dtype == B200FP4_DTYPE_F16) return __half2float(static_cast<const __half*>(p)[at]);
-  return static_cast<const float*>(p)[at];
-}
-
 // a position in a ring of `size` stages
 struct Slot {
   uint32_t at = 0, phase = 0;
@@ -463,7 +449,8 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
   p.status = c.status;
   const int sms = sm_count();
   // Tokens of a tile and blocks that share one: the least time of the busiest block, in cycles.  128 of k take the MMAs four cycles a token, the copies one for each
-  // 57 bytes, and decoding and issue 450.
+  // 57 bytes, and decoding and issue 450.  Shared by this rule / one block a tile, us: M=32 N=4096 K=14336 15.1 / 40.3, M=64 N=K=4096 9.2 / 14.1, M=128 12.4 / 14.4; by it
+  // not shared: M=333 N=K=4096 15.7.
   double best = 1e30;
   unsigned grid = 0;
   const int64_t least = (c.M + kMostTokens - 1) / kMostTokens;
@@ -488,7 +475,7 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
         p.accs = tiles > clusters ? 2 : 1;
         p.acc_cols = (uint32_t)(tokens + 31) / 32 * 32;
         p.stages = (int)std::min<uint32_t>(kMost, std::min<uint32_t>((512 - p.accs * p.acc_cols) / 64, 144 * 1024 / ((uint32_t)tokens * 256)));
-        // A cluster's sums have room of their own where they are small: nobody waits for the others' MMAs then.
+        // A cluster's sums have room of their own where they are small: nobody waits for the others' MMAs then (M=32 N=4096 K=14336 15.1 us / 15.7, M=64 N=K=4096 9.2 / 9.7).
         const uint32_t sums = split > 1 && tokens <= 64 ? (uint32_t)tokens * kMmaRows * 4 : 0;
         p.sums_at = sums > 0 ? kRingBytes - sums : 0;
         p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - sums - (uint32_t)p.stages * tokens * 256) / kWStageBytes);
