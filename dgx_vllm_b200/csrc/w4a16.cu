@@ -494,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   for (int i = 0; i < stages_of(kCols); ++i) fetch();
   pdl_launch_dependents();
   if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
-  if (split > 1) cluster_arrive();                 // the other blocks run before anything is sent to them
+  if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
   // rows are shifted by 16 bytes against each other: no two lanes of a load meet
   const uint32_t row_bytes = (uint32_t)((p.units + split - 1) / split) * (kUnitK * 2) + 16;
   const LinearLayout l = linear_layout(kCols, p.cap, row_bytes, split, p.per + (p.more > 0));
@@ -920,7 +920,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   const uint16_t* const list = reinterpret_cast<const uint16_t*>(smem + l.list);
   Ring<stages_of(kCols)> ring;
   ring.init(base, base + ring_bytes(kCols), warp, lane);
-  if (kWhole && p.split > 1) cluster_arrive();     // the other blocks run before anything is sent to them
+  if (kWhole && p.split > 1) cluster_arrive_relaxed();     // the other blocks run before anything is sent to them
   // The routing is not the first projection's work, and its kernel lets this one start only once what came before it is complete: the second
   // projection finds its slots and asks for its first weights while the first one ends.
   clear_counts(p, smem, l);
@@ -1173,16 +1173,29 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       if (p.split > 1) cluster_sync_any();
       else __syncthreads();
       if ((int)blockIdx.x % p.split != 0 || d.strip0 >= p.strips) return;
-      const int P = p.M * p.topk, count = ((p.strips - d.strip0 + d.strip_step - 1) / d.strip_step) * p.M * 32;
-      for (int i = threadIdx.x; i < count; i += kThreads) {
-        const int hi = (i >> 5) / p.M, m = (i >> 5) - hi * p.M, row = (d.strip0 + hi * d.strip_step) * 32 + (i & 31);
-        if (row >= p.N) continue;
-        const float* const y = reinterpret_cast<const float*>(smem + l.y) + (hi * P + m * p.topk) * 32 + (i & 31);
+      // a warp a token of a strip: its lanes read the routing, then each has a row
+      const int P = p.M * p.topk, count = ((p.strips - d.strip0 + d.strip_step - 1) / d.strip_step) * p.M;
+      for (int i = warp; i < count; i += kWarps) {
+        const int hi = i / p.M, m = i - hi * p.M, row = (d.strip0 + hi * d.strip_step) * 32 + lane;
+        const float* const y = reinterpret_cast<const float*>(smem + l.y) + (hi * P + m * p.topk) * 32 + lane;
         float sum = 0.f;
-#pragma unroll 4
-        for (int s = 0; s < p.topk; ++s)
-          if (expert[m * p.topk + s] != 0xFFFF) sum += weights[m * p.topk + s] * y[s * 32];
-        store_value(p.out, p.out_dtype, (size_t)m * p.N + row, sum);
+        for (int s0 = 0; s0 < p.topk; s0 += 32) {
+          const bool here = s0 + lane < p.topk && expert[m * p.topk + s0 + lane] != 0xFFFF;
+          const float own = here ? weights[m * p.topk + s0 + lane] : 0.f;
+          for (uint32_t left = __ballot_sync(0xffffffffu, here); left != 0;) {
+            float v[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {          // four loads before the first is needed
+              const int s = left != 0 ? __ffs(left) - 1 : 0;
+              const float product = __shfl_sync(0xffffffffu, own, s) * y[(s0 + s) * 32];
+              v[u] = left != 0 ? product : 0.f;
+              left &= left - 1;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) sum += v[u];
+          }
+        }
+        if (row < p.N) store_value(p.out, p.out_dtype, (size_t)m * p.N + row, sum);
       }
       return;
     }

@@ -186,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   pdl_wait();
   pdl_launch_dependents();
   if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
-  if (split > 1) cluster_arrive();                 // the other blocks run before anything is sent to them
+  if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
 
   if (warp == 0) {
     // ------------------------------------------------------------------ copies of the weight
