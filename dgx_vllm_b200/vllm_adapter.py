@@ -130,7 +130,15 @@ def make_w4a16_apply_fn(w13, w2, fused_fn: Optional[Callable] = None):
             if not layer:
                 from .weight_only import W4A16MoE
                 layer.append(W4A16MoE(w13, w2))
-            result = layer[0](hidden_states.contiguous(), topk_weights, topk_ids, apply_router_weight_on_input, expert_map=expert_map)
+            # straight into the output's rows, where they can be written as they are
+            rows = output[:hidden_states.shape[0]]
+            direct = (rows.shape == hidden_states.shape and rows.is_contiguous() and rows.data_ptr() % 16 == 0
+                      and rows.dtype in (torch.bfloat16, torch.float16, torch.float32)
+                      and rows.untyped_storage().data_ptr() != hidden_states.untyped_storage().data_ptr())
+            result = layer[0](hidden_states.contiguous(), topk_weights, topk_ids, apply_router_weight_on_input,
+                              out=rows if direct else None, expert_map=expert_map)
+            if direct:
+                return output
         output[:hidden_states.shape[0]] = result.to(output.dtype)
         return output
 

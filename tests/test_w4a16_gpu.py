@@ -463,6 +463,11 @@ def test_vllm_adapter_on_the_device():
         experts.apply(out, x, None, None, weights, ids, "silu", n, emap, None, None, None, None, None, False)
         _check(out[:M], x, weights, ids, emap, W13, W2)
         assert bool((out[M:] == 5).all())
+        for other in (torch.full((M, H + 8), 5.0, dtype=BF16, device="cuda")[:, :H], torch.cat((x, x))):       # strided rows; the input's own memory
+            hidden = other[:M] if other.is_contiguous() else x
+            experts.apply(other, hidden, None, None, weights, ids, "silu", n, emap, None, None, None, None, None, False)
+            assert torch.equal(other[:M], out[:M])
+            assert torch.equal(other[M:], x if other.is_contiguous() else x[:0])
     codes, block = make_weight(1, 48, 64, 6)
     lin = types.SimpleNamespace(weight=P(codes[0]), weight_scale=P(block[0]), input_global_scale_inv=torch.tensor([8.0], device="cuda"),
                                 alpha=torch.tensor([0.0625], device="cuda"), output_size_per_partition=48)
