@@ -384,12 +384,13 @@ struct StagedRows {
         if (n_parts > 1) {                         // one round then
           if (lane == 0) parts[warp] = make_float2(__uint_as_float(top), squares);
           __syncthreads();
-          squares = 0.f;
-          for (int j = 0; j < n_parts; ++j) {      // in the same order for every warp of the row
-            const float2 u = parts[warp - part + j];
-            top = max(top, __float_as_uint(u.x));
-            squares += u.y;
-          }
+          // one part a lane, and sums in the same order for every warp of the row
+          const float2 u = lane < n_parts ? parts[warp - part + lane] : make_float2(0.f, 0.f);
+          top = __reduce_max_sync(0xffffffffu, __float_as_uint(u.x));
+          squares = u.y;
+          if constexpr (kSquares)
+#pragma unroll
+            for (int d = kWarps / 2; d > 0; d /= 2) squares += __shfl_xor_sync(0xffffffffu, squares, d);
         }
         const int e = kConvert ? row_exponent(top) : 0;
         factor = (uint32_t)(e + 127) * 0x00800080u;
@@ -927,11 +928,22 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   if (!kDown) {
     pdl_wait();
     pdl_launch_dependents();
-  } else {
-    for (int i = threadIdx.x; i < p.M * p.topk; i += kThreads)
-      reinterpret_cast<float*>(smem + l.weights)[i] = p.weight_on_input ? 1.f : p.weights[i];
   }
+  // the weights are on their way with the ids
+  float weight[kDown ? kMaxPairs / kThreads : 1];
+  if constexpr (kDown)
+#pragma unroll
+    for (int q = 0; q < kMaxPairs / kThreads; ++q) {
+      const int i = q * kThreads + threadIdx.x;
+      weight[q] = i < p.M * p.topk && !p.weight_on_input ? p.weights[i] : 1.f;
+    }
   const int n_slots = find_slots(p, smem, l);
+  if constexpr (kDown)
+#pragma unroll
+    for (int q = 0; q < kMaxPairs / kThreads; ++q) {
+      const int i = q * kThreads + threadIdx.x;
+      if (i < p.M * p.topk) reinterpret_cast<float*>(smem + l.weights)[i] = weight[q];
+    }
   // Items (strip, slot) of a slot are neighbours, or (down) those of a strip
   DownItems d;
   if constexpr (kDown) {
