@@ -226,32 +226,39 @@ inline float share_cost(int items, int units, int log_share) {
   const float item = (float)((units + share - 1) / share) + (log_share == 0 ? 0.33f : 0.9f);
   return item * (float)(full * 1400 + (rest > 0 ? std::max(750, (rest + 3) / 4 * 350) : 0));
 }
-inline int share_of(int items, int units) {
-  int log_share = 0;
-  for (int s = 1; s < 5 && (1 << s) <= units; ++s)
+inline int share_of(int items, int units, int least) {
+  int log_share = least;
+  for (int s = least + 1; s < 5 && (1 << s) <= units; ++s)
     if (share_cost(items, units, s) < share_cost(items, units, log_share)) log_share = s;
   return log_share;
 }
+// The least of it where the result is f32: so many warps that each has a chain of the item's k
+inline int least_share(int out_dtype, int units) {
+  int share = 0;
+  while (out_dtype == B200FP4_DTYPE_F32 && share < 4 && (kWarpChain << share) < units) ++share;
+  return share;
+}
 
-// A run of items is done in phases: rounds of an item a warp, then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
+// A run of items is done in phases: rounds of an item a warp (or a group of the least size), then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
 // size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 14.3 / 14.0.
 // share: log2 of the warps of a group.  The plan has that of each number of items under a round, four bits each.
 struct Phase {
   int count, share;
 };
-__device__ __forceinline__ Phase next_phase(int rest, uint64_t plan) {
-  if (rest >= kWarps) return {rest & -kWarps, 0};
+__device__ __forceinline__ Phase next_phase(int rest, uint64_t plan, int least) {
+  const int groups = kWarps >> least;
+  if (rest >= groups) return {rest & -groups, least};
   const int share = (int)(plan >> (rest * 4)) & 15, most = kWarps >> share;
   return {rest < most ? rest : most, share};
 }
-inline uint64_t phase_plan(int units) {
+inline uint64_t phase_plan(int units, int least) {
   static_assert(kWarps == 16, "a plan has 16 numbers of four bits");
   uint64_t plan = 0;
   float cost[kWarps] = {};
   for (int rest = 1; rest < kWarps; ++rest) {
-    int best = 0;
+    int best = least;
     cost[rest] = 1e30f;
-    for (int s = 0; s < 5 && (s == 0 || (1 << s) <= units); ++s) {
+    for (int s = least; s < 5 && (s == least || (1 << s) <= units); ++s) {
       const int count = std::min(rest, kWarps >> s);
       const float all = share_cost(count, units, s) + cost[rest - count] + 400.f;
       if (all < cost[rest]) cost[rest] = all, best = s;
@@ -647,9 +654,10 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
       const int used = (int)std::min<int64_t>(clusters, items), most = (int)((items + used - 1) / used);
       const uint64_t bytes = (uint64_t)linear_layout(kCols, cap, row_bytes, 1, 0).bytes + (split > 1 ? (uint64_t)most * cap * 128 : 0);
       if ((uint64_t)own * 256 > kSmemMost || bytes > kSmemMost) continue;
+      if (kTokens == 0 && p.out_dtype == B200FP4_DTYPE_F32 && own > kWarpChain * kWarps) continue;       // too long a chain for an f32 result
       // The busiest block's units; a cluster's exchange costs some 1500 cycles.  Shared / not shared, us: M=1 N=512 K=16384 6.8 / 8.9, M=8 N=512 K=4096 5.2 / 6.1;
       // by this rule not shared: M=1 N=K=4096 5.2, N=14336 K=4096 9.2.
-      const int log_share = share_of(most, p.units / split);
+      const int log_share = share_of(most, p.units / split, kTokens > 0 ? 0 : least_share(p.out_dtype, own));
       const float cost = share_cost(most, own, log_share) + (split > 1 ? 1500.f : 0.f);
       if (cost < best) {
         best = cost;
@@ -714,6 +722,7 @@ struct MoeParams {
   int strips, units;
   int cap, rows;              // columns of a slot; rows that there is room for
   uint64_t phases;
+  int least;                  // log2 of the warps of an item, at least
   int split;                  // whole strips: blocks of a cluster, which share the slots of a strip
   float rcp_topk, rcp_grid, rcp_strips;
   const int32_t* ids;         // [M, topk]
@@ -989,7 +998,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
           int n_rows;
           turn_end = min(last, turn_of(quotient(phase_end, fast, rcp_fast), n_rows) * fast);
         }
-        const Phase phase = next_phase(turn_end - phase_end, p.phases);
+        const Phase phase = next_phase(turn_end - phase_end, p.phases, p.least);
         ahead_share = phase.share;
         ahead = phase_end + (warp >> ahead_share);
         phase_end += phase.count;
@@ -1050,7 +1059,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       }
       __syncthreads();
       while (done < end) {
-        const Phase phase = next_phase(end - done, p.phases);
+        const Phase phase = next_phase(end - done, p.phases, p.least);
         const Part part = part_of(phase.share);
         for (int item = done + part.group; item < done + phase.count; item += kWarps >> phase.share) {
           const int hi = quotient(item, fast, rcp_fast), strip = item - hi * fast;
@@ -1101,7 +1110,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       return;
     }
     for (int done = first; done < last;) {
-      const Phase phase = next_phase(last - done, p.phases);
+      const Phase phase = next_phase(last - done, p.phases, p.least);
       const Part part = part_of(phase.share);
       for (int item = done + part.group; item < done + phase.count; item += kWarps >> phase.share) {
         const int strip_nth = quotient(item, fast, rcp_fast);
@@ -1347,7 +1356,8 @@ int plan_moe(const MoeParams& given, MoePlan& plan) {
   plan.smem = moe_layout(kCols, pairs, p.E, p.cap, p.rows, row_bytes, strips).bytes;
   if (plan.smem > kSmemMost) return B200FP4_STATUS_NOT_SUPPORTED;
   plan.items = items;
-  p.phases = phase_plan(p.units);
+  p.least = least_share(p.out_dtype, p.units);
+  p.phases = phase_plan(p.units, p.least);
   p.rcp_topk = 1.f / (float)p.topk;
   p.rcp_grid = 1.f / (float)plan.grid;
   p.rcp_strips = 1.f / (float)p.strips;
@@ -1529,6 +1539,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.g = w13_g;
     p.N = (int)(2 * I);
     p.K = (int)H;
+    p.out_dtype = out_dtype;
     p.strips = (int)((I + 15) / 16);
     p.units = (int)w4::units_of(H);
     d.x = p.act;

@@ -49,7 +49,8 @@ struct GemmParams {
   int stages, w_stages;
   int sets;                   // decoding sets at work: no more than stages of either kind, since a set that is further ahead would take a stage's round for the one before
   uint32_t acc_cols;          // columns of an accumulator
-  int accs;                   // accumulators: two where a block does several tiles
+  int accs;                   // accumulators in turn: two where a block does several tiles, or one in several chains
+  int chain, chains;          // units that are summed in one accumulator; one tile: accumulators next to each other, whose sum is the result
   uint32_t sums_at;           // split: where the cluster's sums go; 0: where the token stages were
   int* status;
 };
@@ -143,7 +144,8 @@ struct Slot {
   }
 };
 
-template <typename T>
+// kChains: an f32 result of more units than a chain has; the others' loops are the shorter for it (M=32 N=4096 K=14336 bf16 14.8 us, 15.7 with the chains' counting)
+template <typename T, bool kChains>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const GemmParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* const smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -152,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   const uint32_t full = bars, empty = full + 8 * kMost, w_full = empty + 8 * kMost, w_empty = w_full + 8 * kWMost;
   const uint32_t acc_full = w_empty + 8 * kWMost, acc_empty = acc_full + 16, tmem_ptr = acc_empty + 16;
   const int tokens = p.tokens, split = p.split;
-  const uint32_t stages = p.stages, w_stages = p.w_stages, acc_cols = p.acc_cols, a_col = acc_cols * p.accs;
+  const uint32_t stages = p.stages, w_stages = p.w_stages, acc_cols = p.acc_cols, a_col = acc_cols * (kChains ? max(p.accs, p.chains) : p.accs);
   const uint32_t b_half = (uint32_t)tokens * 128, b_bytes = 2 * b_half, w_ring = base + stages * b_bytes;
   const int rank = split > 1 ? (int)blockIdx.x & (split - 1) : 0;
   const int first_tile = (int)blockIdx.x / split, step = (int)gridDim.x / split;
@@ -243,12 +245,16 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     Slot op, acc;
     bool ok = true;
     acc.phase = 1;
+    uint32_t d = tmem;
     for (int tile = first_tile; tile < p.tiles && ok; tile += step) {
-      ok = mbar_wait_warp(acc_empty + 8 * acc.at, acc.phase, status, 73);
-      if (!ok) break;
-      tcgen05_fence_after();
-      const uint32_t d = tmem + acc.at * acc_cols;
+      int chained = 0;                             // units of this chain
       for (int u = 0; u < n_units; ++u) {
+        if (u == 0 || (kChains && chained == 0 && p.accs > 1)) {
+          ok = mbar_wait_warp(acc_empty + 8 * acc.at, acc.phase, status, 73);
+          if (!ok) break;
+          tcgen05_fence_after();
+          d = tmem + acc.at * acc_cols;
+        }
         // One wait and one commit for 128 of k: with barriers of their own for the two operands the loop took 650 cycles for few tokens.  The next stage is looked at
         // while this one's MMAs are issued.
         if (!ready) ok = mbar_wait_warp(full + 8 * op.at, op.phase, status, 74);
@@ -259,9 +265,18 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
         const bool next = mbar_test_wait(full + 8 * op.at, op.phase);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          tcgen05_mma_ts(leader, d, from + i * 8, desc + (i & 3) * 2 + (i >> 2) * (b_half >> 4), b0_hi, idesc, (u > 0 || i > 0) ? 1u : 0u);
+          tcgen05_mma_ts(leader, d, from + i * 8, desc + (i & 3) * 2 + (i >> 2) * (b_half >> 4), b0_hi, idesc, ((kChains ? chained : u) > 0 || i > 0) ? 1u : 0u);
         tcgen05_commit_if(leader, done);
         if (u == n_units - 1) tcgen05_commit_if(leader, acc_full + 8 * acc.at);
+        if (kChains && ++chained == p.chain) {
+          chained = 0;
+          if (p.accs == 1) {
+            d += acc_cols;
+          } else if (u < n_units - 1) {
+            tcgen05_commit_if(leader, acc_full + 8 * acc.at);
+            acc.next(p.accs);
+          }
+        }
         ready = __all_sync(0xffffffffu, next);
       }
       acc.next(p.accs);
@@ -328,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   const int quarter = warp & 3;
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
   // columns from, from + by, ... of a tile of n tokens, 32 at a time
-  auto write_columns = [&](uint32_t acc, int row, int token0, int n, int from, int by, float g) {
+  auto write_columns = [&](uint32_t acc, int row, int token0, int n, int from, int by, float g, bool more) {
     const float bias = p.bias != nullptr && row < p.N ? load_value(p.bias, p.bias_dtype, row) : 0.f;
     for (int c = from; c < n; c += by) {
       uint32_t r[32];
@@ -349,9 +364,16 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
           if (i < most) to[(size_t)i * p.N] = __float2half_rn(__uint_as_float(r[i]) * g + bias);
       } else {
         float* const to = static_cast<float*>(p.out) + at;
+        if (kChains && more) {
+          // to the sum of the chains before this one: the same lane's, so that the order is the program's
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < most) to[(size_t)i * p.N] = __uint_as_float(r[i]) * g + bias;
+          for (int i = 0; i < 32; ++i)
+            if (i < most) asm volatile("red.relaxed.gpu.global.add.f32 [%0], %1;" ::"l"(to + (size_t)i * p.N), "f"(__uint_as_float(r[i]) * g) : "memory");
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (i < most) to[(size_t)i * p.N] = __uint_as_float(r[i]) * g + bias;
+        }
       }
     }
   };
@@ -362,13 +384,18 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       Slot acc;
       for (int tile = first_tile; tile < p.tiles; tile += step) {
         const int token0 = tile / p.row_tiles * tokens;
-        if (!mbar_wait_warp(acc_full + 8 * acc.at, acc.phase, status, 78)) break;
-        tcgen05_fence_after();
-        write_columns(acc.at * acc_cols, tile % p.row_tiles * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), 0, 32, g);
-        tcgen05_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty + 8 * acc.at);
-        acc.next(2);
+        bool ok = true;
+        for (int u = 0; u < n_units; u += kChains ? p.chain : n_units) {
+          ok = mbar_wait_warp(acc_full + 8 * acc.at, acc.phase, status, 78);
+          if (!ok) break;
+          tcgen05_fence_after();
+          write_columns(acc.at * acc_cols, tile % p.row_tiles * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), 0, 32, g, u > 0);
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(acc_empty + 8 * acc.at);
+          acc.next(2);
+        }
+        if (!ok) break;
       }
     }
   } else {
@@ -380,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     tcgen05_fence_after();
     const float g = *p.g;
     if (split == 1) {
-      if (work && ok) write_columns(0, row_tile * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), nth * 32, 5 * 32, g);
+      if (work && ok) write_columns(0, row_tile * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), nth * 32, 5 * 32, g, false);
     } else {
       // Token t of the tile is finished by block t / (tokens / split): [source][its tokens][128 rows] of f32
       cluster_wait();
@@ -392,6 +419,13 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
           uint32_t r[16];
           tcgen05_ld_32x16(tmem + lanes + c, r);
           tcgen05_wait_ld();
+          for (int u = p.chain, at = acc_cols; kChains && u < n_units; u += p.chain, at += acc_cols) {
+            uint32_t other[16];
+            tcgen05_ld_32x16(tmem + lanes + at + c, other);
+            tcgen05_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) + __uint_as_float(other[i]));
+          }
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int t = c + i, owner = t / own;
@@ -421,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   }
 }
 
-template <typename T>
+template <typename T, bool kChains>
 int launch_gemm(const LinearCall& c, cudaStream_t st) {
   static std::once_flag once[64];
   static bool ready[64];
@@ -429,7 +463,7 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return B200FP4_STATUS_NOT_SUPPORTED;
   std::call_once(once[dev], [&] {
-    ready[dev] = cudaFuncSetAttribute(w4a16_gemm_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) == cudaSuccess;
+    ready[dev] = cudaFuncSetAttribute(w4a16_gemm_kernel<T, kChains>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemBytes) == cudaSuccess;
     cudaGetLastError();
   });
   if (!ready[dev]) return B200FP4_STATUS_EXECUTION_FAILED;
@@ -459,9 +493,13 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
     const int64_t token_tiles = (c.M + tokens - 1) / tokens, tiles = token_tiles * p.row_tiles;
     if (tiles > 0x3FFFFFFF) continue;
     for (int split = 1; split <= kMaxSplit && split <= p.units; split *= 2) {
-      const int clusters = split == 1 ? sms : resident_clusters_of(counts[split], w4a16_gemm_kernel<T>, split, kThreads, kSmemBytes);
+      const int clusters = split == 1 ? sms : resident_clusters_of(counts[split], w4a16_gemm_kernel<T, kChains>, split, kThreads, kSmemBytes);
       if (clusters < 1) break;
       if (split > 1 && tiles > clusters) break;    // a cluster does one tile
+      // An f32 result: chains of all of a block's units (kChain), unless blocks of a cluster, whose chains are all in tensor memory, would need longer ones
+      const int own_units = (p.units + split - 1) / split, wanted = kChains ? (own_units + kChain - 1) / kChain : 1;
+      const int acc_cols = (tokens + 31) / 32 * 32, chains = split == 1 ? 1 : std::min(wanted, (512 - 2 * 64) / acc_cols);
+      if (wanted > 1 && split > 1 && (own_units + chains - 1) / chains > kChain + 1) continue;
       const double unit = std::max(std::max(4.0 * tokens, 450.0), (2.0 * tokens * 128 + 4.0 * kUnitBytes) / 57.0);
       const double waves = (double)((tiles + clusters - 1) / clusters);
       const double cost = waves * ((p.units + split - 1) / split * unit) + 2000.0 + tokens * 20.0 + (split > 1 ? 2000.0 + tokens * 20.0 : 0.0);
@@ -472,9 +510,11 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
         p.split = split;
         // Tensor memory: accumulators (two where a block has several tiles), the rest for the weight.  Shared memory: 144 KB of tokens at most, the rest for packed units, whose
         // copies take longest.
-        p.accs = tiles > clusters ? 2 : 1;
-        p.acc_cols = (uint32_t)(tokens + 31) / 32 * 32;
-        p.stages = (int)std::min<uint32_t>(kMost, std::min<uint32_t>((512 - p.accs * p.acc_cols) / 64, 144 * 1024 / ((uint32_t)tokens * 256)));
+        p.acc_cols = (uint32_t)acc_cols;
+        p.accs = tiles > clusters || (split == 1 && wanted > 1) ? 2 : 1;
+        p.chains = chains;
+        p.chain = split == 1 && wanted > 1 ? kChain : (own_units + chains - 1) / chains;
+        p.stages = (int)std::min<uint32_t>(kMost, std::min<uint32_t>((512 - std::max(p.accs, p.chains) * p.acc_cols) / 64, 144 * 1024 / ((uint32_t)tokens * 256)));
         // A cluster's sums have room of their own where they are small: nobody waits for the others' MMAs then (M=32 N=4096 K=14336 15.1 us / 15.7, M=64 N=K=4096 9.2 / 9.7).
         const uint32_t sums = split > 1 && tokens <= 64 ? (uint32_t)tokens * kMmaRows * 4 : 0;
         p.sums_at = sums > 0 ? kRingBytes - sums : 0;
@@ -487,7 +527,7 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
   if (grid == 0) return B200FP4_STATUS_NOT_SUPPORTED;
   CUtensorMap map;
   if (!make_rows_map(&map, c.x, (uint64_t)c.M, (uint64_t)c.K * 2, (uint64_t)(c.M > 1 ? c.ldx : c.K) * 2, (uint32_t)p.tokens, 128)) return B200FP4_STATUS_INTERNAL_ERROR;
-  if (launch_pdl_cluster(p.split, w4a16_gemm_kernel<T>, dim3(grid), dim3(kThreads), kSmemBytes, st, map, p) != cudaSuccess) {
+  if (launch_pdl_cluster(p.split, w4a16_gemm_kernel<T, kChains>, dim3(grid), dim3(kThreads), kSmemBytes, st, map, p) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
@@ -497,7 +537,9 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
 }  // namespace
 
 int launch_w4a16_gemm(const LinearCall& c, cudaStream_t st) {
-  return c.x_dtype == B200FP4_DTYPE_BF16 ? launch_gemm<__nv_bfloat16>(c, st) : launch_gemm<__half>(c, st);
+  const bool chains = c.out_dtype == B200FP4_DTYPE_F32 && units_of(c.K) > kChain;
+  if (c.x_dtype == B200FP4_DTYPE_BF16) return chains ? launch_gemm<__nv_bfloat16, true>(c, st) : launch_gemm<__nv_bfloat16, false>(c, st);
+  return chains ? launch_gemm<__half, true>(c, st) : launch_gemm<__half, false>(c, st);
 }
 
 }  // namespace b200fp4

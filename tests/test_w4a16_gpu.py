@@ -53,6 +53,12 @@ def _linear(M, N, K, dtype, out_dtype=None, bias_dtype=None, pad=0, exact=True, 
     (2000, 1300, 144, F16, None, F32, 0),
     (18, 20000, 64, BF16, None, None, 8),         # more narrow ones
     (48, 96, 8208, F16, F32, None, 0),            # one tile for a cluster
+    (700, 2300, 4096, F16, F32, BF16, 8),         # f32 results: several chains a tile, more tiles than blocks
+    (190, 1000, 3344, BF16, F32, F32, 0),         # ... one tile a block, the last chain short
+    (130, 260, 4096, BF16, F32, None, 0),         # ... chains of a cluster's blocks
+    (190, 40, 4096, F16, F32, BF16, 0),
+    (5, 5000, 4096, BF16, F32, None, 0),          # ... warps
+    (12, 600, 4096, F16, F32, BF16, 0),
 ])
 def test_linear_exact(M, N, K, dtype, out_dtype, bias_dtype, pad):
     y, ref, _ = _linear(M, N, K, dtype, out_dtype, bias_dtype, pad)
@@ -69,6 +75,16 @@ def test_linear_rounding(M, N, K, dtype, out_dtype):
     y, ref, size = _linear(M, N, K, dtype, out_dtype, exact=False, g=3e-4)
     bound = (K + 2) * 2.0 ** -23 * size + half_eps(out_dtype) * ref.abs() * (1 + 2.0 ** -10) + torch.finfo(out_dtype).tiny
     assert bool(((y.double() - ref).abs() <= bound).all())
+
+
+# An f32 result keeps to f32's precision however long k is: a matrix instruction (16 of k) truncates its sum, by 2^-23 of it at most, and a chain has at most 96 of
+# them; errors of chains add up like the chains themselves.  So the norm of the differences is within
+# 96 * 2^-23 of the result's.
+@pytest.mark.parametrize("M,N,K,dtype", [(1, 900, 14336, BF16), (4, 8192, 14336, BF16), (12, 700, 14336, F16), (32, 4096, 14336, BF16), (150, 1024, 14336, BF16),
+                                         (400, 8192, 14336, F16)])
+def test_linear_f32_results_of_long_sums(M, N, K, dtype):
+    y, ref, _ = _linear(M, N, K, dtype, F32, exact=False, g=3e-4)
+    assert float((y.double() - ref).norm()) <= 96 * 2.0 ** -23 * float(ref.norm())
 
 
 def test_linear_scale_bytes_and_signs():
