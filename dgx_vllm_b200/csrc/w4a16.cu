@@ -240,7 +240,7 @@ inline int least_share(int out_dtype, int units) {
 }
 
 // A run of items is done in phases: rounds of an item a warp (or a group of the least size), then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
-// size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 14.3 / 14.0.
+// size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 14.3 / 14.0 (both 0.3 less by now).
 // share: log2 of the warps of a group.  The plan has that of each number of items under a round, four bits each.
 struct Phase {
   int count, share;
@@ -655,7 +655,7 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
       const uint64_t bytes = (uint64_t)linear_layout(kCols, cap, row_bytes, 1, 0).bytes + (split > 1 ? (uint64_t)most * cap * 128 : 0);
       if ((uint64_t)own * 256 > kSmemMost || bytes > kSmemMost) continue;
       if (kTokens == 0 && p.out_dtype == B200FP4_DTYPE_F32 && own > kWarpChain * kWarps) continue;       // too long a chain for an f32 result
-      // The busiest block's units; a cluster's exchange costs some 1500 cycles.  Shared / not shared, us: M=1 N=512 K=16384 6.8 / 8.9, M=8 N=512 K=4096 5.2 / 6.1;
+      // The busiest block's units; a cluster's exchange costs some 1500 cycles.  Shared / not shared, us: M=1 N=512 K=16384 6.2 / 8.9, M=8 N=512 K=4096 4.7 / 6.1;
       // by this rule not shared: M=1 N=K=4096 5.2, N=14336 K=4096 9.2.
       const int log_share = share_of(most, p.units / split, kTokens > 0 ? 0 : least_share(p.out_dtype, own));
       const float cost = share_cost(most, own, log_share) + (split > 1 ? 1500.f : 0.f);

@@ -11,7 +11,7 @@
 // tiles for them, a cluster shares the k of one and adds up its parts through distributed shared memory, each block some of the tokens.
 // Every wait is bounded (status word), tensor memory is always freed.
 // Bound: with many tokens by the tensor cores, M=4096 N=14336 K=4096 400 us, 1.20 PFLOP/s under the power cap (73 % of the measured burst rate, 88 % of the sustained one), the
-// tensor pipe busy 73 % of active cycles; with few by decoding and the MMA warp's turn, some 450 cycles for 128 of k where HBM brings them in 390: M=32 N=4096 K=14336 15.1 us
+// tensor pipe busy 73 % of active cycles; with few by decoding and the MMA warp's turn, some 450 cycles for 128 of k where HBM brings them in 390: M=32 N=4096 K=14336 14.8 us
 // (33 MB, floor 5.3), M=333 N=K=4096 15.6 (0.72 PFLOP/s).
 #include <algorithm>
 #include <type_traits>
@@ -483,7 +483,7 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
   p.status = c.status;
   const int sms = sm_count();
   // Tokens of a tile and blocks that share one: the least time of the busiest block, in cycles.  128 of k take the MMAs four cycles a token, the copies one for each
-  // 57 bytes, and decoding and issue 450.  Shared by this rule / one block a tile, us: M=32 N=4096 K=14336 15.1 / 40.3, M=64 N=K=4096 9.2 / 14.1, M=128 12.4 / 14.4; by it
+  // 57 bytes, and decoding and issue 450.  Shared by this rule / one block a tile, us: M=32 N=4096 K=14336 14.8 / 40.3, M=64 N=K=4096 8.8 / 14.1, M=128 12.1 / 14.4; by it
   // not shared: M=333 N=K=4096 15.7.
   double best = 1e30;
   unsigned grid = 0;

@@ -494,7 +494,8 @@ B200FP4_API int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, 
 /* out[M,N] = x . W^T * g_scale (+ bias): x [M,K] bf16 or f16, rows ldx elements apart (a multiple of 8, 16-byte aligned), one packed
  * matrix (not gated), g_scale one f32 on the device (weight_scale_2 of a checkpoint), bias [N] of any dtype or NULL, out contiguous
  * in bf16, f16 or f32, not in x's memory.  Products of exact 16-bit values, sums in f32: bf16 rows are brought into f16's range by a power of two each, with
- * which only what is below 2^-39 of a row's largest magnitude can be rounded.  status (on the device) is 0 after the call, or the code of a
+ * which only what is below 2^-39 of a row's largest magnitude can be rounded.  A 16-bit result's sums are the matrix instructions' own; an f32
+ * result is added up, rounded, from sums of at most K = 1024 or so (in memory, where a tile has several: nothing else may write to out).  status (on the device) is 0 after the call, or the code of a
  * bounded wait that ran out: the result is then not valid. */
 B200FP4_API int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, const uint8_t* packed, const float* g_scale,
                                      const void* bias, int bias_dtype, void* out, int out_dtype, int64_t M, int64_t N, int64_t K,
