@@ -240,7 +240,8 @@ inline int least_share(int out_dtype, int units) {
 }
 
 // A run of items is done in phases: rounds of an item a warp (or a group of the least size), then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
-// size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 14.3 / 14.0 (both 0.3 less by now).
+// size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 0.3 us more of
+// its 14, for the longer way to a warp's first weights.
 // share: log2 of the warps of a group.  The plan has that of each number of items under a round, four bits each.
 struct Phase {
   int count, share;
