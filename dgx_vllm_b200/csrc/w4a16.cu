@@ -5,13 +5,13 @@
 //   linear   columns are tokens
 //   gate/up  columns are the (token, expert) pairs of one expert; a tile's rows are eight gate rows and the same eight up rows, so that a
 //            lane holds both halves of its values and applies SiLU(gate) * up to them
-//   down     the value between the projections in f16, brought into its range by a power of two for each pair: eleven bits, where a bf16 result keeps eight.  For an
-//            f16 or f32 result it is two f16, upper and lower part, in two columns: their sum has 22 bits
+//   down     the value between the projections as two f16, upper and lower part, in two columns: their sum has f32's precision ("the value between the projections")
 // Work items are (strip of 32 rows, slot); a slot is a run of one expert's pairs that fits the columns.  A block has a contiguous range of them, groups of
 // warps take items in turn and split k among themselves.
 // The layer is two launches without anything that has to outlast them: both find the slots from the routing by themselves, the first sets the
 // counters of the second, in which the block that finishes a strip's last item adds up its pairs in their order.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <type_traits>
 
@@ -272,18 +272,24 @@ inline uint64_t phase_plan(int units, int least) {
 // Sums of the warps that share an item, [warp][tile][column of eight][j][lane]: each warp adds up some of them, in the order of k, and finishes them.
 // A lane's sums j are row l / 4 (0, 1) or l / 4 + 8 (2, 3) of a tile and columns 2 (l % 4) and the next one; finish gets those of j = kFirst[i] and
 // kSecond[i].  Both barriers are the group's, whichever others there are at the time.
+// finish(t, c, i, a, b, std::false_type) may say, with the whole warp, that it wants these sums a second time, with std::true_type: what is rarely needed stays out of what always is.
 template <int kCols, bool kAcross, typename F>
 __device__ __forceinline__ void finish_item(float* red, int log_share, int in_group, int group, int lane, const float (&acc)[2][kCols][4], F&& finish) {
   const int share = 1 << log_share;
   // kAcross: the pair is the two columns of one row (j, j + 1), otherwise the two rows of one column (j, j + 2)
   constexpr int kSums = 2 * kCols * 4 * 32;
   if (share == 1) {
+    auto all = [&](auto again) {
+      bool done = true;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int c = 0; c < kCols; ++c)
+        for (int c = 0; c < kCols; ++c)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) finish(t, c, i, acc[t][c][kAcross ? 2 * i : i], acc[t][c][kAcross ? 2 * i + 1 : i + 2]);
+          for (int i = 0; i < 2; ++i) done &= finish(t, c, i, acc[t][c][kAcross ? 2 * i : i], acc[t][c][kAcross ? 2 * i + 1 : i + 2], again);
+      return done;
+    };
+    if (!all(std::false_type{})) all(std::true_type{});
     return;
   }
   float* const own = red + group * share * kSums + lane;
@@ -303,7 +309,8 @@ __device__ __forceinline__ void finish_item(float* red, int log_share, int in_gr
       va += a[w * kSums];
       vb += b[w * kSums];
     }
-    finish(kCols == 1 ? tc : tc / kCols, kCols == 1 ? 0 : tc % kCols, i, va, vb);
+    const int t = kCols == 1 ? tc : tc / kCols, c = kCols == 1 ? 0 : tc % kCols;
+    if (!finish(t, c, i, va, vb, std::false_type{})) finish(t, c, i, va, vb, std::true_type{});
   }
   asm volatile("bar.sync %0, %1;" ::"r"((kWarps >> log_share) + group), "r"(share * 32) : "memory");
 }
@@ -311,6 +318,7 @@ __device__ __forceinline__ void finish_item(float* red, int log_share, int in_gr
 // ---- powers of two that bring values into f16's range
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }      // -126 <= e <= 127
+__device__ __forceinline__ int exponent_of(float v) { return (int)(__float_as_uint(v) >> 23) - 127; }     // v not negative
 
 // The exponent that brings a row whose largest magnitude has these bf16 bits below 2^15.  Rows with infinities or NaN, which only give such
 // again, take the least that no finite value overflows with.
@@ -575,9 +583,9 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
         arrived = true;
       }
       const int strip = item - slot * p.strips;
-      finish_item<kCols, false>(reinterpret_cast<float*>(smem + l.red), p.log_share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb) {
+      finish_item<kCols, false>(reinterpret_cast<float*>(smem + l.red), p.log_share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb, auto) {
         const int column = c * 8 + quad * 2 + i, row = t * 16 + row8;
-        if (column >= n) return;
+        if (column >= n) return true;
         const float f = kConvert ? inv[column] : 1.f;
         if (split > 1) {
           // value [row of the strip] is finished by block row / (32 / split): [source][item][column][its rows]
@@ -599,6 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
             }
           }
         }
+        return true;
       });
     }
     done = end;
@@ -714,7 +723,7 @@ constexpr int kMaxPairs = 2048;                // pairs whose slots a block find
 constexpr int kMaxExperts = 4096;
 
 struct MoeParams {
-  const void* x;              // gate/up [M, K], rows ldx apart; down: [pair][part][K] f16
+  const void* x;              // gate/up [M, K], rows ldx apart; down: the rows of act
   int64_t ldx;
   const uint8_t* packed;
   const float* g;             // [E]; gate/up [E][gate, up]
@@ -731,9 +740,11 @@ struct MoeParams {
   const int32_t* map;         // [global_E] or null
   int64_t global_E;
   int topk, E, weight_on_input;
-  __half* act;                // gate/up out
+  __half* act;                // gate/up out: for each pair, rows act_row(I) apart, [part][I] and the levels of its runs (run_at)
   float* act_inv;             // [pair]: the reciprocal of the factor that brought its row of act into f16's range
   float* y;                   // down: [pair][N]
+  uint32_t* leveled;          // `call` of the last call with a run above level 0
+  uint32_t call;
   int* counters;              // [strips of down]
   int n_counters;
   void* out;                  // down [M, N]
@@ -741,6 +752,36 @@ struct MoeParams {
   int* status;
   int clear_status;
 };
+
+// ---- the value between the projections
+//
+// SiLU(gate) * up of a pair is brought below 2^15 by a power of two that goes by a bound, known before any of its values is.  Then it is two f16, v = upper + lower * 2^-12: the
+// rest of the upper part is at most 2^-12 of it, so that the lower part uses f16's range too, and a value is off by the larger of 2^-37 and 2^-23 of itself.
+// A bound may be far from the values (gates of -30: SiLU is 2^-38 of them).  So each run of eight has a level: 2^(28 k) more, with the least k that brings its largest value to 2^-13 or
+// above, where it is off by 2^-24 of that at most.  A level is kept as a bit, 1 << k, none for a run of zeros.  Ordinary layers have no run above level 0; a word says
+// whether a call has one, and only then the second projection looks at the levels: runs of the level above a pair's lowest are brought down to that and split anew, higher
+// ones are less than 2^-28 of the pair's largest value and left out.
+// One f16 of eleven bits instead (bf16 results are then off by 8e-4 of their norm more): 32 tokens, ten of 512 experts, H=2048 I=512, 86.7 us against 90.2; 128 tokens 166.6 / 177; one 14.3 / 14.9.
+// Powers of two of their own for all runs, applied to every operand: 93.8, 185, 14.8.  The looking out of the loops that do without: 94.3 -> 90.2.
+constexpr int kLevel = 28, kLevels = 8;
+constexpr float kLeast = 0x1p-13f, kLower = 4096.f;
+__host__ __device__ __forceinline__ int64_t act_row(int64_t I) { return 2 * I + units_of(I) * 8; }      // halves of a pair: two parts, and 16 bytes for each 128 values
+// Where the level of run n (values 8 n to 8 n + 7) is: lane l of the second projection has its four of a unit in a word, [block l % 4][half of the unit][eight of the block]
+__device__ __forceinline__ int run_at(int n) { return (n >> 4) * 16 + ((n >> 1) & 3) * 4 + ((n >> 3) & 1) * 2 + (n & 1); }
+
+// A lane's eight values of a run, the upper parts or (odd) the lower ones, from one level to the one below it: times 2^-28.  Lanes apart by four have the two parts.
+__device__ __forceinline__ void level_down(uint32_t* b, bool odd, int levels) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, b[j], 4);
+    const float2 hi = __half22float2(as_half2(odd ? other : b[j])), lo = __half22float2(as_half2(odd ? b[j] : other));
+    const float2 v = make_float2((hi.x + lo.x * (1.f / kLower)) * 0x1p-28f, (hi.y + lo.y * (1.f / kLower)) * 0x1p-28f);
+    const __half2 upper = __floats2half2_rn(v.x, v.y);
+    const float2 f = __half22float2(upper);
+    const uint32_t next = odd ? as_u32(__floats2half2_rn((v.x - f.x) * kLower, (v.y - f.y) * kLower)) : as_u32(upper);
+    if (levels > 0) b[j] = levels == 1 ? next : 0u;
+  }
+}
 
 struct RowStat {
   float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
@@ -917,8 +958,8 @@ enum Projection { kGateUp, kDownItems, kDownStrips };       // kDownStrips: whol
 // Bound by the copies of the experts that the routing reaches: 32 tokens, ten of 512 experts, H=2048 I=512, take 91-94 us, gate/up 46 of them at 6.1 TB/s and down 26 at
 // 5.3; the rest is finding the slots (2 us), rows and first units (3), the down projection's start (3) and the strips' last sums (4).  128 tokens 180-187.  Two
 // launches: every value of the first projection is needed by the second, which finds its slots and asks for its first weights while the first one ends.
-// XT: type of the activations (gate/up); kCols: columns of eight; kParts: f16 parts of a value between the projections
-template <typename XT, int kMode, int kCols, int kParts>
+// XT: type of the activations (gate/up); kCols: columns of eight
+template <typename XT, int kMode, int kCols>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr bool kDown = kMode != kGateUp, kWhole = kMode == kDownStrips;
@@ -1081,18 +1122,47 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
             ring.advance();
             if (ring.ok) fetch();
           }
-          finish_item<kCols, false>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float gate, float up) {
-            const int column = c * 8 + quad * 2 + i, I = p.N / 2, i_at = strip * 16 + t * 8 + row8;
-            if (column >= n || i_at >= I) return;
-            const int pair = list[s.y + column];
-            const RowStat st = stats[s.y - row0 + column];
-            const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
-            const float v = silu_f32(gate * f * p.g[2 * e]) * (up * f * p.g[2 * e + 1]) * st.act;
-            const __half hi = __float2half_rn(v);
-            const float rest = v - __half2float(hi);
-            __half* const to = p.act + (size_t)pair * kParts * I + i_at;
-            to[0] = hi;
-            if (kParts == 2) to[I] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
+          const float g_gate = p.g[2 * e], g_up = p.g[2 * e + 1];
+          finish_item<kCols, false>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float gate, float up, auto again) {
+            // a run: eight rows of a tile, a column; I is a multiple of 16, so that it is whole
+            const int column = c * 8 + quad * 2 + i, I = p.N / 2, run = strip * 2 + t;
+            const bool here = column < n && run * 8 < I;
+            float v = 0.f, scale = 1.f;
+            int pair = 0;
+            if (here) {
+              pair = list[s.y + column];
+              const RowStat st = stats[s.y - row0 + column];
+              const float f = p.weight_on_input ? p.weights[pair] * st.inv : st.inv;
+              v = silu_f32(gate * f * g_gate) * (up * f * g_up);
+              scale = st.act;
+            }
+            uint32_t level = 1, large = 15;
+            if constexpr (again.value) {
+              uint32_t top = __float_as_uint(v) & 0x7FFFFFFFu;
+#pragma unroll
+              for (int d = 4; d < 32; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+              const int power = exponent_of(scale), under = exponent_of(kLeast) - (exponent_of(__uint_as_float(top)) + power);
+              const int k = min(max(under + kLevel - 1, 0) / kLevel, min(kLevels - 1, (126 - power) / kLevel));
+              scale = pow2(power + k * kLevel);
+              level = top != 0 ? 1u << k : 0u;
+              if (level > 1 && here) *p.leveled = p.call;
+            } else {
+              // four runs a warp: level 0 where one of a run's values is large enough
+              large = __ballot_sync(0xffffffffu, !here || !(fabsf(v) * scale < kLeast));
+              large |= large >> 16;
+              large |= large >> 8;
+              large |= large >> 4;
+            }
+            if (here) {
+              v *= scale;
+              const __half hi = __float2half_rn(v);
+              const float rest = (v - __half2float(hi)) * kLower;
+              __half* const to = p.act + pair * act_row(I);
+              to[run * 8 + row8] = hi;
+              to[I + run * 8 + row8] = __float2half_rn(isfinite(rest) ? rest : 0.f);        // an infinite or NaN value is the upper part's alone
+              if (row8 == 0) reinterpret_cast<uint8_t*>(to + 2 * I)[run_at(strip * 2) + t] = (uint8_t)level;
+            }
+            return (large & 15) == 15;
           });
         }
         done += phase.count;
@@ -1105,6 +1175,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     pdl_wait();
     pdl_launch_dependents();
     if (kWhole && p.split > 1) cluster_wait();
+    const bool leveled = *p.leveled == p.call;       // otherwise every run of every pair is at level 0, and nobody looks
     if (n_slots == 0) {
       for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < (size_t)p.M * p.N; i += (size_t)gridDim.x * kThreads)
         store_value(p.out, p.out_dtype, i, 0.f);
@@ -1120,8 +1191,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
         const __half* act[kCols];
 #pragma unroll
         for (int c = 0; c < kCols; ++c) {
-          const int i = (c * 8 + row8) / kParts;     // a pair's columns are its parts
-          act[c] = static_cast<const __half*>(p.x) + ((int64_t)list[s.y + (i < n ? i : 0)] * kParts + (kParts == 2 ? row8 & 1 : 0)) * p.ldx + quad * 16;
+          const int i = (c * 8 + row8) / 2;          // a pair's columns are its parts
+          act[c] = static_cast<const __half*>(p.x) + list[s.y + (i < n ? i : 0)] * p.ldx + (row8 & 1) * p.K + quad * 16;
         }
         float acc[2][kCols][4] = {};
         uint32_t b[2][kCols][8];
@@ -1140,50 +1211,90 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
               to[half][c][4] = hi.x, to[half][c][5] = hi.y, to[half][c][6] = hi.z, to[half][c][7] = hi.w;
             }
         };
-        if constexpr (kCols == 1) {                  // a unit ahead, as far as there are registers
-          load_columns(part.k_first, b);
-#pragma unroll 1
-          for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
-            uint32_t after[2][kCols][8];
-            load_columns(k + 1, after);
-            multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
-            ring.advance();
-            if (ring.ok) fetch();
+        auto multiply = [&]() {
+          multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
+          ring.advance();
+          if (ring.ok) fetch();
+        };
+        // Back to the values' own size: this lane's sums are those of pair c * 4 + quad, lowest_of(c) the level that it was brought to.
+        auto scale_sums = [&](auto&& lowest_of) {
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+          for (int c = 0; c < kCols; ++c) {
+            const int column = c * 4 + quad;
+            const float inv = p.act_inv[list[s.y + (column < n ? column : 0)]], f = pow2(exponent_of(inv) - lowest_of(c) * kLevel);
 #pragma unroll
-              for (int j = 0; j < 8; ++j) b[half][0][j] = after[half][0][j];
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[t][c][j] *= j & 1 ? f * (1.f / kLower) : f;
           }
-        } else {
+        };
+        if (__builtin_expect(leveled, 0)) {
+          // four lanes have a pair, each its own words of the levels
+          const bool odd = row8 & 1;
+          auto levels_at = [&](int k, int c) { return reinterpret_cast<const uint32_t*>(act[c] + (odd ? 1 : 2) * p.K - quad * 16 + k * 8)[quad]; };
+          uint32_t levels[kCols];
+#pragma unroll
+          for (int c = 0; c < kCols; ++c) {
+            uint32_t set = 0;
+            for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
+              const int x = k * kUnitK + quad * 16;
+              const uint32_t w = x < p.K ? levels_at(k, c) : 0u;
+              set |= x + 64 < p.K ? w : w & 0xFFFFu;
+            }
+            set |= set >> 16;
+            set = (set | set >> 8) & 0xFFu;
+            set |= __shfl_xor_sync(0xffffffffu, set, 1);
+            levels[c] = set | __shfl_xor_sync(0xffffffffu, set, 2);
+          }
 #pragma unroll 1
           for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
             load_columns(k, b);
-            multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
-            ring.advance();
-            if (ring.ok) fetch();
+#pragma unroll
+            for (int c = 0; c < kCols; ++c) {
+              const uint32_t w = levels_at(k, c);
+#pragma unroll
+              for (int run = 0; run < 4; ++run)      // levels above the pair's lowest; values that are zeros stay so
+                level_down(&b[run >> 1][c][(run & 1) * 4], odd, __ffs((int)((w >> (8 * run)) & 0xFFu)) - __ffs((int)levels[c]));
+            }
+            multiply();
           }
+          scale_sums([&](int c) { return max(__ffs((int)__shfl_sync(0xffffffffu, levels[c], quad * 8)) - 1, 0); });
+        } else {
+          if constexpr (kCols == 1) {                // a unit ahead, as far as there are registers
+            load_columns(part.k_first, b);
+#pragma unroll 1
+            for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
+              uint32_t after[2][kCols][8];
+              load_columns(k + 1, after);
+              multiply();
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) b[half][0][j] = after[half][0][j];
+            }
+          } else {
+#pragma unroll 1
+            for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
+              load_columns(k, b);
+              multiply();
+            }
+          }
+          scale_sums([](int) { return 0; });
         }
-        finish_item<kCols, kParts == 2>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float va, float vb) {
-          // two parts: the columns of one pair in one row; one: two rows of one pair
-          const int column = kParts == 2 ? c * 4 + quad : c * 8 + quad * 2 + i, in_strip = t * 16 + row8 + (kParts == 2 ? i * 8 : 0), row = strip * 32 + in_strip;
-          if (column >= n) return;
+        finish_item<kCols, true>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float va, float vb, auto) {
+          // the two columns of a pair in one row
+          const int column = c * 4 + quad, in_strip = t * 16 + row8 + i * 8;
+          if (column >= n) return true;
           const int pair = list[s.y + column];
-          const float f = p.act_inv[pair] * p.g[e];
+          const float v = (va + vb) * p.g[e];
           if constexpr (kWhole) {
             // [strip of the cluster][pair][32 rows], in its first block
             const uint32_t to = base + l.y + (uint32_t)((strip_nth * p.M * p.topk + pair) * 32 + in_strip) * 4;
-            const uint32_t cluster_to = p.split > 1 ? map_to_cta(to, 0) : to;
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to), "f"(kParts == 2 ? (va + vb) * f : va * f) : "memory");
-            if (kParts == 1) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(cluster_to + 32), "f"(vb * f) : "memory");
-          } else {
-            float* const to = p.y + (size_t)pair * p.N + row;
-            if (kParts == 2) {
-              if (row < p.N) to[0] = (va + vb) * f;
-            } else {
-              if (row < p.N) to[0] = va * f;
-              if (row + 8 < p.N) to[8] = vb * f;
-            }
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(p.split > 1 ? map_to_cta(to, 0) : to), "f"(v) : "memory");
+          } else if (strip * 32 + in_strip < p.N) {
+            p.y[(size_t)pair * p.N + strip * 32 + in_strip] = v;
           }
+          return true;
         });
       }
       done += phase.count;
@@ -1311,17 +1422,17 @@ double slots_of(const MoeParams& p, int cap) {
 }
 
 // What a launch would be, without launching; a status other than success where there is no room for it
-template <typename XT, int kMode, int kCols, int kParts>
+template <typename XT, int kMode, int kCols>
 int plan_moe(const MoeParams& given, MoePlan& plan) {
   static std::once_flag once[64];
   static bool ready[64];
   static ResidentClusters counts[kMaxSplit + 1][64];
-  constexpr auto kernel = w4a16_moe_kernel<XT, kMode, kCols, kParts>;
+  constexpr auto kernel = w4a16_moe_kernel<XT, kMode, kCols>;
   if (!allow_smem(kernel, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
   MoeParams p = given;
   const int pairs = p.M * p.topk, sms = sm_count();
   const uint32_t row_bytes = (uint32_t)p.units * (kUnitK * 2) + 16;
-  p.cap = 8 * kCols / (kMode == kGateUp ? 1 : kParts);
+  p.cap = kMode == kGateUp ? 8 * kCols : 4 * kCols;
   p.rows = 0;
   p.split = 1;
   while (kMode == kGateUp) {
@@ -1366,9 +1477,9 @@ int plan_moe(const MoeParams& given, MoePlan& plan) {
   return B200FP4_STATUS_SUCCESS;
 }
 
-template <typename XT, int kMode, int kCols, int kParts>
+template <typename XT, int kMode, int kCols>
 int launch_moe(const MoePlan& plan, cudaStream_t st) {
-  if (launch_pdl_cluster(plan.p.split, w4a16_moe_kernel<XT, kMode, kCols, kParts>, dim3(plan.grid), dim3(kThreads), plan.smem, st, plan.p) != cudaSuccess) {
+  if (launch_pdl_cluster(plan.p.split, w4a16_moe_kernel<XT, kMode, kCols>, dim3(plan.grid), dim3(kThreads), plan.smem, st, plan.p) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
@@ -1376,40 +1487,35 @@ int launch_moe(const MoePlan& plan, cudaStream_t st) {
 }
 
 // Both projections are planned before the first is launched.
-template <typename T, int kUpCols, int kMode, int kDownCols, int kParts>
+template <typename T, int kUpCols, int kMode, int kDownCols>
 int launch_both(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
   MoePlan u, d;
-  int rc = plan_moe<T, kGateUp, kUpCols, kParts>(up, u);
-  if (rc == B200FP4_STATUS_SUCCESS) rc = plan_moe<__half, kMode, kDownCols, kParts>(down, d);
+  int rc = plan_moe<T, kGateUp, kUpCols>(up, u);
+  if (rc == B200FP4_STATUS_SUCCESS) rc = plan_moe<__half, kMode, kDownCols>(down, d);
   if (rc != B200FP4_STATUS_SUCCESS) return rc;
-  rc = launch_moe<T, kGateUp, kUpCols, kParts>(u, st);
-  return rc == B200FP4_STATUS_SUCCESS ? launch_moe<__half, kMode, kDownCols, kParts>(d, st) : rc;
+  rc = launch_moe<T, kGateUp, kUpCols>(u, st);
+  return rc == B200FP4_STATUS_SUCCESS ? launch_moe<__half, kMode, kDownCols>(d, st) : rc;
 }
 
-template <typename T, int kParts>
+template <typename T>
 int launch_layer_of(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
   // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  One / two of them in both
   // projections, us, eight experts of 4096, H = 4096, bf16: 7.25 pairs an expert 68 / 73, nine 78 / 75, eleven 87 / 78; 64 experts of 768, H = 2048: eight 59.7 / 59.0, twelve
   // 77 / 69.  Below seven few experts have more pairs than one column of eight holds.
   const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
   if (each <= 7) {
-    if (each * kParts > 7) return launch_both<T, 1, kDownItems, 2, kParts>(up, down, st);
+    if (each > 3.5) return launch_both<T, 1, kDownItems, 2>(up, down, st);
     // Whole strips: nothing goes through memory and no block waits for a counter, 1.4 us less for one token (H = 2048, ten experts of 512: 14.0 us against
     // 15.4), but the blocks' shares are less even.  A block reads 36 units in some 2 us: from there on the items are spread over all blocks (12 tokens, eight experts
     // of 4096 and H = 4096, a surplus of 41 units: 53 us against 57).
     MoePlan strips;
-    if (plan_moe<__half, kDownStrips, 1, kParts>(down, strips) == B200FP4_STATUS_SUCCESS &&
+    if (plan_moe<__half, kDownStrips, 1>(down, strips) == B200FP4_STATUS_SUCCESS &&
         (strips.items - slots_of(down, strips.p.cap) * down.strips / sm_count()) * down.units < 36)
-      return launch_both<T, 1, kDownStrips, 1, kParts>(up, down, st);
-    return launch_both<T, 1, kDownItems, 1, kParts>(up, down, st);
+      return launch_both<T, 1, kDownStrips, 1>(up, down, st);
+    return launch_both<T, 1, kDownItems, 1>(up, down, st);
   }
-  return launch_both<T, 2, kDownItems, 2, kParts>(up, down, st);
+  return launch_both<T, 2, kDownItems, 2>(up, down, st);
 }
-template <int kParts>
-int launch_layer(const MoeParams& up, const MoeParams& down, int h_dtype, cudaStream_t st) {
-  return h_dtype == B200FP4_DTYPE_BF16 ? launch_layer_of<__nv_bfloat16, kParts>(up, down, st) : launch_layer_of<__half, kParts>(up, down, st);
-}
-
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
 bool is_16bit(int dtype) { return dtype == B200FP4_DTYPE_F16 || dtype == B200FP4_DTYPE_BF16; }
 bool is_dtype(int dtype) { return is_16bit(dtype) || dtype == B200FP4_DTYPE_F32; }
@@ -1425,16 +1531,17 @@ size_t unit_bytes(int64_t E, int64_t N, int64_t K, int gated) {
 int64_t turn_of(int64_t M, int64_t topk) { return std::min(M, std::max<int64_t>(1, kMaxPairs / topk)); }
 
 struct MoeScratch {
-  size_t act, act_inv, y, counters, bytes;
+  size_t act, act_inv, y, counters, leveled, bytes;
 };
 MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I) {
   MoeScratch s;
   const size_t pairs = (size_t)turn_of(M, topk) * topk;
   s.act = 0;
-  s.act_inv = s.act + pad256(pairs * 2 * I * 2);
+  s.act_inv = s.act + pad256(pairs * act_row(I) * 2);
   s.y = s.act_inv + pad256(pairs * 4);
   s.counters = s.y + pad256(pairs * H * 4);
-  s.bytes = s.counters + pad256((size_t)strips_of(H) * 4);
+  s.leveled = s.counters + pad256((size_t)strips_of(H) * 4);
+  s.bytes = s.leveled + 256;
   return s;
 }
 
@@ -1533,6 +1640,9 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.y = reinterpret_cast<float*>(ws + s.y);
     p.counters = reinterpret_cast<int*>(ws + s.counters);
     p.n_counters = (int)w4::strips_of(H);
+    p.leveled = reinterpret_cast<uint32_t*>(ws + s.leveled);
+    static std::atomic<uint32_t> calls{0};
+    p.call = calls.fetch_add(1, std::memory_order_relaxed);
     MoeParams d = p;
     p.x = static_cast<const unsigned char*>(hidden) + (size_t)m * H * 2;
     p.ldx = H;
@@ -1544,7 +1654,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.strips = (int)((I + 15) / 16);
     p.units = (int)w4::units_of(H);
     d.x = p.act;
-    d.ldx = I;
+    d.ldx = act_row(I);
     d.packed = w2_packed;
     d.g = w2_g;
     d.out = static_cast<unsigned char*>(out) + (size_t)m * H * (out_dtype == B200FP4_DTYPE_F32 ? 4 : 2);
@@ -1553,7 +1663,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     d.K = (int)I;
     d.strips = (int)w4::strips_of(H);
     d.units = (int)w4::units_of(I);
-    const int rc = out_dtype == B200FP4_DTYPE_BF16 ? launch_layer<1>(p, d, h_dtype, st) : launch_layer<2>(p, d, h_dtype, st);
+    const int rc = h_dtype == B200FP4_DTYPE_BF16 ? launch_layer_of<__nv_bfloat16>(p, d, st) : launch_layer_of<__half>(p, d, st);
     if (rc != B200FP4_STATUS_SUCCESS) return rc;
   }
   return B200FP4_STATUS_SUCCESS;

@@ -506,8 +506,7 @@ B200FP4_API int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, co
  * w2 [E, H, I] packed, w13_g [E][gate rows, up rows] (8-byte aligned), w2_g [E]; H and I multiples of 16, H as long as a row fits in shared
  * memory (some 50,000), E up to 4096, topk up to 2048.  out may be hidden (of the same type) or other memory.  Pairs whose expert (after
  * expert_map) is outside [0, E) add nothing; a token without any gives zeros.  flags: B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT or 0.  Between the
- * projections a value is kept in one f16, with a power of two for each pair, where the result is bf16, else as the sum of two.  Results do not
- * depend on the order in which blocks run.  The workspace is a call's own until the call is done. */
+ * projections a value is the sum of two f16, to f32's precision whatever its size.  Results do not depend on the order in which blocks run.  The workspace is a call's own until the call is done. */
 B200FP4_API size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I);
 B200FP4_API int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* topk_weights, const int32_t* topk_ids,
                                   const int32_t* expert_map, int64_t global_E, const uint8_t* w13_packed, const float* w13_g,
