@@ -542,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
         // this lane's column: block (l / 4) % 4 of a half, of the first half and then the second or of token l / 16
         const int token = kTokens == 2 ? row8 >> 2 : 0;
         const bool mine0 = kTokens == 2 ? (row8 & 3) == quad : row8 == quad, mine1 = kTokens == 2 ? mine0 : row8 == quad + 4;
-        const uint32_t row = base + l.rows + token * row_bytes + quad * 32;
+        const uint32_t row = base + l.rows + (token < n ? token : 0) * row_bytes + quad * 32;
         float part[2][2] = {};
         uint32_t b[2][8] = {};
 #pragma unroll 1
@@ -658,7 +658,8 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
     if (clusters < 1) break;
     const int own = (p.units + split - 1) / split;
     const uint32_t row_bytes = (uint32_t)own * (kUnitK * 2) + 16;
-    for (int cap = std::min(8 * kCols, p.M); cap > 0; cap /= 2) {
+    // Rows of fewer tokens where there is no room for all; tokens of a block of k a column are there together or not at all.
+    for (int cap = std::min(8 * kCols, p.M); cap >= std::max(1, kTokens); cap /= 2) {
       const int64_t items = (int64_t)((p.M + cap - 1) / cap) * p.strips;
       if (items > 0x3FFFFFFF) break;
       const int used = (int)std::min<int64_t>(clusters, items), most = (int)((items + used - 1) / used);
