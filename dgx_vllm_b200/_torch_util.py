@@ -37,13 +37,13 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-WS_SHARED, WS_LINEAR, WS_ROUTER, WS_GEMM, WS_W4A16 = 0, 1, 2, 3, 4       # slots of a stream's scratch (csrc/torch_host.cpp)
+WS_SHARED, WS_LINEAR, WS_ROUTER, WS_GEMM, WS_W4A16_STATUS = 0, 1, 2, 3, 5       # slots of a stream's scratch (csrc/torch_host.cpp)
 
 
 def workspace(device: torch.device, nbytes: int, slot: int = WS_SHARED) -> torch.Tensor:
     """Grow-only scratch buffer per (device, current stream, slot), shared with the native host path.  Calls issued on one
-    stream serialise on the GPU, so sharing it between consecutive ops is safe; its address is stable once large enough,
-    which CUDA-graph capture relies on."""
+    stream serialise on the GPU, so sharing it between consecutive ops is safe; scratch whose address a captured graph has is kept
+    when a larger call replaces it."""
     return _lib.host().workspace(torch.cuda.current_device() if device.index is None else device.index, nbytes, slot)
 
 

@@ -23,6 +23,7 @@
 #include <stdexcept>
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "../../include/b200_nvfp4.h"
 
@@ -132,16 +133,23 @@ struct WithoutGil {
   ~WithoutGil() { PyEval_RestoreThread(state); }
 };
 
-// Grow-only scratch per (device, stream): calls issued on one stream serialise on the GPU, so consecutive ops share it; its
-// address is stable once large enough, which CUDA-graph capture relies on.  One slot for each family of ops with a status word of
-// its own (or whose words another's would land on).  The lock is held from the look-up to the last launch of a call: another
+// Grow-only scratch per (device, stream): calls issued on one stream serialise on the GPU, so consecutive ops share it.  A graph keeps
+// the addresses that it was captured with: scratch that a captured call has used is kept for good when a larger call replaces it.  One slot
+// for each family of ops with a status word of its own (or whose words another's would land on); the status word of the weight-only
+// operators has a slot that never grows, so that it is the same word for every call on the stream, captured or not.  The lock is held from the look-up to the last launch of a call: another
 // thread on the same stream neither replaces the scratch under it nor puts a launch between its steps.  It is never waited
 // for with the GIL held.
-enum Slot { kSlotShared = 0, kSlotLinear = 1, kSlotRouter = 2, kSlotGemm = 3, kSlotW4a16 = 4, kSlots = 5 };        // Python names them in _torch_util.py
+enum Slot { kSlotShared = 0, kSlotLinear = 1, kSlotRouter = 2, kSlotGemm = 3, kSlotW4a16 = 4, kSlotW4a16Status = 5, kSlots = 6 };        // Python names them in _torch_util.py
 struct StreamScratch {
   std::mutex mu;
   at::Tensor slots[kSlots];
+  bool captured[kSlots] = {};                      // a graph has the slot's address
+  std::vector<at::Tensor> kept;
 };
+bool capturing(cudaStream_t st) {
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  return cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
+}
 struct StreamKey {
   int dev;
   cudaStream_t stream;
@@ -153,11 +161,21 @@ struct StreamHash {
 
 class Workspace {
  public:
-  Workspace(int dev, cudaStream_t stream, size_t bytes, int slot = kSlotShared) : scratch_(of(dev, stream)), lock_(scratch_.mu), t_(scratch_.slots[slot]) {
-    if (t_.defined() && (size_t)t_.numel() >= bytes) return;
-    t_ = empty({(int64_t)std::max(bytes, (size_t)1 << 20)}, at::kByte, dev);
-    t_.narrow(0, 0, 256).zero_();                  // a status word that no op has written yet reads 0
+  Workspace(int dev, cudaStream_t stream, size_t bytes, int slot = kSlotShared)
+      : scratch_(of(dev, stream)), lock_(scratch_.mu), dev_(dev), captured_(capturing(stream)), t_(take(bytes, slot)) {}
+  // another slot of the stream, under the same lock
+  at::Tensor& take(size_t bytes, int slot) {
+    at::Tensor& t = scratch_.slots[slot];
+    if (!t.defined() || (size_t)t.numel() < bytes) {
+      if (scratch_.captured[slot]) scratch_.kept.push_back(std::move(t));
+      scratch_.captured[slot] = false;
+      t = empty({(int64_t)std::max(bytes, slot == kSlotW4a16Status ? (size_t)256 : (size_t)1 << 20)}, at::kByte, dev_);
+      t.narrow(0, 0, 256).zero_();                 // a status word that no op has written yet reads 0
+    }
+    scratch_.captured[slot] |= captured_;
+    return t;
   }
+  bool captured() const { return captured_; }
   const at::Tensor& tensor() const { return t_; }
   void* data() const { return t_.data_ptr(); }
   size_t bytes() const { return t_.nbytes(); }
@@ -172,6 +190,8 @@ class Workspace {
   }
   StreamScratch& scratch_;
   std::lock_guard<std::mutex> lock_;
+  const int dev_;
+  const bool captured_;
   at::Tensor& t_;
 };
 
@@ -496,21 +516,16 @@ bool meet(const at::Tensor& read, int64_t rows, int64_t cols, int64_t ld, const 
 // share no more than the status word.
 class Scratch {
  public:
-  Scratch(int dev, cudaStream_t st, size_t bytes) : captured_(capturing(st)), shared_(dev, st, 256 + (captured_ ? 0 : bytes), kSlotW4a16) {
-    if (captured_ && bytes > 0) own_ = empty({(int64_t)bytes}, at::kByte, dev);
+  Scratch(int dev, cudaStream_t st, size_t bytes) : status_(dev, st, 256, kSlotW4a16Status) {
+    if (bytes > 0) scratch_ = status_.captured() ? empty({(int64_t)bytes}, at::kByte, dev) : status_.take(bytes, kSlotW4a16);
   }
-  int32_t* status() const { return static_cast<int32_t*>(shared_.data()); }
-  void* data() const { return captured_ ? (own_.defined() ? own_.data_ptr() : nullptr) : static_cast<uint8_t*>(shared_.data()) + 256; }
-  size_t bytes() const { return captured_ ? (own_.defined() ? own_.nbytes() : 0) : shared_.bytes() - 256; }
+  int32_t* status() const { return static_cast<int32_t*>(status_.data()); }
+  void* data() const { return scratch_.data_ptr(); }
+  size_t bytes() const { return scratch_.nbytes(); }
 
  private:
-  static bool capturing(cudaStream_t st) {
-    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-    return cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
-  }
-  bool captured_;
-  Workspace shared_;
-  at::Tensor own_;
+  Workspace status_;
+  at::Tensor scratch_;
 };
 
 // w4a16_linear(x, packed, g_scale, N, K, bias or None, out or None, out_dtype or None) -> out

@@ -16,7 +16,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._torch_util import WS_W4A16, ptr, require, require_cuda, status_word, stream_ptr
+from ._torch_util import WS_W4A16_STATUS, ptr, require, require_cuda, status_word, stream_ptr
 
 
 class PackedNvfp4Weight:
@@ -75,8 +75,8 @@ def w4a16_linear(x: torch.Tensor, weight: PackedNvfp4Weight, bias: torch.Tensor 
 
 def last_w4a16_status(device=None) -> int:
     """Status word of the most recent w4a16_linear or W4A16MoE on the current stream of `device`: 0, or the code of a bounded wait that ran
-    out (that call's result is then not valid).  Synchronises."""
-    return status_word(device, WS_W4A16)
+    out (that call's result is then not valid).  A graph leaves it where the stream that it was captured on has it.  Synchronises."""
+    return status_word(device, WS_W4A16_STATUS)
 
 
 class W4A16MoE:

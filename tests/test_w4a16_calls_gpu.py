@@ -25,3 +25,65 @@ def test_two_tokens_with_long_rows(N, K, dtype):
     for out_dtype in (F32, dtype):
         assert torch.equal(w4a16_linear(x, w, out_dtype=out_dtype), want.to(out_dtype))
     assert last_w4a16_status() == 0
+
+
+def _replayed_after_growth(capture, grow):
+    """`capture()` captured on a stream, then `grow()` on it eagerly; what is allocated then keeps its values through replays.  Returns the captured call's output."""
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        want = capture().clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            out = capture()
+        for _ in range(2):
+            grow()
+            stream.synchronize()
+        others = [torch.full((n,), 7, dtype=torch.int32, device="cuda") for n in [1 << 18] * 24 + [64] * 64 + [1 << 21] * 8]
+        for _ in range(3):
+            out.fill_(0)
+            graph.replay()
+            stream.synchronize()
+            assert torch.equal(out, want)
+        for t in others:
+            assert bool((t == 7).all())
+    del graph
+
+
+def test_graph_beside_larger_calls_on_its_stream():
+    from dgx_vllm_b200 import _torch_util as util
+    from dgx_vllm_b200.weight_only import last_w4a16_status, pack_nvfp4_weight, w4a16_linear
+    layer, x, weights, ids, _, _, _ = _layer(64, 4, 2048, 256, 4, BF16)
+    codes, block = make_weight(1, 64, 2048, 5)
+    w = pack_nvfp4_weight(codes[0], block[0], torch.ones(1, device="cuda"))
+    words = set()
+
+    def status_word():
+        words.add(util.workspace(torch.device("cuda", torch.cuda.current_device()), 256, util.WS_W4A16_STATUS).data_ptr())
+        assert last_w4a16_status() == 0
+
+    def grow():
+        status_word()
+        layer(x, weights, ids)                                          # 2.6 MB of scratch
+        layer(x.repeat(8, 1), weights.repeat(8, 1), ids.repeat(8, 1))   # 20 MB
+        status_word()
+
+    _replayed_after_growth(lambda: layer(x[:1], weights[:1], ids[:1]), grow)
+    _replayed_after_growth(lambda: w4a16_linear(x[:3], w), grow)
+    assert len(words) == 2                                              # one for each of the two streams
+
+
+def test_graph_of_the_sparse_layer_beside_larger_calls_on_its_stream():
+    """The scratch that the 2:4 layer was captured with stays its own as well."""
+    import synth
+    from dgx_vllm_b200.sparse_fp4_v7 import FusedSparseMoE
+    from util import oracle_quantize_fn
+    E, H, I, M, topk = 4, 512, 128, 256, 2
+    w13 = synth.make_sparse_experts(E, 2 * I, H, 1, "cpu", oracle_quantize_fn)
+    w2 = synth.make_sparse_experts(E, H, I, 2, "cpu", oracle_quantize_fn)
+    keys = ("comp_T", "meta_T", "scale_T", "g_scales")
+    layer = FusedSparseMoE(*[w13[k].cuda() for k in keys], *[w2[k].cuda() for k in keys], I)
+    tw, ids = (t.cuda() for t in synth.make_routing(M, E, topk, 3, "cpu"))
+    x = synth.make_hidden(M, H, 4, "cpu").cuda()
+    _replayed_after_growth(lambda: layer(x[:2], tw[:2], ids[:2]),
+                           lambda: layer(x.repeat(8, 1), tw.repeat(8, 1), ids.repeat(8, 1)))
