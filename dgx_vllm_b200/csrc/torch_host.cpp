@@ -512,6 +512,11 @@ bool meet(const at::Tensor& read, int64_t rows, int64_t cols, int64_t ld, const 
   return rows > 0 && cols > 0 && r < w + written.nbytes() && w < r + ((rows - 1) * ld + cols) * (int64_t)read.element_size();
 }
 
+bool is_packed(const at::Tensor& w, int64_t E, int64_t N, int64_t K, int gated) {
+  const size_t bytes = b200fp4_w4a16_packed_bytes(E, N, K, gated);
+  return bytes > 0 && w.scalar_type() == at::kByte && w.is_contiguous() && w.nbytes() == bytes;
+}
+
 // Status word and scratch of a call.  The scratch of a captured call is its own, from its graph's pool: graphs that are replayed at once
 // share no more than the status word.
 class Scratch {
@@ -540,7 +545,7 @@ B200_FN(py_w4a16_linear) {
     const int64_t M = x.size(0);
     require(M == 0 || rows_aligned(x), "the rows of x must be 16-byte aligned");
     require(M < 2 || x.stride(0) >= K, "the rows of x must not overlap");
-    require(w.scalar_type() == at::kByte && w.is_contiguous() && w.nbytes() >= b200fp4_w4a16_packed_bytes(1, N, K, 0), "weight must come from pack_nvfp4_weight");
+    require(is_packed(w, 1, N, K, 0), "weight must come from pack_nvfp4_weight, for [N,K]");
     require(is_f32_scalar(g), "g_scale must be one f32");
     require(bias == nullptr || (bias->dim() == 1 && bias->size(0) == N && is_float(*bias) && bias->is_contiguous()), "bias must be a contiguous [N] tensor in bf16, f16 or f32");
     at::ScalarType dt = x.scalar_type();
@@ -592,9 +597,10 @@ B200_FN(py_w4a16_moe) {
     require(ids_in.dim() == 2 && ids_in.size(0) == M && ids_in.size(1) > 0 && is_2d(tw_in, M, ids_in.size(1)), "topk_weights and topk_ids must be [M, topk]");
     require(ids_in.scalar_type() == at::kInt || ids_in.scalar_type() == at::kLong, "topk_ids must be int32 or int64");
     const int64_t topk = ids_in.size(1);
-    require(w13.nbytes() >= b200fp4_w4a16_packed_bytes(E, 2 * I, H, 1) && w2.nbytes() >= b200fp4_w4a16_packed_bytes(E, H, I, 0) && g13.numel() == 2 * E &&
-                g2.numel() == E,
-            "the weights must come from pack_nvfp4_weight");
+    auto is_factors = [](const at::Tensor& g, int64_t n) { return g.scalar_type() == at::kFloat && g.numel() == n && g.is_contiguous(); };
+    require(is_packed(w13, E, 2 * I, H, 1) && is_packed(w2, E, H, I, 0) && is_factors(g13, 2 * E) && is_factors(g2, E),
+            "the weights must come from pack_nvfp4_weight: w13 [E,2I,H] gated, w2 [E,H,I]");
+    require(emap == nullptr || (emap->scalar_type() == at::kInt && emap->is_contiguous() && emap->numel() > 0), "expert_map must be a contiguous int32 tensor");
     require(given == nullptr || (is_float(*given) && is_2d(*given, M, H) && given->is_contiguous()), "out must be a contiguous [M,H] tensor in bf16, f16 or f32");
     // In place is right: a row of hidden_states is read for the last time before its result is written.
     require(given == nullptr || (given->data_ptr() == x.data_ptr() && given->nbytes() == x.nbytes()) || !meet(x, M, H, H, *given),

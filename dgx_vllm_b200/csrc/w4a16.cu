@@ -30,7 +30,7 @@ struct PackParams {
   const uint8_t* codes;       // [E, N, K/2]
   const uint8_t* scales;      // [E, N, K/16]
   uint8_t* packed;
-  uint32_t* peaks;            // [E], gated [E][gate, up]: behind the units, zeroed before
+  uint32_t* tails;            // [E], gated [E][gate, up]: behind the units, zeroed before
   int64_t strips, units;
   int N, K, gated;
 };
@@ -73,10 +73,10 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
     *reinterpret_cast<uint4*>(dst + (tile * 2 + half) * 512 + chunk_at(lane >> 2, lane & 3)) = make_uint4(word[0].x, word[0].y, word[1].x, word[1].y);
   }
   *reinterpret_cast<uint32_t*>(dst + kUnitScales + lane * 8 + tile * 4) = sc;
-  // magnitudes are not negative: their bits order as they do
+  // magnitudes are not negative: their bits order as they do, above a tag that is the same for all
   for (int r = 0; r <= p.gated; ++r) {
     const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(peak[r]));
-    if (lane == 0) atomicMax(p.peaks + e * (p.gated + 1) + r, top);
+    if (lane == 0) atomicMax(p.tails + e * (p.gated + 1) + r, top | size_tag(p.N, p.K, p.gated));
   }
 }
 
@@ -440,6 +440,7 @@ struct LinearParams {
   const void* x;              // [M, K], rows ldx apart
   int64_t ldx;
   const uint8_t* packed;
+  const uint32_t* tail;
   const float* g;
   void* out;                  // [M, N]
   const void* bias;           // [N] or null
@@ -450,6 +451,7 @@ struct LinearParams {
   int cap;                    // columns of an item
   int per, more;              // items of a cluster: `per`, and one more for the first `more` clusters
   int log_share;
+  uint32_t tag;
   int* status;
 };
 
@@ -510,13 +512,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
 #pragma unroll 1
   for (int i = 0; i < stages_of(kCols); ++i) fetch();
   pdl_launch_dependents();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
+  const bool fits = packed_for(p.tail, p.tag);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = fits ? 0 : kOtherSizes;
   if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
   // rows are shifted by 16 bytes against each other: no two lanes of a load meet
   const uint32_t row_bytes = (uint32_t)((p.units + split - 1) / split) * (kUnitK * 2) + 16;
   const LinearLayout l = linear_layout(kCols, p.cap, row_bytes, split, p.per + (p.more > 0));
   float* const inv = reinterpret_cast<float*>(smem + l.inv);
-  const float g = *p.g;
+  const float g = fits ? *p.g : __int_as_float(0x7FC00000);
   bool arrived = split == 1;
   int item = first + group;
   for (int done = first; done < last;) {
@@ -701,6 +704,8 @@ int launch_linear(const LinearCall& c, cudaStream_t st) {
   p.x = c.x;
   p.ldx = c.ldx;
   p.packed = c.packed;
+  p.tail = c.tail;
+  p.tag = size_tag(c.N, c.K, 0);
   p.g = c.g;
   p.out = c.out;
   p.out_dtype = c.out_dtype;
@@ -728,7 +733,9 @@ struct MoeParams {
   int64_t ldx;
   const uint8_t* packed;
   const float* g;             // [E]; gate/up [E][gate, up]
-  const float* peaks;         // gate/up: [E][gate, up]
+  const uint2* peaks;         // gate/up: [E][gate, up]
+  const uint32_t *tail13, *tail2;        // down: of both projections
+  uint32_t tag13, tag2;
   int M, N, K;
   int strips, units;
   int cap, rows;              // columns of a slot; rows that there is room for
@@ -983,12 +990,15 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   }
   // the weights are on their way with the ids
   float weight[kDown ? kMaxPairs / kThreads : 1];
-  if constexpr (kDown)
+  bool fits = true;
+  if constexpr (kDown) {
+    fits = packed_for(p.tail13, p.tag13) && packed_for(p.tail2, p.tag2);
 #pragma unroll
     for (int q = 0; q < kMaxPairs / kThreads; ++q) {
       const int i = q * kThreads + threadIdx.x;
-      weight[q] = i < p.M * p.topk && !p.weight_on_input ? p.weights[i] : 1.f;
+      weight[q] = !fits ? __int_as_float(0x7FC00000) : i < p.M * p.topk && !p.weight_on_input ? p.weights[i] : 1.f;
     }
+  }
   const int n_slots = find_slots(p, smem, l);
   if constexpr (kDown)
 #pragma unroll
@@ -1078,7 +1088,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       const int own = (int)threadIdx.x < n_rows ? list[row0 + threadIdx.x] : -1;
       if (own >= 0) {
         g = reinterpret_cast<const float2*>(p.g)[expert[own]];
-        peak = reinterpret_cast<const float2*>(p.peaks)[expert[own]];
+        const uint2 words = p.peaks[expert[own]];
+        peak = make_float2(peak_of(words.x), peak_of(words.y));
         if (p.weight_on_input) w = p.weights[own];
       }
       if (end == first)
@@ -1177,6 +1188,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     pdl_launch_dependents();
     if (kWhole && p.split > 1) cluster_wait();
     const bool leveled = *p.leveled == p.call;       // otherwise every run of every pair is at level 0, and nobody looks
+    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) *p.status = kOtherSizes;
     if (n_slots == 0) {
       for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < (size_t)p.M * p.N; i += (size_t)gridDim.x * kThreads)
         store_value(p.out, p.out_dtype, i, 0.f);
@@ -1571,8 +1583,8 @@ extern "C" int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, i
   p.gated = gated != 0;
   const int64_t n = E * p.strips * p.units * 2;
   if ((n + 7) / 8 > 0x7FFFFFFF) return B200FP4_STATUS_NOT_SUPPORTED;
-  p.peaks = reinterpret_cast<uint32_t*>(packed + unit_bytes(E, N, K, gated));
-  if (cudaMemsetAsync(p.peaks, 0, (size_t)E * (gated ? 2 : 1) * 4, static_cast<cudaStream_t>(stream)) != cudaSuccess) {
+  p.tails = reinterpret_cast<uint32_t*>(packed + unit_bytes(E, N, K, gated));
+  if (cudaMemsetAsync(p.tails, 0, (size_t)E * (gated ? 2 : 1) * 4, static_cast<cudaStream_t>(stream)) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
@@ -1589,7 +1601,7 @@ extern "C" int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, con
   if (x == nullptr || packed == nullptr || g_scale == nullptr || out == nullptr || status == nullptr) return B200FP4_STATUS_INVALID_VALUE;
   if (!aligned(x, 16) || !aligned(packed, 16) || !aligned(out, 16) || ldx % 8 != 0 || (M > 1 && ldx < K)) return B200FP4_STATUS_INVALID_VALUE;
   if (!fits_int(M) || !fits_int(N + 64) || !fits_int(K + 128)) return B200FP4_STATUS_NOT_SUPPORTED;
-  const LinearCall c = {x, x_dtype, ldx, packed, g_scale, bias, bias_dtype, out, out_dtype, M, N, K, status};
+  const LinearCall c = {x, x_dtype, ldx, packed, reinterpret_cast<const uint32_t*>(packed + unit_bytes(1, N, K, 0)), g_scale, bias, bias_dtype, out, out_dtype, M, N, K, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (few_tokens(c)) {
     const int rc = x_dtype == B200FP4_DTYPE_BF16 ? launch_linear<__nv_bfloat16>(c, st) : launch_linear<__half>(c, st);
@@ -1637,7 +1649,11 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.weight_on_input = flags & B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT ? 1 : 0;
     p.act = reinterpret_cast<__half*>(ws + s.act);
     p.act_inv = reinterpret_cast<float*>(ws + s.act_inv);
-    p.peaks = reinterpret_cast<const float*>(w13_packed + unit_bytes(E, 2 * I, H, 1));
+    p.peaks = reinterpret_cast<const uint2*>(w13_packed + unit_bytes(E, 2 * I, H, 1));
+    p.tail13 = reinterpret_cast<const uint32_t*>(p.peaks);
+    p.tail2 = reinterpret_cast<const uint32_t*>(w2_packed + unit_bytes(E, H, I, 0));
+    p.tag13 = size_tag(2 * I, H, 1);
+    p.tag2 = size_tag(H, I, 0);
     p.y = reinterpret_cast<float*>(ws + s.y);
     p.counters = reinterpret_cast<int*>(ws + s.counters);
     p.n_counters = (int)w4::strips_of(H);

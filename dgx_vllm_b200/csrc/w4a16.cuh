@@ -18,7 +18,9 @@
 // The chunks are ordered so that no two lanes meet in a bank when each reads its 16 bytes, nor when a lane is one of 32 rows and reads the 8 bytes of a
 // block (the decoding of w4a16_gemm.cu).  Negative scales give their sign to their codes when the weight is packed.
 // Gated: the 16 rows of a tile are eight gate rows and the same eight up rows, so that a lane holds both of a value's products.
-// Behind the units: for each matrix the largest magnitude of code times scale, f32 (two of them, gate rows and up rows, where gated).
+// Behind the units, for each matrix (gated: for its gate rows and its up rows) a word: the largest magnitude of code times scale, which the upper half of an f32 holds exactly, and
+// in the lower half a tag of the sizes.  Packed bytes do not tell K = 112 from 128, or [64, 128] from [32, 256]: kernels compare the tag with
+// the sizes that they are called with, and results of a weight that was packed for others are NaN (status kOtherSizes).
 #pragma once
 
 #include "common.cuh"
@@ -27,6 +29,14 @@ namespace b200fp4 {
 namespace w4 {
 
 constexpr int kUnitBytes = 2304, kUnitScales = 2048, kUnitK = 128, kUnitRows = 32;
+constexpr int kOtherSizes = 63;
+
+// the same for no two sizes within 64 rows and 64 blocks of 16 of each other
+__host__ __device__ __forceinline__ uint32_t size_tag(int64_t N, int64_t K, int gated) {
+  return (uint32_t)((uint64_t)N * 40503u + (uint64_t)(K / 16) * 30011u + (gated ? 0x5555u : 0u)) & 0xFFFFu;
+}
+__device__ __forceinline__ bool packed_for(const uint32_t* tail, uint32_t tag) { return (*tail & 0xFFFFu) == tag; }
+__device__ __forceinline__ float peak_of(uint32_t word) { return __uint_as_float(word & 0xFFFF0000u); }
 
 __host__ __device__ __forceinline__ int64_t strips_of(int64_t rows) { return (rows + kUnitRows - 1) / kUnitRows; }      // of 32 rows
 __host__ __device__ __forceinline__ int64_t units_of(int64_t K) { return (K + kUnitK - 1) / kUnitK; }

@@ -37,6 +37,7 @@ constexpr int kMaxSplit = 8;
 
 struct GemmParams {
   const uint8_t* packed;
+  const uint32_t* tail;
   const float* g;
   const void* bias;
   void* out;
@@ -51,6 +52,7 @@ struct GemmParams {
   uint32_t acc_cols;          // columns of an accumulator
   int accs;                   // accumulators in turn: two where a block does several tiles, or one in several chains
   int chain, chains;          // units that are summed in one accumulator; one tile: accumulators next to each other, whose sum is the result
+  uint32_t tag;
   uint32_t sums_at;           // split: where the cluster's sums go; 0: where the token stages were
   int* status;
 };
@@ -187,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   const uint32_t tmem = lds32(tmem_ptr);
   pdl_wait();
   pdl_launch_dependents();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *status = packed_for(p.tail, p.tag) ? 0 : kOtherSizes;
   if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
 
   if (warp == 0) {
@@ -342,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   // ---------------------------------------------------------------------- epilogue: a lane is a row of the weight, a column a token
   const int quarter = warp & 3;
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+  auto factor = [&]() { return packed_for(p.tail, p.tag) ? *p.g : __int_as_float(0x7FC00000); };
   // columns from, from + by, ... of a tile of n tokens, 32 at a time
   auto write_columns = [&](uint32_t acc, int row, int token0, int n, int from, int by, float g, bool more) {
     const float bias = p.bias != nullptr && row < p.N ? load_value(p.bias, p.bias_dtype, row) : 0.f;
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   if (p.accs > 1) {
     // several tiles: four warps, while the others go on
     if (warp >= 2 && warp < kFirstDecode) {
-      const float g = *p.g;
+      const float g = factor();
       Slot acc;
       for (int tile = first_tile; tile < p.tiles; tile += step) {
         const int token0 = tile / p.row_tiles * tokens;
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     bool ok = true;
     if (work) ok = mbar_wait_warp(acc_full, 0, status, 79);
     tcgen05_fence_after();
-    const float g = *p.g;
+    const float g = factor();
     if (split == 1) {
       if (work && ok) write_columns(0, row_tile * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), nth * 32, 5 * 32, g, false);
     } else {
@@ -469,6 +472,8 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
   if (!ready[dev]) return B200FP4_STATUS_EXECUTION_FAILED;
   GemmParams p = {};
   p.packed = c.packed;
+  p.tail = c.tail;
+  p.tag = size_tag(c.N, c.K, 0);
   p.g = c.g;
   p.bias = c.bias;
   p.bias_dtype = c.bias_dtype;

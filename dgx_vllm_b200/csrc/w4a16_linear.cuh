@@ -10,6 +10,7 @@ struct LinearCall {
   int x_dtype;
   int64_t ldx;
   const uint8_t* packed;
+  const uint32_t* tail;       // behind its units
   const float* g;
   const void* bias;           // [N] or null
   int bias_dtype;

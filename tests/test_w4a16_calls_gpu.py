@@ -87,3 +87,62 @@ def test_graph_of_the_sparse_layer_beside_larger_calls_on_its_stream():
     x = synth.make_hidden(M, H, 4, "cpu").cuda()
     _replayed_after_growth(lambda: layer(x[:2], tw[:2], ids[:2]),
                            lambda: layer(x.repeat(8, 1), tw.repeat(8, 1), ids.repeat(8, 1)))
+
+
+@pytest.mark.parametrize("M", [1, 2, 5, 40, 300])
+@pytest.mark.parametrize("packed_for,called_with", [((96, 128), (96, 112)), ((96, 128), (95, 128)), ((65, 128), (96, 128)), ((64, 128), (32, 256)), ((32, 256), (64, 128))])
+def test_linear_op_with_sizes_that_its_weight_has_not(packed_for, called_with, M):
+    """Packed bytes are as many for both; the result says so."""
+    import dgx_vllm_b200.torch_ops  # noqa: F401
+    from dgx_vllm_b200.weight_only import last_w4a16_status, pack_nvfp4_weight
+    codes, block = make_weight(1, *packed_for, 4)
+    w = pack_nvfp4_weight(codes[0], block[0], torch.ones(1, device="cuda"))
+    N, K = called_with
+    for out_dtype in (F32, None):
+        y = torch.ops.b200_nvfp4.w4a16_linear(make_x(M, K, 1, BF16), w.packed, w.g_scale, N, None, out_dtype)
+        assert tuple(y.shape) == (M, N) and bool(torch.isnan(y).all()) and last_w4a16_status() == 63
+    y = torch.ops.b200_nvfp4.w4a16_linear(make_x(M, packed_for[1], 1, BF16), w.packed, w.g_scale, packed_for[0], None, F32)
+    assert not bool(torch.isnan(y).any()) and last_w4a16_status() == 0
+
+
+@pytest.mark.parametrize("M", [1, 6, 40])
+def test_layer_op_with_sizes_that_its_weights_have_not(M):
+    import dgx_vllm_b200.torch_ops  # noqa: F401
+    from dgx_vllm_b200.weight_only import last_w4a16_status
+    layer, x, weights, ids, _, _, _ = _layer(M, 4, 128, 64, 2, BF16)
+    ids[0] = -1
+    op = torch.ops.b200_nvfp4.w4a16_moe
+    hidden = x[:, :112].contiguous()                                # as many bytes
+    for on_input in (False, True):
+        out = op(hidden, weights, ids, None, *layer._weights, 64, on_input)
+        assert bool((out[0] == 0).all()) and bool(torch.isnan(out[1:]).all()) and last_w4a16_status() == 63
+    with pytest.raises(RuntimeError):
+        op(x, weights, ids, None, *layer._weights, 48, False)
+    assert torch.equal(op(x, weights, ids, None, *layer._weights, 64, False), layer(x, weights, ids)) and last_w4a16_status() == 0
+
+
+def test_tensors_that_are_no_packed_weights_are_refused():
+    import dgx_vllm_b200.torch_ops  # noqa: F401
+    from dgx_vllm_b200 import _lib
+    from dgx_vllm_b200.weight_only import pack_nvfp4_weight
+    codes, block = make_weight(1, 96, 128, 4)
+    one = torch.ones(1, device="cuda")
+    w = pack_nvfp4_weight(codes[0], block[0], one)
+    x = make_x(5, 128, 1, BF16)
+    linear = lambda packed, g=one, n=96, x=x: torch.ops.b200_nvfp4.w4a16_linear(x, packed, g, n, None, None)
+    stub = torch.zeros(1, dtype=torch.uint8, device="cuda").expand(w.packed.numel())
+    for bad in (lambda: linear(w.packed[:-4]), lambda: linear(torch.cat((w.packed, w.packed))), lambda: linear(w.packed.view(torch.int32)), lambda: linear(stub),
+                lambda: linear(w.packed, one.double()), lambda: linear(w.packed, one.to(BF16)), lambda: linear(w.packed, n=0), lambda: linear(w.packed, n=97),
+                lambda: linear(pack_nvfp4_weight(codes[0], block[0], one, gated=True).packed), lambda: linear(w.packed, x=make_x(5, 256, 1, BF16))):
+        with pytest.raises(RuntimeError):
+            bad()
+    layer, x, weights, ids, emap, _, _ = _layer(6, 4, 128, 64, 2, BF16, parallel=2)
+    w13, g13, w2, g2 = layer._weights
+    call = lambda *w, m=emap, out=None: _lib.host().w4a16_moe(*w, m, 128, 64, 4, x, weights, ids, False, out)
+    for bad in (lambda: call(w13, g13, w2, g2.double()), lambda: call(w13, g13.to(BF16), w2, g2), lambda: call(w13, g13.T, w2, g2), lambda: call(w2, g13, w13, g2),
+                lambda: call(w13.view(torch.int32), g13, w2, g2), lambda: call(w13[:-8], g13, w2, g2), lambda: call(w13, g13, w2[4:], g2),
+                lambda: call(w13, g13, torch.zeros(1, dtype=torch.uint8, device="cuda").expand(w2.numel()), g2),
+                lambda: call(w13, g13, w2, g2, m=emap.long()), lambda: call(w13, g13, w2, g2, m=emap[::2])):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert torch.equal(call(w13, g13, w2, g2), layer(x, weights, ids))
