@@ -558,6 +558,7 @@ B200_FN(py_w4a16_linear) {
     require(dt == at::kBFloat16 || dt == at::kHalf || dt == at::kFloat, "out_dtype must be bfloat16, float16 or float32");
     require(given == nullptr || (given->scalar_type() == dt && is_2d(*given, M, N) && given->is_contiguous()), "out must be a contiguous [M,N] tensor of out_dtype");
     require(given == nullptr || !meet(x, M, K, M > 1 ? x.stride(0) : K, *given), "out must not overlap x");
+    require(given == nullptr || bias == nullptr || !meet(*bias, 1, N, N, *given), "out must not overlap bias");
     at::Tensor out;
     {
       WithoutGil nogil;
@@ -605,6 +606,10 @@ B200_FN(py_w4a16_moe) {
     // In place is right: a row of hidden_states is read for the last time before its result is written.
     require(given == nullptr || (given->data_ptr() == x.data_ptr() && given->nbytes() == x.nbytes()) || !meet(x, M, H, H, *given),
             "out must be hidden_states or not overlap it");
+    // every pair's id and weight is read again while results are written
+    require(given == nullptr || (!meet(tw_in, M, topk, tw_in.stride(0), *given) && !meet(ids_in, M, topk, ids_in.stride(0), *given) &&
+                                 (emap == nullptr || !meet(*emap, 1, emap->numel(), emap->numel(), *given))),
+            "out must not overlap the routing");
     at::Tensor out;
     {
       WithoutGil nogil;

@@ -146,3 +146,24 @@ def test_tensors_that_are_no_packed_weights_are_refused():
         with pytest.raises(RuntimeError):
             bad()
     assert torch.equal(call(w13, g13, w2, g2), layer(x, weights, ids))
+
+
+def test_results_in_the_memory_of_other_arguments_are_refused():
+    from dgx_vllm_b200.weight_only import pack_nvfp4_weight, w4a16_linear
+    codes, block = make_weight(1, 64, 64, 3)
+    w = pack_nvfp4_weight(codes[0], block[0], torch.ones(1, device="cuda"))
+    room = torch.zeros(6 * 64, device="cuda")
+    x = make_x(4, 64, 1, BF16)
+    with pytest.raises(RuntimeError, match="overlap"):
+        w4a16_linear(x, w, room[:64], out=room[:256].view(4, 64))
+    w4a16_linear(x, w, room[256:320], out=room[:256].view(4, 64))
+    layer, x, weights, ids, emap, _, _ = _layer(4, 4, 64, 32, 2, BF16, parallel=2)
+    out = torch.zeros(4, 64, device="cuda")
+    flat = out.view(-1)
+    flat[:8].copy_(weights.view(-1))
+    flat[16:24].view(torch.int32).copy_(ids.view(-1))
+    flat[32:40].view(torch.int32).copy_(emap)
+    for args in ((x, flat[:8].view(4, 2), ids, False, out), (x, weights, flat[16:24].view(torch.int32).view(4, 2), False, out),
+                 (x, weights, ids, False, out, flat[32:40].view(torch.int32))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            layer(*args)
