@@ -11,7 +11,8 @@ Sparse MoE experts -- the counterpart of the reference's sparse_kernel patch
                                 reference (:334-362), and routes vLLM's dense NVFP4 entry points here
 Dense NVFP4 experts with 16-bit activations (what MarlinExperts does, weights as they are in the checkpoint):
   * `make_w4a16_apply_fn`, `process_moe_layer_weight_only`   the same hook over weight_only.W4A16MoE;
-                                `patch_vllm(weight_only=True)` or B200_NVFP4_WEIGHT_ONLY=1 installs it in place of the 2:4 one
+                                `patch_vllm(weight_only=True)` or B200_NVFP4_WEIGHT_ONLY=1 installs it in place of the 2:4 one, and
+                                makes `linear_kernel_class(weight_only=True)` the first of vLLM's NVFP4 linear kernels
 Dense NVFP4 linears:
   * `Nvfp4LinearCore` / `linear_kernel_class()`   an NvFp4LinearKernel (vllm/model_executor/kernels/linear/nvfp4/
                                 base.py) whose quantizer and GEMM are this library's;
@@ -172,24 +173,41 @@ def process_moe_layer_weight_only(method, layer, original: Callable, pack_fn: Op
 
 
 _original_process_weights = None
+_patched_weight_only = False
+
+
+def _prefer_weight_only_linears() -> None:
+    """The weight-only linear kernel becomes the first that vLLM tries for a dense NVFP4 layer on CUDA."""
+    import vllm.model_executor.kernels.linear as kernels
+    table = getattr(kernels, "_POSSIBLE_NVFP4_KERNELS", {})
+    platforms = [p for p in table if getattr(p, "name", p) == "CUDA"]
+    if not platforms:
+        raise RuntimeError("vLLM's table of NVFP4 linear kernels was not found: its dense layers would quantize their activations")
+    table[platforms[0]] = [linear_kernel_class(weight_only=True), *table[platforms[0]]]
 
 
 def patch_vllm(force: bool = False, weight_only: Optional[bool] = None) -> bool:
-    """Install the hook on vLLM's ModelOptNvFp4FusedMoE and route its dense NVFP4 ops to this library.  Like the
-    reference's module it acts only when VLLM_NVFP4_SPARSE_V7=1, or B200_NVFP4_WEIGHT_ONLY=1 for experts whose weights are not
-    pruned (or force=True; weight_only chooses between the two hooks).  Idempotent."""
-    global _original_process_weights
+    """Install the hook on vLLM's ModelOptNvFp4FusedMoE and route its dense NVFP4 ops to this library; call it before the model is built.  Like
+    the reference's module it acts only when VLLM_NVFP4_SPARSE_V7=1, or B200_NVFP4_WEIGHT_ONLY=1 for experts and dense layers whose weights are
+    neither pruned nor met by quantized activations, or when the caller says so: force=True, or weight_only True or False, which chooses
+    between the two forms.  Idempotent; a second call for the other form raises."""
+    global _original_process_weights, _patched_weight_only
     asked = {name: os.environ.get(name, "0") == "1" for name in ("VLLM_NVFP4_SPARSE_V7", "B200_NVFP4_WEIGHT_ONLY")}
-    if not force and not any(asked.values()):
+    if not force and weight_only is None and not any(asked.values()):
         return False
+    if _original_process_weights is not None:
+        if weight_only not in (None, _patched_weight_only):
+            raise RuntimeError(f"vLLM is patched already, for {'weight-only' if _patched_weight_only else 'sparse 2:4'} experts")
+        return True
     if weight_only is None:
         weight_only = asked["B200_NVFP4_WEIGHT_ONLY"] and not asked["VLLM_NVFP4_SPARSE_V7"]
-    if _original_process_weights is not None:
-        return True
     from vllm.model_executor.layers.quantization.modelopt import ModelOptNvFp4FusedMoE
 
     from .torch_ops import install_into_vllm
+    if weight_only:
+        _prefer_weight_only_linears()
     _original_process_weights = ModelOptNvFp4FusedMoE.process_weights_after_loading
+    _patched_weight_only = bool(weight_only)
 
     process = process_moe_layer_weight_only if weight_only else process_moe_layer
 
@@ -198,7 +216,8 @@ def patch_vllm(force: bool = False, weight_only: Optional[bool] = None) -> bool:
 
     ModelOptNvFp4FusedMoE.process_weights_after_loading = patched
     install_into_vllm()
-    logger.info("[b200] vLLM patched: %s MoE experts and dense NVFP4 ops run on libb200nvfp4", "weight-only" if weight_only else "sparse 2:4")
+    logger.info("[b200] vLLM patched: %s and dense NVFP4 ops run on libb200nvfp4",
+                "weight-only MoE experts, weight-only linears" if weight_only else "sparse 2:4 MoE experts")
     return True
 
 
