@@ -161,14 +161,16 @@ def process_moe_layer_weight_only(method, layer, original: Callable, pack_fn: Op
         from .weight_only import pack_nvfp4_weight as pack_fn
     if device is None:
         device = src["w13_weight"].device if src["w13_weight"].is_cuda else "cuda"
-    g2 = src["w2_weight_scale_2"]
-    w13 = pack_fn(src["w13_weight"], src["w13_weight_scale"], src["w13_weight_scale_2"], gated=True, device=device)
-    w2 = pack_fn(src["w2_weight"], src["w2_weight_scale"], g2[:, 0] if g2.dim() > 1 else g2, gated=False, device=device)
+    one = lambda g: g[:, 0] if g.dim() > 1 else g
+    n_experts = src["w13_weight"].shape[0]
+    # the copies of a projection go as soon as it is packed: a layer is held twice at most
+    w13 = pack_fn(src.pop("w13_weight"), src.pop("w13_weight_scale"), src.pop("w13_weight_scale_2"), gated=True, device=device)
+    w2 = pack_fn(src.pop("w2_weight"), src.pop("w2_weight_scale"), one(src.pop("w2_weight_scale_2")), gated=False, device=device)
     experts.apply = make_apply(w13, w2)
     freed = sum(_zero_stride_stub(getattr(layer, name)) for name in _STUBBED_PARAMS if hasattr(layer, name))
     if torch.cuda.is_available():
         torch.cuda.empty_cache()
-    logger.info("[b200 weight-only] %d experts packed, %.1f MB of repacked weights released", src["w13_weight"].shape[0], freed / 1e6)
+    logger.info("[b200 weight-only] %d experts packed, %.1f MB of repacked weights released", n_experts, freed / 1e6)
     return True
 
 

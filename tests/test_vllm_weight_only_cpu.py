@@ -5,6 +5,8 @@ import types
 import pytest
 import torch
 
+from test_vllm_adapter_cpu import _fake_moe_layer
+
 
 @pytest.fixture
 def fake_vllm(monkeypatch):
@@ -112,3 +114,22 @@ def test_weight_only_linear_kernel_class(fake_vllm, monkeypatch):
     k.process_weights_after_loading(layer)
     y = k.apply_weights(layer, torch.zeros(2, 3, 32))
     assert tuple(y.shape) == (2, 3, 8) and bool((y == 2.0).all())
+
+
+def test_hook_lets_go_of_the_checkpoint_tensors_before_memory_is_given_back(monkeypatch):
+    import weakref
+    from dgx_vllm_b200 import vllm_adapter as va
+    layer, _, _ = _fake_moe_layer()
+    refs, alive = [], []
+
+    def pack(codes, scales, g, gated, device):
+        if not gated:
+            alive.append([r() is not None for r in refs])           # the first projection's, while the second one's are packed
+        refs.extend(weakref.ref(t) for t in (codes, scales, g))
+        return "packed"
+
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "empty_cache", lambda: alive.append([r() is not None for r in refs]))
+    method = types.SimpleNamespace(moe_mk=types.SimpleNamespace(fused_experts=types.SimpleNamespace(apply=None)))
+    assert va.process_moe_layer_weight_only(method, layer, lambda m, l: None, pack_fn=pack, device="cpu", make_apply=lambda a, b: None)
+    assert alive == [[False] * 3, [False] * 6]
