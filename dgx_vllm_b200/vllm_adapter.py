@@ -131,12 +131,15 @@ def make_w4a16_apply_fn(w13, w2, fused_fn: Optional[Callable] = None):
             if not layer:
                 from .weight_only import W4A16MoE
                 layer.append(W4A16MoE(w13, w2))
+            hidden_states = hidden_states.contiguous()
+            if hidden_states.data_ptr() % 16:
+                hidden_states = hidden_states.clone()
             # straight into the output's rows, where they can be written as they are
             rows = output[:hidden_states.shape[0]]
             direct = (rows.shape == hidden_states.shape and rows.is_contiguous() and rows.data_ptr() % 16 == 0
                       and rows.dtype in (torch.bfloat16, torch.float16, torch.float32)
                       and rows.untyped_storage().data_ptr() != hidden_states.untyped_storage().data_ptr())
-            result = layer[0](hidden_states.contiguous(), topk_weights, topk_ids, apply_router_weight_on_input,
+            result = layer[0](hidden_states, topk_weights, topk_ids, apply_router_weight_on_input,
                               out=rows if direct else None, expert_map=expert_map)
             if direct:
                 return output
@@ -277,8 +280,8 @@ class Nvfp4WeightOnlyLinearCore:
         x2 = x.reshape(-1, x.shape[-1])
         if self._linear is None:
             from .weight_only import w4a16_linear as linear
-            if x2.stride(-1) != 1 or x2.data_ptr() % 16 or (x2.shape[0] > 1 and x2.stride(0) % 8):
-                x2 = x2.clone(memory_format=torch.contiguous_format)          # rows of some slice that are not 16-byte aligned
+            if x2.stride(-1) != 1 or x2.data_ptr() % 16 or (x2.shape[0] > 1 and (x2.stride(0) % 8 or x2.stride(0) < x2.shape[1])):
+                x2 = x2.clone(memory_format=torch.contiguous_format)          # rows of some slice that are not 16-byte aligned, or one row many times
         else:
             linear = self._linear
         return linear(x2, layer.w4a16_weight, bias).view(*out_shape)

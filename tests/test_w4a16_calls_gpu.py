@@ -167,3 +167,37 @@ def test_results_in_the_memory_of_other_arguments_are_refused():
                  (x, weights, ids, False, out, flat[32:40].view(torch.int32))):
         with pytest.raises(RuntimeError, match="overlap"):
             layer(*args)
+
+
+def test_vllm_adapter_takes_activations_as_they_come():
+    """Rows 8 bytes off, one row many times, every other row: the operators' own alignment is the adapter's business."""
+    import types
+    from dgx_vllm_b200 import vllm_adapter as va
+    from dgx_vllm_b200.weight_only import pack_nvfp4_weight, w4a16_linear
+    codes, block = make_weight(1, 48, 64, 6)
+    w = pack_nvfp4_weight(codes[0], block[0], torch.ones(1, device="cuda"))
+    lin = types.SimpleNamespace(w4a16_weight=w, output_size_per_partition=48)
+    core = va.Nvfp4WeightOnlyLinearCore()
+    x = make_x(6, 64, 1, BF16)
+    room = torch.zeros(6 * 64 + 4, dtype=BF16, device="cuda")
+    off = room[4:].view(6, 64).copy_(x)
+    wide = torch.cat((x, x), 1).view(12, 64)
+    for given in (x, off, x[2:3].expand(6, 64), x.view(6, 1, 64).expand(6, 3, 64), wide[::2], x[0], x[:0]):
+        want = w4a16_linear(given.reshape(-1, 64).contiguous().clone(), w)
+        assert torch.equal(core.apply_weights(lin, given), want.view(*given.shape[:-1], 48))
+    layer, x, weights, ids, _, _, _ = _layer(6, 4, 64, 32, 2, BF16)
+    off = room[4:].view(6, 64).copy_(x)
+    moe = va.make_w4a16_apply_fn(*_packed(4, 64, 32))
+    for given in (x, off, torch.cat((x, x), 1)[:, :64]):
+        out = torch.full((8, 64), 5.0, dtype=BF16, device="cuda")
+        moe(out, given, None, None, weights, ids, "silu", 4, None, None, None, None, None, None, False)
+        assert torch.equal(out[:6], layer(x, weights, ids)) and bool((out[6:] == 5).all())
+
+
+def _packed(E, H, I, seed=0, M=6):
+    """The weights of _layer(M, E, H, I, ...)."""
+    from dgx_vllm_b200.weight_only import pack_nvfp4_weight
+    gen = torch.Generator().manual_seed(seed + M + E)
+    g13 = (torch.rand(E, 1, generator=gen) + 0.5).cuda() / (12.0 * H ** 0.5)
+    g2 = (torch.rand(E, generator=gen) + 0.5).cuda() / (3.0 * I ** 0.5)
+    return pack_nvfp4_weight(*make_weight(E, 2 * I, H, seed + 1), g13.squeeze(1), gated=True), pack_nvfp4_weight(*make_weight(E, H, I, seed + 2), g2)
