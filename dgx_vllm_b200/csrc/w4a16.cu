@@ -455,7 +455,7 @@ struct LinearParams {
   int* status;
 };
 
-// Shared memory behind the rings and barriers: partial sums of warps | factors' reciprocals | parts of the rows' statistics | rows in f16 | sums of a
+// Shared memory behind the rings and barriers: partial sums of warps | factors' reciprocals, the weight's factor | parts of the rows' statistics | rows in f16 | sums of a
 // cluster's items, [source block][value], of this block's share of the values
 struct LinearLayout {
   uint32_t red, inv, parts, rows, sums, bytes;
@@ -464,7 +464,7 @@ __host__ __device__ __forceinline__ LinearLayout linear_layout(int cols, int cap
   LinearLayout l;
   l.red = pad16(ring_bytes(cols) + bar_bytes(cols));
   l.inv = l.red + red_bytes(cols);
-  l.parts = pad16(l.inv + (uint32_t)cap * 4);
+  l.parts = pad16(l.inv + (uint32_t)(cap + 1) * 4);
   l.rows = l.parts + kWarps * 8;
   l.sums = l.rows + (uint32_t)cap * row_bytes;
   // strips of an item are 32 rows: each block of the cluster finishes 32 / split of them
@@ -512,14 +512,18 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
 #pragma unroll 1
   for (int i = 0; i < stages_of(kCols); ++i) fetch();
   pdl_launch_dependents();
-  const bool fits = packed_for(p.tail, p.tag);
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = fits ? 0 : kOtherSizes;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
   if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
   // rows are shifted by 16 bytes against each other: no two lanes of a load meet
   const uint32_t row_bytes = (uint32_t)((p.units + split - 1) / split) * (kUnitK * 2) + 16;
   const LinearLayout l = linear_layout(kCols, p.cap, row_bytes, split, p.per + (p.more > 0));
   float* const inv = reinterpret_cast<float*>(smem + l.inv);
-  const float g = fits ? *p.g : __int_as_float(0x7FC00000);
+  uint32_t tail = p.tag;                           // on their way with the rows
+  float given = 0.f;
+  if (threadIdx.x == kThreads - 1) {
+    tail = *p.tail;
+    given = *p.g;
+  }
   bool arrived = split == 1;
   int item = first + group;
   for (int done = first; done < last;) {
@@ -532,6 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
       staged.ask(n, k_begin, k_end, row_at);
     }
     staged.finish(k_stop, smem + l.rows, row_bytes, reinterpret_cast<float2*>(smem + l.parts), row_at, [&](int r, float v, float) { inv[r] = v; });
+    if (threadIdx.x == kThreads - 1) inv[p.cap] = packed_for(tail, p.tag) ? given : __int_as_float(0x7FC00000);
     __syncthreads();
     uint32_t col[kCols];
 #pragma unroll
@@ -589,7 +594,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
       finish_item<kCols, false>(reinterpret_cast<float*>(smem + l.red), p.log_share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb, auto) {
         const int column = c * 8 + quad * 2 + i, row = t * 16 + row8;
         if (column >= n) return true;
-        const float f = kConvert ? inv[column] : 1.f;
+        const float f = kConvert ? inv[column] : 1.f, g = inv[p.cap];
         if (split > 1) {
           // value [row of the strip] is finished by block row / (32 / split): [source][item][column][its rows]
           const int rows = 32 / split;
@@ -616,6 +621,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
     done = end;
   }
   ring.drain();
+  if (blockIdx.x == 0 && threadIdx.x == kThreads - 1 && !packed_for(tail, p.tag)) *p.status = kOtherSizes;
   if (split > 1) {
     if (!arrived) cluster_wait();
     cluster_sync_any();                            // the parts of k have arrived; they are added in their order
@@ -627,7 +633,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
       if (m >= p.M || row >= p.N) continue;
       float v = 0.f;
       for (int s = 0; s < split; ++s) v += sums[s * items * p.cap * rows + i];
-      v *= g;
+      v *= inv[p.cap];
       if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
       store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
     }
@@ -990,21 +996,23 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   }
   // the weights are on their way with the ids
   float weight[kDown ? kMaxPairs / kThreads : 1];
-  bool fits = true;
+  uint32_t tail13 = 0, tail2 = 0;
   if constexpr (kDown) {
-    fits = packed_for(p.tail13, p.tag13) && packed_for(p.tail2, p.tag2);
+    tail13 = *p.tail13;
+    tail2 = *p.tail2;
 #pragma unroll
     for (int q = 0; q < kMaxPairs / kThreads; ++q) {
       const int i = q * kThreads + threadIdx.x;
-      weight[q] = !fits ? __int_as_float(0x7FC00000) : i < p.M * p.topk && !p.weight_on_input ? p.weights[i] : 1.f;
+      weight[q] = i < p.M * p.topk && !p.weight_on_input ? p.weights[i] : 1.f;
     }
   }
   const int n_slots = find_slots(p, smem, l);
+  const bool fits = !kDown || (packed_for(tail13, p.tag13) && packed_for(tail2, p.tag2));
   if constexpr (kDown)
 #pragma unroll
     for (int q = 0; q < kMaxPairs / kThreads; ++q) {
       const int i = q * kThreads + threadIdx.x;
-      if (i < p.M * p.topk) reinterpret_cast<float*>(smem + l.weights)[i] = weight[q];
+      if (i < p.M * p.topk) reinterpret_cast<float*>(smem + l.weights)[i] = fits ? weight[q] : __int_as_float(0x7FC00000);
     }
   // Items (strip, slot) of a slot are neighbours, or (down) those of a strip
   DownItems d;

@@ -35,7 +35,7 @@ constexpr int kOtherSizes = 63;
 __host__ __device__ __forceinline__ uint32_t size_tag(int64_t N, int64_t K, int gated) {
   return (uint32_t)((uint64_t)N * 40503u + (uint64_t)(K / 16) * 30011u + (gated ? 0x5555u : 0u)) & 0xFFFFu;
 }
-__device__ __forceinline__ bool packed_for(const uint32_t* tail, uint32_t tag) { return (*tail & 0xFFFFu) == tag; }
+__device__ __forceinline__ bool packed_for(uint32_t tail, uint32_t tag) { return (tail & 0xFFFFu) == tag; }
 __device__ __forceinline__ float peak_of(uint32_t word) { return __uint_as_float(word & 0xFFFF0000u); }
 
 __host__ __device__ __forceinline__ int64_t strips_of(int64_t rows) { return (rows + kUnitRows - 1) / kUnitRows; }      // of 32 rows

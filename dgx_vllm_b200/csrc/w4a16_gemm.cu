@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   const uint32_t tmem = lds32(tmem_ptr);
   pdl_wait();
   pdl_launch_dependents();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *status = packed_for(p.tail, p.tag) ? 0 : kOtherSizes;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
   if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
 
   if (warp == 0) {
@@ -344,7 +344,11 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   // ---------------------------------------------------------------------- epilogue: a lane is a row of the weight, a column a token
   const int quarter = warp & 3;
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-  auto factor = [&]() { return packed_for(p.tail, p.tag) ? *p.g : __int_as_float(0x7FC00000); };
+  auto factor = [&]() {
+    const uint32_t tail = *p.tail;
+    const float g = *p.g;
+    return packed_for(tail, p.tag) ? g : __int_as_float(0x7FC00000);
+  };
   // columns from, from + by, ... of a tile of n tokens, 32 at a time
   auto write_columns = [&](uint32_t acc, int row, int token0, int n, int from, int by, float g, bool more) {
     const float bias = p.bias != nullptr && row < p.N ? load_value(p.bias, p.bias_dtype, row) : 0.f;
@@ -380,6 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       }
     }
   };
+  if (blockIdx.x == 0 && threadIdx.x == 0 && !packed_for(*p.tail, p.tag)) *status = kOtherSizes;
   if (p.accs > 1) {
     // several tiles: four warps, while the others go on
     if (warp >= 2 && warp < kFirstDecode) {
