@@ -239,27 +239,26 @@ inline int least_share(int out_dtype, int units) {
   return share;
 }
 
-// A run of items is done in phases: rounds of an item a warp (or a group of the least size), then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
+// A run of items is done in phases: rounds of an item a warp, then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
 // size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 0.3 us more of
 // its 14, for the longer way to a warp's first weights.
 // share: log2 of the warps of a group.  The plan has that of each number of items under a round, four bits each.
 struct Phase {
   int count, share;
 };
-__device__ __forceinline__ Phase next_phase(int rest, uint64_t plan, int least) {
-  const int groups = kWarps >> least;
-  if (rest >= groups) return {rest & -groups, least};
+__device__ __forceinline__ Phase next_phase(int rest, uint64_t plan) {
+  if (rest >= kWarps) return {rest & -kWarps, 0};
   const int share = (int)(plan >> (rest * 4)) & 15, most = kWarps >> share;
   return {rest < most ? rest : most, share};
 }
-inline uint64_t phase_plan(int units, int least) {
+inline uint64_t phase_plan(int units) {
   static_assert(kWarps == 16, "a plan has 16 numbers of four bits");
   uint64_t plan = 0;
   float cost[kWarps] = {};
   for (int rest = 1; rest < kWarps; ++rest) {
-    int best = least;
+    int best = 0;
     cost[rest] = 1e30f;
-    for (int s = least; s < 5 && (s == least || (1 << s) <= units); ++s) {
+    for (int s = 0; s < 5 && (1 << s) <= units; ++s) {
       const int count = std::min(rest, kWarps >> s);
       const float all = share_cost(count, units, s) + cost[rest - count] + 400.f;
       if (all < cost[rest]) cost[rest] = all, best = s;
@@ -267,6 +266,30 @@ inline uint64_t phase_plan(int units, int least) {
     plan |= (uint64_t)best << (rest * 4);
   }
   return plan;
+}
+
+// An f32 result's chains (kWarpChain): the sums of one to those of the chains before it, in the room where warps exchange theirs, and all of them back.
+template <int kCols>
+__device__ __forceinline__ void put_aside(float* own, bool first, float (&acc)[2][kCols][4]) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float& sum = own[((t * kCols + c) * 4 + j) * 32];
+        sum = first ? acc[t][c][j] : sum + acc[t][c][j];
+        acc[t][c][j] = 0.f;
+      }
+}
+template <int kCols>
+__device__ __forceinline__ void take_back(const float* own, float (&acc)[2][kCols][4]) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int c = 0; c < kCols; ++c)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[t][c][j] += own[((t * kCols + c) * 4 + j) * 32];
 }
 
 // Sums of the warps that share an item, [warp][tile][column of eight][j][lane]: each warp adds up some of them, in the order of k, and finishes them.
@@ -746,7 +769,6 @@ struct MoeParams {
   int strips, units;
   int cap, rows;              // columns of a slot; rows that there is room for
   uint64_t phases;
-  int least;                  // log2 of the warps of an item, at least
   int split;                  // whole strips: blocks of a cluster, which share the slots of a strip
   float rcp_topk, rcp_grid, rcp_strips;
   const int32_t* ids;         // [M, topk]
@@ -972,8 +994,8 @@ enum Projection { kGateUp, kDownItems, kDownStrips };       // kDownStrips: whol
 // Bound by the copies of the experts that the routing reaches: 32 tokens, ten of 512 experts, H=2048 I=512, take 91-94 us, gate/up 46 of them at 6.1 TB/s and down 26 at
 // 5.3; the rest is finding the slots (2 us), rows and first units (3), the down projection's start (3) and the strips' last sums (4).  128 tokens 180-187.  Two
 // launches: every value of the first projection is needed by the second, which finds its slots and asks for its first weights while the first one ends.
-// XT: type of the activations (gate/up); kCols: columns of eight
-template <typename XT, int kMode, int kCols>
+// XT: type of the activations (gate/up); kCols: columns of eight; kChains: sums of more than a chain, for an f32 result (as a choice at run time it cost the others 5 to 9 %)
+template <typename XT, int kMode, int kCols, bool kChains>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
   constexpr bool kDown = kMode != kGateUp, kWhole = kMode == kDownStrips;
@@ -1059,7 +1081,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
           int n_rows;
           turn_end = min(last, turn_of(quotient(phase_end, fast, rcp_fast), n_rows) * fast);
         }
-        const Phase phase = next_phase(turn_end - phase_end, p.phases, p.least);
+        const Phase phase = next_phase(turn_end - phase_end, p.phases);
         ahead_share = phase.share;
         ahead = phase_end + (warp >> ahead_share);
         phase_end += phase.count;
@@ -1075,6 +1097,22 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     --ahead_left;
   };
   float* const red = reinterpret_cast<float*>(smem + l.red);
+  // units(from, to): some of an item's part; their sums in acc
+  auto in_chains = [&](const Part& part, float (&acc)[2][kCols][4], auto&& units) {
+    if constexpr (kChains) {
+      float* const own = red + warp * (2 * kCols * 4 * 32) + lane;
+      for (int k = part.k_first, rest = part.n_units;;) {
+        const int n = min(rest, kWarpChain);
+        units(k, k + n);
+        k += n;
+        if ((rest -= n) == 0) break;
+        put_aside<kCols>(own, k == part.k_first + kWarpChain, acc);
+      }
+      if (part.n_units > kWarpChain) take_back<kCols>(own, acc);
+    } else {
+      units(part.k_first, part.k_first + part.n_units);
+    }
+  };
 
   if constexpr (!kDown) {
     if (blockIdx.x == 0) {
@@ -1121,7 +1159,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       }
       __syncthreads();
       while (done < end) {
-        const Phase phase = next_phase(end - done, p.phases, p.least);
+        const Phase phase = next_phase(end - done, p.phases);
         const Part part = part_of(phase.share);
         for (int item = done + part.group; item < done + phase.count; item += kWarps >> phase.share) {
           const int hi = quotient(item, fast, rcp_fast), strip = item - hi * fast;
@@ -1134,14 +1172,16 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
             col[c] = base + l.rows + (s.y - row0 + (i < n ? i : 0)) * row_bytes + quad * 32;
           }
           float acc[2][kCols][4] = {};
+          in_chains(part, acc, [&](int k, int end) {
 #pragma unroll 1
-          for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
-            uint32_t b[2][kCols][8];
-            staged_columns<kCols>(col, k * (kUnitK * 2), b);
-            multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
-            ring.advance();
-            if (ring.ok) fetch();
-          }
+            for (; k < end; ++k) {
+              uint32_t b[2][kCols][8];
+              staged_columns<kCols>(col, k * (kUnitK * 2), b);
+              multiply_unit<kCols>(ring.wait(p.status), lane, chunk, b, acc);
+              ring.advance();
+              if (ring.ok) fetch();
+            }
+          });
           const float g_gate = p.g[2 * e], g_up = p.g[2 * e + 1];
           finish_item<kCols, false>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float gate, float up, auto again) {
             // a run: eight rows of a tile, a column; I is a multiple of 16, so that it is whole
@@ -1203,7 +1243,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
       return;
     }
     for (int done = first; done < last;) {
-      const Phase phase = next_phase(last - done, p.phases, p.least);
+      const Phase phase = next_phase(last - done, p.phases);
       const Part part = part_of(phase.share);
       for (int item = done + part.group; item < done + phase.count; item += kWarps >> phase.share) {
         const int strip_nth = quotient(item, fast, rcp_fast);
@@ -1267,39 +1307,40 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
             set |= __shfl_xor_sync(0xffffffffu, set, 1);
             levels[c] = set | __shfl_xor_sync(0xffffffffu, set, 2);
           }
+          in_chains(part, acc, [&](int k, int end) {
 #pragma unroll 1
-          for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
-            load_columns(k, b);
+            for (; k < end; ++k) {
+              load_columns(k, b);
 #pragma unroll
-            for (int c = 0; c < kCols; ++c) {
-              const uint32_t w = levels_at(k, c);
+              for (int c = 0; c < kCols; ++c) {
+                const uint32_t w = levels_at(k, c);
 #pragma unroll
-              for (int run = 0; run < 4; ++run)      // levels above the pair's lowest; values that are zeros stay so
-                level_down(&b[run >> 1][c][(run & 1) * 4], odd, __ffs((int)((w >> (8 * run)) & 0xFFu)) - __ffs((int)levels[c]));
+                for (int run = 0; run < 4; ++run)    // levels above the pair's lowest; values that are zeros stay so
+                  level_down(&b[run >> 1][c][(run & 1) * 4], odd, __ffs((int)((w >> (8 * run)) & 0xFFu)) - __ffs((int)levels[c]));
+              }
+              multiply();
             }
-            multiply();
-          }
+          });
           scale_sums([&](int c) { return max(__ffs((int)__shfl_sync(0xffffffffu, levels[c], quad * 8)) - 1, 0); });
         } else {
-          if constexpr (kCols == 1) {                // a unit ahead, as far as there are registers
-            load_columns(part.k_first, b);
+          if constexpr (kCols == 1) load_columns(part.k_first, b);       // a unit ahead, as far as there are registers
+          in_chains(part, acc, [&](int k, int end) {
 #pragma unroll 1
-            for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
-              uint32_t after[2][kCols][8];
-              load_columns(k + 1, after);
-              multiply();
+            for (; k < end; ++k) {
+              if constexpr (kCols == 1) {
+                uint32_t after[2][kCols][8];
+                load_columns(k + 1, after);
+                multiply();
 #pragma unroll
-              for (int half = 0; half < 2; ++half)
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) b[half][0][j] = after[half][0][j];
+                  for (int j = 0; j < 8; ++j) b[half][0][j] = after[half][0][j];
+              } else {
+                load_columns(k, b);
+                multiply();
+              }
             }
-          } else {
-#pragma unroll 1
-            for (int k = part.k_first; k < part.k_first + part.n_units; ++k) {
-              load_columns(k, b);
-              multiply();
-            }
-          }
+          });
           scale_sums([](int) { return 0; });
         }
         finish_item<kCols, true>(red, phase.share, part.in_group, part.group, lane, acc, [&](int t, int c, int i, float va, float vb, auto) {
@@ -1443,12 +1484,12 @@ double slots_of(const MoeParams& p, int cap) {
 }
 
 // What a launch would be, without launching; a status other than success where there is no room for it
-template <typename XT, int kMode, int kCols>
+template <typename XT, int kMode, int kCols, bool kChains>
 int plan_moe(const MoeParams& given, MoePlan& plan) {
   static std::once_flag once[64];
   static bool ready[64];
   static ResidentClusters counts[kMaxSplit + 1][64];
-  constexpr auto kernel = w4a16_moe_kernel<XT, kMode, kCols>;
+  constexpr auto kernel = w4a16_moe_kernel<XT, kMode, kCols, kChains>;
   if (!allow_smem(kernel, once, ready)) return B200FP4_STATUS_EXECUTION_FAILED;
   MoeParams p = given;
   const int pairs = p.M * p.topk, sms = sm_count();
@@ -1489,8 +1530,7 @@ int plan_moe(const MoeParams& given, MoePlan& plan) {
   plan.smem = moe_layout(kCols, pairs, p.E, p.cap, p.rows, row_bytes, strips).bytes;
   if (plan.smem > kSmemMost) return B200FP4_STATUS_NOT_SUPPORTED;
   plan.items = items;
-  p.least = least_share(p.out_dtype, p.units);
-  p.phases = phase_plan(p.units, p.least);
+  p.phases = phase_plan(p.units);
   p.rcp_topk = 1.f / (float)p.topk;
   p.rcp_grid = 1.f / (float)plan.grid;
   p.rcp_strips = 1.f / (float)p.strips;
@@ -1498,9 +1538,9 @@ int plan_moe(const MoeParams& given, MoePlan& plan) {
   return B200FP4_STATUS_SUCCESS;
 }
 
-template <typename XT, int kMode, int kCols>
+template <typename XT, int kMode, int kCols, bool kChains>
 int launch_moe(const MoePlan& plan, cudaStream_t st) {
-  if (launch_pdl_cluster(plan.p.split, w4a16_moe_kernel<XT, kMode, kCols>, dim3(plan.grid), dim3(kThreads), plan.smem, st, plan.p) != cudaSuccess) {
+  if (launch_pdl_cluster(plan.p.split, w4a16_moe_kernel<XT, kMode, kCols, kChains>, dim3(plan.grid), dim3(kThreads), plan.smem, st, plan.p) != cudaSuccess) {
     cudaGetLastError();
     return B200FP4_STATUS_EXECUTION_FAILED;
   }
@@ -1508,35 +1548,41 @@ int launch_moe(const MoePlan& plan, cudaStream_t st) {
 }
 
 // Both projections are planned before the first is launched.
-template <typename T, int kUpCols, int kMode, int kDownCols>
+template <typename T, int kUpCols, int kMode, int kDownCols, bool kChains>
 int launch_both(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
   MoePlan u, d;
-  int rc = plan_moe<T, kGateUp, kUpCols>(up, u);
-  if (rc == B200FP4_STATUS_SUCCESS) rc = plan_moe<__half, kMode, kDownCols>(down, d);
+  int rc = plan_moe<T, kGateUp, kUpCols, kChains>(up, u);
+  if (rc == B200FP4_STATUS_SUCCESS) rc = plan_moe<__half, kMode, kDownCols, kChains>(down, d);
   if (rc != B200FP4_STATUS_SUCCESS) return rc;
-  rc = launch_moe<T, kGateUp, kUpCols>(u, st);
-  return rc == B200FP4_STATUS_SUCCESS ? launch_moe<__half, kMode, kDownCols>(d, st) : rc;
+  rc = launch_moe<T, kGateUp, kUpCols, kChains>(u, st);
+  return rc == B200FP4_STATUS_SUCCESS ? launch_moe<__half, kMode, kDownCols, kChains>(d, st) : rc;
 }
 
-template <typename T>
+template <typename T, bool kChains>
 int launch_layer_of(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
   // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  One / two of them in both
   // projections, us, eight experts of 4096, H = 4096, bf16: 7.25 pairs an expert 68 / 73, nine 78 / 75, eleven 87 / 78; 64 experts of 768, H = 2048: eight 59.7 / 59.0, twelve
   // 77 / 69.  Below seven few experts have more pairs than one column of eight holds.
   const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
   if (each <= 7) {
-    if (each > 3.5) return launch_both<T, 1, kDownItems, 2>(up, down, st);
+    if (each > 3.5) return launch_both<T, 1, kDownItems, 2, kChains>(up, down, st);
     // Whole strips: nothing goes through memory and no block waits for a counter, 1.4 us less for one token (H = 2048, ten experts of 512: 14.0 us against
     // 15.4), but the blocks' shares are less even.  A block reads 36 units in some 2 us: from there on the items are spread over all blocks (12 tokens, eight experts
     // of 4096 and H = 4096, a surplus of 41 units: 53 us against 57).
     MoePlan strips;
-    if (plan_moe<__half, kDownStrips, 1>(down, strips) == B200FP4_STATUS_SUCCESS &&
+    if (plan_moe<__half, kDownStrips, 1, kChains>(down, strips) == B200FP4_STATUS_SUCCESS &&
         (strips.items - slots_of(down, strips.p.cap) * down.strips / sm_count()) * down.units < 36)
-      return launch_both<T, 1, kDownStrips, 1>(up, down, st);
-    return launch_both<T, 1, kDownItems, 1>(up, down, st);
+      return launch_both<T, 1, kDownStrips, 1, kChains>(up, down, st);
+    return launch_both<T, 1, kDownItems, 1, kChains>(up, down, st);
   }
-  return launch_both<T, 2, kDownItems, 2>(up, down, st);
+  return launch_both<T, 2, kDownItems, 2, kChains>(up, down, st);
 }
+template <typename T>
+int launch_layer(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
+  const bool chains = down.out_dtype == B200FP4_DTYPE_F32 && std::max(up.units, down.units) > kWarpChain;
+  return chains ? launch_layer_of<T, true>(up, down, st) : launch_layer_of<T, false>(up, down, st);
+}
+
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }
 bool is_16bit(int dtype) { return dtype == B200FP4_DTYPE_F16 || dtype == B200FP4_DTYPE_BF16; }
 bool is_dtype(int dtype) { return is_16bit(dtype) || dtype == B200FP4_DTYPE_F32; }
@@ -1688,7 +1734,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     d.K = (int)I;
     d.strips = (int)w4::strips_of(H);
     d.units = (int)w4::units_of(I);
-    const int rc = h_dtype == B200FP4_DTYPE_BF16 ? launch_layer_of<__nv_bfloat16>(p, d, st) : launch_layer_of<__half>(p, d, st);
+    const int rc = h_dtype == B200FP4_DTYPE_BF16 ? launch_layer<__nv_bfloat16>(p, d, st) : launch_layer<__half>(p, d, st);
     if (rc != B200FP4_STATUS_SUCCESS) return rc;
   }
   return B200FP4_STATUS_SUCCESS;
