@@ -1560,22 +1560,21 @@ int launch_both(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
 
 template <typename T, bool kChains>
 int launch_layer_of(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
-  // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit is read again.  One / two of them in both
-  // projections, us, eight experts of 4096, H = 4096, bf16: 7.25 pairs an expert 68 / 73, nine 78 / 75, eleven 87 / 78; 64 experts of 768, H = 2048: eight 59.7 / 59.0, twelve
-  // 77 / 69.  Below seven few experts have more pairs than one column of eight holds.
+  // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit (eight; four in the down projection, where a pair
+  // has two columns) is read again, mostly from L2.  Columns of gate/up and of down, us, by pairs an expert, bf16; eight experts of 4096, H = 4096: 7.25 pairs 1/1 83.4,
+  // 1/2 86.9, 2/1 86.4, 2/2 90.2; 8.5 89.0 / 90.8 / 89.4 / 91.3; 9 94.1 / 96.1 / 93.6 / 95.5; 10 96.3 / 96.5 / 95.7 / 96.1; 11 106 / 104 / 100.6 / 99.8.  64 experts of 768,
+  // H = 2048: four 51.4 / 56.2 / 60.8 / 69.9; 8.5 74.3 / 75.5 / 75.3 / 81.1; 9 78.3 / 78.0 / 76.6 / 81.3; 10 83.9 / 84.8 / 79.8 / 82.7; 12 93.6 / 92.0 / 90.8 / 90.1.
   const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
-  if (each <= 7) {
-    if (each > 3.5) return launch_both<T, 1, kDownItems, 2, kChains>(up, down, st);
-    // Whole strips: nothing goes through memory and no block waits for a counter, 1.4 us less for one token (H = 2048, ten experts of 512: 14.0 us against
-    // 15.4), but the blocks' shares are less even.  A block reads 36 units in some 2 us: from there on the items are spread over all blocks (12 tokens, eight experts
-    // of 4096 and H = 4096, a surplus of 41 units: 53 us against 57).
-    MoePlan strips;
-    if (plan_moe<__half, kDownStrips, 1, kChains>(down, strips) == B200FP4_STATUS_SUCCESS &&
-        (strips.items - slots_of(down, strips.p.cap) * down.strips / sm_count()) * down.units < 36)
-      return launch_both<T, 1, kDownStrips, 1, kChains>(up, down, st);
-    return launch_both<T, 1, kDownItems, 1, kChains>(up, down, st);
-  }
-  return launch_both<T, 2, kDownItems, 2, kChains>(up, down, st);
+  if (each > 10.5) return launch_both<T, 2, kDownItems, 2, kChains>(up, down, st);
+  if (each > 8.75) return launch_both<T, 2, kDownItems, 1, kChains>(up, down, st);
+  // Whole strips: nothing goes through memory and no block waits for a counter, 1.6 us less for one token (H = 2048, ten experts of 512: 14.9 against 16.5), but the
+  // blocks' shares are less even.  Items / whole strips, us, by the units that the busiest block has more than its share, eight experts of 4096, H = 4096: 32 units (3 tokens)
+  // 38.7 / 37.6, 41 (4) 46.9 / 44.4, 42 (12) 56.2 / 56.3, 43 (20) 65.5 / 66.4, 52 (24) 70.8 / 71.4, 79 (29) 83.2 / 84.9; eight of 8192, H = 5120, 6 tokens, 185: 90.0 / 97.9.
+  MoePlan strips;
+  if (plan_moe<__half, kDownStrips, 1, kChains>(down, strips) == B200FP4_STATUS_SUCCESS &&
+      (strips.items - slots_of(down, strips.p.cap) * down.strips / sm_count()) * down.units < 43)
+    return launch_both<T, 1, kDownStrips, 1, kChains>(up, down, st);
+  return launch_both<T, 1, kDownItems, 1, kChains>(up, down, st);
 }
 template <typename T>
 int launch_layer(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
