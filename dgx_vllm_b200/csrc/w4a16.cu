@@ -1579,7 +1579,10 @@ int launch_layer_of(const MoeParams& up, const MoeParams& down, cudaStream_t st)
 template <typename T>
 int launch_layer(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
   const bool chains = down.out_dtype == B200FP4_DTYPE_F32 && std::max(up.units, down.units) > kWarpChain;
-  return chains ? launch_layer_of<T, true>(up, down, st) : launch_layer_of<T, false>(up, down, st);
+  const int rc = chains ? launch_layer_of<T, true>(up, down, st) : launch_layer_of<T, false>(up, down, st);
+  if (rc != B200FP4_STATUS_NOT_SUPPORTED) return rc;
+  // Long rows: rings and sums for two columns leave more room than those for one.  So a last turn of few pairs is never refused where the full ones before it were not.
+  return chains ? launch_both<T, 2, kDownItems, 2, true>(up, down, st) : launch_both<T, 2, kDownItems, 2, false>(up, down, st);
 }
 
 bool fits_int(int64_t v) { return v >= 0 && v <= 0x7FFFFFFF; }

@@ -505,7 +505,7 @@ B200FP4_API int b200fp4_w4a16_linear(const void* x, int x_dtype, int64_t ldx, co
 /* One mixture-of-experts layer: gate/up projection -> SiLU(gate)*up -> down projection -> router-weighted sum, in two launches for up
  * to 2048 (token, expert) pairs; more are done in turns.  Arguments as b200fp4_fused_sparse_moe, with w13 [E, 2I, H] packed gated and
  * w2 [E, H, I] packed, w13_g [E][gate rows, up rows] (8-byte aligned), w2_g [E]; H and I multiples of 16, H as long as a row fits in shared
- * memory (some 50,000), E up to 4096, topk up to 2048.  out may be hidden (of the same type) or other memory.  Pairs whose expert (after
+ * memory beside the routing (59,000 for few pairs, 43,000 for 2048 of them, 31,000 where there are thousands of experts too), E up to 4096, topk up to 2048.  out may be hidden (of the same type) or other memory.  Pairs whose expert (after
  * expert_map) is outside [0, E) add nothing; a token without any gives zeros.  flags: B200FP4_MOE_ROUTER_WEIGHT_ON_INPUT or 0.  Between the
  * projections a value is the sum of two f16, to f32's precision whatever its size.  Results do not depend on the order in which blocks run.  The workspace is a call's own until the call is done. */
 B200FP4_API size_t b200fp4_w4a16_moe_workspace_bytes(int64_t M, int64_t topk, int64_t H, int64_t I);

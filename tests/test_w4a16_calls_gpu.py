@@ -201,3 +201,13 @@ def _packed(E, H, I, seed=0, M=6):
     g13 = (torch.rand(E, 1, generator=gen) + 0.5).cuda() / (12.0 * H ** 0.5)
     g2 = (torch.rand(E, generator=gen) + 0.5).cuda() / (3.0 * I ** 0.5)
     return pack_nvfp4_weight(*make_weight(E, 2 * I, H, seed + 1), g13.squeeze(1), gated=True), pack_nvfp4_weight(*make_weight(E, H, I, seed + 2), g2)
+
+
+@pytest.mark.parametrize("M,E,H,topk", [(381, 128, 43008, 8), (256, 256, 40000, 8), (1030, 8, 44032, 2), (3, 4, 59904, 2)])
+def test_layer_of_long_rows_in_turns(M, E, H, topk):
+    """Rows that fit beside the sums of two columns only, in full turns and in a last one of fewer pairs."""
+    from test_w4a16_gpu import _check
+    layer, x, weights, ids, emap, W13, W2 = _layer(M, E, H, 16, topk, BF16)
+    out = layer(x, weights, ids)
+    some = torch.tensor(sorted({0, 1, M // 2, min(255, M - 1), max(0, M - 125), M - 2, M - 1}), device="cuda")
+    _check(out[some], x[some], weights[some], ids[some], emap, W13, W2)
