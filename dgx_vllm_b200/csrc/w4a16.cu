@@ -478,7 +478,7 @@ struct LinearParams {
   int* status;
 };
 
-// Shared memory behind the rings and barriers: partial sums of warps | factors' reciprocals, the weight's factor | parts of the rows' statistics | rows in f16 | sums of a
+// Shared memory behind the rings and barriers: partial sums of warps | factors' reciprocals | parts of the rows' statistics | rows in f16 | sums of a
 // cluster's items, [source block][value], of this block's share of the values
 struct LinearLayout {
   uint32_t red, inv, parts, rows, sums, bytes;
@@ -487,7 +487,7 @@ __host__ __device__ __forceinline__ LinearLayout linear_layout(int cols, int cap
   LinearLayout l;
   l.red = pad16(ring_bytes(cols) + bar_bytes(cols));
   l.inv = l.red + red_bytes(cols);
-  l.parts = pad16(l.inv + (uint32_t)(cap + 1) * 4);
+  l.parts = pad16(l.inv + (uint32_t)cap * 4);
   l.rows = l.parts + kWarps * 8;
   l.sums = l.rows + (uint32_t)cap * row_bytes;
   // strips of an item are 32 rows: each block of the cluster finishes 32 / split of them
@@ -528,25 +528,31 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   };
   const int k_begin = unit_first * kUnitK, k_stop = (unit_first + own_units) * kUnitK, k_end = min(p.K, k_stop);
   StagedRows<XT, false> staged;
-  int m0 = first / p.strips * p.cap;
+  const int first_slot = first / p.strips;
+  int m0 = first_slot * p.cap;
   auto row_at = [&](int r) { return static_cast<const XT*>(p.x) + (m0 + r) * p.ldx; };
   pdl_wait();
   staged.ask(min(p.cap, p.M - m0), k_begin, k_end, row_at);
 #pragma unroll 1
   for (int i = 0; i < stages_of(kCols); ++i) fetch();
   pdl_launch_dependents();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *p.status = 0;
+  const bool reports = blockIdx.x == gridDim.x - split && threadIdx.x == 0;       // this block has the last item of all
+  if (reports) *p.status = 0;
   if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
   // rows are shifted by 16 bytes against each other: no two lanes of a load meet
   const uint32_t row_bytes = (uint32_t)((p.units + split - 1) / split) * (kUnitK * 2) + 16;
   const LinearLayout l = linear_layout(kCols, p.cap, row_bytes, split, p.per + (p.more > 0));
   float* const inv = reinterpret_cast<float*>(smem + l.inv);
-  uint32_t tail = p.tag;                           // on their way with the rows
-  float given = 0.f;
-  if (threadIdx.x == kThreads - 1) {
-    tail = *p.tail;
-    given = *p.g;
-  }
+  const float g = *p.g;
+  // The word behind the units is read by the blocks that read the last strip, next to it: as a page of its own for all of them it cost a tenth of one token's time.  It is looked
+  // at when the strip is done.
+  const uint32_t tail = last >= (first_slot + 1) * p.strips ? *p.tail : p.tag;
+  auto factor = [&](int strip) {
+    if (strip != p.strips - 1) return g;
+    uint32_t word = tail;
+    asm volatile("" : "+r"(word));
+    return packed_for(word, p.tag) ? g : __int_as_float(0x7FC00000);
+  };
   bool arrived = split == 1;
   int item = first + group;
   for (int done = first; done < last;) {
@@ -559,7 +565,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
       staged.ask(n, k_begin, k_end, row_at);
     }
     staged.finish(k_stop, smem + l.rows, row_bytes, reinterpret_cast<float2*>(smem + l.parts), row_at, [&](int r, float v, float) { inv[r] = v; });
-    if (threadIdx.x == kThreads - 1) inv[p.cap] = packed_for(tail, p.tag) ? given : __int_as_float(0x7FC00000);
     __syncthreads();
     uint32_t col[kCols];
 #pragma unroll
@@ -617,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
       finish_item<kCols, false>(reinterpret_cast<float*>(smem + l.red), p.log_share, in_group, group, lane, acc, [&](int t, int c, int i, float va, float vb, auto) {
         const int column = c * 8 + quad * 2 + i, row = t * 16 + row8;
         if (column >= n) return true;
-        const float f = kConvert ? inv[column] : 1.f, g = inv[p.cap];
+        const float f = kConvert ? inv[column] : 1.f;
         if (split > 1) {
           // value [row of the strip] is finished by block row / (32 / split): [source][item][column][its rows]
           const int rows = 32 / split;
@@ -628,11 +633,12 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(map_to_cta(to, owner)), "f"((h ? vb : va) * f) : "memory");
           }
         } else {
+          const float gf = factor(strip);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int at = strip * 32 + row + h * 8;
             if (at < p.N) {
-              float v = (h ? vb : va) * f * g;
+              float v = (h ? vb : va) * f * gf;
               if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, at);
               store_value(p.out, p.out_dtype, (size_t)(m0 + column) * p.N + at, v);
             }
@@ -644,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
     done = end;
   }
   ring.drain();
-  if (blockIdx.x == 0 && threadIdx.x == kThreads - 1 && !packed_for(tail, p.tag)) *p.status = kOtherSizes;
+  if (reports && !packed_for(tail, p.tag)) *p.status = kOtherSizes;
   if (split > 1) {
     if (!arrived) cluster_wait();
     cluster_sync_any();                            // the parts of k have arrived; they are added in their order
@@ -656,7 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
       if (m >= p.M || row >= p.N) continue;
       float v = 0.f;
       for (int s = 0; s < split; ++s) v += sums[s * items * p.cap * rows + i];
-      v *= inv[p.cap];
+      v *= factor(it - slot * p.strips);
       if (p.bias != nullptr) v += load_value(p.bias, p.bias_dtype, row);
       store_value(p.out, p.out_dtype, (size_t)m * p.N + row, v);
     }
@@ -763,7 +769,7 @@ struct MoeParams {
   const uint8_t* packed;
   const float* g;             // [E]; gate/up [E][gate, up]
   const uint2* peaks;         // gate/up: [E][gate, up]
-  const uint32_t *tail13, *tail2;        // down: of both projections
+  const uint32_t *tail13, *tail2;        // behind the units of both projections
   uint32_t tag13, tag2;
   int M, N, K;
   int strips, units;
@@ -779,7 +785,7 @@ struct MoeParams {
   __half* act;                // gate/up out: for each pair, rows act_row(I) apart, [part][I] and the levels of its runs (run_at)
   float* act_inv;             // [pair]: the reciprocal of the factor that brought its row of act into f16's range
   float* y;                   // down: [pair][N]
-  uint32_t* leveled;          // `call` of the last call with a run above level 0
+  uint32_t* said;             // by gate/up: `call` of the last call with a run above level 0 | whether the weights have the call's sizes
   uint32_t call;
   int* counters;              // [strips of down]
   int n_counters;
@@ -1018,23 +1024,27 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
   }
   // the weights are on their way with the ids
   float weight[kDown ? kMaxPairs / kThreads : 1];
-  uint32_t tail13 = 0, tail2 = 0;
-  if constexpr (kDown) {
-    tail13 = *p.tail13;
-    tail2 = *p.tail2;
+  if constexpr (kDown)
 #pragma unroll
     for (int q = 0; q < kMaxPairs / kThreads; ++q) {
       const int i = q * kThreads + threadIdx.x;
       weight[q] = i < p.M * p.topk && !p.weight_on_input ? p.weights[i] : 1.f;
     }
-  }
+  // one thread of gate/up compares the weights' sizes with the call's
+  const bool compares = !kDown && blockIdx.x == 0 && threadIdx.x == kThreads - 1;
+  const uint32_t tail13 = compares ? *p.tail13 : 0, tail2 = compares ? *p.tail2 : 0;
   const int n_slots = find_slots(p, smem, l);
-  const bool fits = !kDown || (packed_for(tail13, p.tag13) && packed_for(tail2, p.tag2));
+  if (compares) {
+    const bool fits = packed_for(tail13, p.tag13) && packed_for(tail2, p.tag2);
+    p.said[1] = fits;
+    if (!fits) *p.status = kOtherSizes;
+    else if (p.clear_status) *p.status = 0;
+  }
   if constexpr (kDown)
 #pragma unroll
     for (int q = 0; q < kMaxPairs / kThreads; ++q) {
       const int i = q * kThreads + threadIdx.x;
-      if (i < p.M * p.topk) reinterpret_cast<float*>(smem + l.weights)[i] = fits ? weight[q] : __int_as_float(0x7FC00000);
+      if (i < p.M * p.topk) reinterpret_cast<float*>(smem + l.weights)[i] = weight[q];
     }
   // Items (strip, slot) of a slot are neighbours, or (down) those of a strip
   DownItems d;
@@ -1116,7 +1126,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
 
   if constexpr (!kDown) {
     if (blockIdx.x == 0) {
-      if (p.clear_status && threadIdx.x == 0) *p.status = 0;
       for (int i = threadIdx.x; i < p.n_counters; i += kThreads) p.counters[i] = 0;
     }
     RowStat* const stats = reinterpret_cast<RowStat*>(smem + l.stats);
@@ -1205,7 +1214,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
               const int k = min(max(under + kLevel - 1, 0) / kLevel, min(kLevels - 1, (126 - power) / kLevel));
               scale = pow2(power + k * kLevel);
               level = top != 0 ? 1u << k : 0u;
-              if (level > 1 && here) *p.leveled = p.call;
+              if (level > 1 && here) p.said[0] = p.call;
             } else {
               // four runs a warp: level 0 where one of a run's values is large enough
               large = __ballot_sync(0xffffffffu, !here || !(fabsf(v) * scale < kLeast));
@@ -1235,8 +1244,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
     pdl_wait();
     pdl_launch_dependents();
     if (kWhole && p.split > 1) cluster_wait();
-    const bool leveled = *p.leveled == p.call;       // otherwise every run of every pair is at level 0, and nobody looks
-    if (!fits && blockIdx.x == 0 && threadIdx.x == 0) *p.status = kOtherSizes;
+    const uint2 said = *reinterpret_cast<const uint2*>(p.said);
+    const bool leveled = said.x == p.call;           // otherwise every run of every pair is at level 0, and nobody looks
+    if (__builtin_expect(said.y == 0, 0))
+      for (int i = threadIdx.x; i < p.M * p.topk; i += kThreads) reinterpret_cast<float*>(smem + l.weights)[i] = __int_as_float(0x7FC00000);
     if (n_slots == 0) {
       for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < (size_t)p.M * p.N; i += (size_t)gridDim.x * kThreads)
         store_value(p.out, p.out_dtype, i, 0.f);
@@ -1600,7 +1611,7 @@ size_t unit_bytes(int64_t E, int64_t N, int64_t K, int gated) {
 int64_t turn_of(int64_t M, int64_t topk) { return std::min(M, std::max<int64_t>(1, kMaxPairs / topk)); }
 
 struct MoeScratch {
-  size_t act, act_inv, y, counters, leveled, bytes;
+  size_t act, act_inv, y, counters, said, bytes;
 };
 MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I) {
   MoeScratch s;
@@ -1609,8 +1620,8 @@ MoeScratch moe_scratch(int64_t M, int64_t topk, int64_t H, int64_t I) {
   s.act_inv = s.act + pad256(pairs * act_row(I) * 2);
   s.y = s.act_inv + pad256(pairs * 4);
   s.counters = s.y + pad256(pairs * H * 4);
-  s.leveled = s.counters + pad256((size_t)strips_of(H) * 4);
-  s.bytes = s.leveled + 256;
+  s.said = s.counters + pad256((size_t)strips_of(H) * 4);
+  s.bytes = s.said + 256;
   return s;
 }
 
@@ -1713,7 +1724,7 @@ extern "C" int b200fp4_w4a16_moe(const void* hidden, int h_dtype, const float* t
     p.y = reinterpret_cast<float*>(ws + s.y);
     p.counters = reinterpret_cast<int*>(ws + s.counters);
     p.n_counters = (int)w4::strips_of(H);
-    p.leveled = reinterpret_cast<uint32_t*>(ws + s.leveled);
+    p.said = reinterpret_cast<uint32_t*>(ws + s.said);
     static std::atomic<uint32_t> calls{0};
     p.call = calls.fetch_add(1, std::memory_order_relaxed);
     MoeParams d = p;

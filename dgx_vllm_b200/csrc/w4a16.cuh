@@ -20,7 +20,7 @@
 // Gated: the 16 rows of a tile are eight gate rows and the same eight up rows, so that a lane holds both of a value's products.
 // Behind the units, for each matrix (gated: for its gate rows and its up rows) a word: the largest magnitude of code times scale, which the upper half of an f32 holds exactly, and
 // in the lower half a tag of the sizes.  Packed bytes do not tell K = 112 from 128, or [64, 128] from [32, 256]: kernels compare the tag with
-// the sizes that they are called with, and results of a weight that was packed for others are NaN (status kOtherSizes).
+// the sizes that they are called with, and every row of a result of a weight that was packed for others has NaN, a linear's in its last 32 columns or more (status kOtherSizes).
 #pragma once
 
 #include "common.cuh"

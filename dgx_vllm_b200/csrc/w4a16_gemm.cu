@@ -53,6 +53,7 @@ struct GemmParams {
   int accs;                   // accumulators in turn: two where a block does several tiles, or one in several chains
   int chain, chains;          // units that are summed in one accumulator; one tile: accumulators next to each other, whose sum is the result
   uint32_t tag;
+  int last_block;             // which has the last tile of all
   uint32_t sums_at;           // split: where the cluster's sums go; 0: where the token stages were
   int* status;
 };
@@ -189,7 +190,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   const uint32_t tmem = lds32(tmem_ptr);
   pdl_wait();
   pdl_launch_dependents();
-  if (blockIdx.x == 0 && threadIdx.x == 0) *status = 0;
+  const bool reports = (int)blockIdx.x == p.last_block && threadIdx.x == 0;
+  if (reports) *status = 0;
   if (split > 1) cluster_arrive_relaxed();         // the other blocks run before anything is sent to them
 
   if (warp == 0) {
@@ -344,11 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
   // ---------------------------------------------------------------------- epilogue: a lane is a row of the weight, a column a token
   const int quarter = warp & 3;
   const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-  auto factor = [&]() {
-    const uint32_t tail = *p.tail;
-    const float g = *p.g;
-    return packed_for(tail, p.tag) ? g : __int_as_float(0x7FC00000);
-  };
+  auto factor = [&](int row_tile) { return row_tile < p.row_tiles - 1 || packed_for(*p.tail, p.tag) ? *p.g : __int_as_float(0x7FC00000); };      // read next to the last rows' units
   // columns from, from + by, ... of a tile of n tokens, 32 at a time
   auto write_columns = [&](uint32_t acc, int row, int token0, int n, int from, int by, float g, bool more) {
     const float bias = p.bias != nullptr && row < p.N ? load_value(p.bias, p.bias_dtype, row) : 0.f;
@@ -384,14 +382,14 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
       }
     }
   };
-  if (blockIdx.x == 0 && threadIdx.x == 0 && !packed_for(*p.tail, p.tag)) *status = kOtherSizes;
+  if (reports && !packed_for(*p.tail, p.tag)) *status = kOtherSizes;
   if (p.accs > 1) {
     // several tiles: four warps, while the others go on
     if (warp >= 2 && warp < kFirstDecode) {
-      const float g = factor();
       Slot acc;
       for (int tile = first_tile; tile < p.tiles; tile += step) {
         const int token0 = tile / p.row_tiles * tokens;
+        const float g = factor(tile % p.row_tiles);
         bool ok = true;
         for (int u = 0; u < n_units; u += kChains ? p.chain : n_units) {
           ok = mbar_wait_warp(acc_full + 8 * acc.at, acc.phase, status, 78);
@@ -413,7 +411,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
     bool ok = true;
     if (work) ok = mbar_wait_warp(acc_full, 0, status, 79);
     tcgen05_fence_after();
-    const float g = factor();
+    const float g = factor(row_tile);
     if (split == 1) {
       if (work && ok) write_columns(0, row_tile * kMmaRows + quarter * 32 + lane, token0, min(tokens, p.M - token0), nth * 32, 5 * 32, g, false);
     } else {
@@ -531,6 +529,7 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
         p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - sums - (uint32_t)p.stages * tokens * 256) / kWStageBytes);
         p.sets = std::min(kDecodeSets, std::min(p.stages, p.w_stages));
         grid = (unsigned)(std::min<int64_t>(clusters, tiles) * split);
+        p.last_block = (int)((tiles - 1) % std::min<int64_t>(clusters, tiles)) * split;
       }
     }
   }

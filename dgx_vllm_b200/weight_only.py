@@ -75,8 +75,8 @@ def w4a16_linear(x: torch.Tensor, weight: PackedNvfp4Weight, bias: torch.Tensor 
 
 def last_w4a16_status(device=None) -> int:
     """Status word of the most recent w4a16_linear or W4A16MoE on the current stream of `device`: 0, or the code of a bounded wait that ran
-    out (that call's result is then not valid), or 63 where a weight was packed for other sizes than the call's (the result is NaN then;
-    only a custom op or a C caller can name other sizes).  A graph leaves it where the stream that it was captured on has it.  Synchronises."""
+    out (that call's result is then not valid), or 63 where a weight was packed for other sizes than the call's (every row of
+    the result has NaN then; only a custom op or a C caller can name other sizes).  A graph leaves it where the stream that it was captured on has it.  Synchronises."""
     return status_word(device, WS_W4A16_STATUS)
 
 

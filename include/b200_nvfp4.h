@@ -486,7 +486,7 @@ B200FP4_API int b200fp4_ep_combine_p2p(const float* parts, int64_t B, int64_t H,
  *   packed b200fp4_w4a16_packed_bytes(E, N, K, gated) bytes (0 for sizes that it refuses), 16-byte aligned
  *   gated  the rows are N/2 gate rows and then N/2 up rows, which the layer wants next to each other
  * Scale bytes 0x7F / 0xFF (NaN) count as 448; a negative scale gives its sign to its codes.
- * A packed weight knows its sizes: calls that name others give NaN, and 63 in the status word.
+ * A packed weight knows its sizes: calls that name others give NaN in every row (the linear at the row's end), and 63 in the status word.
  * ------------------------------------------------------------------------------------------- */
 B200FP4_API size_t b200fp4_w4a16_packed_bytes(int64_t E, int64_t N, int64_t K, int gated);
 B200FP4_API int b200fp4_w4a16_pack(const uint8_t* codes, const uint8_t* scales, int64_t E, int64_t N, int64_t K, int gated,
