@@ -5,9 +5,9 @@
 //   linear   columns are tokens
 //   gate/up  columns are the (token, expert) pairs of one expert; a tile's rows are eight gate rows and the same eight up rows, so that a
 //            lane holds both halves of its values and applies SiLU(gate) * up to them
-//   down     the value between the projections as two f16, upper and lower part, in two columns: their sum has f32's precision ("the value between the projections")
-// Work items are (strip of 32 rows, slot); a slot is a run of one expert's pairs that fits the columns.  A block has a contiguous range of them, groups of
-// warps take items in turn and split k among themselves.
+//   down     the value between the projections as two f16, upper and lower part, in two columns: their sum has f32's precision
+// Work items are (strip of 32 rows, slot); a slot is a run of one expert's pairs that fits the columns.  A block has a contiguous range of them,
+// groups of warps take items in turn and split k among themselves.
 // The layer is two launches without anything that has to outlast them: both find the slots from the routing by themselves, the first sets the
 // counters of the second, in which the block that finishes a strip's last item adds up its pairs in their order.
 #include <algorithm>
@@ -84,7 +84,8 @@ __global__ void __launch_bounds__(256) w4a16_pack_kernel(const PackParams p, int
 
 constexpr int kWarps = 16, kThreads = 32 * kWarps;
 constexpr uint32_t kSmemMost = 227 * 1024;
-// Units of a warp's ring: three, two where partial sums and rows for more columns need the room.  Two keep as much of HBM busy, but bear less unevenness.
+// Units of a warp's ring: three, two where partial sums and rows for more columns need the room.  Two keep as much of HBM busy, but bear less
+// unevenness.
 __host__ __device__ __forceinline__ constexpr int stages_of(int cols) { return cols == 1 ? 3 : 2; }
 __host__ __device__ __forceinline__ constexpr uint32_t ring_bytes(int cols) { return kWarps * stages_of(cols) * kUnitBytes; }
 __host__ __device__ __forceinline__ constexpr uint32_t bar_bytes(int cols) { return kWarps * stages_of(cols) * 8; }
@@ -164,9 +165,10 @@ __device__ __forceinline__ void multiply_unit(uint32_t unit, int lane, uint32_t 
     }
 }
 
-// The same for one or two tokens, without a multiplication by a scale for every pair of values: a column holds one block of 16 of a token's k and zeros elsewhere, so that
-// a matrix instruction's sums stay apart by block (kTokens = 1: the eight blocks of the unit; 2: the four of a half, for each token), and a scale goes with the
-// block's sum.  268 instructions a unit become 200.  Lane l has columns 2 (l % 4) and the next one: part[tile][row l / 4, l / 4 + 8] gets their sum.
+// The same for one or two tokens, without a multiplication by a scale for every pair of values: a column holds one block of 16 of a token's k and
+// zeros elsewhere, so that a matrix instruction's sums stay apart by block (kTokens = 1: the eight blocks of the unit; 2: the four of a half, for
+// each token), and a scale goes with the block's sum.  268 instructions a unit become 200.  Lane l has columns 2 (l % 4) and the next one:
+// part[tile][row l / 4, l / 4 + 8] gets their sum.
 template <int kTokens>
 __device__ __forceinline__ void multiply_unit_by_block(uint32_t unit, int lane, uint32_t chunk, const uint32_t (&b)[2][8], float (&part)[2][2]) {
   const int row8 = lane >> 2, quad = lane & 3;
@@ -219,8 +221,9 @@ __device__ __forceinline__ void staged_columns(const uint32_t (&col)[kCols], uin
     }
 }
 
-// Warps that share the units of an item, as a power of two, given the block's items and the units of one.  A unit takes a warp 750 cycles, and 350 of its scheduler
-// (an SM has four, warp w is with scheduler w % 4); an item's ending a third of a unit where a warp has the item for itself, else nearly one.
+// Warps that share the units of an item, as a power of two, given the block's items and the units of one.  A unit takes a warp 750 cycles, and 350 of
+// its scheduler (an SM has four, warp w is with scheduler w % 4); an item's ending a third of a unit where a warp has the item for itself, else
+// nearly one.
 inline float share_cost(int items, int units, int log_share) {
   const int share = 1 << log_share, full = (items << log_share) / kWarps, rest = (items << log_share) % kWarps;
   const float item = (float)((units + share - 1) / share) + (log_share == 0 ? 0.33f : 0.9f);
@@ -239,9 +242,9 @@ inline int least_share(int out_dtype, int units) {
   return share;
 }
 
-// A run of items is done in phases: rounds of an item a warp, then the rest by groups of warps, so that no warp is without work for more than a part of an item.  Against one
-// size of group for all: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of 512, H = 2048, 0.3 us more of
-// its 14, for the longer way to a warp's first weights.
+// A run of items is done in phases: rounds of an item a warp, then the rest by groups of warps, so that no warp is without work for more than a part
+// of an item.  Against one size of group for all, when they came: 29 tokens, eight experts of 4096, H = 4096, 78 us / 84; one token, ten experts of
+// 512, H = 2048, 0.3 us more of its 14, for the longer way to a warp's first weights.
 // share: log2 of the warps of a group.  The plan has that of each number of items under a round, four bits each.
 struct Phase {
   int count, share;
@@ -295,7 +298,8 @@ __device__ __forceinline__ void take_back(const float* own, float (&acc)[2][kCol
 // Sums of the warps that share an item, [warp][tile][column of eight][j][lane]: each warp adds up some of them, in the order of k, and finishes them.
 // A lane's sums j are row l / 4 (0, 1) or l / 4 + 8 (2, 3) of a tile and columns 2 (l % 4) and the next one; finish gets those of j = kFirst[i] and
 // kSecond[i].  Both barriers are the group's, whichever others there are at the time.
-// finish(t, c, i, a, b, std::false_type) may say, with the whole warp, that it wants these sums a second time, with std::true_type: what is rarely needed stays out of what always is.
+// finish(t, c, i, a, b, std::false_type) may say, with the whole warp, that it wants these sums a second time, with std::true_type: what is rarely
+// needed stays out of what always is.
 template <int kCols, bool kAcross, typename F>
 __device__ __forceinline__ void finish_item(float* red, int log_share, int in_group, int group, int lane, const float (&acc)[2][kCols][4], F&& finish) {
   const int share = 1 << log_share;
@@ -495,9 +499,11 @@ __host__ __device__ __forceinline__ LinearLayout linear_layout(int cols, int cap
   return l;
 }
 
-// The linear layer of few tokens: bound by the copies of the weight, then by decoding it.  An SM's 16 warps decode and multiply a unit in 87 cycles with one column of eight
-// (131 with two), and its share of HBM brings one in 98, so that a layer reaches the copy rate only where it is large: N=14336 K=4096, 33 MB, takes 9.2 us for one token
-// and 11.4 for eight, of which 2 are the launch and the row, 1.5 the first units' way and 5.1 the floor; N=K=2048 4.4, most of it launch.
+// The linear layer of few tokens: bound by the copies of the weight, then by decoding it.  An SM's 16 warps decode and multiply a unit in 87 cycles
+// with one column of eight (131 with two), and its share of HBM brings one in 98: N=14336 K=4096, 33 MB, takes 9.2 us for one token and 10.8 for
+// eight, of which 2 are the launch and the row, 1.5 the first units' way and 5.1 the floor; N=K=2048 4.4, most of it launch.  Large layers stay below
+// the copy rate, since a block or a cluster has whole strips: 448 of them are three or four a block, and 256 one or two, a sixth more than the mean:
+// four tokens, N=8192 K=14336, 66 MB, 18.2 us, 56 % of the copy rate.
 // XT: type of the activations; kCols: columns of eight; kTokens: 1 or 2 where there are no more, else 0
 template <typename XT, int kCols, int kTokens>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearParams p) {
@@ -544,8 +550,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_linear_kernel(const LinearP
   const LinearLayout l = linear_layout(kCols, p.cap, row_bytes, split, p.per + (p.more > 0));
   float* const inv = reinterpret_cast<float*>(smem + l.inv);
   const float g = *p.g;
-  // The word behind the units is read by the blocks that read the last strip, next to it: as a page of its own for all of them it cost a tenth of one token's time.  It is looked
-  // at when the strip is done.
+  // The word behind the units is read by the blocks that read the last strip, next to it: as a page of its own for all of them it cost a tenth of one
+  // token's time.  It is looked at when the strip is done.
   const uint32_t tail = last >= (first_slot + 1) * p.strips ? *p.tail : p.tag;
   auto factor = [&](int strip) {
     if (strip != p.strips - 1) return g;
@@ -704,8 +710,8 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
       const uint64_t bytes = (uint64_t)linear_layout(kCols, cap, row_bytes, 1, 0).bytes + (split > 1 ? (uint64_t)most * cap * 128 : 0);
       if ((uint64_t)own * 256 > kSmemMost || bytes > kSmemMost) continue;
       if (kTokens == 0 && p.out_dtype == B200FP4_DTYPE_F32 && own > kWarpChain * kWarps) continue;       // too long a chain for an f32 result
-      // The busiest block's units; a cluster's exchange costs some 1500 cycles.  Shared / not shared, us: M=1 N=512 K=16384 6.2 / 8.9, M=8 N=512 K=4096 4.7 / 6.1;
-      // by this rule not shared: M=1 N=K=4096 5.2, N=14336 K=4096 9.2.
+      // The busiest block's units; a cluster's exchange costs some 1500 cycles.  Shared / not shared, us: M=1 N=512 K=16384 6.2 / 8.9, M=8 N=512
+      // K=4096 4.7 / 6.1; by this rule not shared: M=1 N=K=4096 5.2, N=14336 K=4096 9.2.
       const int log_share = share_of(most, p.units / split, kTokens > 0 ? 0 : least_share(p.out_dtype, own));
       const float cost = share_cost(most, own, log_share) + (split > 1 ? 1500.f : 0.f);
       if (cost < best) {
@@ -729,8 +735,8 @@ int launch_linear_of(LinearParams p, cudaStream_t st) {
   return finish_launch(1);
 }
 
-// Up to eight tokens fill the columns of one instruction; with up to sixteen, two of them, the tcgen05 kernel is the faster one but for the smallest weights: M=16, us from
-// Python, this / that: N=K=2048 5.7 / 5.9, N=3001 K=4144 9.7 / 7.9, N=K=4096 10.1 / 8.1, N=14336 K=4096 19.7 / 15.1.
+// Up to eight tokens fill the columns of one instruction; with up to sixteen, two of them, the tcgen05 kernel is the faster one but for the smallest
+// weights: M=16, us from Python, this / that: N=K=2048 5.7 / 5.9, N=3001 K=4144 9.7 / 7.9, N=K=4096 10.1 / 8.1, N=14336 K=4096 19.7 / 15.1.
 bool few_tokens(const LinearCall& c) { return c.M <= 8 || (c.M <= 16 && strips_of(c.N) * units_of(c.K) <= 1536); }
 
 template <typename T>
@@ -797,21 +803,25 @@ struct MoeParams {
 
 // ---- the value between the projections
 //
-// SiLU(gate) * up of a pair is brought below 2^15 by a power of two that goes by a bound, known before any of its values is.  Then it is two f16, v = upper + lower * 2^-12: the
-// rest of the upper part is at most 2^-12 of it, so that the lower part uses f16's range too, and a value is off by the larger of 2^-37 and 2^-23 of itself.
-// A bound may be far from the values (gates of -30: SiLU is 2^-38 of them).  So each run of eight has a level: 2^(28 k) more, with the least k that brings its largest value to 2^-13 or
-// above, where it is off by 2^-24 of that at most.  A level is kept as a bit, 1 << k, none for a run of zeros.  Ordinary layers have no run above level 0; a word says
-// whether a call has one, and only then the second projection looks at the levels: runs of the level above a pair's lowest are brought down to that and split anew, higher
-// ones are less than 2^-28 of the pair's largest value and left out.
-// One f16 of eleven bits instead (bf16 results are then off by 8e-4 of their norm more): 32 tokens, ten of 512 experts, H=2048 I=512, 86.7 us against 90.2; 128 tokens 166.6 / 177; one 14.3 / 14.9.
-// Powers of two of their own for all runs, applied to every operand: 93.8, 185, 14.8.  The looking out of the loops that do without: 94.3 -> 90.2.
+// SiLU(gate) * up of a pair is brought below 2^15 by a power of two that goes by a bound, known before any of its values is.  Then it is two f16, v =
+// upper + lower * 2^-12: the rest of the upper part is at most 2^-12 of it, so that the lower part uses f16's range too, and a value is off by the
+// larger of 2^-37 and 2^-23 of itself. A bound may be far from the values (gates of -30: SiLU is 2^-38 of them).  So each run of eight has a level:
+// 2^(28 k) more, with the least k that brings its largest value to 2^-13 or above, where it is off by 2^-24 of that at most.  A level is kept as a
+// bit, 1 << k, none for a run of zeros.  Ordinary layers have no run above level 0; a word says whether a call has one, and only then the second
+// projection looks at the levels: runs of the level above a pair's lowest are brought down to that and split anew, higher ones are less than 2^-28 of
+// the pair's largest value and left out.
+// One f16 of eleven bits instead (bf16 results are then off by 8e-4 of their norm more): 32 tokens, ten of 512 experts, H=2048 I=512, 94 us against
+// 99; 128 tokens 187 / 200; one 14.1 / 14.9.  With the same inputs in every call 32 tokens take 90.2; with a power of two of its own for each run,
+// applied to every operand, 93.8; where the loops that do without levels look at them 94.3.
 constexpr int kLevel = 28, kLevels = 8;
 constexpr float kLeast = 0x1p-13f, kLower = 4096.f;
 __host__ __device__ __forceinline__ int64_t act_row(int64_t I) { return 2 * I + units_of(I) * 8; }      // halves of a pair: two parts, and 16 bytes for each 128 values
-// Where the level of run n (values 8 n to 8 n + 7) is: lane l of the second projection has its four of a unit in a word, [block l % 4][half of the unit][eight of the block]
+// Where the level of run n (values 8 n to 8 n + 7) is: lane l of the second projection has its four of a unit in a word, [block l % 4][half of the
+// unit][eight of the block]
 __device__ __forceinline__ int run_at(int n) { return (n >> 4) * 16 + ((n >> 1) & 3) * 4 + ((n >> 3) & 1) * 2 + (n & 1); }
 
-// A lane's eight values of a run, the upper parts or (odd) the lower ones, from one level to the one below it: times 2^-28.  Lanes apart by four have the two parts.
+// A lane's eight values of a run, the upper parts or (odd) the lower ones, from one level to the one below it: times 2^-28.  Lanes apart by four have
+// the two parts.
 __device__ __forceinline__ void level_down(uint32_t* b, bool odd, int levels) {
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
@@ -828,8 +838,9 @@ __device__ __forceinline__ void level_down(uint32_t* b, bool odd, int levels) {
 struct RowStat {
   float inv, act;             // the reciprocal of the row's factor; what brings the pair's row of act into f16's range
 };
-// Shared memory behind the rings and barriers: partial sums of warps | expert of a pair | pairs by expert, and as they came | first place of an expert | slots | scan |
-// routing weights (down) | statistics of the staged rows | parts of those | the rows in f16, and before them an expert's pairs | products of whole strips
+// Shared memory behind the rings and barriers: partial sums of warps | expert of a pair | pairs by expert, and as they came | first place of an
+// expert | slots | scan | routing weights (down) | statistics of the staged rows | parts of those | the rows in f16, and before them an expert's
+// pairs | products of whole strips
 struct MoeLayout {
   uint32_t red, expert, list, came, start, slots, scan, weights, stats, parts, rows, y, bytes;
 };
@@ -862,8 +873,8 @@ __device__ __forceinline__ int quotient(int n, int d, float rcp) {
   return q;
 }
 
-// Items of a block of the down projection, of the pairs' slots and the strips of the result: a run of all of them, strip by strip; or a cluster has whole strips
-// and each of its blocks some of the slots.
+// Items of a block of the down projection, of the pairs' slots and the strips of the result: a run of all of them, strip by strip; or a cluster has
+// whole strips and each of its blocks some of the slots.
 struct DownItems {
   int first, last, fast;      // items; slots of a strip
   int strip0, strip_step, slot0;
@@ -899,9 +910,9 @@ __device__ __forceinline__ void clear_counts(const MoeParams& p, unsigned char* 
   for (int i = threadIdx.x; i < p.E; i += kThreads) reinterpret_cast<int*>(smem + l.rows)[i] = 0;
 }
 
-// Slots (expert | pairs << 16, first place in the list): runs of at most `cap` pairs of one expert, experts in order and pairs in theirs.  Every block finds the
-// same ones, whatever the order in which its threads run: pairs are counted and gathered by expert as they come, and then each takes the place that the number
-// of smaller ones in its expert's run gives it.  Returns the number of slots.
+// Slots (expert | pairs << 16, first place in the list): runs of at most `cap` pairs of one expert, experts in order and pairs in theirs.  Every
+// block finds the same ones, whatever the order in which its threads run: pairs are counted and gathered by expert as they come, and then each takes
+// the place that the number of smaller ones in its expert's run gives it.  Returns the number of slots.
 __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* smem, const MoeLayout& l) {
   constexpr int kMost = kMaxPairs / kThreads;
   const int cap = p.cap, P = p.M * p.topk, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -997,10 +1008,15 @@ __device__ __forceinline__ int find_slots(const MoeParams& p, unsigned char* sme
 
 enum Projection { kGateUp, kDownItems, kDownStrips };       // kDownStrips: whole strips
 
-// Bound by the copies of the experts that the routing reaches: 32 tokens, ten of 512 experts, H=2048 I=512, take 91-94 us, gate/up 46 of them at 6.1 TB/s and down 26 at
-// 5.3; the rest is finding the slots (2 us), rows and first units (3), the down projection's start (3) and the strips' last sums (4).  128 tokens 180-187.  Two
-// launches: every value of the first projection is needed by the second, which finds its slots and asks for its first weights while the first one ends.
-// XT: type of the activations (gate/up); kCols: columns of eight; kChains: sums of more than a chain, for an f32 result (as a choice at run time it cost the others 5 to 9 %)
+// Bound by the copies of the experts that the routing reaches: 32 tokens, ten of 512 experts, H=2048 I=512, take 99 us with inputs that change from
+// call to call, of which their 420 MB would take 66 at the copy rate; finding the slots takes 2, rows and first units 3, the down projection's start 3
+// and the strips' last sums 4.  Alone and cold gate/up takes 57 us and down 44.  128 tokens 200.  The kernels over items are at the limit of 128
+// registers and spill (12 bytes stored, 28 loaded).
+// A prompt goes through in turns of kMaxPairs pairs, each of which reads the experts again: 8192 tokens 9.7 ms.
+// Two launches: every value of the first projection is needed by the second, which finds its slots and asks for its first weights while the first one
+// ends.
+// XT: type of the activations (gate/up); kCols: columns of eight; kChains: sums of more than a chain, for an f32 result (as a choice at run time it
+// cost the others 5 to 9 %)
 template <typename XT, int kMode, int kCols, bool kChains>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams p) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -1156,8 +1172,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_moe_kernel(const MoeParams 
                     [&](int r, float inv, float squares) { stats[r] = {inv, squares}; });
       __syncthreads();
       if (own >= 0) {
-        // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the bound is
-        // far above the values costs little: f16 reaches 40 binades down.
+        // |gate|, |up| <= |x| * sqrt(K) * the matrix's largest magnitude, and |SiLU(gate)| <= |gate|.  The product is brought below 2^15; that the
+        // bound is far above the values costs little: f16 reaches 40 binades down.
         // Where the squares have left f32's range, |x| <= 2^16 inv sqrt(K) is the bound that is left.
         const float squares = stats[threadIdx.x].act, root = sqrtf((float)p.K);
         const float norm = (squares > 1e-30f && squares < 1e30f ? sqrtf(squares) : 65536.f * stats[threadIdx.x].inv * root) * root * w;
@@ -1571,16 +1587,18 @@ int launch_both(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
 
 template <typename T, bool kChains>
 int launch_layer_of(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
-  // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit (eight; four in the down projection, where a pair
-  // has two columns) is read again, mostly from L2.  Columns of gate/up and of down, us, by pairs an expert, bf16; eight experts of 4096, H = 4096: 7.25 pairs 1/1 83.4,
-  // 1/2 86.9, 2/1 86.4, 2/2 90.2; 8.5 89.0 / 90.8 / 89.4 / 91.3; 9 94.1 / 96.1 / 93.6 / 95.5; 10 96.3 / 96.5 / 95.7 / 96.1; 11 106 / 104 / 100.6 / 99.8.  64 experts of 768,
-  // H = 2048: four 51.4 / 56.2 / 60.8 / 69.9; 8.5 74.3 / 75.5 / 75.3 / 81.1; 9 78.3 / 78.0 / 76.6 / 81.3; 10 83.9 / 84.8 / 79.8 / 82.7; 12 93.6 / 92.0 / 90.8 / 90.1.
+  // Columns of eight, one or two: with two a unit takes half as long again, with one an expert of more pairs than fit (eight; four in the down
+  // projection, where a pair has two columns) is read again, mostly from L2.  Columns of gate/up and of down, us, by pairs an expert, bf16; eight
+  // experts of 4096, H = 4096: 7.25 pairs 1/1 83.4, 1/2 86.9, 2/1 86.4, 2/2 90.2; 8.5 89.0 / 90.8 / 89.4 / 91.3; 9 94.1 / 96.1 / 93.6 / 95.5; 10 96.3
+  // / 96.5 / 95.7 / 96.1; 11 106 / 104 / 100.6 / 99.8.  64 experts of 768, H = 2048: four 51.4 / 56.2 / 60.8 / 69.9; 8.5 74.3 / 75.5 / 75.3 / 81.1; 9
+  // 78.3 / 78.0 / 76.6 / 81.3; 10 83.9 / 84.8 / 79.8 / 82.7; 12 93.6 / 92.0 / 90.8 / 90.1.
   const double each = (double)up.M * up.topk / (double)(up.map != nullptr ? std::max<int64_t>(up.global_E, up.E) : up.E);
   if (each > 10.5) return launch_both<T, 2, kDownItems, 2, kChains>(up, down, st);
   if (each > 8.75) return launch_both<T, 2, kDownItems, 1, kChains>(up, down, st);
-  // Whole strips: nothing goes through memory and no block waits for a counter, 1.6 us less for one token (H = 2048, ten experts of 512: 14.9 against 16.5), but the
-  // blocks' shares are less even.  Items / whole strips, us, by the units that the busiest block has more than its share, eight experts of 4096, H = 4096: 32 units (3 tokens)
-  // 38.7 / 37.6, 41 (4) 46.9 / 44.4, 42 (12) 56.2 / 56.3, 43 (20) 65.5 / 66.4, 52 (24) 70.8 / 71.4, 79 (29) 83.2 / 84.9; eight of 8192, H = 5120, 6 tokens, 185: 90.0 / 97.9.
+  // Whole strips: nothing goes through memory and no block waits for a counter, 1.6 us less for one token (H = 2048, ten experts of 512: 14.9 against
+  // 16.5), but the blocks' shares are less even.  Items / whole strips, us, by the units that the busiest block has more than its share, eight
+  // experts of 4096, H = 4096: 32 units (3 tokens) 38.7 / 37.6, 41 (4) 46.9 / 44.4, 42 (12) 56.2 / 56.3, 43 (20) 65.5 / 66.4, 52 (24) 70.8 / 71.4, 79
+  // (29) 83.2 / 84.9; eight of 8192, H = 5120, 6 tokens, 185: 90.0 / 97.9.
   MoePlan strips;
   if (plan_moe<__half, kDownStrips, 1, kChains>(down, strips) == B200FP4_STATUS_SUCCESS &&
       (strips.items - slots_of(down, strips.p.cap) * down.strips / sm_count()) * down.units < 43)
@@ -1592,7 +1610,8 @@ int launch_layer(const MoeParams& up, const MoeParams& down, cudaStream_t st) {
   const bool chains = down.out_dtype == B200FP4_DTYPE_F32 && std::max(up.units, down.units) > kWarpChain;
   const int rc = chains ? launch_layer_of<T, true>(up, down, st) : launch_layer_of<T, false>(up, down, st);
   if (rc != B200FP4_STATUS_NOT_SUPPORTED) return rc;
-  // Long rows: rings and sums for two columns leave more room than those for one.  So a last turn of few pairs is never refused where the full ones before it were not.
+  // Long rows: rings and sums for two columns leave more room than those for one.  So a last turn of few pairs is never refused where the full ones
+  // before it were not.
   return chains ? launch_both<T, 2, kDownItems, 2, true>(up, down, st) : launch_both<T, 2, kDownItems, 2, false>(up, down, st);
 }
 

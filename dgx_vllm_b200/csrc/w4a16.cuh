@@ -8,19 +8,19 @@
 // become f16 exactly, after a power of two for each row has brought its largest value below 2^15: what is then below f16's
 // smallest, 2^-39 of that largest value, is the only part that can be rounded.
 //
-// Packed weight: units of 32 rows x 128 of k, 2304 bytes, [matrix][128 rows][k / 128][32 rows][unit] (fewer rows in a last block): one copy brings 128 rows x 128 of
-// k, and one a unit.  A unit is two tiles of the 16x8x16 matrix
-// instruction, whose lane l holds rows l / 4 and l / 4 + 8 and four k of each: with the k of an instruction taken from four blocks of 16,
-// lane l needs block l % 4 only, so it converts one scale a row for four instructions, and its operands of a whole block are 16
-// neighbouring values:
+// Packed weight: units of 32 rows x 128 of k, 2304 bytes, [matrix][128 rows][k / 128][32 rows][unit] (fewer rows in a last block): one copy brings
+// 128 rows x 128 of k, and one a unit.  A unit is two tiles of the 16x8x16 matrix instruction, whose lane l holds rows l / 4 and l / 4 + 8 and four k
+// of each: with the k of an instruction taken from four blocks of 16, lane l needs block l % 4 only, so it converts one scale a row for four
+// instructions, and its operands of a whole block are 16 neighbouring values:
 //   codes   [tile][half: 64 of k][chunk_at(l / 4, l % 4)][16 bytes: row l / 4, k 0..15 | row l / 4 + 8, k 0..15]
 //   scales  [lane][tile][4 bytes: half 0 row l / 4, row l / 4 + 8 | half 1 likewise]
-// The chunks are ordered so that no two lanes meet in a bank when each reads its 16 bytes, nor when a lane is one of 32 rows and reads the 8 bytes of a
-// block (the decoding of w4a16_gemm.cu).  Negative scales give their sign to their codes when the weight is packed.
+// The chunks are ordered so that no two lanes meet in a bank when each reads its 16 bytes, nor when a lane is one of 32 rows and reads the 8 bytes of
+// a block (the decoding of w4a16_gemm.cu).  Negative scales give their sign to their codes when the weight is packed.
 // Gated: the 16 rows of a tile are eight gate rows and the same eight up rows, so that a lane holds both of a value's products.
-// Behind the units, for each matrix (gated: for its gate rows and its up rows) a word: the largest magnitude of code times scale, which the upper half of an f32 holds exactly, and
-// in the lower half a tag of the sizes.  Packed bytes do not tell K = 112 from 128, or [64, 128] from [32, 256]: kernels compare the tag with
-// the sizes that they are called with, and every row of a result of a weight that was packed for others has NaN, a linear's in its last 32 columns or more (status kOtherSizes).
+// Behind the units, for each matrix (gated: for its gate rows and its up rows) a word: the largest magnitude of code times scale, which the upper half
+// of an f32 holds exactly, and in the lower half a tag of the sizes.  Packed bytes do not tell K = 112 from 128, or [64, 128] from [32, 256]: kernels
+// compare the tag with the sizes that they are called with, and every row of a result of a weight that was packed for others has NaN, a linear's in the
+// columns of its last strip (status kOtherSizes).
 #pragma once
 
 #include "common.cuh"

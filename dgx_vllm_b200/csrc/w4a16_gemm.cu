@@ -4,15 +4,15 @@
 // them straight into tensor memory, from where the MMA takes its A operand: a decoded weight never is in shared memory, and it is decoded once for
 // up to 192 tokens.  The activations are the B operand as they lie in memory, brought in by TMA, in the type they have: products are exact in bf16
 // and in f16 alike.
-// Roles (23 warps): 0 copies of the weight, 22 of the tokens, 1 MMAs and tensor memory, 2-5 (in the end 2-21) epilogue, 6-21 decoding (four sets of four, a warp 32 rows of the tile
-// and every fourth 128 of k).  One warp that brought in weight and tokens, four copies for 128 rows, took 1040 cycles for 128 of k and was what all waited for.
-// Tensor memory: accumulators, and the rest for A stages of 64 columns (128 rows x 128 of k): the MMA warp's waits, MMAs and commits take 300 cycles a
-// stage however few the tokens are.  Persistent blocks, one to an SM; where there are too few
-// tiles for them, a cluster shares the k of one and adds up its parts through distributed shared memory, each block some of the tokens.
-// Every wait is bounded (status word), tensor memory is always freed.
-// Bound: with many tokens by the tensor cores, M=4096 N=14336 K=4096 400 us, 1.20 PFLOP/s under the power cap (73 % of the measured burst rate, 88 % of the sustained one), the
-// tensor pipe busy 73 % of active cycles; with few by decoding and the MMA warp's turn, some 450 cycles for 128 of k where HBM brings them in 390: M=32 N=4096 K=14336 14.8 us
-// (33 MB, floor 5.3), M=333 N=K=4096 15.6 (0.72 PFLOP/s).
+// Roles (23 warps): 0 copies of the weight, 22 of the tokens, 1 MMAs and tensor memory, 2-5 (in the end 2-21) epilogue, 6-21 decoding (four sets of
+// four, a warp 32 rows of the tile and every fourth 128 of k).  One warp that brought in weight and tokens, four copies for 128 rows, took 1040
+// cycles for 128 of k and was what all waited for. Tensor memory: accumulators, and the rest for A stages of 64 columns (128 rows x 128 of k): the
+// MMA warp's waits, MMAs and commits take 300 cycles a stage however few the tokens are.  Persistent blocks, one to an SM; where there are too few
+// tiles for them, a cluster shares the k of one and adds up its parts through distributed shared memory, each block some of the tokens. Every wait is
+// bounded (status word), tensor memory is always freed.
+// Bound: with many tokens by the tensor cores, M=4096 N=14336 K=4096 400 us, 1.20 PFLOP/s under the power cap (73 % of the measured burst rate, 88 %
+// of the sustained one), the tensor pipe busy 73 % of active cycles; with few by decoding and the MMA warp's turn, some 450 cycles for 128 of k where
+// HBM brings them in 390: M=32 N=4096 K=14336 15.1 us (33 MB, floor 5.3), M=333 N=K=4096 15.9 (0.70 PFLOP/s).
 #include <algorithm>
 #include <type_traits>
 
@@ -28,8 +28,8 @@ using namespace w4;
 constexpr int kMmaRows = 128, kMostTokens = 192;
 constexpr int kDecodeSets = 4, kFirstDecode = 6, kTokenWarp = kFirstDecode + 4 * kDecodeSets;
 constexpr int kThreads = 32 * (kTokenWarp + 1);
-// Stages at most; how many there are goes by the tokens of a tile.  Of the MMA's operands: 128 rows x 128 of k in tensor memory, beside the accumulators, and
-// tokens x 128 of k in shared memory, two boxes of 64; of packed units of 128 rows x 128 of k.
+// Stages at most; how many there are goes by the tokens of a tile.  Of the MMA's operands: 128 rows x 128 of k in tensor memory, beside the
+// accumulators, and tokens x 128 of k in shared memory, two boxes of 64; of packed units of 128 rows x 128 of k.
 constexpr int kMost = 6, kWMost = 12;
 constexpr uint32_t kWStageBytes = 4 * kUnitBytes, kRingBytes = 212 * 1024;
 constexpr uint32_t kSmemBytes = 1024 + kRingBytes + 1024;
@@ -58,8 +58,9 @@ struct GemmParams {
   int* status;
 };
 
-// A pair of codes' f16 values times a block's scale, in the operand's type; both products are exact.  To bf16 by way of two f32, which a mixed-precision
-// multiplication gives at once: 54 cycles of an SM for 32 rows x 64 of k, against 75 where the bits are moved and multiplied in bf16, and 34 in f16.
+// A pair of codes' f16 values times a block's scale, in the operand's type; both products are exact.  To bf16 by way of two f32, which a
+// mixed-precision multiplication gives at once: 54 cycles of an SM for 32 rows x 64 of k, against 75 where the bits are moved and multiplied in bf16,
+// and 34 in f16.
 template <typename T>
 __device__ __forceinline__ uint32_t scaled(uint32_t pair, uint32_t scale);
 template <>
@@ -97,8 +98,8 @@ __device__ __forceinline__ void tcgen05_st_32x32(uint32_t taddr, const uint32_t 
       "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
-// D += A . B^T, A in tensor memory; by the lane whose `issue` is set.  Predicates instead of a branch: in a branch of one lane every operand is moved to the uniform
-// registers that the instruction wants.
+// D += A . B^T, A in tensor memory; by the lane whose `issue` is set.  Predicates instead of a branch: in a branch of one lane every operand is moved
+// to the uniform registers that the instruction wants.
 __device__ __forceinline__ void tcgen05_mma_ts(uint32_t issue, uint32_t d_tmem, uint32_t a_tmem, uint32_t b_desc_lo, uint32_t b_desc_hi, uint32_t idesc,
                                                uint32_t accumulate) {
   asm volatile(
@@ -147,7 +148,8 @@ struct Slot {
   }
 };
 
-// kChains: an f32 result of more units than a chain has; the others' loops are the shorter for it (M=32 N=4096 K=14336 bf16 14.8 us, 15.7 with the chains' counting)
+// kChains: an f32 result of more units than a chain has; the others' loops are the shorter for it (M=32 N=4096 K=14336 bf16 14.8 us, 15.7 with the
+// chains' counting)
 template <typename T, bool kChains>
 __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const GemmParams p) {
   extern __shared__ unsigned char smem_raw[];
@@ -259,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_gemm_kernel(const __grid_co
           tcgen05_fence_after();
           d = tmem + acc.at * acc_cols;
         }
-        // One wait and one commit for 128 of k: with barriers of their own for the two operands the loop took 650 cycles for few tokens.  The next stage is looked at
-        // while this one's MMAs are issued.
+        // One wait and one commit for 128 of k: with barriers of their own for the two operands the loop took 650 cycles for few tokens.  The next
+        // stage is looked at while this one's MMAs are issued.
         if (!ready) ok = mbar_wait_warp(full + 8 * op.at, op.phase, status, 74);
         if (!ok) break;
         tcgen05_fence_after();
@@ -490,9 +492,9 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
   p.row_tiles = (int)((c.N + kMmaRows - 1) / kMmaRows);
   p.status = c.status;
   const int sms = sm_count();
-  // Tokens of a tile and blocks that share one: the least time of the busiest block, in cycles.  128 of k take the MMAs four cycles a token, the copies one for each
-  // 57 bytes, and decoding and issue 450.  Shared by this rule / one block a tile, us: M=32 N=4096 K=14336 14.8 / 40.3, M=64 N=K=4096 8.8 / 14.1, M=128 12.1 / 14.4; by it
-  // not shared: M=333 N=K=4096 15.7.
+  // Tokens of a tile and blocks that share one: the least time of the busiest block, in cycles.  128 of k take the MMAs four cycles a token, the
+  // copies one for each 57 bytes, and decoding and issue 450.  Shared by this rule / one block a tile, us: M=32 N=4096 K=14336 14.8 / 40.3, M=64
+  // N=K=4096 8.8 / 14.1, M=128 12.1 / 14.4; by it not shared: M=333 N=K=4096 15.7.
   double best = 1e30;
   unsigned grid = 0;
   const int64_t least = (c.M + kMostTokens - 1) / kMostTokens;
@@ -504,7 +506,8 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
       const int clusters = split == 1 ? sms : resident_clusters_of(counts[split], w4a16_gemm_kernel<T, kChains>, split, kThreads, kSmemBytes);
       if (clusters < 1) break;
       if (split > 1 && tiles > clusters) break;    // a cluster does one tile
-      // An f32 result: chains of all of a block's units (kChain), unless blocks of a cluster, whose chains are all in tensor memory, would need longer ones
+      // An f32 result: chains of all of a block's units (kChain), unless blocks of a cluster, whose chains are all in tensor memory, would need
+      // longer ones
       const int own_units = (p.units + split - 1) / split, wanted = kChains ? (own_units + kChain - 1) / kChain : 1;
       const int acc_cols = (tokens + 31) / 32 * 32, chains = split == 1 ? 1 : std::min(wanted, (512 - 2 * 64) / acc_cols);
       if (wanted > 1 && split > 1 && (own_units + chains - 1) / chains > kChain + 1) continue;
@@ -516,14 +519,15 @@ int launch_gemm(const LinearCall& c, cudaStream_t st) {
         p.tokens = tokens;
         p.tiles = (int)tiles;
         p.split = split;
-        // Tensor memory: accumulators (two where a block has several tiles), the rest for the weight.  Shared memory: 144 KB of tokens at most, the rest for packed units, whose
-        // copies take longest.
+        // Tensor memory: accumulators (two where a block has several tiles), the rest for the weight.  Shared memory: 144 KB of tokens at most, the
+        // rest for packed units, whose copies take longest.
         p.acc_cols = (uint32_t)acc_cols;
         p.accs = tiles > clusters || (split == 1 && wanted > 1) ? 2 : 1;
         p.chains = chains;
         p.chain = split == 1 && wanted > 1 ? kChain : (own_units + chains - 1) / chains;
         p.stages = (int)std::min<uint32_t>(kMost, std::min<uint32_t>((512 - std::max(p.accs, p.chains) * p.acc_cols) / 64, 144 * 1024 / ((uint32_t)tokens * 256)));
-        // A cluster's sums have room of their own where they are small: nobody waits for the others' MMAs then (M=32 N=4096 K=14336 15.1 us / 15.7, M=64 N=K=4096 9.2 / 9.7).
+        // A cluster's sums have room of their own where they are small: nobody waits for the others' MMAs then (M=32 N=4096 K=14336 15.1 us / 15.7,
+        // M=64 N=K=4096 9.2 / 9.7).
         const uint32_t sums = split > 1 && tokens <= 64 ? (uint32_t)tokens * kMmaRows * 4 : 0;
         p.sums_at = sums > 0 ? kRingBytes - sums : 0;
         p.w_stages = (int)std::min<uint32_t>(kWMost, (kRingBytes - sums - (uint32_t)p.stages * tokens * 256) / kWStageBytes);
