@@ -133,3 +133,22 @@ def test_values_of_one_pair_spread_over_many_powers():
     out = layer(x, weights, ids)
     check(out, x, weights, ids, W13, W2)
     assert bool((out[2] == 0).all())
+
+
+def test_one_graph_with_ordinary_and_with_small_values():
+    """Replays on inputs of both kinds, in turn: what a replay says of its values is at most looked at needlessly by the next."""
+    layer, x, W13, W2 = _signed_layer(6, 3, 256, 160, 30.0, -1)
+    ids = (torch.arange(6, dtype=torch.int32, device="cuda") % 3)[:, None].contiguous()
+    weights = torch.full((6, 1), 0.75, device="cuda")
+    kinds = [x, -x, x * 0.25, torch.zeros_like(x)]                  # all gates near -30, near 30, near -8; nothing
+    want = [layer(k, weights, ids).clone() for k in kinds]
+    for k, w in zip(kinds, want):
+        check(w, k, weights, ids, W13, W2)
+    given = x.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = layer(given, weights, ids)
+    for i in (1, 0, 1, 2, 3, 0, 2, 3):
+        given.copy_(kinds[i])
+        graph.replay()
+        assert torch.equal(out, want[i])
