@@ -148,7 +148,9 @@ struct StreamScratch {
 };
 bool capturing(cudaStream_t st) {
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
-  return cudaStreamIsCapturing(st, &cap) == cudaSuccess && cap != cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &cap) == cudaSuccess) return cap != cudaStreamCaptureStatusNone;
+  cudaGetLastError();                              // the legacy stream beside another's capture: nobody else's error
+  return false;
 }
 struct StreamKey {
   int dev;
